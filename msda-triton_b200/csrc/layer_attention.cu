@@ -1,0 +1,207 @@
+// C ABI of masked attention (declared in include/msda_layer_b200.h): argument
+// checks, the choice of kernel and the workspace's layout.
+#include <cmath>
+
+#include "layer_attention.cuh"
+
+namespace {
+
+using namespace msda;
+using namespace msda::abi;
+
+// Query rows (queries x heads that share a key head) up to which the few-rows
+// kernels run, whose CTAs split the keys.
+constexpr int64_t kTokenRows = 64;
+constexpr int kMaxSplits = 64;
+
+enum class Path { kSimt, kToken };
+
+int check(const char* fn, const msda_attention_args* a, bool backward) {
+  if (!a) return fail(MSDA_ERR_INVALID_ARGUMENT, "%s: null arguments", fn);
+  if (elem_size(a->dtype) == 0) return fail(MSDA_ERR_UNSUPPORTED, "%s: unsupported dtype code %d (0=f32, 1=f16, 2=bf16)", fn, a->dtype);
+  if (a->batch < 0 || a->num_queries < 0 || a->num_keys < 0) return fail(MSDA_ERR_INVALID_ARGUMENT, "%s: negative size", fn);
+  if (a->num_heads < 1 || a->num_key_heads < 1 || a->num_heads % a->num_key_heads)
+    return fail(MSDA_ERR_INVALID_ARGUMENT, "%s: num_heads=%d must be a multiple of num_key_heads=%d", fn, a->num_heads, a->num_key_heads);
+  if (a->head_dim < 1 || a->head_dim > MSDA_ATTENTION_MAX_HEAD_DIM)
+    return fail(MSDA_ERR_UNSUPPORTED, "%s: head_dim=%d outside [1, %d]", fn, a->head_dim, MSDA_ATTENTION_MAX_HEAD_DIM);
+  if (a->batch > 65535 || a->num_heads > 4096 || a->num_queries > (1 << 24) || a->num_keys > (1 << 30))
+    return fail(MSDA_ERR_UNSUPPORTED, "%s: sizes exceed batch 65535, 4096 heads, 2^24 queries or 2^30 keys", fn);
+  if (!std::isfinite(a->scale) || !std::isfinite(a->softcap) || a->softcap < 0)
+    return fail(MSDA_ERR_INVALID_ARGUMENT, "%s: scale must be finite, softcap finite and >= 0", fn);
+  if (!a->query_documents != !a->key_documents)
+    return fail(MSDA_ERR_INVALID_ARGUMENT, "%s: documents of queries and keys come together", fn);
+  if (a->prefix_lengths && !a->causal) return fail(MSDA_ERR_INVALID_ARGUMENT, "%s: prefix_lengths needs causal", fn);
+  if (a->batch == 0) return MSDA_OK;
+  const int es = elem_size(a->dtype);
+  if (a->num_queries > 0 && (!a->query || !a->out)) return fail(MSDA_ERR_INVALID_ARGUMENT, "%s: null pointer argument", fn);
+  if (a->num_keys > 0 && (!a->key || !a->value)) return fail(MSDA_ERR_INVALID_ARGUMENT, "%s: null pointer argument", fn);
+  const void* data[] = {a->query, a->key, a->value, a->out, a->out_residue, a->grad_out, a->grad_query, a->grad_key, a->grad_value};
+  for (const void* p : data)
+    if (!aligned(p, es)) return fail(MSDA_ERR_INVALID_ARGUMENT, "%s: misaligned buffer", fn);
+  const void* words[] = {a->lse, a->distance_slopes, a->query_documents, a->key_documents, a->prefix_lengths, a->key_lengths};
+  for (const void* p : words)
+    if (!aligned(p, 4)) return fail(MSDA_ERR_INVALID_ARGUMENT, "%s: misaligned buffer", fn);
+  if (backward) {
+    if (a->num_queries > 0 && (!a->lse || !a->grad_out || !a->grad_query))
+      return fail(MSDA_ERR_INVALID_ARGUMENT, "%s: null pointer argument", fn);
+    if (a->num_keys > 0 && (!a->grad_key || !a->grad_value)) return fail(MSDA_ERR_INVALID_ARGUMENT, "%s: null pointer argument", fn);
+  }
+  return MSDA_OK;
+}
+
+// 16-byte loads of 8 channels: the tensor-core kernels' layout.
+bool rows_of_16(const void* p, const int64_t (&s)[3], const int64_t (&n)[3]) {
+  for (int i = 0; i < 3; ++i)
+    if (n[i] > 1 && (s[i] <= 0 || s[i] % 8)) return false;
+  return aligned(p, 16);
+}
+
+bool tensor_layout(const msda_attention_args* a) {
+  if (a->dtype == MSDA_DTYPE_F32 || a->head_dim % 8 || a->head_dim > 128) return false;
+  const int64_t nq[3] = {a->batch, a->num_queries, a->num_heads}, nk[3] = {a->batch, a->num_keys, a->num_key_heads};
+  return rows_of_16(a->query, a->query_strides, nq) && rows_of_16(a->key, a->key_strides, nk) &&
+         rows_of_16(a->value, a->value_strides, nk);
+}
+
+struct Plan {
+  Path path = Path::kSimt;
+  int splits = 1;
+  int64_t q_tiles = 0, k_tiles = 0;  // document summary entries
+  size_t delta = 0, part_ml = 0, part_o = 0, bytes = 0;  // byte offsets, after the summary; total
+};
+
+Plan plan_of(const msda_attention_args* a, bool backward) {
+  Plan p;
+  const int64_t group = a->num_heads / a->num_key_heads, rows = a->num_queries * group;
+  if (!backward && rows <= kTokenRows) {
+    const bool tensor = tensor_layout(a);
+    p.path = tensor ? Path::kToken : Path::kSimt;
+    // Parts of at least 128 keys, enough of them for 16 CTAs an SM, so that
+    // streams of different lengths even out.
+    const int64_t tiles = tensor ? (rows + 15) / 16 : (rows + 31) / 32;
+    const int64_t ctas = a->batch * a->num_key_heads * tiles;
+    int64_t s = 16 * (int64_t)sm_count() / (ctas > 0 ? ctas : 1);
+    const int64_t most = (a->num_keys + 127) / 128;
+    if (s > most) s = most;
+    if (s > kMaxSplits) s = kMaxSplits;
+    p.splits = s < 1 ? 1 : (int)s;
+    if (!tensor && p.splits < 2 && a->num_keys > 64) p.splits = 2;  // the packed rows' form
+  }
+  size_t at = 0;
+  const bool documents = a->query_documents && p.path != Path::kToken && p.splits == 1;
+  if (documents) {
+    p.q_tiles = a->batch * ((a->num_queries + kDocTile - 1) / kDocTile);
+    p.k_tiles = a->batch * ((a->num_keys + kDocTile - 1) / kDocTile);
+    at = align256((p.q_tiles + p.k_tiles) * sizeof(DocTile));
+  }
+  const size_t all = (size_t)a->batch * a->num_heads * a->num_queries;
+  if (backward) {
+    p.delta = at;
+    at += align256(all * 4);
+  }
+  if (p.splits > 1) {
+    p.part_ml = at;
+    at += align256(all * p.splits * 8);
+    p.part_o = at;
+    at += align256(all * p.splits * a->head_dim * 4);
+  }
+  p.bytes = at;
+  return p;
+}
+
+void copy3(int64_t (&to)[3], const int64_t (&from)[3]) {
+  for (int i = 0; i < 3; ++i) to[i] = from[i];
+}
+
+AttnParams params_of(const msda_attention_args* a, const Plan& plan) {
+  AttnParams p = {};
+  p.q = a->query, p.k = a->key, p.v = a->value, p.go = a->grad_out;
+  p.o = a->out, p.residue = a->dtype == MSDA_DTYPE_F32 ? nullptr : a->out_residue, p.dq = a->grad_query, p.dk = a->grad_key, p.dv = a->grad_value;
+  p.lse = a->lse;
+  copy3(p.qs, a->query_strides);
+  copy3(p.ks, a->key_strides);
+  copy3(p.vs, a->value_strides);
+  copy3(p.gs, a->grad_out_strides);
+  p.slopes = a->distance_slopes;
+  p.qdoc = a->query_documents, p.kdoc = a->key_documents;
+  p.prefix = a->prefix_lengths, p.klen = a->key_lengths;
+  p.B = (int)a->batch, p.Sq = (int)a->num_queries, p.Sk = (int)a->num_keys;
+  p.H = a->num_heads, p.Hkv = a->num_key_heads, p.D = a->head_dim;
+  p.scale = a->scale, p.cap = a->softcap;
+  p.shared = a->shared_document < 0 ? -1 : a->shared_document;
+  p.causal = a->causal != 0;
+  p.splits = plan.splits;
+  char* ws = static_cast<char*>(a->workspace);
+  if (plan.q_tiles + plan.k_tiles > 0) {
+    p.qtile = reinterpret_cast<DocTile*>(ws);
+    p.ktile = p.qtile + plan.q_tiles;
+  }
+  p.delta = reinterpret_cast<float*>(ws + plan.delta);
+  p.part_ml = reinterpret_cast<float2*>(ws + plan.part_ml);
+  p.part_o = reinterpret_cast<float*>(ws + plan.part_o);
+  return p;
+}
+
+int check_workspace(const char* fn, const msda_attention_args* a, const Plan& plan) {
+  if (plan.bytes && (!a->workspace || a->workspace_bytes < plan.bytes || !aligned(a->workspace, 16)))
+    return fail(MSDA_ERR_INVALID_ARGUMENT, "%s: workspace of %zu bytes (16-byte aligned), needs %zu", fn,
+                a->workspace ? a->workspace_bytes : 0, plan.bytes);
+  return MSDA_OK;
+}
+
+cudaError_t documents(const AttnParams& p, const Plan& plan, cudaStream_t st) {
+  if (plan.q_tiles + plan.k_tiles == 0) return cudaSuccess;
+  return attn_documents_launch(p, const_cast<DocTile*>(p.qtile), const_cast<DocTile*>(p.ktile), st);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t msda_attention_workspace_size(const msda_attention_args* a, int32_t backward) {
+  if (!a || elem_size(a->dtype) == 0 || a->batch < 1 || a->num_queries < 1 || a->num_keys < 0 || a->num_heads < 1 ||
+      a->num_key_heads < 1 || a->num_heads % a->num_key_heads || a->head_dim < 1 || a->head_dim > MSDA_ATTENTION_MAX_HEAD_DIM)
+    return 0;
+  return plan_of(a, backward != 0).bytes;
+}
+
+int msda_attention_forward(const msda_attention_args* a, void* stream) {
+  const char* fn = "msda_attention_forward";
+  if (int rc = check(fn, a, false)) return rc;
+  if (a->batch == 0 || a->num_queries == 0) return succeed();
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const Plan plan = plan_of(a, false);
+  if (int rc = check_workspace(fn, a, plan)) return rc;
+  const AttnParams p = params_of(a, plan);
+  cudaError_t e = documents(p, plan, st);
+  if (e == cudaSuccess)
+    e = plan.path == Path::kToken ? attn_token_forward(p, a->dtype, st) : attn_simt_forward(p, a->dtype, st);
+  if (e == cudaSuccess && plan.splits > 1) e = attn_combine_launch(p, a->dtype, st);
+  if (e != cudaSuccess) return cuda_fail(e, "attention launch");
+  return succeed();
+}
+
+int msda_attention_backward(const msda_attention_args* a, void* stream) {
+  const char* fn = "msda_attention_backward";
+  if (int rc = check(fn, a, true)) return rc;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (a->batch == 0) return succeed();
+  if (a->num_queries == 0 || a->num_keys == 0) {
+    const size_t row = (size_t)a->batch * a->head_dim * elem_size(a->dtype);
+    cudaError_t e = cudaSuccess;
+    if (a->num_queries > 0) e = cudaMemsetAsync(a->grad_query, 0, row * a->num_queries * a->num_heads, st);
+    if (e == cudaSuccess && a->num_keys > 0) e = cudaMemsetAsync(a->grad_key, 0, row * a->num_keys * a->num_key_heads, st);
+    if (e == cudaSuccess && a->num_keys > 0) e = cudaMemsetAsync(a->grad_value, 0, row * a->num_keys * a->num_key_heads, st);
+    if (e != cudaSuccess) return cuda_fail(e, "attention zero-fill");
+    return succeed();
+  }
+  const Plan plan = plan_of(a, true);
+  if (int rc = check_workspace(fn, a, plan)) return rc;
+  const AttnParams p = params_of(a, plan);
+  cudaError_t e = documents(p, plan, st);
+  if (e == cudaSuccess) e = attn_simt_backward(p, a->dtype, st);
+  if (e != cudaSuccess) return cuda_fail(e, "attention backward launch");
+  return succeed();
+}
+
+}  // extern "C"

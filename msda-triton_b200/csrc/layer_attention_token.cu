@@ -1,0 +1,308 @@
+// Attention of a few queries over a long cache, fp16 and bf16: the form for
+// single tokens.
+//
+// Bound by HBM: the visible keys and values are read once. The heads that share
+// a key head and the queries are packed into the 16 rows of an m16n8k16 product,
+// so that shared heads cost no further reads. Keys and values go from global
+// memory straight to the registers of that product, 16 bytes a thread: the
+// order of channels within a product is free as long as both sides agree, so a
+// thread takes 8 neighbouring channels of a key for four k-slots of two products;
+// for the values a thread takes a few neighbouring channels of four keys and
+// pairs the keys by byte permutes. No shared memory, no barrier in the loop: the
+// latency is covered by the loads of the SM's other warps. The keys are split
+// over CTAs, whose parts the combining kernel joins.
+#include "layer_attention.cuh"
+
+namespace msda {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kStep = 16;  // keys a warp takes at once
+
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  Pack<T, 2> u;
+  u.e[0] = from_f32<T>(a);
+  u.e[1] = from_f32<T>(b);
+  return u.raw;
+}
+
+// 16 bytes of the cache, which is read once: past L1.
+__device__ __forceinline__ uint4 load_cache(const void* p) {
+  uint4 r;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+  return r;
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kWarps * 32, DP == 128 ? 2 : 4) attn_token_kernel(const AttnParams p) {
+  constexpr int KC = DP / 32;               // 32-channel chunks of a key
+  constexpr int VE = DP == 32 ? 4 : 8;      // neighbouring channels of a value that a thread takes
+  constexpr int VC = DP / (8 * VE);         // groups of them
+  constexpr int NT = DP / 8;                // output tiles of 8 channels
+  __shared__ float part_o[kWarps - 1][16][DP + 4];
+  __shared__ float2 part_ml[kWarps][16];
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, t = lane % 4;
+  const int group = p.H / p.Hkv, rows = p.Sq * group;
+  const int tiles = (rows + 15) / 16;
+  const int hk = blockIdx.y / tiles, r0 = blockIdx.y % tiles * 16, b = blockIdx.z, split = blockIdx.x;
+  const int length = attn_length(p, b);
+  int first, last;
+  split_range(rows_limit(p, b, (min(r0 + 16, rows) + group - 1) / group, length), p.splits, split, first, last);
+  const T* kb = static_cast<const T*>(p.k) + b * p.ks[0] + hk * p.ks[2];
+  const T* vb = static_cast<const T*>(p.v) + b * p.vs[0] + hk * p.vs[2];
+  const int* kdoc = p.kdoc ? p.kdoc + (int64_t)b * p.Sk : nullptr;
+  ScoreForm f = score_form(p, 0);
+  RowView row[2];
+  float slope[2];
+  uint32_t qa[KC][2][4];  // products' left sides: rows g and g + 8, channels 8 t ... of each chunk
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = r0 + g + 8 * i, at = r / group, h = hk * group + r % group;
+    const bool in = r < rows;
+    row[i] = row_view(p, b, in ? at : p.Sq, length);
+    slope[i] = in && p.slopes ? __ldg(p.slopes + h) * kLog2e : 0.0f;
+    const T* q = static_cast<const T*>(p.q) + b * p.qs[0] + at * p.qs[1] + h * p.qs[2];
+#pragma unroll
+    for (int c = 0; c < KC; ++c) {
+      const int d = c * 32 + t * 8;
+      uint4 u = make_uint4(0, 0, 0, 0);
+      if (in && d < p.D) u = __ldg(reinterpret_cast<const uint4*>(q + d));
+      qa[c][0][i] = u.x, qa[c][0][2 + i] = u.y, qa[c][1][i] = u.z, qa[c][1][2 + i] = u.w;
+    }
+  }
+  float o[NT][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[n][i] = 0.0f;
+
+  for (int j0 = first + warp * kStep; j0 < last; j0 += kWarps * kStep) {
+    uint4 kr[2][KC];
+    uint32_t vr[4][VC][VE / 2];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const int j = j0 + g + 8 * n;
+      const bool in = j < last && (!kdoc || __ldg(kdoc + j) >= 0);
+#pragma unroll
+      for (int c = 0; c < KC; ++c) {
+        const int d = c * 32 + t * 8;
+        kr[n][c] = make_uint4(0, 0, 0, 0);
+        if (in && d < p.D) kr[n][c] = load_cache(kb + j * p.ks[1] + d);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const int j = j0 + t * 2 + (n & 1) + (n >> 1) * 8;
+      const bool in = j < last && (!kdoc || __ldg(kdoc + j) >= 0);
+#pragma unroll
+      for (int c = 0; c < VC; ++c) {
+        const int d = c * 64 + g * VE;
+        const T* v = vb + j * p.vs[1] + d;
+        if constexpr (VE == 8) {
+          uint4 u = make_uint4(0, 0, 0, 0);
+          if (in && d < p.D) u = load_cache(v);
+          vr[n][c][0] = u.x, vr[n][c][1] = u.y, vr[n][c][2] = u.z, vr[n][c][3] = u.w;
+        } else {
+          uint2 u = make_uint2(0, 0);
+          if (in && d < p.D) u = __ldg(reinterpret_cast<const uint2*>(v));
+          vr[n][c][0] = u.x, vr[n][c][1] = u.y;
+        }
+      }
+    }
+    float s[2][4];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+#pragma unroll
+      for (int c = 0; c < KC; ++c) {
+        mma16816<T>(s[n], qa[c][0], kr[n][c].x, kr[n][c].y);
+        mma16816<T>(s[n], qa[c][1], kr[n][c].z, kr[n][c].w);
+      }
+    }
+    // s[n][2 i + e]: row g + 8 i, key j0 + 8 n + 2 t + e.
+    float top[2] = {m[0], m[1]};
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int j = j0 + 8 * n + 2 * t + e;
+        const int kd = kdoc && j < last ? __ldg(kdoc + j) : 0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float x = s[n][2 * i + e] * f.scale2;
+          if (p.cap != 0.0f) x = tanh_of(s[n][2 * i + e] * f.inv_cap) * f.cap2;
+          if (p.slopes) x = fmaf(-slope[i], (float)abs(row[i].place - j), x);
+          const bool seen = j < last && j < row[i].limit && (!kdoc || same_document(row[i].doc, kd, p.shared));
+          s[n][2 * i + e] = seen ? x : -INFINITY;
+          top[i] = fmaxf(top[i], s[n][2 * i + e]);
+        }
+      }
+    uint32_t pa[4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      top[i] = fmaxf(top[i], __shfl_xor_sync(kFullMask, top[i], 1));
+      top[i] = fmaxf(top[i], __shfl_xor_sync(kFullMask, top[i], 2));
+      const float base = top[i] == -INFINITY ? 0.0f : top[i];
+      const float old = exp2f(m[i] - base);
+      m[i] = top[i];
+      l[i] *= old;
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const float e0 = exp2f(s[n][2 * i] - base), e1 = exp2f(s[n][2 * i + 1] - base);
+        l[i] += e0 + e1;
+        pa[2 * n + i] = pack2<T>(e0, e1);
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        o[n][2 * i] *= old;
+        o[n][2 * i + 1] *= old;
+      }
+    }
+    // Output tile (c, e): channels c * 64 + 8-wide (or 4-wide) groups' element e.
+#pragma unroll
+    for (int c = 0; c < VC; ++c)
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const uint32_t pick = e & 1 ? 0x7632 : 0x5410;
+        const uint32_t b0 = __byte_perm(vr[0][c][e / 2], vr[1][c][e / 2], pick);
+        const uint32_t b1 = __byte_perm(vr[2][c][e / 2], vr[3][c][e / 2], pick);
+        mma16816<T>(o[c * VE + e], pa, b0, b1);
+      }
+  }
+  // Join the CTA's warps.
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    l[i] += __shfl_xor_sync(kFullMask, l[i], 1);
+    l[i] += __shfl_xor_sync(kFullMask, l[i], 2);
+    if (t == 0) part_ml[warp][g + 8 * i] = make_float2(m[i], l[i]);
+  }
+  __syncthreads();
+  float all_m[2], all_l[2], mine[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    all_m[i] = -INFINITY, all_l[i] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) all_m[i] = fmaxf(all_m[i], part_ml[w][g + 8 * i].x);
+    const float base = all_m[i] == -INFINITY ? 0.0f : all_m[i];
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float2 ml = part_ml[w][g + 8 * i];
+      all_l[i] += ml.y * exp2f(ml.x - base);
+    }
+    mine[i] = exp2f(m[i] - base);
+  }
+  // Channel of o[c * VE + e][2 i + x]: c * 64 + (2 t + x) * VE + e.
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        o[n][2 * i + x] *= mine[i];
+        if (warp > 0) part_o[warp - 1][g + 8 * i][n / VE * 64 + (2 * t + x) * VE + n % VE] = o[n][2 * i + x];
+      }
+  __syncthreads();
+  if (warp > 0) return;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = r0 + g + 8 * i;
+    if (r >= rows) continue;
+    const int at = r / group, h = hk * group + r % group;
+    const int64_t out = ((int64_t)b * p.H + h) * p.Sq + at;
+    const int64_t part = (int64_t)split * p.B * p.H * p.Sq + out;
+    const float mul = all_l[i] > 0.0f ? 1.0f / all_l[i] : (all_l[i] == 0.0f ? 0.0f : all_l[i]);
+    if (t == 0) {
+      if (p.splits > 1) p.part_ml[part] = make_float2(all_m[i], all_l[i]);
+      else if (p.lse) p.lse[out] = all_l[i] == 0.0f ? -INFINITY : (all_m[i] + log2f(all_l[i])) * kLn2;
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int d = n / VE * 64 + (2 * t + x) * VE + n % VE;
+        float v = o[n][2 * i + x];
+#pragma unroll
+        for (int w = 0; w < kWarps - 1; ++w) v += part_o[w][g + 8 * i][d];
+        if (d >= p.D) continue;
+        if (p.splits > 1) p.part_o[part * p.D + d] = v;
+        else put_output<T>(p, (((int64_t)b * p.Sq + at) * p.H + h) * p.D + d, v * mul);
+      }
+  }
+}
+
+// Joins the parts of each row in the parts' order: a warp a row.
+template <typename T>
+__global__ void __launch_bounds__(128) attn_combine_kernel(const AttnParams p) {
+  pdl_wait();
+  const int64_t rows = (int64_t)p.B * p.H * p.Sq;
+  const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / 32;
+  if (row >= rows) return;
+  const int lane = threadIdx.x % 32;
+  float top = -INFINITY;
+  for (int s = lane; s < p.splits; s += 32) top = fmaxf(top, __ldcg(&p.part_ml[s * rows + row]).x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, o));
+  const float base = top == -INFINITY ? 0.0f : top;
+  float total = 0.0f, acc[8];
+#pragma unroll
+  for (int c = 0; c < 8; ++c) acc[c] = 0.0f;
+#pragma unroll 4
+  for (int s = 0; s < p.splits; ++s) {
+    const float2 ml = __ldcg(&p.part_ml[s * rows + row]);
+    const float w = exp2f(ml.x - base);
+    total = fmaf(ml.y, w, total);
+    if (ml.y == 0.0f) continue;  // a part without keys
+    const float* o = p.part_o + (s * rows + row) * p.D;
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      if (lane + 32 * c < p.D) acc[c] = fmaf(__ldcg(o + lane + 32 * c), w, acc[c]);
+  }
+  const float mul = total > 0.0f ? 1.0f / total : (total == 0.0f ? 0.0f : total);
+  const int i = (int)(row % p.Sq), h = (int)(row / p.Sq % p.H);
+  const int64_t b = row / p.Sq / p.H;
+  const int64_t out = ((b * p.Sq + i) * p.H + h) * p.D;
+#pragma unroll
+  for (int c = 0; c < 8; ++c)
+    if (lane + 32 * c < p.D) put_output<T>(p, out + lane + 32 * c, acc[c] * mul);
+  if (p.lse && lane == 0) p.lse[row] = total == 0.0f ? -INFINITY : (top + log2f(total)) * kLn2;
+}
+
+template <typename T>
+cudaError_t token_t(const AttnParams& p, cudaStream_t st) {
+  const int rows = p.Sq * (p.H / p.Hkv);
+  const dim3 grid(p.splits, p.Hkv * ((rows + 15) / 16), p.B);
+  if (p.D <= 32) attn_token_kernel<T, 32><<<grid, kWarps * 32, 0, st>>>(p);
+  else if (p.D <= 64) attn_token_kernel<T, 64><<<grid, kWarps * 32, 0, st>>>(p);
+  else attn_token_kernel<T, 128><<<grid, kWarps * 32, 0, st>>>(p);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t attn_token_forward(const AttnParams& p, int dtype, cudaStream_t st) {
+  return dtype == MSDA_DTYPE_F16 ? token_t<__half>(p, st) : token_t<__nv_bfloat16>(p, st);
+}
+
+cudaError_t attn_combine_launch(const AttnParams& p, int dtype, cudaStream_t st) {
+  const int64_t rows = (int64_t)p.B * p.H * p.Sq;
+  const dim3 grid((unsigned)((rows + 3) / 4));
+  if (dtype == MSDA_DTYPE_F32) return launch_ex(attn_combine_kernel<float>, grid, dim3(128), 0, st, true, p);
+  if (dtype == MSDA_DTYPE_F16) return launch_ex(attn_combine_kernel<__half>, grid, dim3(128), 0, st, true, p);
+  return launch_ex(attn_combine_kernel<__nv_bfloat16>, grid, dim3(128), 0, st, true, p);
+}
+
+}  // namespace msda

@@ -1,4 +1,5 @@
-"""ctypes binding of ``libmsda_b200.so`` (C ABI declared in include/msda_b200.h).
+"""ctypes binding of ``libmsda_b200.so`` (C ABI declared in include/msda_b200.h
+and include/msda_layer_b200.h).
 
 The library is loaded lazily on first use. If it is missing or cannot be
 loaded the op raises ``RuntimeError``: there is no fallback implementation.
@@ -28,7 +29,16 @@ MSDA_BWD_FORCE_COUNTED = 8
 MSDA_BWD_DETERMINISTIC = 16
 MSDA_BWD_GRAD_INPUT_NCHW = 32
 
-# Every symbol include/msda_b200.h declares, with (restype, argtypes).
+MSDA_POSITION_F32 = 0
+MSDA_POSITION_I32 = 1
+MSDA_POSITION_I64 = 2
+MSDA_ROTARY_MAX_AXES = 8
+MSDA_ROTARY_MAX_HEAD_DIM = 512
+MSDA_LAYER_NORM_MAX_WIDTH = 1 << 20
+MSDA_ATTENTION_MAX_HEAD_DIM = 256
+
+# Every symbol include/msda_b200.h and include/msda_layer_b200.h declare, with
+# (restype, argtypes).
 _VP = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I32 = ctypes.c_int32
@@ -87,11 +97,54 @@ SIGNATURES = {
         [_VP, _VP, _VP, _VP, ctypes.c_size_t, _I64, _I64, _I64, _I64, _I64, _I32, _I32,
          ctypes.c_float, _I32, _I32, _I32, ctypes.c_uint32, _VP],
     ),
+    # include/msda_layer_b200.h: the operators beside the sampling.
+    "msda_rotary": (
+        ctypes.c_int,
+        [_VP, _VP, _VP, _VP, _VP, _I64, _I64, _I32, _I32, _I32, _VP, _VP, _I64, _I32, _I32, _VP,
+         ctypes.c_double, _I32, _I32, _I32, _I32, _VP],
+    ),
+    "msda_layer_norm_forward": (
+        ctypes.c_int,
+        [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _I64, _I64, _I64, _I64, ctypes.c_float, _I32, _I32, _VP],
+    ),
+    "msda_layer_norm_backward_workspace_size": (ctypes.c_size_t, [_I64, _I64]),
+    "msda_layer_norm_backward": (
+        ctypes.c_int,
+        [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, ctypes.c_size_t,
+         _I64, _I64, _I64, _I64, _I64, _I32, _I32, _VP],
+    ),
+    "msda_attention_workspace_size": (ctypes.c_size_t, [_VP, _I32]),
+    "msda_attention_forward": (ctypes.c_int, [_VP, _VP]),
+    "msda_attention_backward": (ctypes.c_int, [_VP, _VP]),
 }
 
 # Size of the static scratch behind msda_backward_noalloc
 # (MSDA_NOALLOC_SCRATCH_BYTES in include/msda_b200.h).
 MSDA_NOALLOC_SCRATCH_BYTES = 16 << 20
+
+
+class AttentionArgs(ctypes.Structure):
+    """msda_attention_args of include/msda_layer_b200.h."""
+
+    _fields_ = [
+        (n, ctypes.c_void_p) for n in ("query", "key", "value", "out", "out_residue", "lse", "grad_out", "grad_query", "grad_key",
+                                       "grad_value")
+    ] + [
+        (n, ctypes.c_int64) for n in ("batch", "num_queries", "num_keys")
+    ] + [
+        (n, ctypes.c_int32) for n in ("num_heads", "num_key_heads", "head_dim", "dtype")
+    ] + [
+        (n, ctypes.c_int64 * 3) for n in ("query_strides", "key_strides", "value_strides", "grad_out_strides")
+    ] + [
+        ("scale", ctypes.c_float), ("softcap", ctypes.c_float)
+    ] + [
+        (n, ctypes.c_void_p) for n in ("distance_slopes", "query_documents", "key_documents", "prefix_lengths",
+                                       "key_lengths")
+    ] + [
+        ("shared_document", ctypes.c_int32), ("causal", ctypes.c_int32),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
