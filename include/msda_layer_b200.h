@@ -145,6 +145,10 @@ MSDA_API size_t msda_attention_workspace_size(const msda_attention_args* args, i
  * sizes: results are bitwise reproducible. */
 MSDA_API int msda_attention_forward(const msda_attention_args* args, void* stream);
 MSDA_API int msda_attention_backward(const msda_attention_args* args, void* stream);
+/* The tensor-core kernels' waits are bounded: one that gives up (a fault of
+ * the hardware or of this library) leaves NaN in the outputs and is counted.
+ * Reads the current device's count; synchronises with it. */
+MSDA_API int msda_attention_gave_up(int32_t* count);
 
 #ifdef __cplusplus
 }

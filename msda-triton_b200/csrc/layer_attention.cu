@@ -1,8 +1,65 @@
 // C ABI of masked attention (declared in include/msda_layer_b200.h): argument
 // checks, the choice of kernel and the workspace's layout.
+#include <cuda.h>
+
 #include <cmath>
 
 #include "layer_attention.cuh"
+
+namespace msda {
+namespace tc {
+
+int run_f16(const AttnParams& p, bool backward, cudaStream_t st);
+int run_bf16(const AttnParams& p, bool backward, cudaStream_t st);
+cudaError_t gave_up_f16(int* count);
+cudaError_t gave_up_bf16(int* count);
+
+// The map of a (B, S, H, D) tensor by boxes of 64 channels x 1 head x 128 tokens
+// in 128-byte swizzled rows; what lies outside comes as zeros.
+bool make_map(CUtensorMap* map, const void* base, bool bf16, int64_t D, int64_t H, int64_t S, int64_t B,
+              const int64_t (&strides)[3]) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static const Encode encode = [] {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess)
+      fn = nullptr;
+    return reinterpret_cast<Encode>(fn);
+  }();
+  if (!encode) return false;
+  const cuuint64_t size[4] = {(cuuint64_t)D, (cuuint64_t)H, (cuuint64_t)S, (cuuint64_t)B};
+  const int64_t from[3] = {strides[2], strides[1], strides[0]};
+  cuuint64_t stride[3];
+  // A dimension of one element may have any stride; 16 bytes stand for it.
+  for (int i = 0; i < 3; ++i) stride[i] = size[i + 1] > 1 ? (cuuint64_t)from[i] * 2 : 16;
+  const cuuint32_t box[4] = {64, 1, 128, 1}, step[4] = {1, 1, 1, 1};
+  return encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), size,
+                stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace tc
+
+int attn_tc_forward(const AttnParams& p, int dtype, cudaStream_t st) {
+  return dtype == MSDA_DTYPE_F16 ? tc::run_f16(p, false, st) : tc::run_bf16(p, false, st);
+}
+
+int attn_tc_backward(const AttnParams& p, int dtype, cudaStream_t st) {
+  return dtype == MSDA_DTYPE_F16 ? tc::run_f16(p, true, st) : tc::run_bf16(p, true, st);
+}
+
+cudaError_t attn_tc_gave_up(int* count) {
+  int a = 0, b = 0;
+  cudaError_t e = tc::gave_up_f16(&a);
+  if (e == cudaSuccess) e = tc::gave_up_bf16(&b);
+  *count = a + b;
+  return e;
+}
+
+}  // namespace msda
 
 namespace {
 
@@ -14,7 +71,7 @@ using namespace msda::abi;
 constexpr int64_t kTokenRows = 64;
 constexpr int kMaxSplits = 64;
 
-enum class Path { kSimt, kToken };
+enum class Path { kSimt, kToken, kTensor };
 
 int check(const char* fn, const msda_attention_args* a, bool backward) {
   if (!a) return fail(MSDA_ERR_INVALID_ARGUMENT, "%s: null arguments", fn);
@@ -56,11 +113,13 @@ bool rows_of_16(const void* p, const int64_t (&s)[3], const int64_t (&n)[3]) {
   return aligned(p, 16);
 }
 
-bool tensor_layout(const msda_attention_args* a) {
+bool tensor_layout(const msda_attention_args* a, bool backward) {
   if (a->dtype == MSDA_DTYPE_F32 || a->head_dim % 8 || a->head_dim > 128) return false;
   const int64_t nq[3] = {a->batch, a->num_queries, a->num_heads}, nk[3] = {a->batch, a->num_keys, a->num_key_heads};
   return rows_of_16(a->query, a->query_strides, nq) && rows_of_16(a->key, a->key_strides, nk) &&
-         rows_of_16(a->value, a->value_strides, nk);
+         rows_of_16(a->value, a->value_strides, nk) && aligned(a->out, 16) && aligned(a->out_residue, 16) &&
+         (!backward || (rows_of_16(a->grad_out, a->grad_out_strides, nq) && aligned(a->grad_query, 16) &&
+                        aligned(a->grad_key, 16) && aligned(a->grad_value, 16)));
 }
 
 struct Plan {
@@ -73,9 +132,10 @@ struct Plan {
 Plan plan_of(const msda_attention_args* a, bool backward) {
   Plan p;
   const int64_t group = a->num_heads / a->num_key_heads, rows = a->num_queries * group;
+  const bool tensor = tensor_layout(a, backward);
+  if (tensor && a->num_keys > 0) p.path = Path::kTensor;
   if (!backward && rows <= kTokenRows) {
-    const bool tensor = tensor_layout(a);
-    p.path = tensor ? Path::kToken : Path::kSimt;
+    if (tensor) p.path = Path::kToken;
     // Parts of at least 128 keys, enough of them for 16 CTAs an SM, so that
     // streams of different lengths even out.
     const int64_t tiles = tensor ? (rows + 15) / 16 : (rows + 31) / 32;
@@ -174,10 +234,24 @@ int msda_attention_forward(const msda_attention_args* a, void* stream) {
   if (int rc = check_workspace(fn, a, plan)) return rc;
   const AttnParams p = params_of(a, plan);
   cudaError_t e = documents(p, plan, st);
-  if (e == cudaSuccess)
+  if (e == cudaSuccess && plan.path == Path::kTensor) {
+    const int rc = attn_tc_forward(p, a->dtype, st);
+    if (rc < 0) return fail(MSDA_ERR_CUDA, "%s: no tensor map for these sizes and strides", fn);
+    e = (cudaError_t)rc;
+  } else if (e == cudaSuccess) {
     e = plan.path == Path::kToken ? attn_token_forward(p, a->dtype, st) : attn_simt_forward(p, a->dtype, st);
+  }
   if (e == cudaSuccess && plan.splits > 1) e = attn_combine_launch(p, a->dtype, st);
   if (e != cudaSuccess) return cuda_fail(e, "attention launch");
+  return succeed();
+}
+
+int msda_attention_gave_up(int32_t* count) {
+  if (!count) return fail(MSDA_ERR_INVALID_ARGUMENT, "msda_attention_gave_up: null pointer argument");
+  int n = 0;
+  const cudaError_t e = attn_tc_gave_up(&n);
+  if (e != cudaSuccess) return cuda_fail(e, "attention status");
+  *count = n;
   return succeed();
 }
 
@@ -199,7 +273,13 @@ int msda_attention_backward(const msda_attention_args* a, void* stream) {
   if (int rc = check_workspace(fn, a, plan)) return rc;
   const AttnParams p = params_of(a, plan);
   cudaError_t e = documents(p, plan, st);
-  if (e == cudaSuccess) e = attn_simt_backward(p, a->dtype, st);
+  if (e == cudaSuccess && plan.path == Path::kTensor) {
+    const int rc = attn_tc_backward(p, a->dtype, st);
+    if (rc < 0) return fail(MSDA_ERR_CUDA, "%s: no tensor map for these sizes and strides", fn);
+    e = (cudaError_t)rc;
+  } else if (e == cudaSuccess) {
+    e = attn_simt_backward(p, a->dtype, st);
+  }
   if (e != cudaSuccess) return cuda_fail(e, "attention backward launch");
   return succeed();
 }

@@ -23,10 +23,10 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kDocTile = 128;  // tokens one entry of the document summary stands for
 
 // Documents of a tile of kDocTile tokens: those that are no padding lie in
-// [low, high] (low > high: all padding); `mixed`: some are padding, or
-// documents differ; `shared`: some key is of the shared document.
+// [low, high] (low > high: all padding); `padded`: some are padding; `shared`:
+// some key is of the shared document.
 struct DocTile {
-  int low, high, mixed, shared;
+  int low, high, padded, shared;
 };
 
 struct AttnParams {
@@ -45,7 +45,6 @@ struct AttnParams {
   int splits;          // parts of the keys; above 1 the parts' results go to part_o, part_ml
   float* part_o;       // (splits, B, H, Sq, D)
   float2* part_ml;     // (splits, B, H, Sq): maximum (base 2) and sum
-  int* status;         // set to non-zero by a wait that gave up
 };
 
 __device__ __forceinline__ int attn_length(const AttnParams& p, int b) {
@@ -102,18 +101,21 @@ __device__ __forceinline__ bool tiles_apart(const DocTile& q, const DocTile& k) 
 
 // Whether every query of one tile sees every key of the other by their documents.
 __device__ __forceinline__ bool tiles_agree(const DocTile& q, const DocTile& k, int shared) {
-  return !q.mixed && !k.mixed && (q.low == k.low || k.low == shared);
+  return !q.padded && !k.padded && q.low == q.high && k.low == k.high && (q.low == k.low || k.low == shared);
 }
 
-// tanh, to about 2e-7 relative: an odd polynomial near zero (its Taylor series
-// to x^9, truncation below 1e-8 relative for |x| < 0.25), else by the exponential,
-// whose cancellation there would cost digits.
+// tanh, to about 2e-7 relative: near zero an odd polynomial (fitted to the
+// least relative error on |x| < 0.75: 3.3e-8), beyond it the exponential, whose
+// cancellation near zero would cost digits.
+constexpr float kTanhSmall = 0.75f;
+
 __device__ __forceinline__ float tanh_small(float x) {
   const float y = x * x;
-  float r = 0.021869488536155203f;  // 62 / 2835
-  r = fmaf(r, y, -0.053968253968253971f);  // -17 / 315
-  r = fmaf(r, y, 0.13333333333333333f);    // 2 / 15
-  r = fmaf(r, y, -0.33333333333333331f);   // -1 / 3
+  float r = -0.004769488703459501f;
+  r = fmaf(r, y, 0.019664911553263664f);
+  r = fmaf(r, y, -0.0533902570605278f);
+  r = fmaf(r, y, 0.13326521217823029f);
+  r = fmaf(r, y, -0.3333306908607483f);
   return fmaf(r * y, x, x);
 }
 
@@ -122,7 +124,7 @@ __device__ __forceinline__ float tanh_large(float x) {
   return copysignf(__fdividef(1.0f - e, 1.0f + e), x);
 }
 
-__device__ __forceinline__ float tanh_of(float x) { return fabsf(x) < 0.25f ? tanh_small(x) : tanh_large(x); }
+__device__ __forceinline__ float tanh_of(float x) { return fabsf(x) < kTanhSmall ? tanh_small(x) : tanh_large(x); }
 
 // v rounded to T, and what the rounding took.
 template <typename T>
@@ -163,6 +165,13 @@ cudaError_t attn_documents_launch(const AttnParams& p, DocTile* qtile, DocTile* 
 cudaError_t attn_simt_forward(const AttnParams& p, int dtype, cudaStream_t st);
 cudaError_t attn_simt_backward(const AttnParams& p, int dtype, cudaStream_t st);
 cudaError_t attn_token_forward(const AttnParams& p, int dtype, cudaStream_t st);
+// Tensor-core kernels: 16-bit types, D a multiple of 8 up to 128, rows that
+// start on 16 bytes at strides of whole 16 bytes. 0 or a cudaError_t; -1 where a
+// tensor map could not be made.
+int attn_tc_forward(const AttnParams& p, int dtype, cudaStream_t st);
+int attn_tc_backward(const AttnParams& p, int dtype, cudaStream_t st);
+// Waits of the tensor-core kernels that gave up so far (reads device memory).
+cudaError_t attn_tc_gave_up(int* count);
 cudaError_t attn_combine_launch(const AttnParams& p, int dtype, cudaStream_t st);
 
 }  // namespace msda

@@ -466,7 +466,7 @@ __global__ void __launch_bounds__(128) attn_documents_kernel(const AttnParams p,
   low = __reduce_min_sync(kFullMask, low), high = __reduce_max_sync(kFullMask, high);
   pad = __any_sync(kFullMask, pad), shared = __any_sync(kFullMask, shared);
   if (threadIdx.x % 32 == 0) {
-    DocTile out{low, high, pad || low != high, shared};
+    DocTile out{low, high, pad, shared};
     (keys ? ktile + (int64_t)b * nk : qtile + (int64_t)b * nq)[tile] = out;
   }
 }

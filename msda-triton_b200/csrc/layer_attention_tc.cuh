@@ -1,0 +1,935 @@
+// Masked attention on the tensor cores (tcgen05), fp16 and bf16.
+//
+// All tiles are 128 tokens in 128-byte swizzled shared-memory rows, brought by
+// TMA (channels past the head size and tokens past the end come as zeros). The
+// scores land in TMEM, one query (or key) a lane; a thread reads its row's 128
+// (or 64) scores into registers, and writes the probabilities back to TMEM in 16
+// bits over the scores that it has read, from where the second product takes
+// them as its left side: they never pass through shared memory.
+//
+// Roles: one warp loads, one issues the products (one elected lane), eight warps
+// do the softmax. Each wait is bounded (layer_tcgen05.cuh); a kernel whose wait
+// gave up leaves NaN in its outputs.
+#pragma once
+
+#include "layer_attention.cuh"
+#include "layer_tcgen05.cuh"
+
+namespace msda {
+namespace tc {
+
+constexpr int kSoftmaxThreads = 256;
+constexpr int kThreads = kSoftmaxThreads + 128;  // two warpgroups of softmax, one of the other roles
+constexpr int kLoadWarp = 8, kMmaWarp = 9;
+
+// The launch has 168 registers a thread; the softmax takes what the other
+// warpgroup leaves: 256 x 224 + 128 x 56 = 384 x 168.
+__device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 224;"); }
+__device__ __forceinline__ void leave_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 56;"); }
+
+template <typename T> struct IsBf16 { static constexpr bool value = false; };
+template <> struct IsBf16<__nv_bfloat16> { static constexpr bool value = true; };
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
+  uint32_t r;
+  if constexpr (IsBf16<T>::value) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// Scores of a thread's row to base 2 (all but a plain scale, which is folded
+// into the exponent): cap and distance bias. t2 (BWD): 1 - tanh^2.
+template <int N, bool BWD>
+__device__ __forceinline__ void shape_scores(const AttnParams& p, const ScoreForm& f, float (&s)[N], float (&t2)[BWD ? N : 1]) {
+  if (p.cap != 0.0f) {
+    float big = 0.0f;
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      s[c] *= f.inv_cap;
+      big = fmaxf(big, fabsf(s[c]));
+    }
+    // Scores well below the cap, the common case, need no exponential.
+    if (__all_sync(kFullMask, big < kTanhSmall)) {
+#pragma unroll
+      for (int c = 0; c < N; ++c) {
+        const float t = tanh_small(s[c]);
+        if constexpr (BWD) t2[c] = fmaf(-t, t, 1.0f);
+        s[c] = t * f.cap2;
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < N; ++c) {
+        const float t = tanh_of(s[c]);
+        if constexpr (BWD) t2[c] = fmaf(-t, t, 1.0f);
+        s[c] = t * f.cap2;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      if constexpr (BWD) t2[c] = 1.0f;
+      s[c] *= f.scale2;
+    }
+  }
+}
+
+struct TileState {
+  bool skip;    // no query of the rows sees a key of the tile by documents
+  bool agree;   // documents hide nothing
+  bool padded;  // some keys are padding: their values must be cleared
+};
+
+// rows: [i0, i0 + n * 128); keys: tile j.
+__device__ __forceinline__ TileState tile_state(const AttnParams& p, int b, int i0, int n, int j, int length) {
+  TileState s{false, true, (j + 1) * kTileTokens > length && length < p.Sk};
+  if (!p.kdoc) return s;
+  const int nq = (p.Sq + kDocTile - 1) / kDocTile, nk = (p.Sk + kDocTile - 1) / kDocTile;
+  const DocTile k = p.ktile[(int64_t)b * nk + j];
+  s.skip = true;
+  for (int t = 0; t < n && i0 / kDocTile + t < nq; ++t) {
+    const DocTile q = p.qtile[(int64_t)b * nq + i0 / kDocTile + t];
+    s.skip = s.skip && tiles_apart(q, k);
+    s.agree = s.agree && tiles_agree(q, k, p.shared);
+  }
+  s.padded = s.padded || k.padded;
+  return s;
+}
+
+// Clears the rows of a tile whose token is padding (a warp): 0 x NaN is NaN, and
+// a product over tokens would spread what padding holds.
+template <int DP>
+__device__ __forceinline__ void clear_rows(char* tile, const int* doc, int first, int count) {
+  for (int r = threadIdx.x % 32; r < kTileTokens; r += 32) {
+    const int at = first + r;
+    if (at < count && (!doc || __ldg(doc + at) >= 0)) continue;
+#pragma unroll
+    for (int c = 0; c < (DP + kChunk - 1) / kChunk; ++c)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        *reinterpret_cast<uint4*>(tile + c * kChunkBytes + r * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+  }
+  fence_async_smem();
+  __syncwarp();
+}
+
+// ---------------------------------------------------------------------------
+// Forward: 256 queries of a head a CTA, as two tiles that take turns: while one
+// tile's rows are exponentiated the tensor cores work on the other's products.
+// For 128 channels a key tile costs 2 x 1024 cycles of products and, on the
+// 16-a-cycle exponential units, 2 x 1024 cycles too.
+// ---------------------------------------------------------------------------
+template <int DP>
+struct FwdShape {
+  static constexpr int kTile = tile_bytes<DP>();
+  static constexpr int kStages = DP > 64 ? 4 : 6;
+  static constexpr int kSmem = 1024 + (2 + kStages) * kTile;
+};
+
+template <typename T, int DP, bool MODS>
+__global__ void __launch_bounds__(kThreads, 1)
+    attn_tc_fwd_kernel(const AttnParams p, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                       const __grid_constant__ CUtensorMap vmap) {
+  using Shape = FwdShape<DP>;
+  constexpr int NS = Shape::kStages;
+  extern __shared__ char raw[];
+  char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  char* sq = smem;
+  char* ring = smem + 2 * Shape::kTile;
+  __shared__ uint64_t q_full, kv_full[NS], kv_empty[NS], s_full[2], p_full[2], o_full;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+  volatile int* abort = &abort_flag;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int h = blockIdx.y, b = blockIdx.z, hk = h / (p.H / p.Hkv);
+  const int i0 = (gridDim.x - 1 - blockIdx.x) * 2 * kTileTokens;  // long causal rows first
+  const int length = attn_length(p, b);
+  const int limit = rows_limit(p, b, i0 + 2 * kTileTokens, length);
+  const int tiles = (limit + kTileTokens - 1) / kTileTokens;
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    bar_init(&q_full, 1);
+    bar_init(&o_full, 1);
+    for (int i = 0; i < NS; ++i) bar_init(&kv_full[i], 1), bar_init(&kv_empty[i], 1);
+    for (int i = 0; i < 2; ++i) bar_init(&s_full[i], 1), bar_init(&p_full[i], kSoftmaxThreads / 2);
+    fence_async_smem();
+  }
+  if (warp == kMmaWarp) tmem_alloc<512>(&tmem_slot);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = tmem_slot;
+
+  if (warp < kLoadWarp) {
+    take_registers();
+    const int t = warp / 4, i = i0 + threadIdx.x;  // tile and query of this thread
+    const uint32_t lanes = (uint32_t)(warp % 4) << 21;
+    const uint32_t s_at = tmem + lanes + t * 128, o_at = tmem + lanes + 256 + t * DP;
+    const RowView row = row_view(p, b, i, length);
+    const ScoreForm f = score_form(p, h);
+    const int* kdoc = p.kdoc ? p.kdoc + (int64_t)b * p.Sk : nullptr;
+    float m = -INFINITY, l = 0.0f;  // in base 2; m trails the maximum by at most kSlack
+    constexpr float kSlack = 8.0f;
+    bool ok = true;
+    int count = 0;
+    for (int j = 0; j < tiles && ok; ++j) {
+      const TileState st = tile_state(p, b, i0, 2, j, length);
+      if (st.skip) continue;
+      ok = warp_wait(&s_full[t], count & 1, abort);
+      if (!ok) break;
+      fence_after();
+      float s[128];
+#pragma unroll
+      for (int c = 0; c < 128; c += 32) tmem_load32(s_at + c, s + c);
+      tmem_wait_load();
+      const int j0 = j * kTileTokens;
+      float factor = f.scale2;
+      if constexpr (MODS) {
+        float none[1];
+        shape_scores<128, false>(p, f, s, none);
+        if (p.slopes) {
+          const float far = (float)(row.place - j0);
+#pragma unroll
+          for (int c = 0; c < 128; ++c) s[c] = fmaf(-f.slope2, fabsf(far - (float)c), s[c]);
+        }
+        factor = 1.0f;
+      }
+      const int seen = row.limit - j0;
+      if (!__all_sync(kFullMask, seen >= 128)) {
+#pragma unroll
+        for (int c = 0; c < 128; ++c) s[c] = c < seen ? s[c] : -INFINITY;
+      }
+      if (!st.agree) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int at = j0 + q * 32 + lane, mine = at < p.Sk ? __ldg(kdoc + at) : -1;
+#pragma unroll
+          for (int c = 0; c < 32; ++c)
+            if (!same_document(row.doc, __shfl_sync(kFullMask, mine, c), p.shared)) s[q * 32 + c] = -INFINITY;
+        }
+      }
+      float top0 = s[0], top1 = s[1];
+#pragma unroll
+      for (int c = 2; c < 128; c += 2) top0 = fmaxf(top0, s[c]), top1 = fmaxf(top1, s[c + 1]);
+      // The largest scaled score: for a negative scale the largest comes from the smallest.
+      float top = fmaxf(top0, top1) * factor;
+      if constexpr (!MODS) {
+        if (factor <= 0.0f) {
+          top = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < 128; ++c)
+            if (s[c] != -INFINITY) top = fmaxf(top, s[c] * factor);
+        }
+      }
+      // The reference maximum moves only when a row has grown by 2^8 past it, so
+      // that the sums in TMEM are seldom rescaled; 2^8 is far from overflow.
+      if (__any_sync(kFullMask, top > m + kSlack)) {
+        const float next = fmaxf(m, top);
+        const float old = next == -INFINITY ? 1.0f : ex2(m - next);
+        m = next;
+        l *= old;
+        if (count > 0) {
+#pragma unroll
+          for (int c = 0; c < DP; c += 32) {
+            float o[32];
+            tmem_load32(o_at + c, o);
+            tmem_wait_load();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] *= old;
+            tmem_store32(o_at + c, reinterpret_cast<uint32_t*>(o));
+          }
+        }
+      }
+      const float base = m == -INFINITY ? 0.0f : m;
+      float sum0 = 0.0f, sum1 = 0.0f;
+      const bool flip = !MODS && factor <= 0.0f;  // -inf marks must stay so
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t packed[32];
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          const float a = s[half * 64 + 2 * c], d = s[half * 64 + 2 * c + 1];
+          float e0 = ex2(fmaf(a, factor, -base)), e1 = ex2(fmaf(d, factor, -base));
+          if (flip) e0 = a == -INFINITY ? 0.0f : e0, e1 = d == -INFINITY ? 0.0f : e1;
+          sum0 += e0, sum1 += e1;
+          packed[c] = pack_pair<T>(e0, e1);
+        }
+        tmem_store32(s_at + half * 32, packed);
+      }
+      l += sum0 + sum1;
+      tmem_wait_store();
+      fence_before();
+      bar_arrive(&p_full[t]);
+      ++count;
+    }
+    if (ok && count > 0) ok = warp_wait(&o_full, 0, abort);
+    fence_after();
+    const float mul = !ok ? NAN : l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+    const int64_t at = (((int64_t)b * p.Sq + i) * p.H + h) * p.D;
+#pragma unroll
+    for (int c = 0; c < DP; c += 32) {
+      float o[32];
+      if (count > 0) {
+        tmem_load32(o_at + c, o);
+        tmem_wait_load();
+      }
+      if (i < p.Sq) {
+#pragma unroll
+        for (int e = 0; e < 32; e += 8) {
+          if (c + e >= p.D) continue;
+          uint4 high, low;
+          uint32_t* hi = reinterpret_cast<uint32_t*>(&high);
+          uint32_t* lo = reinterpret_cast<uint32_t*>(&low);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const float a = count > 0 ? o[e + 2 * x] * mul : mul, d = count > 0 ? o[e + 2 * x + 1] * mul : mul;
+            hi[x] = pack_pair<T>(a, d);
+            Pack<T, 2> u;
+            u.raw = hi[x];
+            lo[x] = pack_pair<T>(a - to_f32(u.e[0]), d - to_f32(u.e[1]));
+          }
+          *reinterpret_cast<uint4*>(static_cast<T*>(p.o) + at + c + e) = high;
+          if (p.residue) *reinterpret_cast<uint4*>(static_cast<T*>(p.residue) + at + c + e) = low;
+        }
+      }
+    }
+    if (i < p.Sq && p.lse)
+      p.lse[((int64_t)b * p.H + h) * p.Sq + i] = !ok ? NAN : l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+    fence_before();
+  } else {
+    leave_registers();
+    if (warp == kLoadWarp) {
+      int n = 0;  // ring slots filled
+      if (lane == 0 && tiles > 0) {
+        bar_expect(&q_full, 2 * Shape::kTile);
+        tma_tile<DP>(sq, &qmap, &q_full, h, i0, b);
+        tma_tile<DP>(sq + Shape::kTile, &qmap, &q_full, h, i0 + kTileTokens, b);
+        bool ok = true;
+        for (int j = 0; j < tiles && ok; ++j) {
+          if (tile_state(p, b, i0, 2, j, length).skip) continue;
+          for (int kv = 0; kv < 2 && ok; ++kv) {
+            const int slot = n % NS;
+            if (n >= NS) ok = bar_wait(&kv_empty[slot], (n / NS - 1) & 1, abort);
+            if (!ok) break;
+            bar_expect(&kv_full[slot], Shape::kTile);
+            tma_tile<DP>(ring + slot * Shape::kTile, kv ? &vmap : &kmap, &kv_full[slot], hk, j * kTileTokens, b);
+            ++n;
+          }
+        }
+        // Copies in flight end before the CTA does.
+        bar_wait(&q_full, 0, abort);
+        for (int i = max(0, n - NS); i < n; ++i) bar_wait(&kv_full[i % NS], (i / NS) & 1, abort);
+      }
+    } else if (warp == kMmaWarp) {
+      constexpr uint32_t ds = instr_desc<IsBf16<T>::value>(128, false), dv = instr_desc<IsBf16<T>::value>(DP, true);
+      const uint32_t q_addr = smem_u32(sq), ring_addr = smem_u32(ring);
+      bool ok = tiles == 0 || warp_wait(&q_full, 0, abort);
+      int n = 0, prev = -1, prev_slot = 0, count = 0;  // prev: the tile whose scores were issued last
+      bool prev_padded = false;
+      for (int j = 0; j <= tiles && ok; ++j) {
+        TileState st{};
+        if (j < tiles) {
+          st = tile_state(p, b, i0, 2, j, length);
+          if (st.skip) continue;
+        }
+        const int k_slot = n % NS, v_slot = (n + 1) % NS;
+        // Scores of tile j after the values' product of the tile before, for each
+        // tile of queries in turn.
+        if (j < tiles) ok = warp_wait(&kv_full[k_slot], (n / NS) & 1, abort);
+        if (prev >= 0 && ok) {
+          ok = warp_wait(&kv_full[prev_slot], ((n - 1) / NS) & 1, abort);
+          if (prev_padded) clear_rows<DP>(ring + prev_slot * Shape::kTile, p.kdoc ? p.kdoc + (int64_t)b * p.Sk : nullptr, prev * kTileTokens, length);
+        }
+        for (int t = 0; t < 2 && ok; ++t) {
+          if (prev >= 0) {
+            ok = warp_wait(&p_full[t], (count - 1) & 1, abort);
+            if (!ok) break;
+            fence_after();
+            if (lane == 0) product_tokens(tmem + 256 + t * DP, tmem + t * 128, 32, ring_addr + prev_slot * Shape::kTile, dv, count > 1);
+            __syncwarp();
+          }
+          if (lane == 0) {
+            if (j < tiles) product_channels<DP>(tmem + t * 128, q_addr + t * Shape::kTile, ring_addr + k_slot * Shape::kTile, ds);
+            if (j < tiles) commit(&s_full[t]);
+            else if (t == 1) commit(&o_full);
+          }
+          __syncwarp();
+        }
+        if (ok && lane == 0) {
+          if (prev >= 0) commit(&kv_empty[prev_slot]);
+          if (j < tiles) commit(&kv_empty[k_slot]);
+        }
+        __syncwarp();
+        prev = j, prev_slot = v_slot, prev_padded = st.padded;
+        n += 2;
+        ++count;
+      }
+      if (!ok) {
+        if (lane == 0) commit(&o_full);
+        __syncwarp();
+        warp_wait(&o_full, 0, abort);
+      }
+    }
+  }
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    fence_after();
+    tmem_free<512>(tmem);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Backward, in two kernels without atomics: dq by tiles of queries (which also
+// leaves delta_i = g_i . o_i), then dk and dv by tiles of keys. Scores are formed
+// in both: 7 products of a tile pair instead of 5, and a fixed order of sums.
+// Each half of the eight warps takes 64 of the 128 columns, so that a thread
+// holds 64 scores and 64 derivatives. The derivative goes to TMEM in 16 bits
+// without the scale, which its sums get at the end: in fp16 it would cost small
+// gradients digits.
+// ---------------------------------------------------------------------------
+template <int DP>
+struct BwdShape {
+  static constexpr int kTile = tile_bytes<DP>();
+  static constexpr int kSmem = 1024 + 6 * kTile;  // two tiles that stay, two stages of two
+};
+
+// A thread's 64 probabilities from its scores (in place), where row or column
+// masks leave them; `t2` the cap's derivative. seen(c): what the masks say.
+template <bool MODS, typename Seen, typename Far, typename Lse>
+__device__ __forceinline__ void probabilities(const AttnParams& p, const ScoreForm& f, float (&s)[64], float (&t2)[MODS ? 64 : 1],
+                                              bool all, Seen seen, Far far, Lse lse2) {
+  float factor = f.scale2;
+  if constexpr (MODS) {
+    shape_scores<64, true>(p, f, s, t2);
+    if (p.slopes) {
+#pragma unroll
+      for (int c = 0; c < 64; ++c) s[c] = fmaf(-f.slope2, fabsf(far(c)), s[c]);
+    }
+    factor = 1.0f;
+  }
+#pragma unroll
+  for (int c = 0; c < 64; ++c) s[c] = ex2(fmaf(s[c], factor, -lse2(c)));
+  if (!all) {
+#pragma unroll
+    for (int c = 0; c < 64; ++c) s[c] = seen(c) ? s[c] : 0.0f;
+  }
+}
+
+// 64 values of a thread's row to TMEM in 16 bits.
+template <typename T>
+__device__ __forceinline__ void store_row(uint32_t at, const float (&v)[64]) {
+  uint32_t packed[32];
+#pragma unroll
+  for (int c = 0; c < 32; ++c) packed[c] = pack_pair<T>(v[2 * c], v[2 * c + 1]);
+  tmem_store32(at, packed);
+}
+
+// COLS columns of a thread's row of a sum in TMEM, times mul, to global memory.
+template <typename T, int COLS>
+__device__ __forceinline__ void write_row(T* out, bool in, uint32_t at, int first, int D, float mul, bool any) {
+#pragma unroll
+  for (int c = 0; c < COLS; c += 32) {
+    float o[32];
+    if (any) {
+      tmem_load32(at + c, o);
+      tmem_wait_load();
+    }
+    if (!in) continue;
+#pragma unroll
+    for (int e = 0; e < 32; e += 8) {
+      if (first + c + e >= D) continue;
+      uint4 v;
+      uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        w[x] = any ? pack_pair<T>(o[e + 2 * x] * mul, o[e + 2 * x + 1] * mul) : pack_pair<T>(mul - mul, mul - mul);
+      *reinterpret_cast<uint4*>(out + c + e) = v;
+    }
+  }
+}
+
+// Columns of a sum that each half of the warps writes: half of them, or all by
+// the first half where half would be less than a load's 32.
+template <int DP>
+struct HalfColumns {
+  static constexpr int kCols = DP >= 64 ? DP / 2 : DP;
+};
+
+template <typename T, int DP, bool MODS>
+__global__ void __launch_bounds__(kThreads, 1)
+    attn_tc_dq_kernel(const AttnParams p, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                      const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap gmap) {
+  using Shape = BwdShape<DP>;
+  extern __shared__ char raw[];
+  char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  char *sq = smem, *sg = smem + Shape::kTile, *ring = smem + 2 * Shape::kTile;  // stage: key tile, value tile
+  __shared__ uint64_t q_full, kv_full[2], kv_empty[2], s_full[2], dp_full, dp_empty, ds_full, done;
+  __shared__ float delta_part[2][kTileTokens];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+  volatile int* abort = &abort_flag;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int h = blockIdx.y, b = blockIdx.z, hk = h / (p.H / p.Hkv);
+  const int i0 = (gridDim.x - 1 - blockIdx.x) * kTileTokens;
+  const int length = attn_length(p, b);
+  const int limit = rows_limit(p, b, i0 + kTileTokens, length);
+  const int tiles = (limit + kTileTokens - 1) / kTileTokens;
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    bar_init(&q_full, 1);
+    bar_init(&done, 1);
+    for (int i = 0; i < 2; ++i) bar_init(&kv_full[i], 1), bar_init(&kv_empty[i], 1), bar_init(&s_full[i], 1);
+    bar_init(&dp_full, 1);
+    bar_init(&dp_empty, kSoftmaxThreads), bar_init(&ds_full, kSoftmaxThreads);
+    fence_async_smem();
+  }
+  if (warp == kMmaWarp) tmem_alloc<512>(&tmem_slot);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = tmem_slot;  // scores 0..127 and 128..255, derivatives 256..383, dq 384...
+
+  if (warp < kLoadWarp) {
+    take_registers();
+    const int half = warp / 4, r = threadIdx.x % kTileTokens, i = i0 + r;
+    const uint32_t at = tmem + ((uint32_t)(warp % 4) << 21);
+    const RowView row = row_view(p, b, i, length);
+    const ScoreForm f = score_form(p, h);
+    const int* kdoc = p.kdoc ? p.kdoc + (int64_t)b * p.Sk : nullptr;
+    const bool in = i < p.Sq;
+    const int64_t stat = ((int64_t)b * p.H + h) * p.Sq + i;
+    // delta: each half of the warps sums every other 8 channels.
+    float delta = 0.0f;
+    if (in && row.limit > 0) {
+      const int64_t o_at = (((int64_t)b * p.Sq + i) * p.H + h) * p.D;
+      const T* o = static_cast<const T*>(p.o) + o_at;
+      const T* low = p.residue ? static_cast<const T*>(p.residue) + o_at : nullptr;
+      const T* g = static_cast<const T*>(p.go) + b * p.gs[0] + i * p.gs[1] + h * p.gs[2];
+#pragma unroll 4
+      for (int d = half * 8; d < p.D; d += 16) {
+        float x[8], y[8], z[8];
+        load_vec<T, 8>(o + d, x);
+        load_vec<T, 8>(g + d, y);
+        if (low) {
+          load_vec<T, 8>(low + d, z);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] += z[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) delta = fmaf(x[e], y[e], delta);
+      }
+    }
+    delta_part[half][r] = delta;
+    named_barrier(1, kSoftmaxThreads);
+    delta = delta_part[0][r] + delta_part[1][r];
+    if (in && half == 0) p.delta[stat] = delta;
+    const float lse2 = in && row.limit > 0 ? p.lse[stat] * kLog2e : 0.0f;
+    bool ok = true;
+    int n = 0;
+    for (int j = 0; j < tiles && ok; ++j) {
+      const TileState st = tile_state(p, b, i0, 1, j, length);
+      if (st.skip) continue;
+      const int c0 = j * kTileTokens + half * 64;  // the thread's first key
+      const uint32_t s_at = at + (n % 2) * 128 + half * 64;
+      ok = warp_wait(&s_full[n % 2], (n / 2) & 1, abort);
+      if (!ok) break;
+      fence_after();
+      float s[64], t2[MODS ? 64 : 1];
+      tmem_load32(s_at, s);
+      tmem_load32(s_at + 32, s + 32);
+      tmem_wait_load();
+      const int seen = row.limit - c0;
+      const float away = (float)(row.place - c0);
+      probabilities<MODS>(p, f, s, t2, __all_sync(kFullMask, seen >= 64), [&](int c) { return c < seen; },
+                          [&](int c) { return away - (float)c; }, [&](int) { return lse2; });
+      if (!st.agree) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const int k = c0 + q * 32 + lane, mine = k < p.Sk ? __ldg(kdoc + k) : -1;
+#pragma unroll
+          for (int c = 0; c < 32; ++c)
+            if (!same_document(row.doc, __shfl_sync(kFullMask, mine, c), p.shared)) s[q * 32 + c] = 0.0f;
+        }
+      }
+      ok = warp_wait(&dp_full, n & 1, abort);
+      if (!ok) break;
+      fence_after();
+      float dp[64];
+      tmem_load32(at + 256 + half * 64, dp);
+      tmem_load32(at + 256 + half * 64 + 32, dp + 32);
+      tmem_wait_load();
+      fence_before();
+      bar_arrive(&dp_empty);
+#pragma unroll
+      for (int c = 0; c < 64; ++c) {
+        float d = s[c] * (dp[c] - delta);
+        if constexpr (MODS) d *= t2[c];
+        dp[c] = s[c] == 0.0f ? 0.0f : d;  // also where what the masks hide is not finite
+      }
+      store_row<T>(s_at, dp);
+      tmem_wait_store();
+      fence_before();
+      bar_arrive(&ds_full);
+      ++n;
+    }
+    if (ok && n > 0) ok = warp_wait(&done, 0, abort);
+    fence_after();
+    constexpr int cols = HalfColumns<DP>::kCols;
+    if (half * cols < DP)
+      write_row<T, cols>(static_cast<T*>(p.dq) + (((int64_t)b * p.Sq + i) * p.H + h) * p.D + half * cols, in, at + 384 + half * cols,
+                         half * cols, p.D, ok ? p.scale : NAN, n > 0);
+    fence_before();
+  } else {
+    leave_registers();
+    if (warp == kLoadWarp) {
+      if (lane == 0 && tiles > 0) {
+        bar_expect(&q_full, 2 * Shape::kTile);
+        tma_tile<DP>(sq, &qmap, &q_full, h, i0, b);
+        tma_tile<DP>(sg, &gmap, &q_full, h, i0, b);
+        int n = 0;
+        bool ok = true;
+        for (int j = 0; j < tiles && ok; ++j) {
+          if (tile_state(p, b, i0, 1, j, length).skip) continue;
+          const int slot = n % 2;
+          if (n >= 2) ok = bar_wait(&kv_empty[slot], (n / 2 - 1) & 1, abort);
+          if (!ok) break;
+          bar_expect(&kv_full[slot], 2 * Shape::kTile);
+          tma_tile<DP>(ring + slot * 2 * Shape::kTile, &kmap, &kv_full[slot], hk, j * kTileTokens, b);
+          tma_tile<DP>(ring + slot * 2 * Shape::kTile + Shape::kTile, &vmap, &kv_full[slot], hk, j * kTileTokens, b);
+          ++n;
+        }
+        bar_wait(&q_full, 0, abort);
+        for (int i = max(0, n - 2); i < n; ++i) bar_wait(&kv_full[i % 2], (i / 2) & 1, abort);
+      }
+    } else if (warp == kMmaWarp) {
+      constexpr uint32_t ds = instr_desc<IsBf16<T>::value>(128, false), dd = instr_desc<IsBf16<T>::value>(DP, true);
+      const uint32_t q_addr = smem_u32(sq), g_addr = smem_u32(sg), ring_addr = smem_u32(ring);
+      bool ok = tiles == 0 || warp_wait(&q_full, 0, abort);
+      int n = 0;  // tiles begun; tile n - 1 is the one whose dq is due
+      bool prev_padded = false;
+      int prev_j = 0;
+      for (int j = 0; j <= tiles && ok; ++j) {
+        TileState st{};
+        if (j < tiles) {
+          st = tile_state(p, b, i0, 1, j, length);
+          if (st.skip) continue;
+          // Scores into the buffer that the tile before last has left, ahead of
+          // the softmax of the tile before.
+          const uint32_t slot = ring_addr + (n % 2) * 2 * Shape::kTile;
+          ok = warp_wait(&kv_full[n % 2], (n / 2) & 1, abort);
+          if (!ok) break;
+          fence_after();
+          if (lane == 0) {
+            product_channels<DP>(tmem + (n % 2) * 128, q_addr, slot, ds);
+            commit(&s_full[n % 2]);
+          }
+          __syncwarp();
+          if (n > 0) ok = warp_wait(&dp_empty, (n - 1) & 1, abort);
+          if (!ok) break;
+          fence_after();
+          if (lane == 0) {
+            product_channels<DP>(tmem + 256, g_addr, slot + Shape::kTile, ds);
+            commit(&dp_full);
+          }
+          __syncwarp();
+        }
+        if (n > 0) {
+          const int slot = (n - 1) % 2;
+          ok = warp_wait(&ds_full, (n - 1) & 1, abort);
+          if (!ok) break;
+          if (prev_padded)
+            clear_rows<DP>(ring + slot * 2 * Shape::kTile, p.kdoc ? p.kdoc + (int64_t)b * p.Sk : nullptr, prev_j * kTileTokens, length);
+          fence_after();
+          if (lane == 0) {
+            product_tokens(tmem + 384, tmem + slot * 128, 64, ring_addr + slot * 2 * Shape::kTile, dd, n > 1);
+            commit(&kv_empty[slot]);
+            if (j == tiles) commit(&done);
+          }
+          __syncwarp();
+        }
+        prev_padded = st.padded, prev_j = j;
+        ++n;
+      }
+      if (!ok) {
+        if (lane == 0) commit(&done);
+        __syncwarp();
+        warp_wait(&done, 0, abort);
+      }
+    }
+  }
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    fence_after();
+    tmem_free<512>(tmem);
+  }
+}
+
+// What a key-tile thread needs of each query of a tile.
+struct QueryStats {
+  float lse2[kTileTokens], delta[kTileTokens];
+  int limit[kTileTokens], place[kTileTokens], doc[kTileTokens];
+};
+
+template <typename T, int DP, bool MODS>
+__global__ void __launch_bounds__(kThreads, 1)
+    attn_tc_dkv_kernel(const AttnParams p, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                       const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap gmap) {
+  using Shape = BwdShape<DP>;
+  extern __shared__ char raw[];
+  char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  char *sk = smem, *sv = smem + Shape::kTile, *ring = smem + 2 * Shape::kTile;  // stage: query tile, gradient tile
+  __shared__ uint64_t k_full, q_full[2], q_empty[2], s_full, p_full, dp_full, ds_full, done;
+  __shared__ QueryStats stats[2];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+  volatile int* abort = &abort_flag;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int hk = blockIdx.y, b = blockIdx.z, group = p.H / p.Hkv;
+  const int kt = blockIdx.x, j0 = kt * kTileTokens;  // early keys are seen by the most causal queries
+  const int length = attn_length(p, b);
+  const int q_tiles = (p.Sq + kTileTokens - 1) / kTileTokens;
+  const int first = j0 < length ? first_query(p, b, j0, length) / kTileTokens : q_tiles;
+  // Steps: each head of the group, its tiles of queries from `first` on.
+  const int per_head = q_tiles - first, steps = group * per_head;
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    bar_init(&k_full, 1);
+    bar_init(&done, 1);
+    for (int i = 0; i < 2; ++i) bar_init(&q_full[i], 1), bar_init(&q_empty[i], 1);
+    bar_init(&s_full, 1), bar_init(&dp_full, 1);
+    bar_init(&p_full, kSoftmaxThreads), bar_init(&ds_full, kSoftmaxThreads);
+    fence_async_smem();
+  }
+  if (warp == kMmaWarp) tmem_alloc<512>(&tmem_slot);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = tmem_slot;  // scores 0..127, derivatives 128..255, dv 256..., dk 384...
+
+  if (warp < kLoadWarp) {
+    take_registers();
+    const int half = warp / 4, r = threadIdx.x % kTileTokens, j = j0 + r;  // key of this thread
+    const uint32_t at = tmem + ((uint32_t)(warp % 4) << 21) + half * 64;
+    const int kd = p.kdoc && j < length ? __ldg(p.kdoc + (int64_t)b * p.Sk + j) : 0;
+    const bool live = j < length;
+    bool ok = true;
+    int n = 0;
+    // A warp whose wait gave up still comes to the others' barriers.
+    for (int u = 0; u < steps; ++u) {
+      const int h = hk * group + u / per_head, i0 = (first + u % per_head) * kTileTokens;
+      const TileState st = tile_state(p, b, i0, 1, kt, length);
+      if (st.skip) continue;
+      QueryStats& q = stats[n % 2];
+      const ScoreForm f = score_form(p, h);
+      bool whole;  // every query of the tile sees every key of the tile
+      {
+        // Filled two steps ahead of their buffer's next use: every thread has
+        // passed the barrier of the step between.
+        const RowView row = row_view(p, b, i0 + r, length);
+        const int64_t stat = ((int64_t)b * p.H + h) * p.Sq + i0 + r;
+        if (half == 0) {
+          q.lse2[r] = row.limit > 0 ? p.lse[stat] * kLog2e : 0.0f;
+          q.delta[r] = row.limit > 0 ? p.delta[stat] : 0.0f;
+        } else {
+          q.limit[r] = row.limit, q.place[r] = row.place, q.doc[r] = row.doc;
+        }
+        int full;
+        asm volatile("{\n .reg .pred p, q;\n setp.ne.s32 p, %1, 0;\n barrier.cta.red.and.pred q, 1, %2, p;\n selp.s32 %0, 1, 0, q;\n}"
+                     : "=r"(full) : "r"((int)(row.limit >= j0 + kTileTokens)), "r"(kSoftmaxThreads) : "memory");
+        whole = full && st.agree;
+      }
+      ok = ok && warp_wait(&s_full, n & 1, abort);
+      if (!ok) continue;
+      fence_after();
+      float s[64], t2[MODS ? 64 : 1];
+      tmem_load32(at, s);
+      tmem_load32(at + 32, s + 32);
+      tmem_wait_load();
+      const int c0 = half * 64;
+      probabilities<MODS>(p, f, s, t2, whole,
+                          [&](int c) {
+                            return live && j < q.limit[c0 + c] && (!p.kdoc || same_document(q.doc[c0 + c], kd, p.shared));
+                          },
+                          [&](int c) { return (float)(q.place[c0 + c] - j); }, [&](int c) { return q.lse2[c0 + c]; });
+      store_row<T>(at, s);
+      tmem_wait_store();
+      fence_before();
+      bar_arrive(&p_full);
+      ok = warp_wait(&dp_full, n & 1, abort);
+      if (!ok) continue;
+      fence_after();
+      float dp[64];
+      tmem_load32(at + 128, dp);
+      tmem_load32(at + 160, dp + 32);
+      tmem_wait_load();
+#pragma unroll
+      for (int c = 0; c < 64; ++c) {
+        float d = s[c] * (dp[c] - q.delta[c0 + c]);
+        if constexpr (MODS) d *= t2[c];
+        dp[c] = s[c] == 0.0f ? 0.0f : d;
+      }
+      store_row<T>(at + 128, dp);
+      tmem_wait_store();
+      fence_before();
+      bar_arrive(&ds_full);
+      ++n;
+    }
+    if (ok && n > 0) ok = warp_wait(&done, 0, abort);
+    fence_after();
+    const bool in = j < p.Sk;
+    const int64_t out = (((int64_t)b * p.Sk + j) * p.Hkv + hk) * p.D;
+    const uint32_t lanes = tmem + ((uint32_t)(warp % 4) << 21);
+    // The first half of the warps writes dv, the second dk.
+    if (half == 0) write_row<T, DP>(static_cast<T*>(p.dv) + out, in, lanes + 256, 0, p.D, ok ? 1.0f : NAN, n > 0);
+    else write_row<T, DP>(static_cast<T*>(p.dk) + out, in, lanes + 384, 0, p.D, ok ? p.scale : NAN, n > 0);
+    fence_before();
+  } else {
+    leave_registers();
+    if (warp == kLoadWarp) {
+      if (lane == 0 && steps > 0) {
+        bar_expect(&k_full, 2 * Shape::kTile);
+        tma_tile<DP>(sk, &kmap, &k_full, hk, j0, b);
+        tma_tile<DP>(sv, &vmap, &k_full, hk, j0, b);
+        int n = 0;
+        bool ok = true;
+        for (int u = 0; u < steps && ok; ++u) {
+          const int h = hk * group + u / per_head, i0 = (first + u % per_head) * kTileTokens;
+          if (tile_state(p, b, i0, 1, kt, length).skip) continue;
+          const int slot = n % 2;
+          if (n >= 2) ok = bar_wait(&q_empty[slot], (n / 2 - 1) & 1, abort);
+          if (!ok) break;
+          bar_expect(&q_full[slot], 2 * Shape::kTile);
+          tma_tile<DP>(ring + slot * 2 * Shape::kTile, &qmap, &q_full[slot], h, i0, b);
+          tma_tile<DP>(ring + slot * 2 * Shape::kTile + Shape::kTile, &gmap, &q_full[slot], h, i0, b);
+          ++n;
+        }
+        bar_wait(&k_full, 0, abort);
+        for (int i = max(0, n - 2); i < n; ++i) bar_wait(&q_full[i % 2], (i / 2) & 1, abort);
+      }
+    } else if (warp == kMmaWarp) {
+      constexpr uint32_t ds = instr_desc<IsBf16<T>::value>(128, false), dd = instr_desc<IsBf16<T>::value>(DP, true);
+      const uint32_t k_addr = smem_u32(sk), v_addr = smem_u32(sv), ring_addr = smem_u32(ring);
+      bool ok = steps == 0 || warp_wait(&k_full, 0, abort);
+      int n = 0;
+      for (int u = 0; u <= steps && ok; ++u) {
+        const int i0 = u < steps ? (first + u % per_head) * kTileTokens : 0;
+        if (u < steps && tile_state(p, b, i0, 1, kt, length).skip) continue;
+        const uint32_t next = ring_addr + (n % 2) * 2 * Shape::kTile, prev = ring_addr + ((n - 1) & 1) * 2 * Shape::kTile;
+        // dv of the step before, then this step's scores over its probabilities;
+        // dk of the step before, then this step's derivatives: each product runs
+        // while the softmax works on the other half.
+        if (n > 0) {
+          ok = warp_wait(&p_full, (n - 1) & 1, abort);
+          if (!ok) break;
+          fence_after();
+          if (lane == 0) product_tokens(tmem + 256, tmem, 64, prev + Shape::kTile, dd, n > 1);
+          __syncwarp();
+        }
+        if (u < steps) {
+          ok = warp_wait(&q_full[n % 2], (n / 2) & 1, abort);
+          if (!ok) break;
+          fence_after();
+          if (p.qdoc) {
+            // Padded queries' rows and gradients, whatever they hold, count for nothing.
+            const int nq = (p.Sq + kDocTile - 1) / kDocTile;
+            if (p.qtile[(int64_t)b * nq + i0 / kDocTile].padded) {
+              char* stage = ring + (n % 2) * 2 * Shape::kTile;
+              clear_rows<DP>(stage, p.qdoc + (int64_t)b * p.Sq, i0, p.Sq);
+              clear_rows<DP>(stage + Shape::kTile, p.qdoc + (int64_t)b * p.Sq, i0, p.Sq);
+            }
+          }
+          if (lane == 0) {
+            product_channels<DP>(tmem, k_addr, next, ds);
+            commit(&s_full);
+          }
+          __syncwarp();
+        }
+        if (n > 0) {
+          ok = warp_wait(&ds_full, (n - 1) & 1, abort);
+          if (!ok) break;
+          fence_after();
+          if (lane == 0) {
+            product_tokens(tmem + 384, tmem + 128, 64, prev, dd, n > 1);
+            commit(&q_empty[(n - 1) & 1]);
+            if (u == steps) commit(&done);
+          }
+          __syncwarp();
+        }
+        if (u < steps) {
+          if (lane == 0) {
+            product_channels<DP>(tmem + 128, v_addr, next + Shape::kTile, ds);
+            commit(&dp_full);
+          }
+          __syncwarp();
+        }
+        ++n;
+      }
+      if (!ok) {
+        if (lane == 0) commit(&done);
+        __syncwarp();
+        warp_wait(&done, 0, abort);
+      }
+    }
+  }
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    fence_after();
+    tmem_free<512>(tmem);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Launches
+// ---------------------------------------------------------------------------
+bool make_map(CUtensorMap* map, const void* base, bool bf16, int64_t D, int64_t H, int64_t S, int64_t B, const int64_t (&strides)[3]);
+
+template <typename T, int DP, bool MODS>
+cudaError_t launch_fwd(const AttnParams& p, const CUtensorMap (&m)[4], cudaStream_t st) {
+  using Shape = FwdShape<DP>;
+  cudaError_t e = cudaFuncSetAttribute(attn_tc_fwd_kernel<T, DP, MODS>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem);
+  if (e != cudaSuccess) return e;
+  const dim3 grid((p.Sq + 2 * kTileTokens - 1) / (2 * kTileTokens), p.H, p.B);
+  attn_tc_fwd_kernel<T, DP, MODS><<<grid, kThreads, Shape::kSmem, st>>>(p, m[0], m[1], m[2]);
+  return cudaGetLastError();
+}
+
+template <typename T, int DP, bool MODS>
+cudaError_t launch_bwd(const AttnParams& p, const CUtensorMap (&m)[4], cudaStream_t st) {
+  using Shape = BwdShape<DP>;
+  cudaError_t e = cudaFuncSetAttribute(attn_tc_dq_kernel<T, DP, MODS>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(attn_tc_dkv_kernel<T, DP, MODS>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem);
+  if (e != cudaSuccess) return e;
+  attn_tc_dq_kernel<T, DP, MODS><<<dim3((p.Sq + kTileTokens - 1) / kTileTokens, p.H, p.B), kThreads, Shape::kSmem, st>>>(p, m[0], m[1], m[2], m[3]);
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  attn_tc_dkv_kernel<T, DP, MODS><<<dim3((p.Sk + kTileTokens - 1) / kTileTokens, p.Hkv, p.B), kThreads, Shape::kSmem, st>>>(p, m[0], m[1], m[2], m[3]);
+  return cudaGetLastError();
+}
+
+template <typename T, bool MODS>
+cudaError_t launch_by_size(const AttnParams& p, const CUtensorMap (&m)[4], bool backward, cudaStream_t st) {
+  if (p.D <= 32) return backward ? launch_bwd<T, 32, MODS>(p, m, st) : launch_fwd<T, 32, MODS>(p, m, st);
+  if (p.D <= 64) return backward ? launch_bwd<T, 64, MODS>(p, m, st) : launch_fwd<T, 64, MODS>(p, m, st);
+  return backward ? launch_bwd<T, 128, MODS>(p, m, st) : launch_fwd<T, 128, MODS>(p, m, st);
+}
+
+template <typename T>
+int run(const AttnParams& p, bool backward, cudaStream_t st) {
+  constexpr bool bf16 = IsBf16<T>::value;
+  CUtensorMap m[4];
+  if (!make_map(&m[0], p.q, bf16, p.D, p.H, p.Sq, p.B, p.qs) || !make_map(&m[1], p.k, bf16, p.D, p.Hkv, p.Sk, p.B, p.ks) ||
+      !make_map(&m[2], p.v, bf16, p.D, p.Hkv, p.Sk, p.B, p.vs) ||
+      (backward && !make_map(&m[3], p.go, bf16, p.D, p.H, p.Sq, p.B, p.gs)))
+    return -1;
+  const bool mods = p.cap != 0.0f || p.slopes;
+  return (int)(mods ? launch_by_size<T, true>(p, m, backward, st) : launch_by_size<T, false>(p, m, backward, st));
+}
+
+}  // namespace tc
+}  // namespace msda

@@ -116,6 +116,7 @@ SIGNATURES = {
     "msda_attention_workspace_size": (ctypes.c_size_t, [_VP, _I32]),
     "msda_attention_forward": (ctypes.c_int, [_VP, _VP]),
     "msda_attention_backward": (ctypes.c_int, [_VP, _VP]),
+    "msda_attention_gave_up": (ctypes.c_int, [ctypes.POINTER(_I32)]),
 }
 
 # Size of the static scratch behind msda_backward_noalloc

@@ -333,7 +333,7 @@ def _check(q, k, v, dtype, train=True, size=64, **how):
     out, got_lse = attention(q, k, v, return_lse=True, **how)
     tol = (3, 12) if dtype != torch.float32 else (size, 16 * size)
     close(out.detach(), want, dtype, *tol, floor=0.02, what="out")
-    assert torch.equal(out.detach() == 0, want == 0) or dtype == torch.float16
+    assert not out.detach()[want == 0].any()  # rows that see no key
     close(got_lse, lse, torch.float32, size, 16 * size, floor=1.0, what="lse")
     if train:
         got = torch.autograd.grad(out, (q, k, v), g)
