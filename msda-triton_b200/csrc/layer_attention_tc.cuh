@@ -351,17 +351,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             ok = warp_wait(&p_full[t], (count - 1) & 1, abort);
             if (!ok) break;
             fence_after();
-            if (lane == 0) product_tokens(tmem + 256 + t * DP, tmem + t * 128, 32, ring_addr + prev_slot * Shape::kTile, dv, count > 1);
+            if (elect_one()) product_tokens(tmem + 256 + t * DP, tmem + t * 128, 32, ring_addr + prev_slot * Shape::kTile, dv, count > 1);
             __syncwarp();
           }
-          if (lane == 0) {
+          if (elect_one()) {
             if (j < tiles) product_channels<DP>(tmem + t * 128, q_addr + t * Shape::kTile, ring_addr + k_slot * Shape::kTile, ds);
             if (j < tiles) commit(&s_full[t]);
             else if (t == 1) commit(&o_full);
           }
           __syncwarp();
         }
-        if (ok && lane == 0) {
+        if (ok && elect_one()) {
           if (prev >= 0) commit(&kv_empty[prev_slot]);
           if (j < tiles) commit(&kv_empty[k_slot]);
         }
@@ -371,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++count;
       }
       if (!ok) {
-        if (lane == 0) commit(&o_full);
+        if (elect_one()) commit(&o_full);
         __syncwarp();
         warp_wait(&o_full, 0, abort);
       }
@@ -625,7 +625,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = warp_wait(&kv_full[n % 2], (n / 2) & 1, abort);
           if (!ok) break;
           fence_after();
-          if (lane == 0) {
+          if (elect_one()) {
             product_channels<DP>(tmem + (n % 2) * 128, q_addr, slot, ds);
             commit(&s_full[n % 2]);
           }
@@ -633,7 +633,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (n > 0) ok = warp_wait(&dp_empty, (n - 1) & 1, abort);
           if (!ok) break;
           fence_after();
-          if (lane == 0) {
+          if (elect_one()) {
             product_channels<DP>(tmem + 256, g_addr, slot + Shape::kTile, ds);
             commit(&dp_full);
           }
@@ -646,7 +646,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (prev_padded)
             clear_rows<DP>(ring + slot * 2 * Shape::kTile, p.kdoc ? p.kdoc + (int64_t)b * p.Sk : nullptr, prev_j * kTileTokens, length);
           fence_after();
-          if (lane == 0) {
+          if (elect_one()) {
             product_tokens(tmem + 384, tmem + slot * 128, 64, ring_addr + slot * 2 * Shape::kTile, dd, n > 1);
             commit(&kv_empty[slot]);
             if (j == tiles) commit(&done);
@@ -657,7 +657,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++n;
       }
       if (!ok) {
-        if (lane == 0) commit(&done);
+        if (elect_one()) commit(&done);
         __syncwarp();
         warp_wait(&done, 0, abort);
       }
@@ -828,7 +828,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = warp_wait(&p_full, (n - 1) & 1, abort);
           if (!ok) break;
           fence_after();
-          if (lane == 0) product_tokens(tmem + 256, tmem, 64, prev + Shape::kTile, dd, n > 1);
+          if (elect_one()) product_tokens(tmem + 256, tmem, 64, prev + Shape::kTile, dd, n > 1);
           __syncwarp();
         }
         if (u < steps) {
@@ -844,7 +844,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               clear_rows<DP>(stage + Shape::kTile, p.qdoc + (int64_t)b * p.Sq, i0, p.Sq);
             }
           }
-          if (lane == 0) {
+          if (elect_one()) {
             product_channels<DP>(tmem, k_addr, next, ds);
             commit(&s_full);
           }
@@ -854,7 +854,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = warp_wait(&ds_full, (n - 1) & 1, abort);
           if (!ok) break;
           fence_after();
-          if (lane == 0) {
+          if (elect_one()) {
             product_tokens(tmem + 384, tmem + 128, 64, prev, dd, n > 1);
             commit(&q_empty[(n - 1) & 1]);
             if (u == steps) commit(&done);
@@ -862,7 +862,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
         }
         if (u < steps) {
-          if (lane == 0) {
+          if (elect_one()) {
             product_channels<DP>(tmem + 128, v_addr, next + Shape::kTile, ds);
             commit(&dp_full);
           }
@@ -871,7 +871,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++n;
       }
       if (!ok) {
-        if (lane == 0) commit(&done);
+        if (elect_one()) commit(&done);
         __syncwarp();
         warp_wait(&done, 0, abort);
       }

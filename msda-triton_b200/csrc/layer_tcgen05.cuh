@@ -15,6 +15,15 @@ constexpr int kChunkBytes = kTileTokens * 128;  // one chunk of a tile
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
+// One lane of a whole warp, always the same: it issues the products and their
+// commits. (With a test of the lane number instead, the compiler does not know
+// that a single thread runs, and a product cost about 100 cycles to issue.)
+__device__ __forceinline__ bool elect_one() {
+  uint32_t pred;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.b32 %0, 1, 0, p;\n}" : "=r"(pred));
+  return pred != 0;
+}
+
 // --- mbarriers -------------------------------------------------------------
 __device__ __forceinline__ void bar_init(uint64_t* bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
