@@ -475,7 +475,8 @@ template <typename T, int DP, int RM, bool PACK>
 cudaError_t fwd(const AttnParams& p, cudaStream_t st) {
   using G = Tile<DP, RM>;
   constexpr int smem = (G::kRowFloats + 2 * G::kColFloats + G::kProbFloats) * 4;
-  cudaError_t e = cudaFuncSetAttribute(attn_simt_fwd_kernel<T, DP, RM, PACK>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<uint64_t> set{0};
+  cudaError_t e = abi::allow_smem(attn_simt_fwd_kernel<T, DP, RM, PACK>, smem, set);
   if (e != cudaSuccess) return e;
   const int rows = PACK ? p.Sq * (p.H / p.Hkv) : p.Sq;
   const dim3 grid((rows + G::kRows - 1) / G::kRows * p.splits, PACK ? p.Hkv : p.H, p.B);
@@ -489,9 +490,9 @@ cudaError_t bwd(const AttnParams& p, cudaStream_t st) {
   using K = Tile<DP, RMK>;
   constexpr int smem_q = (2 * Q::kRowFloats + 2 * Q::kColFloats + Q::kProbFloats) * 4;
   constexpr int smem_k = (2 * K::kRowFloats + 2 * K::kColFloats + K::kProbFloats) * 4;
-  cudaError_t e = cudaFuncSetAttribute(attn_simt_dq_kernel<T, DP, RMQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_q);
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(attn_simt_dkv_kernel<T, DP, RMK>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_k);
+  static std::atomic<uint64_t> set_q{0}, set_k{0};
+  cudaError_t e = abi::allow_smem(attn_simt_dq_kernel<T, DP, RMQ>, smem_q, set_q);
+  if (e == cudaSuccess) e = abi::allow_smem(attn_simt_dkv_kernel<T, DP, RMK>, smem_k, set_k);
   if (e != cudaSuccess) return e;
   attn_simt_dq_kernel<T, DP, RMQ><<<dim3((p.Sq + Q::kRows - 1) / Q::kRows, p.H, p.B), kThreads, smem_q, st>>>(p);
   attn_simt_dkv_kernel<T, DP, RMK><<<dim3((p.Sk + K::kRows - 1) / K::kRows, p.Hkv, p.B), kThreads, smem_k, st>>>(p);

@@ -892,7 +892,8 @@ bool make_map(CUtensorMap* map, const void* base, bool bf16, int64_t D, int64_t 
 template <typename T, int DP, bool MODS>
 cudaError_t launch_fwd(const AttnParams& p, const CUtensorMap (&m)[4], cudaStream_t st) {
   using Shape = FwdShape<DP>;
-  cudaError_t e = cudaFuncSetAttribute(attn_tc_fwd_kernel<T, DP, MODS>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem);
+  static std::atomic<uint64_t> set{0};
+  cudaError_t e = abi::allow_smem(attn_tc_fwd_kernel<T, DP, MODS>, Shape::kSmem, set);
   if (e != cudaSuccess) return e;
   const dim3 grid((p.Sq + 2 * kTileTokens - 1) / (2 * kTileTokens), p.H, p.B);
   attn_tc_fwd_kernel<T, DP, MODS><<<grid, kThreads, Shape::kSmem, st>>>(p, m[0], m[1], m[2]);
@@ -902,9 +903,9 @@ cudaError_t launch_fwd(const AttnParams& p, const CUtensorMap (&m)[4], cudaStrea
 template <typename T, int DP, bool MODS>
 cudaError_t launch_bwd(const AttnParams& p, const CUtensorMap (&m)[4], cudaStream_t st) {
   using Shape = BwdShape<DP>;
-  cudaError_t e = cudaFuncSetAttribute(attn_tc_dq_kernel<T, DP, MODS>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem);
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(attn_tc_dkv_kernel<T, DP, MODS>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem);
+  static std::atomic<uint64_t> set_q{0}, set_k{0};
+  cudaError_t e = abi::allow_smem(attn_tc_dq_kernel<T, DP, MODS>, Shape::kSmem, set_q);
+  if (e == cudaSuccess) e = abi::allow_smem(attn_tc_dkv_kernel<T, DP, MODS>, Shape::kSmem, set_k);
   if (e != cudaSuccess) return e;
   attn_tc_dq_kernel<T, DP, MODS><<<dim3((p.Sq + kTileTokens - 1) / kTileTokens, p.H, p.B), kThreads, Shape::kSmem, st>>>(p, m[0], m[1], m[2], m[3]);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;

@@ -3,6 +3,7 @@
 // choice of the channel-vector kernels.
 #pragma once
 
+#include <atomic>
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
@@ -66,6 +67,20 @@ inline int sm_count() {
   int dev = 0, n = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
   return n;
+}
+
+// Lets `kernel` take `bytes` of dynamic shared memory, once for each device.
+// `set`: the kernel's own record, a bit a device.
+template <typename K>
+cudaError_t allow_smem(K kernel, int bytes, std::atomic<uint64_t>& set) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = uint64_t(1) << (dev & 63);
+  if (dev < 64 && (set.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) set.fetch_or(bit, std::memory_order_relaxed);
+  return e;
 }
 
 // Picks the lane layout for a channel count D (a head dim, or the channels

@@ -10,14 +10,17 @@ reproducible. There is no CPU path.
 
 from __future__ import annotations
 
-import ctypes
 import math
+import struct
 
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import _DTYPE_CODE, _FLOAT_DTYPES, _device_guard, _stream
+from .ops import _DTYPE_CODE, _FLOAT_DTYPES, _device_guard, _raw_stream
+
+# msda_attention_args of include/msda_layer_b200.h, packed in one call.
+_ARGS = struct.Struct("@10P3q4i12q2f5P2iPN")
 
 
 def _laid_out(x: torch.Tensor) -> torch.Tensor:
@@ -33,49 +36,54 @@ def _laid_out(x: torch.Tensor) -> torch.Tensor:
     return x
 
 
-def _args(query, key, value, out, residue, lse, options) -> _lib.AttentionArgs:
-    a = _lib.AttentionArgs()
-    a.query, a.key, a.value, a.out = query.data_ptr(), key.data_ptr(), value.data_ptr(), out.data_ptr()
-    a.out_residue = residue.data_ptr() if residue is not None else None
-    a.lse = lse.data_ptr() if lse is not None else None
-    a.batch, a.num_queries, a.num_heads, a.head_dim = query.shape
-    a.num_keys, a.num_key_heads = key.shape[1], key.shape[2]
-    a.dtype = _DTYPE_CODE[query.dtype]
-    a.query_strides[:], a.key_strides[:], a.value_strides[:] = query.stride()[:3], key.stride()[:3], value.stride()[:3]
-    a.scale, a.softcap, a.causal, shared, tensors = options
-    a.shared_document = shared
-    (a.distance_slopes, a.query_documents, a.key_documents, a.prefix_lengths,
-     a.key_lengths) = (t.data_ptr() if t is not None else None for t in tensors)
-    return a
+def _pack(query, key, value, out, residue, lse, grads, options, tensors, ws=0, nbytes=0) -> bytes:
+    """`grads`: (grad_out, and the three gradients' buffers), or None."""
+    B, Sq, H, D = query.shape
+    scale, softcap, causal, shared = options
+    go, dq, dk, dv = (0, 0, 0, 0) if grads is None else [t.data_ptr() for t in grads]
+    gs = (0, 0, 0) if grads is None else grads[0].stride()[:3]
+    return _ARGS.pack(
+        query.data_ptr(), key.data_ptr(), value.data_ptr(), out.data_ptr(),
+        0 if residue is None else residue.data_ptr(), 0 if lse is None else lse.data_ptr(), go, dq, dk, dv,
+        B, Sq, key.shape[1], H, key.shape[2], D, _DTYPE_CODE[query.dtype],
+        *query.stride()[:3], *key.stride()[:3], *value.stride()[:3], *gs, scale, softcap,
+        *[0 if t is None else t.data_ptr() for t in tensors], shared, causal, ws, nbytes)
 
 
-def _call(fn: str, a: _lib.AttentionArgs, backward: int, device: torch.device) -> None:
+def _call(fn, name: str, args, backward: int) -> None:
     lib = _lib.load()
-    nbytes = lib.msda_attention_workspace_size(ctypes.byref(a), backward)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-    if ws is not None:
-        a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
+    packed = _pack(*args)
+    device = args[0].device
     with _device_guard(device):
-        rc = getattr(lib, fn)(ctypes.byref(a), _stream(device))
-    _lib.check(fn, rc)
+        nbytes = lib.msda_attention_workspace_size(packed, backward)
+        if nbytes:
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            packed = packed[:-16] + struct.pack("@PN", ws.data_ptr(), nbytes)
+        rc = fn(packed, _raw_stream(device))
+    if rc:
+        _lib.check(name, rc)
+
+
+def _forward(query, key, value, options, tensors, want_lse, grad):
+    """(out, lse or None, query, key, value as they were read, residue or None)."""
+    query, key, value = _laid_out(query), _laid_out(key), _laid_out(value)
+    B, Sq, H, _ = query.shape
+    out = query.new_empty(query.shape)
+    lse = torch.empty(B, H, Sq, dtype=torch.float32, device=query.device) if grad or want_lse else None
+    residue = torch.empty_like(out) if grad and query.element_size() == 2 else None
+    if out.numel():
+        _call(_lib.load().msda_attention_forward, "msda_attention_forward",
+              (query, key, value, out, residue, lse, None, options, tensors), 0)
+    return out, lse, query, key, value, residue
 
 
 class _AttentionFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, query, key, value, options, want_lse):
-        B, Sq, H, D = query.shape
-        query, key, value = _laid_out(query), _laid_out(key), _laid_out(value)
-        out = query.new_empty(B, Sq, H, D)
-        grad = any(ctx.needs_input_grad)
-        lse = torch.empty(B, H, Sq, dtype=torch.float32, device=query.device) if grad or want_lse else None
-        residue = torch.empty_like(out) if grad and out.element_size() == 2 else None
-        if out.numel():
-            _call("msda_attention_forward", _args(query, key, value, out, residue, lse, options), 0, query.device)
-        if grad:
-            ctx.save_for_backward(query, key, value, out, residue, lse, *options[4])
-        ctx.options = options[:4]
-        if lse is not None:
-            ctx.mark_non_differentiable(lse)
+    def forward(ctx, query, key, value, options, tensors):
+        out, lse, *saved = _forward(query, key, value, options, tensors, True, True)
+        ctx.save_for_backward(out, lse, *saved, *tensors)
+        ctx.options = options
+        ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
         return out, lse
 
@@ -84,14 +92,11 @@ class _AttentionFunction(torch.autograd.Function):
     def backward(ctx, grad_out, _):
         if grad_out is None:
             return (None,) * 5
-        query, key, value, out, residue, lse, *tensors = ctx.saved_tensors
-        grad_out = _laid_out(grad_out.to(query.dtype))
-        dq = query.new_empty(query.shape)
-        dk, dv = key.new_empty(key.shape), value.new_empty(value.shape)
-        a = _args(query, key, value, out, residue, lse, (*ctx.options, tensors))
-        a.grad_out, a.grad_query, a.grad_key, a.grad_value = (t.data_ptr() for t in (grad_out, dq, dk, dv))
-        a.grad_out_strides[:] = grad_out.stride()[:3]
-        _call("msda_attention_backward", a, 1, query.device)
+        out, lse, query, key, value, residue, *tensors = ctx.saved_tensors
+        grad_out = _laid_out(grad_out if grad_out.dtype == query.dtype else grad_out.to(query.dtype))
+        dq, dk, dv = query.new_empty(query.shape), key.new_empty(key.shape), key.new_empty(key.shape)
+        _call(_lib.load().msda_attention_backward, "msda_attention_backward",
+              (query, key, value, out, residue, lse, (grad_out, dq, dk, dv), ctx.options, tensors), 1)
         return dq, dk, dv, None, None
 
 
@@ -169,22 +174,29 @@ def attention(
         raise ValueError("attention: shared_document is an id >= 0 and needs documents")
     if prefix_lengths is not None and not causal:
         raise ValueError("attention: prefix_lengths needs causal=True")
-    masks = (("distance_slopes", distance_slopes, (H,), torch.float32),
-             ("query_documents", query_documents, (B, Sq), torch.int32),
-             ("key_documents", key_documents, (B, Sk), torch.int32),
-             ("prefix_lengths", prefix_lengths, (B,), torch.int32),
-             ("key_lengths", key_lengths, (B,), torch.int32))
-    for name, t, shape, dtype in masks:
-        if t is not None and (tuple(t.shape) != shape or t.dtype != dtype):
-            raise ValueError(f"attention: {name} must be {shape} {dtype}, got {tuple(t.shape)} {t.dtype}")
-    if distance_slopes is not None and distance_slopes.requires_grad:
-        raise ValueError("attention: distance_slopes are constants and may not require a gradient; detach() them")
-    if query.device.type != "cuda":
+    device = query.device
+    tensors = (distance_slopes, query_documents, key_documents, prefix_lengths, key_lengths)
+    if any(t is not None for t in tensors):
+        shapes = ((H,), (B, Sq), (B, Sk), (B,), (B,))
+        for name, t, shape in zip(("distance_slopes", "query_documents", "key_documents", "prefix_lengths",
+                                   "key_lengths"), tensors, shapes):
+            if t is None:
+                continue
+            dtype = torch.float32 if t is distance_slopes else torch.int32
+            if t.shape != shape or t.dtype != dtype:
+                raise ValueError(f"attention: {name} must be {shape} {dtype}, got {tuple(t.shape)} {t.dtype}")
+            if t.device != device:
+                raise ValueError("attention: all tensors must be on the same CUDA device")
+        if distance_slopes is not None and distance_slopes.requires_grad:
+            raise ValueError("attention: distance_slopes are constants and may not require a gradient; detach() them")
+        tensors = tuple(None if t is None else t.contiguous() for t in tensors)
+    if device.type != "cuda":
         raise ValueError("attention requires CUDA tensors on a B200 (sm_100a) GPU")
-    if any(t.device != query.device for t in (key, value, *(m[1] for m in masks)) if t is not None):
+    if key.device != device or value.device != device:
         raise ValueError("attention: all tensors must be on the same CUDA device")
-    _lib.load()
-    options = (scale, softcap, int(bool(causal)), -1 if shared_document is None else int(shared_document),
-               tuple(m[1].contiguous() if m[1] is not None else None for m in masks))
-    out, lse = _AttentionFunction.apply(query, key, value, options, bool(return_lse))
+    options = (scale, softcap, 1 if causal else 0, -1 if shared_document is None else int(shared_document))
+    if (query.requires_grad or key.requires_grad or value.requires_grad) and torch.is_grad_enabled():
+        out, lse = _AttentionFunction.apply(query, key, value, options, tensors)
+    else:
+        out, lse, *_ = _forward(query, key, value, options, tensors, return_lse, False)
     return (out, lse) if return_lse else out

@@ -13,67 +13,88 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import _DTYPE_CODE, _FLOAT_DTYPES, _device_guard, _ptr, _stream
+from .ops import _DTYPE_CODE, _FLOAT_DTYPES, _device_guard, _raw_stream
 
 
 def _as_rows(x: torch.Tensor) -> torch.Tensor:
     """x (..., C) as (N, C) rows of contiguous channels: a view where the
     strides allow one, else a copy."""
-    x = x.reshape(-1, x.shape[-1])
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1])
     return x if x.shape[1] == 1 or x.stride(1) == 1 else x.contiguous()
+
+
+def _address(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
+def _param_code(code: int, weight, bias) -> int:
+    param = weight if weight is not None else bias
+    return code if param is None else _DTYPE_CODE[param.dtype]
+
+
+def _forward(x, residual, weight, bias, eps, want_sum, grad):
+    """(y, sum or None, rows, residual rows, statistics or None)."""
+    rows = _as_rows(x)
+    res = None if residual is None else _as_rows(residual)
+    N, C = rows.shape
+    y = x.new_empty(x.shape)
+    total = x.new_empty(x.shape) if want_sum else None
+    stats = mean = rstd = None
+    if grad:  # means, then reciprocal deviations
+        stats = torch.empty(2 * N, dtype=torch.float32, device=x.device)
+        mean = stats.data_ptr()
+        rstd = mean + 4 * N
+    code = _DTYPE_CODE[x.dtype]
+    device = x.device
+    with _device_guard(device):
+        rc = _lib.load().msda_layer_norm_forward(
+            rows.data_ptr(), _address(res), _address(weight), _address(bias), y.data_ptr(), _address(total),
+            mean, rstd, N, C, rows.stride(0), 0 if res is None else res.stride(0), eps, code,
+            _param_code(code, weight, bias), _raw_stream(device))
+    if rc:
+        _lib.check("msda_layer_norm_forward", rc)
+    return y, total, rows, res, stats
 
 
 class _LayerNormFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, bias, eps, want_sum):
-        rows = _as_rows(x)
-        res = _as_rows(residual) if residual is not None else None
-        N, C = rows.shape
-        y = rows.new_empty(x.shape)
-        total = rows.new_empty(x.shape) if want_sum else None
-        grad = any(ctx.needs_input_grad)
-        stats = torch.empty(2, N, dtype=torch.float32, device=x.device) if grad else None
-        param = weight if weight is not None else bias
-        code = _DTYPE_CODE[x.dtype]
-        lib = _lib.load()
-        with _device_guard(x.device):
-            rc = lib.msda_layer_norm_forward(
-                _ptr(rows), _ptr(res), _ptr(weight), _ptr(bias), _ptr(y), _ptr(total),
-                _ptr(stats[0] if grad else None), _ptr(stats[1] if grad else None), N, C, rows.stride(0),
-                res.stride(0) if res is not None else 0, eps, code,
-                _DTYPE_CODE[param.dtype] if param is not None else code, _stream(x.device))
-        _lib.check("msda_layer_norm_forward", rc)
-        if grad:
-            ctx.save_for_backward(rows, res, weight, bias, stats)
+        y, total, *saved = _forward(x, residual, weight, bias, eps, want_sum, True)
+        ctx.save_for_backward(weight, bias, *saved)
         ctx.shape = x.shape
         ctx.set_materialize_grads(False)
-        return y, total
+        return (y, total) if want_sum else y
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, grad_y, grad_sum):
-        rows, res, weight, bias, stats = ctx.saved_tensors
+    def backward(ctx, grad_y, grad_sum=None):
+        weight, bias, rows, res, stats = ctx.saved_tensors
         N, C = rows.shape
         if grad_y is None:
             grad_y = rows.new_zeros(N, C)
-        g = _as_rows(grad_y.to(rows.dtype))
-        gs = _as_rows(grad_sum.to(rows.dtype)).contiguous() if grad_sum is not None else None
+        g = _as_rows(grad_y if grad_y.dtype == rows.dtype else grad_y.to(rows.dtype))
+        gs = None if grad_sum is None else _as_rows(grad_sum.to(rows.dtype)).contiguous()
         dx = rows.new_empty(ctx.shape)
         dw = torch.empty_like(weight) if weight is not None and ctx.needs_input_grad[2] else None
         db = torch.empty_like(bias) if bias is not None and ctx.needs_input_grad[3] else None
         lib = _lib.load()
-        columns = dw is not None or db is not None
-        nbytes = lib.msda_layer_norm_backward_workspace_size(N, C) if columns else 0
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=rows.device) if nbytes else None
+        nbytes, ws = 0, None
+        if dw is not None or db is not None:
+            nbytes = lib.msda_layer_norm_backward_workspace_size(N, C)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=rows.device)
         code = _DTYPE_CODE[rows.dtype]
-        param = weight if weight is not None else bias
-        with _device_guard(rows.device):
+        device = rows.device
+        mean = stats.data_ptr()
+        with _device_guard(device):
             rc = lib.msda_layer_norm_backward(
-                _ptr(rows), _ptr(res), _ptr(weight), _ptr(stats[0]), _ptr(stats[1]), _ptr(g), _ptr(gs), _ptr(dx),
-                _ptr(dw), _ptr(db), _ptr(ws), nbytes, N, C, rows.stride(0), res.stride(0) if res is not None else 0,
-                g.stride(0), code, _DTYPE_CODE[param.dtype] if param is not None else code, _stream(rows.device))
-        _lib.check("msda_layer_norm_backward", rc)
-        return dx, dx if res is not None else None, dw, db, None, None
+                rows.data_ptr(), _address(res), _address(weight), mean, mean + 4 * N, g.data_ptr(), _address(gs),
+                dx.data_ptr(), _address(dw), _address(db), _address(ws), nbytes, N, C, rows.stride(0),
+                0 if res is None else res.stride(0), g.stride(0), code, _param_code(code, weight, bias),
+                _raw_stream(device))
+        if rc:
+            _lib.check("msda_layer_norm_backward", rc)
+        return dx, None if res is None else dx, dw, db, None, None
 
 
 def layer_norm(
@@ -105,26 +126,34 @@ def layer_norm(
     C = x.shape[-1]
     if C > _lib.MSDA_LAYER_NORM_MAX_WIDTH:
         raise ValueError(f"layer_norm: C={C} exceeds {_lib.MSDA_LAYER_NORM_MAX_WIDTH}")
-    if x.dtype not in _FLOAT_DTYPES:
-        raise ValueError(f"layer_norm: unsupported dtype {x.dtype}; use fp32, fp16 or bf16")
-    params = [p for p in (weight, bias) if p is not None]
-    for p in params:
-        if p.shape != (C,):
+    dtype, device = x.dtype, x.device
+    if dtype not in _FLOAT_DTYPES:
+        raise ValueError(f"layer_norm: unsupported dtype {dtype}; use fp32, fp16 or bf16")
+    for p in (weight, bias):
+        if p is not None and p.shape != (C,):
             raise ValueError(f"layer_norm: weight and bias must be ({C},), got {tuple(p.shape)}")
-        if p.dtype != params[0].dtype or p.dtype not in (x.dtype, torch.float32):
-            raise ValueError(f"layer_norm: weight and bias must both be {x.dtype} or fp32, got "
-                             f"{'/'.join(str(q.dtype) for q in params)}")
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
-        raise ValueError(f"layer_norm: residual must be {tuple(x.shape)} {x.dtype}, got "
+        if p is not None and (p.dtype not in (dtype, torch.float32) or
+                              (weight is not None and p.dtype != weight.dtype)):
+            raise ValueError(f"layer_norm: weight and bias must both be {dtype} or fp32, got "
+                             f"{'/'.join(str(q.dtype) for q in (weight, bias) if q is not None)}")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != dtype):
+        raise ValueError(f"layer_norm: residual must be {tuple(x.shape)} {dtype}, got "
                          f"{tuple(residual.shape)} {residual.dtype}")
     if not eps >= 0:
         raise ValueError(f"layer_norm: eps must be >= 0, got {eps}")
-    if x.device.type != "cuda":
+    if device.type != "cuda":
         raise ValueError("layer_norm requires CUDA tensors on a B200 (sm_100a) GPU")
-    if any(t.device != x.device for t in params + ([residual] if residual is not None else [])):
-        raise ValueError("layer_norm: all tensors must be on the same CUDA device")
-    _lib.load()
-    y, total = _LayerNormFunction.apply(
-        x, residual, weight.contiguous() if weight is not None else None,
-        bias.contiguous() if bias is not None else None, float(eps), bool(return_sum))
+    grad = x.requires_grad
+    for t in (weight, bias, residual):
+        if t is not None:
+            if t.device != device:
+                raise ValueError("layer_norm: all tensors must be on the same CUDA device")
+            grad = grad or t.requires_grad
+    if weight is not None:
+        weight = weight.contiguous()
+    if bias is not None:
+        bias = bias.contiguous()
+    if grad and torch.is_grad_enabled():
+        return _LayerNormFunction.apply(x, residual, weight, bias, float(eps), bool(return_sum))
+    y, total, *_ = _forward(x, residual, weight, bias, float(eps), return_sum, False)
     return (y, total) if return_sum else y

@@ -72,6 +72,17 @@ def _stream(device: torch.device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+# The current stream's handle by the device's index, without the Stream object
+# that torch.cuda.current_stream builds (2 us a call).
+_stream_of_index = torch._C._cuda_getCurrentRawStream
+
+
+def _raw_stream(device: torch.device) -> int:
+    """The device's current stream as a cudaStream_t."""
+    index = device.index
+    return _stream_of_index(torch.cuda.current_device() if index is None else index)
+
+
 def _forward(value, spatial_shapes, level_start_index, sampling_locations, attention_weights):
     B, S, M, D = value.shape
     _, Q, _, L, K, _ = sampling_locations.shape

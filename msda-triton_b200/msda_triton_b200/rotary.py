@@ -15,12 +15,13 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import _DTYPE_CODE, _FLOAT_DTYPES, _device_guard, _ptr, _stream
+from .ops import _DTYPE_CODE, _FLOAT_DTYPES, _device_guard, _raw_stream
 
 _LADDER = {"axis": 0, "shared": 1}
 _PAIRING = {"half": 0, "interleaved": 1}
 _POSITION = {torch.float32: _lib.MSDA_POSITION_F32, torch.int32: _lib.MSDA_POSITION_I32,
              torch.int64: _lib.MSDA_POSITION_I64}
+_Strides = ctypes.c_int64 * 3
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
@@ -28,48 +29,45 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
     return x if x.shape[-1] <= 1 or x.stride(-1) == 1 else x.contiguous()
 
 
-def _strides(x: torch.Tensor):
-    return (ctypes.c_int64 * 3)(*x.stride()[:3])
-
-
-def _turn(query, key, positions, axis_dims, base, ladder, pairing, inverse):
+def _turn(query, key, positions, axes, base, ladder, pairing, inverse):
     B, S, H, D = query.shape
     query = _rows(query)
     out = query.new_empty(B, S, H, D)
-    key_out, Hkv = None, 0
+    key_out, key_at, key_to, key_strides, Hkv = None, None, None, None, 0
     if key is not None:
         key, Hkv = _rows(key), key.shape[2]
         key_out = key.new_empty(B, S, Hkv, D)
-    axes = (ctypes.c_int32 * len(axis_dims))(*axis_dims)
-    lib = _lib.load()
-    with _device_guard(query.device):
-        rc = lib.msda_rotary(
-            _ptr(query), _ptr(key), _ptr(positions), _ptr(out), _ptr(key_out), B, S, H, Hkv, D,
-            _strides(query), _strides(key) if key is not None else None,
-            positions.stride(0) if positions.dim() == 3 else 0, _POSITION[positions.dtype], len(axis_dims), axes,
-            base, ladder, pairing, inverse, _DTYPE_CODE[query.dtype], _stream(query.device))
-    _lib.check("msda_rotary", rc)
+        key_at, key_to, key_strides = key.data_ptr(), key_out.data_ptr(), _Strides(*key.stride()[:3])
+    device = query.device
+    with _device_guard(device):
+        rc = _lib.load().msda_rotary(
+            query.data_ptr(), key_at, positions.data_ptr(), out.data_ptr(), key_to, B, S, H, Hkv, D,
+            _Strides(*query.stride()[:3]), key_strides, positions.stride(0) if positions.dim() == 3 else 0,
+            _POSITION[positions.dtype], len(axes), axes, base, ladder, pairing, inverse, _DTYPE_CODE[query.dtype],
+            _raw_stream(device))
+    if rc:
+        _lib.check("msda_rotary", rc)
     return out, key_out
 
 
 class _RotaryFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, query, key, positions, axis_dims, base, ladder, pairing):
+    def forward(ctx, query, key, positions, axes, base, ladder, pairing):
         ctx.save_for_backward(positions)
-        ctx.cfg = (axis_dims, base, ladder, pairing)
+        ctx.cfg = (axes, base, ladder, pairing)
         ctx.set_materialize_grads(False)
-        return _turn(query, key, positions, axis_dims, base, ladder, pairing, 0)
+        out, key_out = _turn(query, key, positions, axes, base, ladder, pairing, 0)
+        return out if key is None else (out, key_out)
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, grad_query, grad_key):
+    def backward(ctx, grad_query, grad_key=None):
         positions, = ctx.saved_tensors
-        grads = [g for g in (grad_query, grad_key) if g is not None]
-        if not grads:
+        if grad_query is None and grad_key is None:
             return (None,) * 7
-        turned = _turn(grads[0], grads[1] if len(grads) > 1 else None, positions, *ctx.cfg, 1)
         if grad_query is None:
-            return None, turned[0], None, None, None, None, None
+            return None, _turn(grad_key, None, positions, *ctx.cfg, 1)[0], None, None, None, None, None
+        turned = _turn(grad_query, grad_key, positions, *ctx.cfg, 1)
         return turned[0], turned[1], None, None, None, None, None
 
 
@@ -112,13 +110,16 @@ def rotary(
     if query.dim() != 4:
         raise ValueError(f"rotary: query must be (B, S, H, D), got {tuple(query.shape)}")
     B, S, H, D = query.shape
-    axis_dims = tuple(int(d) for d in axis_dims)
+    axis_dims = tuple(axis_dims)
     A = len(axis_dims)
     if not 1 <= A <= _lib.MSDA_ROTARY_MAX_AXES:
         raise ValueError(f"rotary: axis_dims must name 1 to {_lib.MSDA_ROTARY_MAX_AXES} axes, got {A}")
-    if any(d < 0 or d % 2 for d in axis_dims) or sum(axis_dims) > D:
+    total = 0
+    for d in axis_dims:
+        total = D + 1 if d < 0 or d % 2 else total + d
+    if total > D:
         raise ValueError(f"rotary: axis_dims must be even and sum to at most D={D}, got {axis_dims}")
-    if tuple(positions.shape) not in ((B, S, A), (S, A)):
+    if positions.shape != (B, S, A) and positions.shape != (S, A):
         raise ValueError(f"rotary: positions must be {(B, S, A)} or {(S, A)}, got {tuple(positions.shape)}")
     if positions.dtype not in _POSITION:
         raise ValueError(f"rotary: positions must be fp32, int32 or int64, got {positions.dtype}")
@@ -139,9 +140,11 @@ def rotary(
         raise ValueError("rotary requires CUDA tensors on a B200 (sm_100a) GPU")
     if positions.device != query.device or (key is not None and key.device != query.device):
         raise ValueError("rotary: query, key and positions must be on the same CUDA device")
-    _lib.load()
     if query.numel() == 0 and (key is None or key.numel() == 0):
         return query.clone() if key is None else (query.clone(), key.clone())
-    out, key_out = _RotaryFunction.apply(query, key, positions.contiguous(), axis_dims, float(base),
-                                         _LADDER[ladder], _PAIRING[pairing])
+    args = (query, key, positions.contiguous(), (ctypes.c_int32 * A)(*axis_dims), float(base), _LADDER[ladder],
+            _PAIRING[pairing])
+    if (query.requires_grad or (key is not None and key.requires_grad)) and torch.is_grad_enabled():
+        return _RotaryFunction.apply(*args)
+    out, key_out = _turn(*args, 0)
     return out if key is None else (out, key_out)
