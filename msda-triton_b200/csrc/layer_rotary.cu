@@ -19,6 +19,7 @@ namespace {
 constexpr int kRotaryThreads = 256;
 constexpr int kMaxPairs = MSDA_ROTARY_MAX_HEAD_DIM / 2;
 constexpr int kMaxCached = 1024;  // cosine / sine pairs a CTA holds (8 KB)
+constexpr int kMaxTokens = 128;   // tokens a CTA holds
 
 struct RotaryTable {
   // Frequencies in turns per unit of position, as the sum of two fp32 numbers.
@@ -58,15 +59,23 @@ __device__ __forceinline__ float position_at(const RotaryParams& p, int64_t at) 
 template <typename T, int VP, bool HALF>
 __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryParams p,
                                                                 const __grid_constant__ RotaryTable table) {
-  constexpr int N = VP == 0 ? 1 : VP;       // pairs an item
+  constexpr int N = VP == 0 ? 1 : VP;                   // pairs an item
   constexpr int W = HALF ? N : (VP == 0 ? 1 : 2 * VP);  // elements a load
+  constexpr bool TWO = HALF || VP == 0;                 // an item is two loads
+  constexpr int U = 4;                                  // items in flight a thread
+  using Raw = typename Pack<T, W>::Raw;
   __shared__ float2 turn[kMaxCached];
+  __shared__ int64_t from[2][kMaxTokens];  // the tokens' rows of query and key
   const int64_t token0 = (int64_t)blockIdx.x * p.tokens_per_cta;
   const int count = (int)min((int64_t)p.tokens_per_cta, p.tokens - token0);
+  if ((int)threadIdx.x < 2 * count) {
+    const int which = threadIdx.x & 1, t = threadIdx.x >> 1;
+    const int64_t b = (token0 + t) / p.seq, s = token0 + t - b * p.seq;
+    from[which][t] = b * p.stride[which][0] + s * p.stride[which][1];
+  }
   for (int i = threadIdx.x; i < count * p.pairs; i += kRotaryThreads) {
     const int t = i / p.pairs, k = i - t * p.pairs;
-    const int64_t token = token0 + t;
-    const int64_t b = token / p.seq, s = token - b * p.seq;
+    const int64_t b = (token0 + t) / p.seq, s = token0 + t - b * p.seq;
     const float pos = position_at(p, b * p.position_batch_stride + s * p.num_axes + table.axis[k]);
     // pos * frequency exactly, as h + l; whole turns leave h without a rounding.
     const float f = table.hi[k], h = pos * f, l = fmaf(pos, f, -h);
@@ -78,49 +87,66 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryPara
   __syncthreads();
   const int pair_items = p.pairs / N;
   const uint32_t work = (uint32_t)count * p.all_heads * p.items;
-  for (uint32_t i = threadIdx.x; i < work; i += kRotaryThreads) {
-    const uint32_t row = quotient(i, p.items, p.items_magic), item = i - row * p.items;
-    const uint32_t t = quotient(row, p.all_heads, p.heads_magic);
-    uint32_t h = row - t * p.all_heads;
-    const int64_t token = token0 + t;
-    const int64_t b = token / p.seq, s = token - b * p.seq;
-    const int which = h >= (uint32_t)p.heads[0];
-    if (which) h -= p.heads[0];
-    const T* x = static_cast<const T*>(p.x[which]) + b * p.stride[which][0] + s * p.stride[which][1] +
-                 h * p.stride[which][2];
-    T* y = static_cast<T*>(p.y[which]) + (token * p.heads[which] + h) * (int64_t)p.D;
-    if ((int)item >= pair_items) {  // a channel group that passes through
-      const int c = 2 * p.pairs + ((int)item - pair_items) * W;
-      *reinterpret_cast<typename Pack<T, W>::Raw*>(y + c) = load_raw<T, W>(x + c);
-      continue;
+  for (uint32_t i0 = threadIdx.x; i0 < work; i0 += U * kRotaryThreads) {
+    Raw first[U], second[U];
+    T* y[U];
+    int at[U], apart[U];  // pair in `turn` (-1: passes through), the second load's distance
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t i = i0 + u * kRotaryThreads;
+      y[u] = nullptr;
+      if (i >= work) continue;
+      const uint32_t row = quotient(i, p.items, p.items_magic);
+      const int item = (int)(i - row * p.items);
+      const uint32_t t = quotient(row, p.all_heads, p.heads_magic);
+      uint32_t h = row - t * p.all_heads;
+      const int which = h >= (uint32_t)p.heads[0];
+      if (which) h -= p.heads[0];
+      int c = 2 * p.pairs + (item - pair_items) * W;
+      at[u] = -1, apart[u] = 0;
+      if (item < pair_items) {
+        const int k = item * N;
+        at[u] = t * p.pairs + k;
+        if constexpr (TWO) c = table.first[k], apart[u] = table.second[k] - c;
+        else c = 2 * k;
+      }
+      const T* x = static_cast<const T*>(p.x[which]) + from[which][t] + h * p.stride[which][2] + c;
+      y[u] = static_cast<T*>(p.y[which]) + ((token0 + t) * p.heads[which] + h) * (int64_t)p.D + c;
+      first[u] = load_raw<T, W>(x);
+      if (TWO && at[u] >= 0) second[u] = load_raw<T, W>(x + apart[u]);
     }
-    const int k = (int)item * N;
-    const float2* cs = turn + t * p.pairs + k;
-    if constexpr (HALF || VP == 0) {
-      const int c0 = table.first[k], c1 = table.second[k];
-      float a[N], d[N];
-      load_vec<T, N>(x + c0, a);
-      load_vec<T, N>(x + c1, d);
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const float2 r = cs[j];
-        const float u = a[j] * r.x - d[j] * r.y;
-        d[j] = a[j] * r.y + d[j] * r.x;
-        a[j] = u;
+    for (int u = 0; u < U; ++u) {
+      if (!y[u]) continue;
+      if (at[u] < 0) {
+        *reinterpret_cast<Raw*>(y[u]) = first[u];
+        continue;
       }
-      store_vec<T, N>(y + c0, a);
-      store_vec<T, N>(y + c1, d);
-    } else {
-      float v[W];
-      load_vec<T, W>(x + 2 * k, v);
+      const float2* cs = turn + at[u];
+      float a[W];
+      unpack_raw<T, W>(first[u], a);
+      if constexpr (TWO) {
+        float d[W];
+        unpack_raw<T, W>(second[u], d);
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const float2 r = cs[j];
-        const float u = v[2 * j] * r.x - v[2 * j + 1] * r.y;
-        v[2 * j + 1] = v[2 * j] * r.y + v[2 * j + 1] * r.x;
-        v[2 * j] = u;
+        for (int j = 0; j < N; ++j) {
+          const float2 r = cs[j];
+          const float v = a[j] * r.x - d[j] * r.y;
+          d[j] = a[j] * r.y + d[j] * r.x;
+          a[j] = v;
+        }
+        store_vec<T, W>(y[u], a);
+        store_vec<T, W>(y[u] + apart[u], d);
+      } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          const float2 r = cs[j];
+          const float v = a[2 * j] * r.x - a[2 * j + 1] * r.y;
+          a[2 * j + 1] = a[2 * j] * r.y + a[2 * j + 1] * r.x;
+          a[2 * j] = v;
+        }
+        store_vec<T, W>(y[u], a);
       }
-      store_vec<T, W>(y + 2 * k, v);
     }
   }
 }
@@ -263,6 +289,7 @@ extern "C" int msda_rotary(const void* query, const void* key, const void* posit
   if (per_token > (int64_t(1) << 22)) return fail(MSDA_ERR_UNSUPPORTED, "%s: num_heads * head_dim too large", fn);
   int64_t tpc = 4096 / per_token;
   if (k > 0 && tpc > kMaxCached / k) tpc = kMaxCached / k;
+  if (tpc > kMaxTokens) tpc = kMaxTokens;
   const int64_t fill = p.tokens / (2 * sm_count());
   if (tpc > fill) tpc = fill;
   if (tpc < 1) tpc = 1;
