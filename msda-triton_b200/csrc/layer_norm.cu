@@ -6,31 +6,27 @@
 //   dw = sum_rows g z,  db = sum_rows g
 //
 // Bound by HBM: a row is read once, kept in registers by the threads that
-// share it, and written once; the variance is taken about the mean, from the
-// registers. Rows are dealt to a grid that fits the GPU, so that a thread keeps
-// its channels' weights, and in the backward their gradients' running sums, in
-// registers from row to row. What matters is how many bytes are in flight:
-//   - up to 512 channels a warp has a row, and loads the next one while it
-//     reduces this one;
-//   - up to 8192 channels a CTA has a row, and bulk copies bring the next ones
-//     to a ring in shared memory. (With the rows in registers alone, 256 to 1024
-//     threads each, the backward of 4095 x 5001 in fp32 took 92 to 117 us.)
-//   - wider rows are read again from L2 for each step.
-// Each CTA leaves one partial row of the two column sums; a second kernel adds
-// the partial rows in a fixed order.
+// share it (a warp up to 512 channels, 128 to 512 threads up to 8192), and
+// written once; the variance is taken about the mean, from the registers. Rows
+// are dealt to a grid that fits the GPU, so that a thread keeps its channels'
+// weights, and in the backward their gradients' running sums, in registers from
+// row to row, and the next row's loads are in flight while a row is reduced.
+// Longer rows are bound by the latency of their sums over the CTA, so that these
+// go in pairs. (Staging rows in shared memory by bulk copies was slower: 20000 x
+// 1000 bf16 forward 91 us for 29.) Rows wider than 8192 are read again from L2
+// for each step. Each CTA leaves one partial row of the two column sums; a second
+// kernel adds the partial rows in a fixed order.
 #include <algorithm>
 
 #include "msda_abi.cuh"
 #include "msda_common.cuh"
-#include "layer_tcgen05.cuh"
 #include "msda_layer_b200.h"
 
 namespace msda {
 namespace {
 
 constexpr int kNormThreads = 256;
-constexpr int kWarpWidth = 512;       // widest row of a warp
-constexpr int kRegisterWidth = 8192;  // widest row of a CTA
+constexpr int kRegisterWidth = 8192;  // widest row held in registers
 constexpr int kWideThreads = 1024;    // a CTA of the wider rows' kernels
 constexpr int kNormSms = 148;         // grids and workspaces go by this, not by the device
 
@@ -61,19 +57,25 @@ __device__ __forceinline__ float param_at(const void* p, int f32, int c) {
   return to_f32(*reinterpret_cast<const T*>(&bits));
 }
 
-// Sum over the TPR threads that share a row, the same in each of them. `red`:
-// one float for each warp of the CTA in each of a few buffers; consecutive
-// calls take different ones, so that one barrier a call is enough.
+// Sums of two values over the TPR threads that share a row, the same in each of
+// them. `red`: a pair for each warp of the CTA in each of two buffers, which
+// consecutive calls take in turn, so that one barrier a call is enough.
 template <int TPR>
-__device__ __forceinline__ float row_sum(float v, float (*red)[32], int buffer) {
+__device__ __forceinline__ float2 row_sums(float2 v, float2 (*red)[32], int buffer) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
+  for (int o = 16; o > 0; o >>= 1) {
+    v.x += __shfl_xor_sync(kFullMask, v.x, o);
+    v.y += __shfl_xor_sync(kFullMask, v.y, o);
+  }
   if constexpr (TPR > 32) {
     if ((threadIdx.x & 31) == 0) red[buffer][threadIdx.x >> 5] = v;
     __syncthreads();
-    v = (threadIdx.x & 31) < TPR / 32 ? red[buffer][threadIdx.x & 31] : 0.0f;
+    v = red[buffer][threadIdx.x & (TPR / 32 - 1)];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
+    for (int o = TPR / 64; o > 0; o >>= 1) {
+      v.x += __shfl_xor_sync(kFullMask, v.x, o);
+      v.y += __shfl_xor_sync(kFullMask, v.y, o);
+    }
   }
   return v;
 }
@@ -94,15 +96,6 @@ struct RowTile {
     for (int v = 0; v < NV; ++v) {
       raw[v] = Raw{};
       if (any && column(v) < width) raw[v] = load_raw<T, VEC>(p + column(v));
-    }
-  }
-
-  // The same from shared memory.
-  static __device__ __forceinline__ void staged(const char* row, int width, Raw (&raw)[NV]) {
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      raw[v] = Raw{};
-      if (column(v) < width) raw[v] = *reinterpret_cast<const Raw*>(row + column(v) * (int)sizeof(T));
     }
   }
 
@@ -145,75 +138,34 @@ struct RowTile {
       }
   }
 
-  // A row h = x (+ r) to y, its mean and reciprocal deviation. scale(e, z): the
-  // normalised channel with its weight and bias.
-  template <typename Scale>
-  static __device__ __forceinline__ void normalise(const NormParams& p, int64_t row, float (&h)[E], float (*red)[32], float inv,
-                                                   Scale scale) {
-    const int width = p.width;
-    if (p.sum_out) store(p.sum_out, row * width, width, h);
-    float s = 0.0f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) s += h[e];
-    const float mean = row_sum<TPR>(s, red, 0) * inv;
-    // The mean's rounding is taken out again: it would show where the row
-    // lies many deviations from zero.
-    float rest = 0.0f;
-    s = 0.0f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      h[e] = inside(e, width) ? h[e] - mean : 0.0f;
-      rest += h[e];
-      s = fmaf(h[e], h[e], s);
-    }
-    rest = row_sum<TPR>(rest, red, 1) * inv;
-    const float rstd = rsqrtf(fmaf(-rest, rest, row_sum<TPR>(s, red, 2) * inv) + p.eps);
-#pragma unroll
-    for (int e = 0; e < E; ++e) h[e] = scale(e, (h[e] - rest) * rstd);
-    store(p.y, row * width, width, h);
-    if (p.mean && threadIdx.x % TPR == 0) {
-      p.mean[row] = mean;
-      p.rstd[row] = rstd;
-    }
-  }
-
-  // The gradient of row h = x (+ r) from g, and the column sums' share.
-  template <typename Weight>
-  static __device__ __forceinline__ void differentiate(const NormParams& p, int64_t row, float mean, float rstd, float (&h)[E],
-                                                       float (&g)[E], float (&dw)[E], float (&db)[E], float (*red)[32], float inv,
-                                                       Weight weight) {
-    const int width = p.width;
-    float s1 = 0.0f, s2 = 0.0f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      h[e] = inside(e, width) ? (h[e] - mean) * rstd : 0.0f;
-      db[e] += g[e];
-      dw[e] = fmaf(g[e], h[e], dw[e]);
-      g[e] *= weight(e);
-      s1 += g[e];
-      s2 = fmaf(g[e], h[e], s2);
-    }
-    const float c1 = row_sum<TPR>(s1, red, 0) * inv, c2 = row_sum<TPR>(s2, red, 1) * inv;
-#pragma unroll
-    for (int e = 0; e < E; ++e) g[e] = (g[e] - c1 - h[e] * c2) * rstd;
-    if (p.grad_sum) {
-      Raw sum[NV];
-      fetch(p.grad_sum, row * width, width, true, sum);
-      add(sum, g);
-    }
-    store(p.grad_x, row * width, width, g);
-  }
 };
 
-// A warp a row.
-template <typename T, int VEC, int NV>
-__global__ void __launch_bounds__(kNormThreads) norm_fwd_kernel(const NormParams p) {
-  using R = RowTile<T, VEC, NV, 32>;
+// A CTA's threads, and the rows that it works on at once.
+template <int TPR>
+__host__ __device__ constexpr int norm_threads() {
+  return TPR == 32 ? kNormThreads : TPR;
+}
+template <int TPR>
+__host__ __device__ constexpr int norm_rows() {
+  return TPR == 32 ? kNormThreads / 32 : 1;
+}
+
+// Rows of 16 channels a thread and more than a warp have no registers left for
+// the next row in the backward.
+template <int TPR, int E, bool BWD>
+__host__ __device__ constexpr bool norm_ahead() {
+  return !(BWD && TPR > 32 && E > 8);
+}
+
+template <typename T, int VEC, int NV, int TPR>
+__global__ void __launch_bounds__(norm_threads<TPR>()) norm_fwd_kernel(const NormParams p) {
+  using R = RowTile<T, VEC, NV, TPR>;
   constexpr int E = R::E;
+  __shared__ float2 red[2][32];
   const int width = p.width;
   const float inv = 1.0f / (float)width;
-  const int64_t step = (int64_t)gridDim.x * (kNormThreads / 32);
-  int64_t row = (int64_t)blockIdx.x * (kNormThreads / 32) + threadIdx.x / 32;
+  const int64_t step = (int64_t)gridDim.x * norm_rows<TPR>();
+  int64_t row = (int64_t)blockIdx.x * norm_rows<TPR>() + (TPR == 32 ? threadIdx.x / 32 : 0);
   typename R::Raw next[NV], more[NV];
   R::fetch(p.x, row * p.x_stride, width, row < p.rows, next);
   R::fetch(p.residual, row * p.residual_stride, width, row < p.rows && p.residual, more);
@@ -226,203 +178,90 @@ __global__ void __launch_bounds__(kNormThreads) norm_fwd_kernel(const NormParams
     if (p.residual) R::add(more, h);
     R::fetch(p.x, (row + step) * p.x_stride, width, row + step < p.rows, next);
     if (p.residual) R::fetch(p.residual, (row + step) * p.residual_stride, width, row + step < p.rows, more);
-    R::normalise(p, row, h, nullptr, inv, [&](int e, float z) { return fmaf(z, w[e], b[e]); });
+    if (p.sum_out) R::store(p.sum_out, row * width, width, h);
+    float2 s = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int e = 0; e < E; ++e) s.x += h[e];
+    const float mean = row_sums<TPR>(s, red, 0).x * inv;
+    // The mean's rounding is taken out again: it would show where the row
+    // lies many deviations from zero.
+    s = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      h[e] = R::inside(e, width) ? h[e] - mean : 0.0f;
+      s.x += h[e];
+      s.y = fmaf(h[e], h[e], s.y);
+    }
+    s = row_sums<TPR>(s, red, 1);
+    const float rest = s.x * inv;
+    const float rstd = rsqrtf(fmaf(-rest, rest, s.y * inv) + p.eps);
+#pragma unroll
+    for (int e = 0; e < E; ++e) h[e] = fmaf((h[e] - rest) * rstd, w[e], b[e]);
+    R::store(p.y, row * width, width, h);
+    if (p.mean && threadIdx.x % TPR == 0) {
+      p.mean[row] = mean;
+      p.rstd[row] = rstd;
+    }
   }
 }
 
-template <typename T, int VEC, int NV>
-__global__ void __launch_bounds__(kNormThreads) norm_bwd_kernel(const NormParams p) {
-  using R = RowTile<T, VEC, NV, 32>;
-  constexpr int E = R::E, kRows = kNormThreads / 32;
+template <typename T, int VEC, int NV, int TPR>
+__global__ void __launch_bounds__(norm_threads<TPR>()) norm_bwd_kernel(const NormParams p) {
+  using R = RowTile<T, VEC, NV, TPR>;
+  constexpr int E = R::E, kRows = norm_rows<TPR>();
+  constexpr bool kAhead = norm_ahead<TPR, E, true>();
+  __shared__ float2 red[2][32];
   const int width = p.width;
   const float inv = 1.0f / (float)width;
   const int64_t step = (int64_t)gridDim.x * kRows;
-  int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / 32;
+  int64_t row = (int64_t)blockIdx.x * kRows + (TPR == 32 ? threadIdx.x / 32 : 0);
   typename R::Raw next[NV], more[NV], grad[NV];
-  R::fetch(p.x, row * p.x_stride, width, row < p.rows, next);
-  R::fetch(p.grad_y, row * p.grad_stride, width, row < p.rows, grad);
-  R::fetch(p.residual, row * p.residual_stride, width, row < p.rows && p.residual, more);
   float mean = 0.0f, rstd = 0.0f;
-  if (row < p.rows) mean = __ldg(p.mean + row), rstd = __ldg(p.rstd + row);
+  const auto fetch = [&](int64_t r, bool any) {
+    R::fetch(p.x, r * p.x_stride, width, any, next);
+    R::fetch(p.grad_y, r * p.grad_stride, width, any, grad);
+    if (p.residual) R::fetch(p.residual, r * p.residual_stride, width, any, more);
+    if (any) mean = __ldg(p.mean + r), rstd = __ldg(p.rstd + r);
+  };
+  if (kAhead) fetch(row, row < p.rows);
   float w[E], dw[E], db[E];
   R::params(p.weight, p.param_f32, width, 1.0f, w);
 #pragma unroll
   for (int e = 0; e < E; ++e) dw[e] = db[e] = 0.0f;
-  for (; row < p.rows; row += step) {
+  int turn = 0;
+  for (; row < p.rows; row += step, turn ^= 1) {
+    if (!kAhead) fetch(row, true);
     float h[E], g[E];
     R::unpack(next, h);
     R::unpack(grad, g);
     if (p.residual) R::add(more, h);
     const float mu = mean, rs = rstd;
-    const bool again = row + step < p.rows;
-    R::fetch(p.x, (row + step) * p.x_stride, width, again, next);
-    R::fetch(p.grad_y, (row + step) * p.grad_stride, width, again, grad);
-    if (p.residual) R::fetch(p.residual, (row + step) * p.residual_stride, width, again, more);
-    if (again) mean = __ldg(p.mean + row + step), rstd = __ldg(p.rstd + row + step);
-    R::differentiate(p, row, mu, rs, h, g, dw, db, nullptr, inv, [&](int e) { return w[e]; });
+    if (kAhead) fetch(row + step, row + step < p.rows);
+    float2 s = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      h[e] = R::inside(e, width) ? (h[e] - mu) * rs : 0.0f;
+      db[e] += g[e];
+      dw[e] = fmaf(g[e], h[e], dw[e]);
+      g[e] *= w[e];
+      s.x += g[e];
+      s.y = fmaf(g[e], h[e], s.y);
+    }
+    s = row_sums<TPR>(s, red, turn);
+    s.x *= inv, s.y *= inv;
+#pragma unroll
+    for (int e = 0; e < E; ++e) g[e] = (g[e] - s.x - h[e] * s.y) * rs;
+    if (p.grad_sum) {
+      typename R::Raw sum[NV];
+      R::fetch(p.grad_sum, row * width, width, true, sum);
+      R::add(sum, g);
+    }
+    R::store(p.grad_x, row * width, width, g);
   }
   if (!p.want_columns) return;
-  // The CTA's warps add their sums in turn, in shared memory.
-  __shared__ float sum[2][32 * E];
-  for (int r = 0; r < kRows; ++r) {
-    if ((int)(threadIdx.x / 32) == r) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int at = e * 32 + (threadIdx.x & 31);
-        sum[0][at] = r ? sum[0][at] + dw[e] : dw[e];
-        sum[1][at] = r ? sum[1][at] + db[e] : db[e];
-      }
-    }
-    __syncthreads();
-  }
   float* out = p.partial + (int64_t)blockIdx.x * width;
   const int64_t second = (int64_t)gridDim.x * width;
-  for (int i = threadIdx.x; i < 32 * E; i += kNormThreads) {
-    const int e = i / 32, lane = i & 31;
-    const int c = ((e / VEC) * 32 + lane) * VEC + e % VEC;
-    if (c < width) {
-      out[c] = sum[0][i];
-      out[second + c] = sum[1][i];
-    }
-  }
-}
-
-// A CTA a row, from a ring of staged rows. A slot holds the row of each input
-// (x, gradient, residual) with the 16-byte pieces that its ends lie in; the last
-// piece of a row after which the buffer may end is left out, and loaded apart.
-struct NormSlots {
-  const char* base[3];
-  int64_t stride[3];  // bytes
-  int inputs, slots, slot_row;  // slot_row: bytes of one input's row in a slot
-};
-
-__device__ __forceinline__ void stage_row(const NormSlots& s, char* slot, uint64_t* bar, int64_t row, int bytes, bool last) {
-  uint32_t total = 0;
-  for (int i = 0; i < s.inputs; ++i) {
-    const uintptr_t at = reinterpret_cast<uintptr_t>(s.base[i] + row * s.stride[i]), end = at + bytes;
-    const uintptr_t low = at & ~uintptr_t(15), high = last ? end & ~uintptr_t(15) : (end + 15) & ~uintptr_t(15);
-    if (high > low) total += (uint32_t)(high - low);
-  }
-  tc::bar_expect(bar, total);
-  for (int i = 0; i < s.inputs; ++i) {
-    const uintptr_t at = reinterpret_cast<uintptr_t>(s.base[i] + row * s.stride[i]), end = at + bytes;
-    const uintptr_t low = at & ~uintptr_t(15), high = last ? end & ~uintptr_t(15) : (end + 15) & ~uintptr_t(15);
-    if (high > low)
-      asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                   ::"r"(tc::smem_u32(slot + i * s.slot_row)), "l"(low), "r"((uint32_t)(high - low)), "r"(tc::smem_u32(bar))
-                   : "memory");
-  }
-}
-
-// CTAs an SM that the ring is laid out for.
-template <int E, bool BWD>
-constexpr int staged_resident() {
-  return E == 32 ? (BWD ? 1 : 2) : E == 16 ? (BWD ? 2 : 3) : (BWD ? 3 : 4);
-}
-
-template <typename T, int VEC, int NV, bool BWD>
-__global__ void __launch_bounds__(kNormThreads, (staged_resident<VEC * NV, BWD>()))
-    norm_staged_kernel(const NormParams p, const NormSlots s) {
-  using R = RowTile<T, VEC, NV, kNormThreads>;
-  constexpr int E = R::E, kMost = 8;
-  extern __shared__ __align__(128) char ring[];
-  __shared__ uint64_t full[kMost];
-  __shared__ float red[3][32];
-  __shared__ int abort_flag;
-  const int width = p.width, bytes = width * (int)sizeof(T);
-  const float inv = 1.0f / (float)width;
-  float* ws = reinterpret_cast<float*>(ring + s.slots * s.inputs * s.slot_row);  // weights, then biases
-  if (threadIdx.x == 0) {
-    abort_flag = 0;
-    for (int i = 0; i < s.slots; ++i) tc::bar_init(&full[i], 1);
-    tc::fence_async_smem();
-  }
-  // Whether the buffer may end with this row.
-  const auto last = [&](int64_t row) {
-    bool l = row + 1 == p.rows;
-    for (int i = 0; i < s.inputs; ++i) l = l || s.stride[i] < bytes;
-    return l;
-  };
-  __syncthreads();
-  if (threadIdx.x == 0)
-    for (int i = 0; i < s.slots; ++i) {
-      const int64_t row = blockIdx.x + (int64_t)i * gridDim.x;
-      if (row < p.rows) stage_row(s, ring + i * s.inputs * s.slot_row, &full[i], row, bytes, last(row));
-    }
-  float w[E], b[BWD ? 1 : E], dw[BWD ? E : 1], db[BWD ? E : 1];
-  constexpr bool kHold = E == 8;  // the parameters in registers; else in shared memory
-  if constexpr (kHold) {
-    R::params(p.weight, p.param_f32, width, 1.0f, w);
-    if constexpr (!BWD) R::params(p.bias, p.param_f32, width, 0.0f, b);
-  } else {
-    for (int c = threadIdx.x; c < width; c += kNormThreads) {
-      ws[c] = 1.0f;
-      if (p.weight) ws[c] = param_at<T>(p.weight, p.param_f32, c);
-      if constexpr (!BWD) {
-        ws[width + c] = 0.0f;
-        if (p.bias) ws[width + c] = param_at<T>(p.bias, p.param_f32, c);
-      }
-    }
-    __syncthreads();
-  }
-  if constexpr (BWD) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) dw[e] = db[e] = 0.0f;
-  }
-  int n = 0;
-  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, ++n) {
-    const int at = n % s.slots;
-    char* slot = ring + at * s.inputs * s.slot_row;
-    float mean = 0.0f, rstd = 0.0f;
-    if constexpr (BWD) mean = __ldg(p.mean + row), rstd = __ldg(p.rstd + row);
-    bool ok = tc::bar_wait(&full[at], (n / s.slots) & 1, &abort_flag);
-    // Where an input's row starts in the slot.
-    const auto from = [&](int i) { return slot + i * s.slot_row + (reinterpret_cast<uintptr_t>(s.base[i] + row * s.stride[i]) & 15); };
-    if (last(row)) {  // the pieces left out
-      for (int i = 0; i < s.inputs; ++i) {
-        const T* src = reinterpret_cast<const T*>(s.base[i] + row * s.stride[i]);
-        const uintptr_t start = reinterpret_cast<uintptr_t>(src), cut = (start + bytes) & ~uintptr_t(15);
-        const int c = (cut > start ? (int)((cut - start) / sizeof(T)) : 0) + threadIdx.x;
-        if (c < width) reinterpret_cast<T*>(from(i))[c] = src[c];
-      }
-      __syncthreads();
-    }
-    typename R::Raw raw[NV];
-    float h[E];
-    R::staged(from(0), width, raw);
-    R::unpack(raw, h);
-    if (p.residual) {
-      R::staged(from(BWD ? 2 : 1), width, raw);
-      R::add(raw, h);
-    }
-    if constexpr (BWD) {
-      float g[E];
-      R::staged(from(1), width, raw);
-      R::unpack(raw, g);
-      if (!ok) mean = NAN;
-      R::differentiate(p, row, mean, rstd, h, g, dw, db, red, inv, [&](int e) {
-        if constexpr (kHold) return w[e];
-        return ws[min(R::column(e / VEC) + e % VEC, width - 1)];
-      });
-    } else {
-      if (!ok) h[0] = NAN;
-      R::normalise(p, row, h, red, inv, [&](int e, float z) {
-        if constexpr (kHold) return fmaf(z, w[e], b[e]);
-        const int c = min(R::column(e / VEC) + e % VEC, width - 1);
-        return fmaf(z, ws[c], ws[width + c]);
-      });
-    }
-    // Every thread has read the slot: all have come to the row's sums since.
-    const int64_t later = row + (int64_t)s.slots * gridDim.x;
-    if (threadIdx.x == 0 && later < p.rows && ok) {
-      tc::fence_async_smem();
-      stage_row(s, slot, &full[at], later, bytes, last(later));
-    }
-  }
-  if constexpr (BWD) {
-    if (!p.want_columns) return;
-    float* out = p.partial + (int64_t)blockIdx.x * width;
-    const int64_t second = (int64_t)gridDim.x * width;
+  if constexpr (kRows == 1) {
 #pragma unroll
     for (int e = 0; e < E; ++e)
       if (R::inside(e, width)) {
@@ -430,6 +269,28 @@ __global__ void __launch_bounds__(kNormThreads, (staged_resident<VEC * NV, BWD>(
         out[c] = dw[e];
         out[second + c] = db[e];
       }
+  } else {
+    // The CTA's warps add their sums in turn, in shared memory.
+    __shared__ float sum[2][32 * E];
+    for (int r = 0; r < kRows; ++r) {
+      if ((int)(threadIdx.x / 32) == r) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const int at = e * 32 + (threadIdx.x & 31);
+          sum[0][at] = r ? sum[0][at] + dw[e] : dw[e];
+          sum[1][at] = r ? sum[1][at] + db[e] : db[e];
+        }
+      }
+      __syncthreads();
+    }
+    for (int i = threadIdx.x; i < 32 * E; i += kNormThreads) {
+      const int e = i / 32, lane = i & 31;
+      const int c = ((e / VEC) * 32 + lane) * VEC + e % VEC;
+      if (c < width) {
+        out[c] = sum[0][i];
+        out[second + c] = sum[1][i];
+      }
+    }
   }
 }
 
@@ -442,21 +303,20 @@ __device__ __forceinline__ float wide_at(const NormParams& p, int64_t row, int c
 
 template <typename T>
 __global__ void __launch_bounds__(kWideThreads) norm_wide_fwd_kernel(const NormParams p) {
-  __shared__ float red[3][32];
+  __shared__ float2 red[2][32];
   const float inv = 1.0f / (float)p.width;
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-    float s = 0.0f;
-    for (int c = threadIdx.x; c < p.width; c += kWideThreads) s += wide_at<T>(p, row, c);
-    const float mean = row_sum<kWideThreads>(s, red, 0) * inv;
-    float rest = 0.0f;
-    s = 0.0f;
+    float2 s = make_float2(0.0f, 0.0f);
+    for (int c = threadIdx.x; c < p.width; c += kWideThreads) s.x += wide_at<T>(p, row, c);
+    const float mean = row_sums<kWideThreads>(s, red, 0).x * inv;
+    s = make_float2(0.0f, 0.0f);
     for (int c = threadIdx.x; c < p.width; c += kWideThreads) {
       const float d = wide_at<T>(p, row, c) - mean;
-      rest += d;
-      s = fmaf(d, d, s);
+      s.x += d;
+      s.y = fmaf(d, d, s.y);
     }
-    rest = row_sum<kWideThreads>(rest, red, 1) * inv;
-    const float rstd = rsqrtf(fmaf(-rest, rest, row_sum<kWideThreads>(s, red, 2) * inv) + p.eps);
+    s = row_sums<kWideThreads>(s, red, 1);
+    const float rest = s.x * inv, rstd = rsqrtf(fmaf(-rest, rest, s.y * inv) + p.eps);
     for (int c = threadIdx.x; c < p.width; c += kWideThreads) {
       const float h = wide_at<T>(p, row, c);
       const float w = p.weight ? param_at<T>(p.weight, p.param_f32, c) : 1.0f;
@@ -473,18 +333,21 @@ __global__ void __launch_bounds__(kWideThreads) norm_wide_fwd_kernel(const NormP
 
 template <typename T>
 __global__ void __launch_bounds__(kWideThreads) norm_wide_bwd_kernel(const NormParams p) {
-  __shared__ float red[3][32];
+  __shared__ float2 red[2][32];
   const float inv = 1.0f / (float)p.width;
+  int turn = 0;
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
     const float mean = __ldg(p.mean + row), rstd = __ldg(p.rstd + row);
     const T* g = static_cast<const T*>(p.grad_y) + row * p.grad_stride;
-    float s1 = 0.0f, s2 = 0.0f;
+    float2 s = make_float2(0.0f, 0.0f);
     for (int c = threadIdx.x; c < p.width; c += kWideThreads) {
       const float gw = to_f32(__ldg(g + c)) * (p.weight ? param_at<T>(p.weight, p.param_f32, c) : 1.0f);
-      s1 += gw;
-      s2 = fmaf(gw, (wide_at<T>(p, row, c) - mean) * rstd, s2);
+      s.x += gw;
+      s.y = fmaf(gw, (wide_at<T>(p, row, c) - mean) * rstd, s.y);
     }
-    const float c1 = row_sum<kWideThreads>(s1, red, 0) * inv, c2 = row_sum<kWideThreads>(s2, red, 1) * inv;
+    s = row_sums<kWideThreads>(s, red, turn);
+    turn ^= 1;
+    const float c1 = s.x * inv, c2 = s.y * inv;
     for (int c = threadIdx.x; c < p.width; c += kWideThreads) {
       const float gw = to_f32(__ldg(g + c)) * (p.weight ? param_at<T>(p.weight, p.param_f32, c) : 1.0f);
       float d = (gw - c1 - (wide_at<T>(p, row, c) - mean) * rstd * c2) * rstd;
@@ -541,76 +404,42 @@ __global__ void __launch_bounds__(1024) norm_columns_kernel(const float* partial
 using namespace abi;
 
 struct NormShape {
-  int vec, nv;
-  bool staged, wide;
+  int vec, nv, tpr;
 };
 
-// Channels a thread of a CTA's row: 8, or more where that does not hold it.
-int staged_channels(int64_t width) { return width <= 8 * kNormThreads ? 8 : width <= 16 * kNormThreads ? 16 : 32; }
+// Threads a row and channels a thread by the width alone: 8 channels, or 16
+// where a warp (up to 512) or 512 threads (up to 8192) hold the row with them.
+int norm_threads_of(int64_t width) { return width <= 512 ? 32 : width <= 1024 ? 128 : width <= 2048 ? 256 : 512; }
+int norm_channels_of(int64_t width) { return width <= 8 * norm_threads_of(width) ? 8 : 16; }
 
 // The vector is the widest of 16 bytes, 4 bytes and one element that the
-// width, the strides and the buffers allow. `whole`: the inputs' buffers start on
-// 16 bytes, as staging takes them.
-NormShape norm_shape(int64_t width, int es, int64_t unit, bool whole) {
+// width, the strides and the buffers allow.
+NormShape norm_shape(int64_t width, int es, int64_t unit) {
   const int v16 = 16 / es, v4 = 4 / es;
   NormShape s;
   s.vec = unit % v16 == 0 ? v16 : unit % v4 == 0 ? v4 : 1;
-  s.staged = width > kWarpWidth && width <= kRegisterWidth && whole;
-  s.wide = width > kWarpWidth && !s.staged;
-  if (s.staged) s.nv = staged_channels(width) / s.vec;
-  else s.nv = width <= 32 && s.vec == 1 ? 1 : (width <= 256 ? 8 : 16) / s.vec;
+  s.tpr = norm_threads_of(width);
+  s.nv = width <= 32 && s.vec == 1 ? 1 : norm_channels_of(width) / s.vec;
   return s;
 }
 
 // Most CTAs of a backward, each of which leaves a partial row.
 int64_t norm_backward_most(int64_t width) {
-  if (width <= kWarpWidth) return kNormSms * (width <= 256 ? 4 : 2);
   if (width > kRegisterWidth) return kNormSms * 2;
-  const int e = staged_channels(width);
-  return kNormSms * (e == 8 ? staged_resident<8, true>() : e == 16 ? staged_resident<16, true>() : staged_resident<32, true>());
+  return kNormSms * (norm_threads_of(width) <= 256 ? 4 : norm_channels_of(width) == 8 ? 2 : 1);
 }
 
 int norm_grid(int64_t rows, const NormShape& s, bool backward, int64_t width) {
-  const int64_t per_cta = s.staged || s.wide ? 1 : kNormThreads / 32;
-  const int64_t ctas = (rows + per_cta - 1) / per_cta;
-  int64_t most = norm_backward_most(width);
-  if (!backward) {
-    const int e = staged_channels(width);
-    most = kNormSms * (s.wide ? 2 : !s.staged ? 8 : e == 8 ? staged_resident<8, false>() : e == 16 ? staged_resident<16, false>()
-                                                                                                    : staged_resident<32, false>());
-  }
+  const bool warps = s.tpr == 32;
+  const int64_t ctas = warps ? (rows + kNormThreads / 32 - 1) / (kNormThreads / 32) : rows;
+  const int64_t most = backward ? norm_backward_most(width)
+                                : kNormSms * (width > kRegisterWidth ? 2 : 2048 / (warps ? kNormThreads : s.tpr));
   return (int)(ctas < most ? ctas : most);
-}
-
-template <typename T, int VEC, int NV, bool BWD>
-cudaError_t staged_launch(const NormParams& p, int grid, cudaStream_t st) {
-  constexpr int E = VEC * NV;
-  NormSlots s = {};
-  int n = 0;
-  const auto input = [&](const void* base, int64_t stride) {
-    s.base[n] = static_cast<const char*>(base);
-    s.stride[n++] = stride * (int64_t)sizeof(T);
-  };
-  input(p.x, p.x_stride);
-  if (BWD) input(p.grad_y, p.grad_stride);
-  if (p.residual) input(p.residual, p.residual_stride);
-  s.inputs = n;
-  s.slot_row = (p.width * (int)sizeof(T) + 15) / 16 * 16 + 16;
-  // The ring takes what the CTA's share of an SM's shared memory leaves.
-  const int room = 220 * 1024 / staged_resident<E, BWD>() - 2048 - (E == 8 ? 0 : (BWD ? 4 : 8) * p.width);
-  s.slots = std::min(8, room / (s.inputs * s.slot_row));
-  if (s.slots < 1) s.slots = 1;
-  const int smem = s.slots * s.inputs * s.slot_row + (E == 8 ? 0 : (BWD ? 4 : 8) * p.width);
-  static std::atomic<uint64_t> set{0};
-  cudaError_t e = allow_smem(norm_staged_kernel<T, VEC, NV, BWD>, 220 * 1024, set);
-  if (e != cudaSuccess) return e;
-  norm_staged_kernel<T, VEC, NV, BWD><<<grid, kNormThreads, smem, st>>>(p, s);
-  return cudaGetLastError();
 }
 
 template <typename T>
 cudaError_t norm_launch(const NormParams& p, const NormShape& s, bool backward, int grid, cudaStream_t st) {
-  if (s.wide) {
+  if (p.width > kRegisterWidth) {
     if (!backward) {
       norm_wide_fwd_kernel<T><<<grid, kWideThreads, 0, st>>>(p);
     } else {
@@ -620,26 +449,22 @@ cudaError_t norm_launch(const NormParams& p, const NormShape& s, bool backward, 
     }
     return cudaGetLastError();
   }
-#define MSDA_NORM(VEC_, NV_)                                                                 \
-  if (!s.staged && s.vec == VEC_ && s.nv == NV_) {                                           \
-    if (backward) norm_bwd_kernel<T, VEC_, NV_><<<grid, kNormThreads, 0, st>>>(p);           \
-    else norm_fwd_kernel<T, VEC_, NV_><<<grid, kNormThreads, 0, st>>>(p);                    \
-    return cudaGetLastError();                                                               \
+#define MSDA_NORM(VEC_, NV_, TPR_)                                                                  \
+  if (s.vec == VEC_ && s.nv == NV_ && s.tpr == TPR_) {                                              \
+    if (backward) norm_bwd_kernel<T, VEC_, NV_, TPR_><<<grid, norm_threads<TPR_>(), 0, st>>>(p);    \
+    else norm_fwd_kernel<T, VEC_, NV_, TPR_><<<grid, norm_threads<TPR_>(), 0, st>>>(p);             \
+    return cudaGetLastError();                                                                      \
   }
-#define MSDA_NORM_STAGED(VEC_, NV_)                                                          \
-  if (s.staged && s.vec == VEC_ && s.nv == NV_)                                              \
-    return backward ? staged_launch<T, VEC_, NV_, true>(p, grid, st) : staged_launch<T, VEC_, NV_, false>(p, grid, st);
-#define MSDA_NORM_VEC(VEC_)                                                                  \
-  MSDA_NORM(VEC_, 8 / (VEC_)) MSDA_NORM(VEC_, 16 / (VEC_)) MSDA_NORM_STAGED(VEC_, 8 / (VEC_)) \
-  MSDA_NORM_STAGED(VEC_, 16 / (VEC_)) MSDA_NORM_STAGED(VEC_, 32 / (VEC_))
+#define MSDA_NORM_VEC(VEC_)                                                                         \
+  MSDA_NORM(VEC_, 8 / (VEC_), 32) MSDA_NORM(VEC_, 16 / (VEC_), 32) MSDA_NORM(VEC_, 8 / (VEC_), 128) \
+  MSDA_NORM(VEC_, 8 / (VEC_), 256) MSDA_NORM(VEC_, 8 / (VEC_), 512) MSDA_NORM(VEC_, 16 / (VEC_), 512)
   MSDA_NORM_VEC(16 / (int)sizeof(T))
   if constexpr (sizeof(T) == 2) {
     MSDA_NORM_VEC(2)
   }
-  MSDA_NORM(1, 1)
+  MSDA_NORM(1, 1, 32)
   MSDA_NORM_VEC(1)
 #undef MSDA_NORM_VEC
-#undef MSDA_NORM_STAGED
 #undef MSDA_NORM
   return cudaErrorInvalidConfiguration;
 }
@@ -704,7 +529,7 @@ int msda_layer_norm_forward(const void* x, const void* residual, const void* wei
   p.mean = mean, p.rstd = rstd;
   p.rows = rows, p.width = (int32_t)width, p.x_stride = x_stride, p.residual_stride = residual_stride, p.eps = eps;
   p.param_f32 = param_dtype == MSDA_DTYPE_F32;
-  const NormShape s = norm_shape(width, es, u.unit, aligned(x, 16) && aligned(residual, 16));
+  const NormShape s = norm_shape(width, es, u.unit);
   const int grid = norm_grid(rows, s, false, width);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e = dtype == MSDA_DTYPE_F32   ? norm_launch<float>(p, s, false, grid, st)
@@ -762,7 +587,7 @@ int msda_layer_norm_backward(const void* x, const void* residual, const void* we
   p.rows = rows, p.width = (int32_t)width, p.x_stride = x_stride, p.residual_stride = residual_stride;
   p.grad_stride = grad_stride;
   p.param_f32 = param_dtype == MSDA_DTYPE_F32, p.want_columns = columns;
-  const NormShape s = norm_shape(width, es, u.unit, aligned(x, 16) && aligned(residual, 16) && aligned(grad_y, 16));
+  const NormShape s = norm_shape(width, es, u.unit);
   const int grid = norm_grid(rows, s, true, width);
   cudaError_t e = dtype == MSDA_DTYPE_F32   ? norm_launch<float>(p, s, true, grid, st)
                   : dtype == MSDA_DTYPE_F16 ? norm_launch<__half>(p, s, true, grid, st)
