@@ -44,39 +44,67 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 
-// Scores of a thread's row to base 2 (all but a plain scale, which is folded
-// into the exponent): cap and distance bias. t2 (BWD): 1 - tanh^2.
-template <int N, bool BWD>
-__device__ __forceinline__ void shape_scores(const AttnParams& p, const ScoreForm& f, float (&s)[N], float (&t2)[BWD ? N : 1]) {
-  if (p.cap != 0.0f) {
-    float big = 0.0f;
+// Two fp32 values in a register pair: one instruction does both.
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) { return f2_pack(lo, hi); }
+__device__ __forceinline__ uint64_t pair_mul(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t pair_add(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// A row's largest value: four chains.
+template <int N>
+__device__ __forceinline__ float row_max(const float (&s)[N]) {
+  float m0 = s[0], m1 = s[1], m2 = s[2], m3 = s[3];
 #pragma unroll
-    for (int c = 0; c < N; ++c) {
-      s[c] *= f.inv_cap;
-      big = fmaxf(big, fabsf(s[c]));
+  for (int c = 4; c < N; c += 8) {
+    m0 = fmaxf(fmaxf(m0, s[c]), s[c + 4 < N ? c + 4 : c]);
+    m1 = fmaxf(fmaxf(m1, s[c + 1]), s[c + 4 < N ? c + 5 : c]);
+    m2 = fmaxf(fmaxf(m2, s[c + 2]), s[c + 4 < N ? c + 6 : c]);
+    m3 = fmaxf(fmaxf(m3, s[c + 3]), s[c + 4 < N ? c + 7 : c]);
+  }
+  return fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
+}
+
+// Scores of a thread's row to base 2, capped: cap2 tanh(inv_cap s). Well below
+// the cap, the common case, by tanh_small's polynomial with the factors worked
+// into its coefficients, two columns an instruction; else one by one.
+template <int N>
+__device__ __forceinline__ void cap_scores(const ScoreForm& f, float (&s)[N]) {
+  const float i2 = f.inv_cap * f.inv_cap;
+  float top0 = 0.0f, top1 = 0.0f;
+#pragma unroll
+  for (int c = 0; c < N; c += 2) top0 = fmaxf(top0, fabsf(s[c])), top1 = fmaxf(top1, fabsf(s[c + 1]));
+  if (__all_sync(kFullMask, fmaxf(top0, top1) * fabsf(f.inv_cap) < kTanhSmall)) {
+    const float unit = f.cap2 * f.inv_cap;
+    const uint64_t k = pair_of(unit, unit);
+    uint64_t a[5];
+    float factor = i2;
+    const float poly[5] = {-0.3333306908607483f, 0.13326521217823029f, -0.0533902570605278f, 0.019664911553263664f,
+                           -0.004769488703459501f};
+#pragma unroll
+    for (int i = 0; i < 5; ++i) {
+      a[i] = pair_of(poly[i] * factor, poly[i] * factor);
+      factor *= i2;
     }
-    // Scores well below the cap, the common case, need no exponential.
-    if (__all_sync(kFullMask, big < kTanhSmall)) {
 #pragma unroll
-      for (int c = 0; c < N; ++c) {
-        const float t = tanh_small(s[c]);
-        if constexpr (BWD) t2[c] = fmaf(-t, t, 1.0f);
-        s[c] = t * f.cap2;
-      }
-    } else {
-#pragma unroll
-      for (int c = 0; c < N; ++c) {
-        const float t = tanh_of(s[c]);
-        if constexpr (BWD) t2[c] = fmaf(-t, t, 1.0f);
-        s[c] = t * f.cap2;
-      }
+    for (int c = 0; c < N; c += 2) {
+      const uint64_t x = pair_of(s[c], s[c + 1]), y = pair_mul(x, x), u = pair_mul(x, k);
+      uint64_t r = f2_fma(a[4], y, a[3]);
+      r = f2_fma(r, y, a[2]);
+      r = f2_fma(r, y, a[1]);
+      r = f2_fma(r, y, a[0]);
+      r = f2_fma(pair_mul(u, y), r, u);
+      f2_unpack(r, s[c], s[c + 1]);
     }
   } else {
 #pragma unroll
-    for (int c = 0; c < N; ++c) {
-      if constexpr (BWD) t2[c] = 1.0f;
-      s[c] *= f.scale2;
-    }
+    for (int c = 0; c < N; ++c) s[c] = tanh_of(s[c] * f.inv_cap) * f.cap2;
   }
 }
 
@@ -142,7 +170,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   char* sq = smem;
   char* ring = smem + 2 * Shape::kTile;
-  __shared__ uint64_t q_full, kv_full[NS], kv_empty[NS], s_full[2], p_full[2], o_full;
+  __shared__ uint64_t q_full, kv_full[NS], kv_empty[NS], s_full[2], p_half[2], p_full[2], o_full;
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   volatile int* abort = &abort_flag;
@@ -157,7 +185,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     bar_init(&q_full, 1);
     bar_init(&o_full, 1);
     for (int i = 0; i < NS; ++i) bar_init(&kv_full[i], 1), bar_init(&kv_empty[i], 1);
-    for (int i = 0; i < 2; ++i) bar_init(&s_full[i], 1), bar_init(&p_full[i], kSoftmaxThreads / 2);
+    for (int i = 0; i < 2; ++i) bar_init(&s_full[i], 1), bar_init(&p_half[i], 4), bar_init(&p_full[i], 4);
     fence_async_smem();
   }
   if (warp == kMmaWarp) tmem_alloc<512>(&tmem_slot);
@@ -191,14 +219,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int j0 = j * kTileTokens;
       float factor = f.scale2;
       if constexpr (MODS) {
-        float none[1];
-        shape_scores<128, false>(p, f, s, none);
+        if (p.cap != 0.0f) {
+          cap_scores(f, s);
+          factor = 1.0f;
+        }
         if (p.slopes) {
           const float far = (float)(row.place - j0);
 #pragma unroll
-          for (int c = 0; c < 128; ++c) s[c] = fmaf(-f.slope2, fabsf(far - (float)c), s[c]);
+          for (int c = 0; c < 128; ++c) s[c] = fmaf(-f.slope2, fabsf(far - (float)c), s[c] * factor);
+          factor = 1.0f;
         }
-        factor = 1.0f;
       }
       const int seen = row.limit - j0;
       if (!__all_sync(kFullMask, seen >= 128)) {
@@ -214,19 +244,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!same_document(row.doc, __shfl_sync(kFullMask, mine, c), p.shared)) s[q * 32 + c] = -INFINITY;
         }
       }
-      float top0 = s[0], top1 = s[1];
+      if (factor <= 0.0f) {  // a negative scale: its own factor now, so that the largest score is the largest value
 #pragma unroll
-      for (int c = 2; c < 128; c += 2) top0 = fmaxf(top0, s[c]), top1 = fmaxf(top1, s[c + 1]);
-      // The largest scaled score: for a negative scale the largest comes from the smallest.
-      float top = fmaxf(top0, top1) * factor;
-      if constexpr (!MODS) {
-        if (factor <= 0.0f) {
-          top = -INFINITY;
-#pragma unroll
-          for (int c = 0; c < 128; ++c)
-            if (s[c] != -INFINITY) top = fmaxf(top, s[c] * factor);
-        }
+        for (int c = 0; c < 128; ++c) s[c] = s[c] == -INFINITY ? -INFINITY : s[c] * factor;
+        factor = 1.0f;
       }
+      const float top = row_max(s) * factor;
       // The reference maximum moves only when a row has grown by 2^8 past it, so
       // that the sums in TMEM are seldom rescaled; 2^8 is far from overflow.
       if (__any_sync(kFullMask, top > m + kSlack)) {
@@ -246,26 +269,33 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      const float base = m == -INFINITY ? 0.0f : m;
-      float sum0 = 0.0f, sum1 = 0.0f;
-      const bool flip = !MODS && factor <= 0.0f;  // -inf marks must stay so
+      const float base = m == -INFINITY ? 0.0f : -m;
+      const uint64_t factor2 = pair_of(factor, factor), base2 = pair_of(base, base);
+      uint64_t sum0 = 0, sum1 = 0;  // pairs of zeros
+      // The first half of the keys goes to the products ahead of the second.
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         uint32_t packed[32];
 #pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          const float a = s[half * 64 + 2 * c], d = s[half * 64 + 2 * c + 1];
-          float e0 = ex2(fmaf(a, factor, -base)), e1 = ex2(fmaf(d, factor, -base));
-          if (flip) e0 = a == -INFINITY ? 0.0f : e0, e1 = d == -INFINITY ? 0.0f : e1;
-          sum0 += e0, sum1 += e1;
+        for (int c = 0; c < 32; c += 2) {
+          float e0, e1, e2, e3;
+          f2_unpack(f2_fma(pair_of(s[half * 64 + 2 * c], s[half * 64 + 2 * c + 1]), factor2, base2), e0, e1);
+          f2_unpack(f2_fma(pair_of(s[half * 64 + 2 * c + 2], s[half * 64 + 2 * c + 3]), factor2, base2), e2, e3);
+          e0 = ex2(e0), e1 = ex2(e1), e2 = ex2(e2), e3 = ex2(e3);
+          sum0 = pair_add(sum0, pair_of(e0, e1)), sum1 = pair_add(sum1, pair_of(e2, e3));
           packed[c] = pack_pair<T>(e0, e1);
+          packed[c + 1] = pack_pair<T>(e2, e3);
         }
         tmem_store32(s_at + half * 32, packed);
+        tmem_wait_store();
+        fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(half ? &p_full[t] : &p_half[t]);
       }
-      l += sum0 + sum1;
-      tmem_wait_store();
-      fence_before();
-      bar_arrive(&p_full[t]);
+      float part[4];
+      f2_unpack(sum0, part[0], part[1]);
+      f2_unpack(sum1, part[2], part[3]);
+      l += (part[0] + part[1]) + (part[2] + part[3]);
       ++count;
     }
     if (ok && count > 0) ok = warp_wait(&o_full, 0, abort);
@@ -348,11 +378,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int t = 0; t < 2 && ok; ++t) {
           if (prev >= 0) {
-            ok = warp_wait(&p_full[t], (count - 1) & 1, abort);
+            for (int half = 0; half < 2 && ok; ++half) {
+              ok = warp_wait(half ? &p_full[t] : &p_half[t], (count - 1) & 1, abort);
+              fence_after();
+              if (ok && elect_one())
+                product_half(tmem + 256 + t * DP, tmem + t * 128 + half * 32, ring_addr + prev_slot * Shape::kTile, half, dv, count > 1);
+              __syncwarp();
+            }
             if (!ok) break;
-            fence_after();
-            if (elect_one()) product_tokens(tmem + 256 + t * DP, tmem + t * 128, 32, ring_addr + prev_slot * Shape::kTile, dv, count > 1);
-            __syncwarp();
           }
           if (elect_one()) {
             if (j < tiles) product_channels<DP>(tmem + t * 128, q_addr + t * Shape::kTile, ring_addr + k_slot * Shape::kTile, ds);
@@ -399,25 +432,63 @@ struct BwdShape {
   static constexpr int kSmem = 1024 + 6 * kTile;  // two tiles that stay, two stages of two
 };
 
-// A thread's 64 probabilities from its scores (in place), where row or column
-// masks leave them; `t2` the cap's derivative. seen(c): what the masks say.
-template <bool MODS, typename Seen, typename Far, typename Lse>
-__device__ __forceinline__ void probabilities(const AttnParams& p, const ScoreForm& f, float (&s)[64], float (&t2)[MODS ? 64 : 1],
-                                              bool all, Seen seen, Far far, Lse lse2) {
+// A thread's 64 probabilities from its scores, in place; with a cap its
+// derivative 1 - tanh^2 in t2. far(c): places between query and key; lse(c, i):
+// minus the log-sum-exp, to base 2, of columns c and c + 1 (i = 0) or c + 2 and
+// c + 3.
+template <bool MODS, typename Far, typename Lse>
+__device__ __forceinline__ void probabilities(const AttnParams& p, const ScoreForm& f, float (&s)[64], float (&t2)[MODS ? 64 : 2],
+                                              Far far, Lse lse) {
   float factor = f.scale2;
   if constexpr (MODS) {
-    shape_scores<64, true>(p, f, s, t2);
+    if (p.cap != 0.0f) {
+      cap_scores(f, s);
+      const float inv = -1.0f / (f.cap2 * f.cap2);
+      const uint64_t inv2 = pair_of(inv, inv), one = pair_of(1.0f, 1.0f);
+#pragma unroll
+      for (int c = 0; c < 64; c += 2) {
+        const uint64_t x = pair_of(s[c], s[c + 1]);
+        f2_unpack(f2_fma(pair_mul(x, x), inv2, one), t2[c], t2[c + 1]);
+      }
+      factor = 1.0f;
+    }
     if (p.slopes) {
 #pragma unroll
-      for (int c = 0; c < 64; ++c) s[c] = fmaf(-f.slope2, fabsf(far(c)), s[c]);
+      for (int c = 0; c < 64; ++c) s[c] = fmaf(-f.slope2, fabsf(far(c)), s[c] * factor);
+      factor = 1.0f;
     }
-    factor = 1.0f;
   }
+  const uint64_t factor2 = pair_of(factor, factor);
 #pragma unroll
-  for (int c = 0; c < 64; ++c) s[c] = ex2(fmaf(s[c], factor, -lse2(c)));
-  if (!all) {
+  for (int c = 0; c < 64; c += 4) {
+    uint64_t l0, l1;
+    lse(c, l0, l1);
+    f2_unpack(f2_fma(pair_of(s[c], s[c + 1]), factor2, l0), s[c], s[c + 1]);
+    f2_unpack(f2_fma(pair_of(s[c + 2], s[c + 3]), factor2, l1), s[c + 2], s[c + 3]);
 #pragma unroll
-    for (int c = 0; c < 64; ++c) s[c] = seen(c) ? s[c] : 0.0f;
+    for (int e = 0; e < 4; ++e) s[c + e] = ex2(s[c + e]);
+  }
+}
+
+__device__ __forceinline__ void multiply(float (&s)[64], const float (&t)[64]) {
+#pragma unroll
+  for (int c = 0; c < 64; c += 2) f2_unpack(pair_mul(pair_of(s[c], s[c + 1]), pair_of(t[c], t[c + 1])), s[c], s[c + 1]);
+}
+
+// dp <- s (dp - delta); delta(c, ..): minus the columns' row sums, as lse above.
+// `clean`: masked columns (s = 0) stay 0 whatever dp holds there.
+template <typename Delta>
+__device__ __forceinline__ void derivatives(const float (&s)[64], float (&dp)[64], bool clean, Delta delta) {
+#pragma unroll
+  for (int c = 0; c < 64; c += 4) {
+    uint64_t d0, d1;
+    delta(c, d0, d1);
+    f2_unpack(pair_mul(pair_add(pair_of(dp[c], dp[c + 1]), d0), pair_of(s[c], s[c + 1])), dp[c], dp[c + 1]);
+    f2_unpack(pair_mul(pair_add(pair_of(dp[c + 2], dp[c + 3]), d1), pair_of(s[c + 2], s[c + 3])), dp[c + 2], dp[c + 3]);
+  }
+  if (clean) {
+#pragma unroll
+    for (int c = 0; c < 64; ++c) dp[c] = s[c] == 0.0f ? 0.0f : dp[c];
   }
 }
 
@@ -486,7 +557,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     bar_init(&done, 1);
     for (int i = 0; i < 2; ++i) bar_init(&kv_full[i], 1), bar_init(&kv_empty[i], 1), bar_init(&s_full[i], 1);
     bar_init(&dp_full, 1);
-    bar_init(&dp_empty, kSoftmaxThreads), bar_init(&ds_full, kSoftmaxThreads);
+    bar_init(&dp_empty, kSoftmaxThreads / 32), bar_init(&ds_full, kSoftmaxThreads / 32);
     fence_async_smem();
   }
   if (warp == kMmaWarp) tmem_alloc<512>(&tmem_slot);
@@ -529,7 +600,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     named_barrier(1, kSoftmaxThreads);
     delta = delta_part[0][r] + delta_part[1][r];
     if (in && half == 0) p.delta[stat] = delta;
-    const float lse2 = in && row.limit > 0 ? p.lse[stat] * kLog2e : 0.0f;
+    const float lse = in && row.limit > 0 ? p.lse[stat] * -kLog2e : 0.0f;
+    const uint64_t lse2 = pair_of(lse, lse), delta2 = pair_of(-delta, -delta);
     bool ok = true;
     int n = 0;
     for (int j = 0; j < tiles && ok; ++j) {
@@ -540,15 +612,24 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = warp_wait(&s_full[n % 2], (n / 2) & 1, abort);
       if (!ok) break;
       fence_after();
-      float s[64], t2[MODS ? 64 : 1];
+      float s[64], t2[MODS ? 64 : 2];
       tmem_load32(s_at, s);
       tmem_load32(s_at + 32, s + 32);
       tmem_wait_load();
       const int seen = row.limit - c0;
       const float away = (float)(row.place - c0);
-      probabilities<MODS>(p, f, s, t2, __all_sync(kFullMask, seen >= 64), [&](int c) { return c < seen; },
-                          [&](int c) { return away - (float)c; }, [&](int) { return lse2; });
+      probabilities<MODS>(p, f, s, t2, [&](int c) { return away - (float)c; }, [&](int, uint64_t& a, uint64_t& d) { a = d = lse2; });
+      if constexpr (MODS) {
+        if (p.cap != 0.0f) multiply(s, t2);
+      }
+      bool masked = false;
+      if (!__all_sync(kFullMask, seen >= 64)) {
+        masked = true;
+#pragma unroll
+        for (int c = 0; c < 64; ++c) s[c] = c < seen ? s[c] : 0.0f;
+      }
       if (!st.agree) {
+        masked = true;
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
           const int k = c0 + q * 32 + lane, mine = k < p.Sk ? __ldg(kdoc + k) : -1;
@@ -565,17 +646,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_load32(at + 256 + half * 64 + 32, dp + 32);
       tmem_wait_load();
       fence_before();
-      bar_arrive(&dp_empty);
-#pragma unroll
-      for (int c = 0; c < 64; ++c) {
-        float d = s[c] * (dp[c] - delta);
-        if constexpr (MODS) d *= t2[c];
-        dp[c] = s[c] == 0.0f ? 0.0f : d;  // also where what the masks hide is not finite
-      }
+      __syncwarp();
+      if (lane == 0) bar_arrive(&dp_empty);
+      derivatives(s, dp, masked, [&](int, uint64_t& a, uint64_t& d) { a = d = delta2; });
       store_row<T>(s_at, dp);
       tmem_wait_store();
       fence_before();
-      bar_arrive(&ds_full);
+      __syncwarp();
+      if (lane == 0) bar_arrive(&ds_full);
       ++n;
     }
     if (ok && n > 0) ok = warp_wait(&done, 0, abort);
@@ -671,8 +749,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // What a key-tile thread needs of each query of a tile.
-struct QueryStats {
-  float lse2[kTileTokens], delta[kTileTokens];
+struct __align__(16) QueryStats {
+  float lse[kTileTokens], delta[kTileTokens];  // negative; lse to base 2
   int limit[kTileTokens], place[kTileTokens], doc[kTileTokens];
 };
 
@@ -703,7 +781,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     bar_init(&done, 1);
     for (int i = 0; i < 2; ++i) bar_init(&q_full[i], 1), bar_init(&q_empty[i], 1);
     bar_init(&s_full, 1), bar_init(&dp_full, 1);
-    bar_init(&p_full, kSoftmaxThreads), bar_init(&ds_full, kSoftmaxThreads);
+    bar_init(&p_full, kSoftmaxThreads / 32), bar_init(&ds_full, kSoftmaxThreads / 32);
     fence_async_smem();
   }
   if (warp == kMmaWarp) tmem_alloc<512>(&tmem_slot);
@@ -734,8 +812,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const RowView row = row_view(p, b, i0 + r, length);
         const int64_t stat = ((int64_t)b * p.H + h) * p.Sq + i0 + r;
         if (half == 0) {
-          q.lse2[r] = row.limit > 0 ? p.lse[stat] * kLog2e : 0.0f;
-          q.delta[r] = row.limit > 0 ? p.delta[stat] : 0.0f;
+          q.lse[r] = row.limit > 0 ? p.lse[stat] * -kLog2e : 0.0f;
+          q.delta[r] = row.limit > 0 ? -p.delta[stat] : 0.0f;
         } else {
           q.limit[r] = row.limit, q.place[r] = row.place, q.doc[r] = row.doc;
         }
@@ -747,20 +825,47 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = ok && warp_wait(&s_full, n & 1, abort);
       if (!ok) continue;
       fence_after();
-      float s[64], t2[MODS ? 64 : 1];
+      float s[64], t2[MODS ? 64 : 2];
       tmem_load32(at, s);
       tmem_load32(at + 32, s + 32);
       tmem_wait_load();
       const int c0 = half * 64;
-      probabilities<MODS>(p, f, s, t2, whole,
-                          [&](int c) {
-                            return live && j < q.limit[c0 + c] && (!p.kdoc || same_document(q.doc[c0 + c], kd, p.shared));
-                          },
-                          [&](int c) { return (float)(q.place[c0 + c] - j); }, [&](int c) { return q.lse2[c0 + c]; });
+      const auto pairs = [&](const float* from, int c, uint64_t& a, uint64_t& d) {
+        const float4 v = *reinterpret_cast<const float4*>(from + c0 + c);
+        a = pair_of(v.x, v.y), d = pair_of(v.z, v.w);
+      };
+      probabilities<MODS>(p, f, s, t2, [&](int c) { return (float)(q.place[c0 + c] - j); },
+                          [&](int c, uint64_t& a, uint64_t& d) { pairs(q.lse, c, a, d); });
+      if (!whole) {
+#pragma unroll
+        for (int c = 0; c < 64; c += 4) {
+          const int4 limit = *reinterpret_cast<const int4*>(q.limit + c0 + c);
+          s[c] = live & (j < limit.x) ? s[c] : 0.0f;
+          s[c + 1] = live & (j < limit.y) ? s[c + 1] : 0.0f;
+          s[c + 2] = live & (j < limit.z) ? s[c + 2] : 0.0f;
+          s[c + 3] = live & (j < limit.w) ? s[c + 3] : 0.0f;
+        }
+        if (!st.agree) {
+          // A key of the shared document is of every query's; a padded key of none.
+          const bool any = kd >= 0 && kd == p.shared;
+#pragma unroll
+          for (int c = 0; c < 64; c += 4) {
+            const int4 doc = *reinterpret_cast<const int4*>(q.doc + c0 + c);
+            s[c] = (any | (doc.x == kd)) ? s[c] : 0.0f;
+            s[c + 1] = (any | (doc.y == kd)) ? s[c + 1] : 0.0f;
+            s[c + 2] = (any | (doc.z == kd)) ? s[c + 2] : 0.0f;
+            s[c + 3] = (any | (doc.w == kd)) ? s[c + 3] : 0.0f;
+          }
+        }
+      }
       store_row<T>(at, s);
       tmem_wait_store();
       fence_before();
-      bar_arrive(&p_full);
+      __syncwarp();
+      if (lane == 0) bar_arrive(&p_full);
+      if constexpr (MODS) {
+        if (p.cap != 0.0f) multiply(s, t2);
+      }
       ok = warp_wait(&dp_full, n & 1, abort);
       if (!ok) continue;
       fence_after();
@@ -768,16 +873,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_load32(at + 128, dp);
       tmem_load32(at + 160, dp + 32);
       tmem_wait_load();
-#pragma unroll
-      for (int c = 0; c < 64; ++c) {
-        float d = s[c] * (dp[c] - q.delta[c0 + c]);
-        if constexpr (MODS) d *= t2[c];
-        dp[c] = s[c] == 0.0f ? 0.0f : d;
-      }
+      derivatives(s, dp, !whole, [&](int c, uint64_t& a, uint64_t& d) { pairs(q.delta, c, a, d); });
       store_row<T>(at + 128, dp);
       tmem_wait_store();
       fence_before();
-      bar_arrive(&ds_full);
+      __syncwarp();
+      if (lane == 0) bar_arrive(&ds_full);
       ++n;
     }
     if (ok && n > 0) ok = warp_wait(&done, 0, abort);

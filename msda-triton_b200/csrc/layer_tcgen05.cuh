@@ -142,12 +142,16 @@ __device__ __forceinline__ void product_channels(uint32_t d, uint32_t a_tile, ui
   for (int k = 0; k < DP / 16; ++k) mma_ss(d, desc_channels(a_tile, k), desc_channels(b_tile, k), idesc, k > 0);
 }
 
-// d (128 x DP) += p . t over 128 tokens: p 16-bit in TMEM, tokens 0..63 from
-// column p, 64..127 from column p + high.
-__device__ __forceinline__ void product_tokens(uint32_t d, uint32_t p, int high, uint32_t tile, uint32_t idesc, bool add) {
+// d (128 x DP) += p . t over half of a tile's 128 tokens: p 16-bit in TMEM.
+__device__ __forceinline__ void product_half(uint32_t d, uint32_t p, uint32_t tile, int half, uint32_t idesc, bool add) {
 #pragma unroll
-  for (int k = 0; k < 8; ++k)
-    mma_ts(d, p + (k < 4 ? k * 8 : high + (k - 4) * 8), desc_tokens(tile, k), idesc, add || k > 0);
+  for (int k = 0; k < 4; ++k) mma_ts(d, p + k * 8, desc_tokens(tile, half * 4 + k), idesc, add || half || k > 0);
+}
+
+// The same over all of them: tokens 64... from column p + high.
+__device__ __forceinline__ void product_tokens(uint32_t d, uint32_t p, int high, uint32_t tile, uint32_t idesc, bool add) {
+  product_half(d, p, tile, 0, idesc, add);
+  product_half(d, p + high, tile, 1, idesc, add);
 }
 
 __device__ __forceinline__ void commit(uint64_t* bar) {
