@@ -147,11 +147,52 @@ __device__ __forceinline__ void clear_rows(char* tile, const int* doc, int first
   __syncwarp();
 }
 
+// The steps of 64 keys that a block of queries goes through: the halves of its
+// key tiles, less those that the limit or the documents leave out. Every role
+// walks them by itself.
+struct KeySteps {
+  int j, half, n;  // key tile, its half, the tile's number among those visited
+  int tiles, halves;  // key tiles below the limit; halves of the last of them
+  bool done;
+  TileState state;
+
+  __device__ __forceinline__ void seek(const AttnParams& p, int b, int i0, int rows, int length) {
+    if (!p.kdoc) {
+      done = j >= tiles;
+      state = TileState{false, true, j * kTileTokens + kTileTokens > length && length < p.Sk};
+      return;
+    }
+    for (;; ++j) {
+      done = j >= tiles;
+      if (done) return;
+      state = tile_state(p, b, i0, rows, j, length);
+      if (!state.skip) return;
+    }
+  }
+  __device__ __forceinline__ KeySteps(const AttnParams& p, int b, int i0, int rows, int limit, int length)
+      : j(0), half(0), n(0), tiles((limit + kTileTokens - 1) / kTileTokens), halves((limit - 1) % kTileTokens < 64 ? 1 : 2) {
+    seek(p, b, i0, rows, length);
+  }
+  __device__ __forceinline__ int count() const { return j + 1 == tiles ? halves : 2; }
+  __device__ __forceinline__ void next_tile(const AttnParams& p, int b, int i0, int rows, int length) {
+    half = 0, ++j, ++n;
+    seek(p, b, i0, rows, length);
+  }
+  __device__ __forceinline__ void advance(const AttnParams& p, int b, int i0, int rows, int length) {
+    if (half + 1 == count()) next_tile(p, b, i0, rows, length);
+    else half = 1;
+  }
+};
+
 // ---------------------------------------------------------------------------
-// Forward: 256 queries of a head a CTA, as two tiles that take turns: while one
-// tile's rows are exponentiated the tensor cores work on the other's products.
-// For 128 channels a key tile costs 2 x 1024 cycles of products and, on the
-// 16-a-cycle exponential units, 2 x 1024 cycles too.
+// Forward: 256 queries of a head a CTA, as two tiles of 128, each with two
+// buffers for the scores of 64 keys: while a buffer is exponentiated the other
+// one's scores are formed, so that the softmax waits for a product only where the
+// tensor cores are the bound. For 128 channels 64 keys cost the two tiles 1280
+// cycles of products (the scores' run at two thirds of their rate: 64 columns are
+// bound by shared memory) and 1024 of the exponential units, 16 a cycle. With one
+// buffer of 128 keys each, the softmax waited half of the time (8192 x 16 heads
+// x 128 channels, no mask: 662 us).
 // ---------------------------------------------------------------------------
 template <int DP>
 struct FwdShape {
@@ -160,8 +201,10 @@ struct FwdShape {
   static constexpr int kSmem = 1024 + (2 + kStages) * kTile;
 };
 
+constexpr int kFwdThreads = kSoftmaxThreads + 64;
+
 template <typename T, int DP, bool MODS>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kFwdThreads, 1)
     attn_tc_fwd_kernel(const AttnParams p, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                        const __grid_constant__ CUtensorMap vmap) {
   using Shape = FwdShape<DP>;
@@ -169,8 +212,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ char raw[];
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   char* sq = smem;
-  char* ring = smem + 2 * Shape::kTile;
-  __shared__ uint64_t q_full, kv_full[NS], kv_empty[NS], s_full[2], p_half[2], p_full[2], o_full;
+  char* ring = smem + 2 * Shape::kTile;  // slots: a visited tile's keys, then its values
+  __shared__ uint64_t q_full, kv_full[NS], kv_empty[NS], s_full[2][2], p_full[2][2], o_done[2][2], cleared;
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   volatile int* abort = &abort_flag;
@@ -179,44 +222,43 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int i0 = (gridDim.x - 1 - blockIdx.x) * 2 * kTileTokens;  // long causal rows first
   const int length = attn_length(p, b);
   const int limit = rows_limit(p, b, i0 + 2 * kTileTokens, length);
-  const int tiles = (limit + kTileTokens - 1) / kTileTokens;
   if (threadIdx.x == 0) {
     abort_flag = 0;
     bar_init(&q_full, 1);
-    bar_init(&o_full, 1);
+    bar_init(&cleared, 1);
     for (int i = 0; i < NS; ++i) bar_init(&kv_full[i], 1), bar_init(&kv_empty[i], 1);
-    for (int i = 0; i < 2; ++i) bar_init(&s_full[i], 1), bar_init(&p_half[i], 4), bar_init(&p_full[i], 4);
+    for (int t = 0; t < 2; ++t) {
+      for (int i = 0; i < 2; ++i) bar_init(&s_full[t][i], 1), bar_init(&p_full[t][i], 4), bar_init(&o_done[t][i], 1);
+    }
     fence_async_smem();
   }
   if (warp == kMmaWarp) tmem_alloc<512>(&tmem_slot);
   fence_before();
   __syncthreads();
   fence_after();
-  const uint32_t tmem = tmem_slot;
+  const uint32_t tmem = tmem_slot;  // scores: 128 t + 64 buffer; sums: 256 + DP t
 
   if (warp < kLoadWarp) {
-    take_registers();
     const int t = warp / 4, i = i0 + threadIdx.x;  // tile and query of this thread
     const uint32_t lanes = (uint32_t)(warp % 4) << 21;
-    const uint32_t s_at = tmem + lanes + t * 128, o_at = tmem + lanes + 256 + t * DP;
+    const uint32_t o_at = tmem + lanes + 256 + t * DP;
     const RowView row = row_view(p, b, i, length);
     const ScoreForm f = score_form(p, h);
     const int* kdoc = p.kdoc ? p.kdoc + (int64_t)b * p.Sk : nullptr;
     float m = -INFINITY, l = 0.0f;  // in base 2; m trails the maximum by at most kSlack
     constexpr float kSlack = 8.0f;
     bool ok = true;
-    int count = 0;
-    for (int j = 0; j < tiles && ok; ++j) {
-      const TileState st = tile_state(p, b, i0, 2, j, length);
-      if (st.skip) continue;
-      ok = warp_wait(&s_full[t], count & 1, abort);
+    int u = 0;
+    for (KeySteps at(p, b, i0, 2, limit, length); !at.done && ok; at.advance(p, b, i0, 2, length), ++u) {
+      const uint32_t s_at = tmem + lanes + t * 128 + (u & 1) * 64;
+      ok = warp_wait(&s_full[t][u & 1], (u >> 1) & 1, abort);
       if (!ok) break;
       fence_after();
-      float s[128];
-#pragma unroll
-      for (int c = 0; c < 128; c += 32) tmem_load32(s_at + c, s + c);
+      float s[64];
+      tmem_load32(s_at, s);
+      tmem_load32(s_at + 32, s + 32);
       tmem_wait_load();
-      const int j0 = j * kTileTokens;
+      const int j0 = at.j * kTileTokens + at.half * 64;
       float factor = f.scale2;
       if constexpr (MODS) {
         if (p.cap != 0.0f) {
@@ -226,19 +268,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (p.slopes) {
           const float far = (float)(row.place - j0);
 #pragma unroll
-          for (int c = 0; c < 128; ++c) s[c] = fmaf(-f.slope2, fabsf(far - (float)c), s[c] * factor);
+          for (int c = 0; c < 64; ++c) s[c] = fmaf(-f.slope2, fabsf(far - (float)c), s[c] * factor);
           factor = 1.0f;
         }
       }
       const int seen = row.limit - j0;
-      if (!__all_sync(kFullMask, seen >= 128)) {
+      if (!__all_sync(kFullMask, seen >= 64)) {
 #pragma unroll
-        for (int c = 0; c < 128; ++c) s[c] = c < seen ? s[c] : -INFINITY;
+        for (int c = 0; c < 64; ++c) s[c] = c < seen ? s[c] : -INFINITY;
       }
-      if (!st.agree) {
+      if (!at.state.agree) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int at = j0 + q * 32 + lane, mine = at < p.Sk ? __ldg(kdoc + at) : -1;
+        for (int q = 0; q < 2; ++q) {
+          const int k = j0 + q * 32 + lane, mine = k < p.Sk ? __ldg(kdoc + k) : -1;
 #pragma unroll
           for (int c = 0; c < 32; ++c)
             if (!same_document(row.doc, __shfl_sync(kFullMask, mine, c), p.shared)) s[q * 32 + c] = -INFINITY;
@@ -246,7 +288,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (factor <= 0.0f) {  // a negative scale: its own factor now, so that the largest score is the largest value
 #pragma unroll
-        for (int c = 0; c < 128; ++c) s[c] = s[c] == -INFINITY ? -INFINITY : s[c] * factor;
+        for (int c = 0; c < 64; ++c) s[c] = s[c] == -INFINITY ? -INFINITY : s[c] * factor;
         factor = 1.0f;
       }
       const float top = row_max(s) * factor;
@@ -257,7 +299,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float old = next == -INFINITY ? 1.0f : ex2(m - next);
         m = next;
         l *= old;
-        if (count > 0) {
+        if (u > 0) {
+          ok = warp_wait(&o_done[t][(u - 1) & 1], ((u - 1) >> 1) & 1, abort);
+          if (!ok) break;
+          fence_after();
 #pragma unroll
           for (int c = 0; c < DP; c += 32) {
             float o[32];
@@ -272,40 +317,35 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float base = m == -INFINITY ? 0.0f : -m;
       const uint64_t factor2 = pair_of(factor, factor), base2 = pair_of(base, base);
       uint64_t sum0 = 0, sum1 = 0;  // pairs of zeros
-      // The first half of the keys goes to the products ahead of the second.
+      uint32_t packed[32];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t packed[32];
-#pragma unroll
-        for (int c = 0; c < 32; c += 2) {
-          float e0, e1, e2, e3;
-          f2_unpack(f2_fma(pair_of(s[half * 64 + 2 * c], s[half * 64 + 2 * c + 1]), factor2, base2), e0, e1);
-          f2_unpack(f2_fma(pair_of(s[half * 64 + 2 * c + 2], s[half * 64 + 2 * c + 3]), factor2, base2), e2, e3);
-          e0 = ex2(e0), e1 = ex2(e1), e2 = ex2(e2), e3 = ex2(e3);
-          sum0 = pair_add(sum0, pair_of(e0, e1)), sum1 = pair_add(sum1, pair_of(e2, e3));
-          packed[c] = pack_pair<T>(e0, e1);
-          packed[c + 1] = pack_pair<T>(e2, e3);
-        }
-        tmem_store32(s_at + half * 32, packed);
-        tmem_wait_store();
-        fence_before();
-        __syncwarp();
-        if (lane == 0) bar_arrive(half ? &p_full[t] : &p_half[t]);
+      for (int c = 0; c < 32; c += 2) {
+        float e0, e1, e2, e3;
+        f2_unpack(f2_fma(pair_of(s[2 * c], s[2 * c + 1]), factor2, base2), e0, e1);
+        f2_unpack(f2_fma(pair_of(s[2 * c + 2], s[2 * c + 3]), factor2, base2), e2, e3);
+        e0 = ex2(e0), e1 = ex2(e1), e2 = ex2(e2), e3 = ex2(e3);
+        sum0 = pair_add(sum0, pair_of(e0, e1)), sum1 = pair_add(sum1, pair_of(e2, e3));
+        packed[c] = pack_pair<T>(e0, e1);
+        packed[c + 1] = pack_pair<T>(e2, e3);
       }
+      tmem_store32(s_at, packed);
+      tmem_wait_store();
+      fence_before();
+      __syncwarp();
+      if (lane == 0) bar_arrive(&p_full[t][u & 1]);
       float part[4];
       f2_unpack(sum0, part[0], part[1]);
       f2_unpack(sum1, part[2], part[3]);
       l += (part[0] + part[1]) + (part[2] + part[3]);
-      ++count;
     }
-    if (ok && count > 0) ok = warp_wait(&o_full, 0, abort);
+    if (ok && u > 0) ok = warp_wait(&o_done[t][(u - 1) & 1], ((u - 1) >> 1) & 1, abort);
     fence_after();
     const float mul = !ok ? NAN : l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
     const int64_t at = (((int64_t)b * p.Sq + i) * p.H + h) * p.D;
 #pragma unroll
     for (int c = 0; c < DP; c += 32) {
       float o[32];
-      if (count > 0) {
+      if (u > 0) {
         tmem_load32(o_at + c, o);
         tmem_wait_load();
       }
@@ -318,11 +358,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint32_t* lo = reinterpret_cast<uint32_t*>(&low);
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
-            const float a = count > 0 ? o[e + 2 * x] * mul : mul, d = count > 0 ? o[e + 2 * x + 1] * mul : mul;
+            const float a = u > 0 ? o[e + 2 * x] * mul : mul, d = u > 0 ? o[e + 2 * x + 1] * mul : mul;
             hi[x] = pack_pair<T>(a, d);
-            Pack<T, 2> u;
-            u.raw = hi[x];
-            lo[x] = pack_pair<T>(a - to_f32(u.e[0]), d - to_f32(u.e[1]));
+            Pack<T, 2> v;
+            v.raw = hi[x];
+            lo[x] = pack_pair<T>(a - to_f32(v.e[0]), d - to_f32(v.e[1]));
           }
           *reinterpret_cast<uint4*>(static_cast<T*>(p.o) + at + c + e) = high;
           if (p.residue) *reinterpret_cast<uint4*>(static_cast<T*>(p.residue) + at + c + e) = low;
@@ -332,82 +372,95 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (i < p.Sq && p.lse)
       p.lse[((int64_t)b * p.H + h) * p.Sq + i] = !ok ? NAN : l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
     fence_before();
-  } else {
-    leave_registers();
-    if (warp == kLoadWarp) {
-      int n = 0;  // ring slots filled
-      if (lane == 0 && tiles > 0) {
+  } else if (warp == kLoadWarp) {
+    const int* kdoc = p.kdoc ? p.kdoc + (int64_t)b * p.Sk : nullptr;
+    int n = 0;  // ring slots filled
+    bool ok = true;
+    if (limit > 0) {
+      if (lane == 0) {
         bar_expect(&q_full, 2 * Shape::kTile);
         tma_tile<DP>(sq, &qmap, &q_full, h, i0, b);
         tma_tile<DP>(sq + Shape::kTile, &qmap, &q_full, h, i0 + kTileTokens, b);
-        bool ok = true;
-        for (int j = 0; j < tiles && ok; ++j) {
-          if (tile_state(p, b, i0, 2, j, length).skip) continue;
-          for (int kv = 0; kv < 2 && ok; ++kv) {
-            const int slot = n % NS;
-            if (n >= NS) ok = bar_wait(&kv_empty[slot], (n / NS - 1) & 1, abort);
-            if (!ok) break;
-            bar_expect(&kv_full[slot], Shape::kTile);
-            tma_tile<DP>(ring + slot * Shape::kTile, kv ? &vmap : &kmap, &kv_full[slot], hk, j * kTileTokens, b);
-            ++n;
-          }
-        }
-        // Copies in flight end before the CTA does.
-        bar_wait(&q_full, 0, abort);
-        for (int i = max(0, n - NS); i < n; ++i) bar_wait(&kv_full[i % NS], (i / NS) & 1, abort);
       }
-    } else if (warp == kMmaWarp) {
-      constexpr uint32_t ds = instr_desc<IsBf16<T>::value>(128, false), dv = instr_desc<IsBf16<T>::value>(DP, true);
-      const uint32_t q_addr = smem_u32(sq), ring_addr = smem_u32(ring);
-      bool ok = tiles == 0 || warp_wait(&q_full, 0, abort);
-      int n = 0, prev = -1, prev_slot = 0, count = 0;  // prev: the tile whose scores were issued last
-      bool prev_padded = false;
-      for (int j = 0; j <= tiles && ok; ++j) {
-        TileState st{};
-        if (j < tiles) {
-          st = tile_state(p, b, i0, 2, j, length);
-          if (st.skip) continue;
-        }
-        const int k_slot = n % NS, v_slot = (n + 1) % NS;
-        // Scores of tile j after the values' product of the tile before, for each
-        // tile of queries in turn.
-        if (j < tiles) ok = warp_wait(&kv_full[k_slot], (n / NS) & 1, abort);
-        if (prev >= 0 && ok) {
-          ok = warp_wait(&kv_full[prev_slot], ((n - 1) / NS) & 1, abort);
-          if (prev_padded) clear_rows<DP>(ring + prev_slot * Shape::kTile, p.kdoc ? p.kdoc + (int64_t)b * p.Sk : nullptr, prev * kTileTokens, length);
-        }
-        for (int t = 0; t < 2 && ok; ++t) {
-          if (prev >= 0) {
-            for (int half = 0; half < 2 && ok; ++half) {
-              ok = warp_wait(half ? &p_full[t] : &p_half[t], (count - 1) & 1, abort);
-              fence_after();
-              if (ok && elect_one())
-                product_half(tmem + 256 + t * DP, tmem + t * 128 + half * 32, ring_addr + prev_slot * Shape::kTile, half, dv, count > 1);
-              __syncwarp();
-            }
-            if (!ok) break;
-          }
-          if (elect_one()) {
-            if (j < tiles) product_channels<DP>(tmem + t * 128, q_addr + t * Shape::kTile, ring_addr + k_slot * Shape::kTile, ds);
-            if (j < tiles) commit(&s_full[t]);
-            else if (t == 1) commit(&o_full);
+      for (KeySteps at(p, b, i0, 2, limit, length); !at.done && ok; at.next_tile(p, b, i0, 2, length)) {
+        for (int kv = 0; kv < 2 && ok; ++kv, ++n) {
+          const int slot = n % NS;
+          if (n >= NS) ok = warp_wait(&kv_empty[slot], (n / NS - 1) & 1, abort);
+          if (!ok) break;
+          if (lane == 0) {
+            bar_expect(&kv_full[slot], Shape::kTile);
+            tma_tile<DP>(ring + slot * Shape::kTile, kv ? &vmap : &kmap, &kv_full[slot], hk, at.j * kTileTokens, b);
           }
           __syncwarp();
+          if (kv && at.state.padded) {  // padded keys' values are cleared before their product
+            ok = warp_wait(&kv_full[slot], (n / NS) & 1, abort);
+            clear_rows<DP>(ring + slot * Shape::kTile, kdoc, at.j * kTileTokens, length);
+            if (lane == 0) bar_arrive(&cleared);
+          }
         }
-        if (ok && elect_one()) {
-          if (prev >= 0) commit(&kv_empty[prev_slot]);
-          if (j < tiles) commit(&kv_empty[k_slot]);
+      }
+      // Copies in flight end before the CTA does.
+      warp_wait(&q_full, 0, abort);
+      for (int i = max(0, n - NS); i < n; ++i) warp_wait(&kv_full[i % NS], (i / NS) & 1, abort);
+    }
+  } else if (elect_one()) {
+    // One thread issues: with its whole warp in step, the waits and elections
+    // between the products cost more than the products of small heads.
+    constexpr uint32_t ds = instr_desc<IsBf16<T>::value>(64, false), dv = instr_desc<IsBf16<T>::value>(DP, true);
+    constexpr uint64_t kHalfTile = 64 * 128 >> 4, kSlot = Shape::kTile >> 4;
+    const uint64_t q_desc = by_channels(smem_u32(sq)), k_desc = by_channels(smem_u32(ring)), v_desc = by_tokens(smem_u32(ring));
+    bool ok = limit == 0 || bar_wait(&q_full, 0, abort);
+    KeySteps at(p, b, i0, 2, limit, length);
+    int slot = 0, clears = 0;  // of the tile's keys; its values': the next
+    uint32_t phase = 0;
+    // Scores of both halves of the first tile; then the values' products of a
+    // tile's halves, each followed by the same half's scores of the next tile.
+    if (!at.done && ok) {
+      ok = bar_wait(&kv_full[0], 0, abort);
+      fence_after();
+      for (int half = 0; half < at.count() && ok; ++half)
+        for (int t = 0; t < 2; ++t) {
+          product_channels<DP>(tmem + t * 128 + half * 64, q_desc + t * kSlot, k_desc + half * kHalfTile, ds);
+          commit(&s_full[t][half]);
         }
-        __syncwarp();
-        prev = j, prev_slot = v_slot, prev_padded = st.padded;
-        n += 2;
-        ++count;
+      if (ok) commit(&kv_empty[0]);
+    }
+    while (!at.done && ok) {
+      const int count = at.count(), v_slot = slot + 1;
+      const uint32_t n = at.n & 1;
+      ok = bar_wait(&kv_full[v_slot], phase, abort);
+      if (ok && at.state.padded) ok = bar_wait(&cleared, clears++ & 1, abort);
+      const bool add = at.n > 0;
+      const uint64_t v = v_desc + v_slot * kSlot;
+      at.next_tile(p, b, i0, 2, length);
+      slot += 2;
+      if (slot == NS) slot = 0, phase ^= 1;
+      const int next = at.done ? 0 : at.count();
+      const uint64_t k = k_desc + slot * kSlot;
+      if (next && ok) ok = bar_wait(&kv_full[slot], phase, abort);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        if (half >= count || !ok) break;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          ok = ok && bar_wait(&p_full[t][half], n, abort);
+          fence_after();
+          if (!ok) break;
+          product_half(tmem + 256 + t * DP, tmem + t * 128 + half * 64, v + half * 4 * kTokenStep, dv, add || half > 0);
+          commit(&o_done[t][half]);
+          if (half < next) {
+            product_channels<DP>(tmem + t * 128 + half * 64, q_desc + t * kSlot, k + half * kHalfTile, ds);
+            commit(&s_full[t][half]);
+          }
+        }
       }
-      if (!ok) {
-        if (elect_one()) commit(&o_full);
-        __syncwarp();
-        warp_wait(&o_full, 0, abort);
-      }
+      if (!ok) break;
+      commit(&kv_empty[v_slot]);
+      if (next) commit(&kv_empty[slot]);
+    }
+    if (!ok) {
+      commit(&q_full);
+      bar_wait(&q_full, 1, abort);
     }
   }
   __syncthreads();
@@ -704,7 +757,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!ok) break;
           fence_after();
           if (elect_one()) {
-            product_channels<DP>(tmem + (n % 2) * 128, q_addr, slot, ds);
+            product_channels<DP>(tmem + (n % 2) * 128, by_channels(q_addr), by_channels(slot), ds);
             commit(&s_full[n % 2]);
           }
           __syncwarp();
@@ -712,7 +765,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!ok) break;
           fence_after();
           if (elect_one()) {
-            product_channels<DP>(tmem + 256, g_addr, slot + Shape::kTile, ds);
+            product_channels<DP>(tmem + 256, by_channels(g_addr), by_channels(slot + Shape::kTile), ds);
             commit(&dp_full);
           }
           __syncwarp();
@@ -725,7 +778,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             clear_rows<DP>(ring + slot * 2 * Shape::kTile, p.kdoc ? p.kdoc + (int64_t)b * p.Sk : nullptr, prev_j * kTileTokens, length);
           fence_after();
           if (elect_one()) {
-            product_tokens(tmem + 384, tmem + slot * 128, 64, ring_addr + slot * 2 * Shape::kTile, dd, n > 1);
+            product_tokens(tmem + 384, tmem + slot * 128, 64, by_tokens(ring_addr + slot * 2 * Shape::kTile), dd, n > 1);
             commit(&kv_empty[slot]);
             if (j == tiles) commit(&done);
           }
@@ -929,7 +982,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = warp_wait(&p_full, (n - 1) & 1, abort);
           if (!ok) break;
           fence_after();
-          if (elect_one()) product_tokens(tmem + 256, tmem, 64, prev + Shape::kTile, dd, n > 1);
+          if (elect_one()) product_tokens(tmem + 256, tmem, 64, by_tokens(prev + Shape::kTile), dd, n > 1);
           __syncwarp();
         }
         if (u < steps) {
@@ -946,7 +999,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           if (elect_one()) {
-            product_channels<DP>(tmem, k_addr, next, ds);
+            product_channels<DP>(tmem, by_channels(k_addr), by_channels(next), ds);
             commit(&s_full);
           }
           __syncwarp();
@@ -956,7 +1009,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!ok) break;
           fence_after();
           if (elect_one()) {
-            product_tokens(tmem + 384, tmem + 128, 64, prev, dd, n > 1);
+            product_tokens(tmem + 384, tmem + 128, 64, by_tokens(prev), dd, n > 1);
             commit(&q_empty[(n - 1) & 1]);
             if (u == steps) commit(&done);
           }
@@ -964,7 +1017,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (u < steps) {
           if (elect_one()) {
-            product_channels<DP>(tmem + 128, v_addr, next + Shape::kTile, ds);
+            product_channels<DP>(tmem + 128, by_channels(v_addr), by_channels(next + Shape::kTile), ds);
             commit(&dp_full);
           }
           __syncwarp();
@@ -997,7 +1050,7 @@ cudaError_t launch_fwd(const AttnParams& p, const CUtensorMap (&m)[4], cudaStrea
   cudaError_t e = abi::allow_smem(attn_tc_fwd_kernel<T, DP, MODS>, Shape::kSmem, set);
   if (e != cudaSuccess) return e;
   const dim3 grid((p.Sq + 2 * kTileTokens - 1) / (2 * kTileTokens), p.H, p.B);
-  attn_tc_fwd_kernel<T, DP, MODS><<<grid, kThreads, Shape::kSmem, st>>>(p, m[0], m[1], m[2]);
+  attn_tc_fwd_kernel<T, DP, MODS><<<grid, kFwdThreads, Shape::kSmem, st>>>(p, m[0], m[1], m[2]);
   return cudaGetLastError();
 }
 

@@ -105,15 +105,13 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead) {
          (uint64_t)2 << 61;
 }
 
-// Channels are the inner (contracted) dimension: step k takes 16 of them.
-__device__ __forceinline__ uint64_t desc_channels(uint32_t tile, int k) {
-  return smem_desc(tile + (k / 4) * kChunkBytes + (k % 4) * 32, 16);
-}
+// A tile as an operand whose contracted dimension is its channels, or its tokens.
+__device__ __forceinline__ uint64_t by_channels(uint32_t tile) { return smem_desc(tile, 16); }
+__device__ __forceinline__ uint64_t by_tokens(uint32_t tile) { return smem_desc(tile, kChunkBytes); }
 
-// Tokens are the inner dimension: step k takes 16 of them, all channels.
-__device__ __forceinline__ uint64_t desc_tokens(uint32_t tile, int k) {
-  return smem_desc(tile + k * 2048, kChunkBytes);
-}
+// What 16 channels, or 16 tokens, further on adds to the descriptor.
+constexpr uint64_t kTokenStep = 16 * 128 >> 4;
+__host__ __device__ constexpr uint64_t channel_offset(int k) { return (uint64_t)((k / 4) * kChunkBytes + (k % 4) * 32) >> 4; }
 
 // 128 x N product of 16-bit inputs with fp32 sums; outer_b: B's tokens are the
 // contracted dimension.
@@ -135,23 +133,23 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
       ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
 }
 
-// d (128 x 128) = a . b^T over DP channels, both tiles token-major.
+// d = a . b^T over DP channels of two tiles (by_channels).
 template <int DP>
-__device__ __forceinline__ void product_channels(uint32_t d, uint32_t a_tile, uint32_t b_tile, uint32_t idesc) {
+__device__ __forceinline__ void product_channels(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
 #pragma unroll
-  for (int k = 0; k < DP / 16; ++k) mma_ss(d, desc_channels(a_tile, k), desc_channels(b_tile, k), idesc, k > 0);
+  for (int k = 0; k < DP / 16; ++k) mma_ss(d, a + channel_offset(k), b + channel_offset(k), idesc, k > 0);
 }
 
-// d (128 x DP) += p . t over half of a tile's 128 tokens: p 16-bit in TMEM.
-__device__ __forceinline__ void product_half(uint32_t d, uint32_t p, uint32_t tile, int half, uint32_t idesc, bool add) {
+// d (128 x DP) += p . t over 64 tokens of a tile (by_tokens): p 16-bit in TMEM.
+__device__ __forceinline__ void product_half(uint32_t d, uint32_t p, uint64_t t, uint32_t idesc, bool add) {
 #pragma unroll
-  for (int k = 0; k < 4; ++k) mma_ts(d, p + k * 8, desc_tokens(tile, half * 4 + k), idesc, add || half || k > 0);
+  for (int k = 0; k < 4; ++k) mma_ts(d, p + k * 8, t + k * kTokenStep, idesc, add || k > 0);
 }
 
-// The same over all of them: tokens 64... from column p + high.
-__device__ __forceinline__ void product_tokens(uint32_t d, uint32_t p, int high, uint32_t tile, uint32_t idesc, bool add) {
-  product_half(d, p, tile, 0, idesc, add);
-  product_half(d, p + high, tile, 1, idesc, add);
+// The same over 128 tokens: tokens 64... of p from column p + high.
+__device__ __forceinline__ void product_tokens(uint32_t d, uint32_t p, int high, uint64_t t, uint32_t idesc, bool add) {
+  product_half(d, p, t, idesc, add);
+  product_half(d, p + high, t + 4 * kTokenStep, idesc, true);
 }
 
 __device__ __forceinline__ void commit(uint64_t* bar) {
