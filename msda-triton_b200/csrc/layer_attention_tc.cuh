@@ -147,9 +147,10 @@ __device__ __forceinline__ void clear_rows(char* tile, const int* doc, int first
   __syncwarp();
 }
 
-// The steps of 64 keys that a block of queries goes through: the halves of its
-// key tiles, less those that the limit or the documents leave out. Every role
-// walks them by itself.
+// The steps that a block of queries goes through: its key tiles, or with STEP 64
+// their halves, less what the limit or the documents leave out. Every role walks
+// them by itself.
+template <int STEP>
 struct KeySteps {
   int j, half, n;  // key tile, its half, the tile's number among those visited
   int tiles, halves;  // key tiles below the limit; halves of the last of them
@@ -170,10 +171,10 @@ struct KeySteps {
     }
   }
   __device__ __forceinline__ KeySteps(const AttnParams& p, int b, int i0, int rows, int limit, int length)
-      : j(0), half(0), n(0), tiles((limit + kTileTokens - 1) / kTileTokens), halves((limit - 1) % kTileTokens < 64 ? 1 : 2) {
+      : j(0), half(0), n(0), tiles((limit + kTileTokens - 1) / kTileTokens), halves(STEP == 128 || (limit - 1) % kTileTokens < 64 ? 1 : 2) {
     seek(p, b, i0, rows, length);
   }
-  __device__ __forceinline__ int count() const { return j + 1 == tiles ? halves : 2; }
+  __device__ __forceinline__ int count() const { return STEP == 128 || j + 1 == tiles ? halves : 2; }
   __device__ __forceinline__ void next_tile(const AttnParams& p, int b, int i0, int rows, int length) {
     half = 0, ++j, ++n;
     seek(p, b, i0, rows, length);
@@ -185,35 +186,42 @@ struct KeySteps {
 };
 
 // ---------------------------------------------------------------------------
-// Forward: 256 queries of a head a CTA, as two tiles of 128, each with two
-// buffers for the scores of 64 keys: while a buffer is exponentiated the other
-// one's scores are formed, so that the softmax waits for a product only where the
-// tensor cores are the bound. For 128 channels 64 keys cost the two tiles 1280
-// cycles of products (the scores' run at two thirds of their rate: 64 columns are
-// bound by shared memory) and 1024 of the exponential units, 16 a cycle. With one
-// buffer of 128 keys each, the softmax waited half of the time (8192 x 16 heads
-// x 128 channels, no mask: 662 us).
+// Forward: 256 queries of a head a CTA, as two tiles of 128 that take turns: while
+// one tile's rows are exponentiated the tensor cores work on the other's products.
+// Above 64 channels a step is 128 keys, 2 x 1024 cycles of products, and on the
+// 16-a-cycle exponential units 2 x 1024 cycles too; the sums take half of TMEM,
+// one CTA an SM. Up to 64 channels the exponentials are the bound, and what
+// counts is that warps are there to keep them busy: steps of 64 keys and half of
+// TMEM let two CTAs share an SM, four warps for each of its schedulers. (Two
+// buffers of 64 keys a tile with one CTA took 606 us and 544 us for 8192 x 16
+// heads of 128 and of 32 channels: products of 64 columns run at half rate, and
+// two warps left the exponential units idle for half of the time.)
 // ---------------------------------------------------------------------------
 template <int DP>
 struct FwdShape {
   static constexpr int kTile = tile_bytes<DP>();
-  static constexpr int kStages = DP > 64 ? 4 : 6;
+  static constexpr int kStages = 4;
   static constexpr int kSmem = 1024 + (2 + kStages) * kTile;
+  static constexpr int kStep = DP > 64 ? 128 : 64;
+  static constexpr int kCtas = DP > 64 ? 1 : 2;
+  // With 128 scores a thread the softmax takes registers from the other roles'
+  // warpgroup.
+  static constexpr bool kSplit = DP > 64;
+  static constexpr int kThreads = kSplit ? tc::kThreads : kSoftmaxThreads + 64;
+  static constexpr int kColumns = DP > 64 ? 512 : 256;
 };
 
-constexpr int kFwdThreads = kSoftmaxThreads + 64;
-
 template <typename T, int DP, bool MODS>
-__global__ void __launch_bounds__(kFwdThreads, 1)
+__global__ void __launch_bounds__(FwdShape<DP>::kThreads, FwdShape<DP>::kCtas)
     attn_tc_fwd_kernel(const AttnParams p, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                        const __grid_constant__ CUtensorMap vmap) {
   using Shape = FwdShape<DP>;
-  constexpr int NS = Shape::kStages;
+  constexpr int NS = Shape::kStages, STEP = Shape::kStep, OUT = 2 * STEP;  // OUT: first TMEM column of the sums
   extern __shared__ char raw[];
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   char* sq = smem;
   char* ring = smem + 2 * Shape::kTile;  // slots: a visited tile's keys, then its values
-  __shared__ uint64_t q_full, kv_full[NS], kv_empty[NS], s_full[2][2], p_full[2][2], o_done[2][2], cleared;
+  __shared__ uint64_t q_full, kv_full[NS], kv_empty[NS], s_full[2], p_full[2], o_full[2], cleared;
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   volatile int* abort = &abort_flag;
@@ -227,21 +235,20 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     bar_init(&q_full, 1);
     bar_init(&cleared, 1);
     for (int i = 0; i < NS; ++i) bar_init(&kv_full[i], 1), bar_init(&kv_empty[i], 1);
-    for (int t = 0; t < 2; ++t) {
-      for (int i = 0; i < 2; ++i) bar_init(&s_full[t][i], 1), bar_init(&p_full[t][i], 4), bar_init(&o_done[t][i], 1);
-    }
+    for (int t = 0; t < 2; ++t) bar_init(&s_full[t], 1), bar_init(&p_full[t], 4), bar_init(&o_full[t], 1);
     fence_async_smem();
   }
-  if (warp == kMmaWarp) tmem_alloc<512>(&tmem_slot);
+  if (warp == kMmaWarp) tmem_alloc<Shape::kColumns>(&tmem_slot);
   fence_before();
   __syncthreads();
   fence_after();
-  const uint32_t tmem = tmem_slot;  // scores: 128 t + 64 buffer; sums: 256 + DP t
+  const uint32_t tmem = tmem_slot;
 
   if (warp < kLoadWarp) {
+    if constexpr (Shape::kSplit) take_registers();
     const int t = warp / 4, i = i0 + threadIdx.x;  // tile and query of this thread
     const uint32_t lanes = (uint32_t)(warp % 4) << 21;
-    const uint32_t o_at = tmem + lanes + 256 + t * DP;
+    const uint32_t s_at = tmem + lanes + t * STEP, o_at = tmem + lanes + OUT + t * DP;
     const RowView row = row_view(p, b, i, length);
     const ScoreForm f = score_form(p, h);
     const int* kdoc = p.kdoc ? p.kdoc + (int64_t)b * p.Sk : nullptr;
@@ -249,14 +256,13 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     constexpr float kSlack = 8.0f;
     bool ok = true;
     int u = 0;
-    for (KeySteps at(p, b, i0, 2, limit, length); !at.done && ok; at.advance(p, b, i0, 2, length), ++u) {
-      const uint32_t s_at = tmem + lanes + t * 128 + (u & 1) * 64;
-      ok = warp_wait(&s_full[t][u & 1], (u >> 1) & 1, abort);
+    for (KeySteps<STEP> at(p, b, i0, 2, limit, length); !at.done && ok; at.advance(p, b, i0, 2, length), ++u) {
+      ok = warp_wait(&s_full[t], u & 1, abort);
       if (!ok) break;
       fence_after();
-      float s[64];
-      tmem_load32(s_at, s);
-      tmem_load32(s_at + 32, s + 32);
+      float s[STEP];
+#pragma unroll
+      for (int c = 0; c < STEP; c += 32) tmem_load32(s_at + c, s + c);
       tmem_wait_load();
       const int j0 = at.j * kTileTokens + at.half * 64;
       float factor = f.scale2;
@@ -268,18 +274,18 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         if (p.slopes) {
           const float far = (float)(row.place - j0);
 #pragma unroll
-          for (int c = 0; c < 64; ++c) s[c] = fmaf(-f.slope2, fabsf(far - (float)c), s[c] * factor);
+          for (int c = 0; c < STEP; ++c) s[c] = fmaf(-f.slope2, fabsf(far - (float)c), s[c] * factor);
           factor = 1.0f;
         }
       }
       const int seen = row.limit - j0;
-      if (!__all_sync(kFullMask, seen >= 64)) {
+      if (!__all_sync(kFullMask, seen >= STEP)) {
 #pragma unroll
-        for (int c = 0; c < 64; ++c) s[c] = c < seen ? s[c] : -INFINITY;
+        for (int c = 0; c < STEP; ++c) s[c] = c < seen ? s[c] : -INFINITY;
       }
       if (!at.state.agree) {
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
+        for (int q = 0; q < STEP / 32; ++q) {
           const int k = j0 + q * 32 + lane, mine = k < p.Sk ? __ldg(kdoc + k) : -1;
 #pragma unroll
           for (int c = 0; c < 32; ++c)
@@ -288,7 +294,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       }
       if (factor <= 0.0f) {  // a negative scale: its own factor now, so that the largest score is the largest value
 #pragma unroll
-        for (int c = 0; c < 64; ++c) s[c] = s[c] == -INFINITY ? -INFINITY : s[c] * factor;
+        for (int c = 0; c < STEP; ++c) s[c] = s[c] == -INFINITY ? -INFINITY : s[c] * factor;
         factor = 1.0f;
       }
       const float top = row_max(s) * factor;
@@ -300,45 +306,47 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         m = next;
         l *= old;
         if (u > 0) {
-          ok = warp_wait(&o_done[t][(u - 1) & 1], ((u - 1) >> 1) & 1, abort);
-          if (!ok) break;
-          fence_after();
-#pragma unroll
-          for (int c = 0; c < DP; c += 32) {
-            float o[32];
-            tmem_load32(o_at + c, o);
+          // The scores came after the product of the step before: the sums rest.
+#pragma unroll 1
+          for (int c = 0; c < DP; c += 8) {
+            float o[8];
+            tmem_load8(o_at + c, o);
             tmem_wait_load();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] *= old;
-            tmem_store32(o_at + c, reinterpret_cast<uint32_t*>(o));
+            for (int e = 0; e < 8; ++e) o[e] *= old;
+            tmem_store8(o_at + c, reinterpret_cast<uint32_t*>(o));
           }
         }
       }
       const float base = m == -INFINITY ? 0.0f : -m;
       const uint64_t factor2 = pair_of(factor, factor), base2 = pair_of(base, base);
       uint64_t sum0 = 0, sum1 = 0;  // pairs of zeros
-      uint32_t packed[32];
 #pragma unroll
-      for (int c = 0; c < 32; c += 2) {
-        float e0, e1, e2, e3;
-        f2_unpack(f2_fma(pair_of(s[2 * c], s[2 * c + 1]), factor2, base2), e0, e1);
-        f2_unpack(f2_fma(pair_of(s[2 * c + 2], s[2 * c + 3]), factor2, base2), e2, e3);
-        e0 = ex2(e0), e1 = ex2(e1), e2 = ex2(e2), e3 = ex2(e3);
-        sum0 = pair_add(sum0, pair_of(e0, e1)), sum1 = pair_add(sum1, pair_of(e2, e3));
-        packed[c] = pack_pair<T>(e0, e1);
-        packed[c + 1] = pack_pair<T>(e2, e3);
+      for (int from = 0; from < STEP; from += 32) {
+        uint32_t packed[16];
+#pragma unroll
+        for (int c = 0; c < 16; c += 2) {
+          const float* x = s + from + 2 * c;
+          float e0, e1, e2, e3;
+          f2_unpack(f2_fma(pair_of(x[0], x[1]), factor2, base2), e0, e1);
+          f2_unpack(f2_fma(pair_of(x[2], x[3]), factor2, base2), e2, e3);
+          e0 = ex2(e0), e1 = ex2(e1), e2 = ex2(e2), e3 = ex2(e3);
+          sum0 = pair_add(sum0, pair_of(e0, e1)), sum1 = pair_add(sum1, pair_of(e2, e3));
+          packed[c] = pack_pair<T>(e0, e1);
+          packed[c + 1] = pack_pair<T>(e2, e3);
+        }
+        tmem_store16(s_at + from / 2, packed);
       }
-      tmem_store32(s_at, packed);
       tmem_wait_store();
       fence_before();
       __syncwarp();
-      if (lane == 0) bar_arrive(&p_full[t][u & 1]);
+      if (lane == 0) bar_arrive(&p_full[t]);
       float part[4];
       f2_unpack(sum0, part[0], part[1]);
       f2_unpack(sum1, part[2], part[3]);
       l += (part[0] + part[1]) + (part[2] + part[3]);
     }
-    if (ok && u > 0) ok = warp_wait(&o_done[t][(u - 1) & 1], ((u - 1) >> 1) & 1, abort);
+    if (ok && u > 0) ok = warp_wait(&o_full[t], 0, abort);
     fence_after();
     const float mul = !ok ? NAN : l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
     const int64_t at = (((int64_t)b * p.Sq + i) * p.H + h) * p.D;
@@ -372,7 +380,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     if (i < p.Sq && p.lse)
       p.lse[((int64_t)b * p.H + h) * p.Sq + i] = !ok ? NAN : l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
     fence_before();
-  } else if (warp == kLoadWarp) {
+  } else {
+    if constexpr (Shape::kSplit) leave_registers();
+    if (warp == kLoadWarp) {
     const int* kdoc = p.kdoc ? p.kdoc + (int64_t)b * p.Sk : nullptr;
     int n = 0;  // ring slots filled
     bool ok = true;
@@ -382,7 +392,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         tma_tile<DP>(sq, &qmap, &q_full, h, i0, b);
         tma_tile<DP>(sq + Shape::kTile, &qmap, &q_full, h, i0 + kTileTokens, b);
       }
-      for (KeySteps at(p, b, i0, 2, limit, length); !at.done && ok; at.next_tile(p, b, i0, 2, length)) {
+      for (KeySteps<STEP> at(p, b, i0, 2, limit, length); !at.done && ok; at.next_tile(p, b, i0, 2, length)) {
         for (int kv = 0; kv < 2 && ok; ++kv, ++n) {
           const int slot = n % NS;
           if (n >= NS) ok = warp_wait(&kv_empty[slot], (n / NS - 1) & 1, abort);
@@ -403,70 +413,71 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       warp_wait(&q_full, 0, abort);
       for (int i = max(0, n - NS); i < n; ++i) warp_wait(&kv_full[i % NS], (i / NS) & 1, abort);
     }
-  } else if (elect_one()) {
+    } else if (warp == kMmaWarp && elect_one()) {
     // One thread issues: with its whole warp in step, the waits and elections
     // between the products cost more than the products of small heads.
-    constexpr uint32_t ds = instr_desc<IsBf16<T>::value>(64, false), dv = instr_desc<IsBf16<T>::value>(DP, true);
+    constexpr uint32_t ds = instr_desc<IsBf16<T>::value>(STEP, false), dv = instr_desc<IsBf16<T>::value>(DP, true);
     constexpr uint64_t kHalfTile = 64 * 128 >> 4, kSlot = Shape::kTile >> 4;
     const uint64_t q_desc = by_channels(smem_u32(sq)), k_desc = by_channels(smem_u32(ring)), v_desc = by_tokens(smem_u32(ring));
     bool ok = limit == 0 || bar_wait(&q_full, 0, abort);
-    KeySteps at(p, b, i0, 2, limit, length);
-    int slot = 0, clears = 0;  // of the tile's keys; its values': the next
-    uint32_t phase = 0;
-    // Scores of both halves of the first tile; then the values' products of a
-    // tile's halves, each followed by the same half's scores of the next tile.
+    KeySteps<STEP> at(p, b, i0, 2, limit, length);
+    int slot = 0, clears = 0;  // slot of the tile's keys; its values': the next
+    uint32_t phase = 0, turn = 0;
+    const auto scores = [&](int t, uint64_t k) {
+      product_channels<DP>(tmem + t * STEP, q_desc + t * kSlot, k, ds);
+      commit(&s_full[t]);
+    };
     if (!at.done && ok) {
       ok = bar_wait(&kv_full[0], 0, abort);
       fence_after();
-      for (int half = 0; half < at.count() && ok; ++half)
-        for (int t = 0; t < 2; ++t) {
-          product_channels<DP>(tmem + t * 128 + half * 64, q_desc + t * kSlot, k_desc + half * kHalfTile, ds);
-          commit(&s_full[t][half]);
-        }
-      if (ok) commit(&kv_empty[0]);
+      if (ok) {
+        scores(0, k_desc);
+        scores(1, k_desc);
+        if (at.count() == 1) commit(&kv_empty[0]);
+      }
     }
+    bool add = false;
     while (!at.done && ok) {
-      const int count = at.count(), v_slot = slot + 1;
-      const uint32_t n = at.n & 1;
+      const int count = at.count(), k_slot = slot, v_slot = slot + 1;
+      const uint64_t v = v_desc + v_slot * kSlot;
       ok = bar_wait(&kv_full[v_slot], phase, abort);
       if (ok && at.state.padded) ok = bar_wait(&cleared, clears++ & 1, abort);
-      const bool add = at.n > 0;
-      const uint64_t v = v_desc + v_slot * kSlot;
       at.next_tile(p, b, i0, 2, length);
       slot += 2;
       if (slot == NS) slot = 0, phase ^= 1;
-      const int next = at.done ? 0 : at.count();
-      const uint64_t k = k_desc + slot * kSlot;
-      if (next && ok) ok = bar_wait(&kv_full[slot], phase, abort);
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        if (half >= count || !ok) break;
+      // A step's values' products, each followed by the next step's scores.
+      for (int half = 0; half < count && ok; ++half) {
+        const bool same = half + 1 < count, more = same || !at.done;
+        const uint64_t k = same ? k_desc + k_slot * kSlot + kHalfTile : k_desc + slot * kSlot;
+        if (!same && more) ok = bar_wait(&kv_full[slot], phase, abort);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          ok = ok && bar_wait(&p_full[t][half], n, abort);
+          ok = ok && bar_wait(&p_full[t], turn, abort);
           fence_after();
           if (!ok) break;
-          product_half(tmem + 256 + t * DP, tmem + t * 128 + half * 64, v + half * 4 * kTokenStep, dv, add || half > 0);
-          commit(&o_done[t][half]);
-          if (half < next) {
-            product_channels<DP>(tmem + t * 128 + half * 64, q_desc + t * kSlot, k + half * kHalfTile, ds);
-            commit(&s_full[t][half]);
-          }
+          product_half(tmem + OUT + t * DP, tmem + t * STEP, v + half * 4 * kTokenStep, dv, add);
+          if constexpr (STEP == 128) product_half(tmem + OUT + t * DP, tmem + t * STEP + 32, v + 4 * kTokenStep, dv, true);
+          if (more) scores(t, k);
+          else commit(&o_full[t]);
         }
+        add = true;
+        turn ^= 1;
+        if (!ok) break;
+        if (same) commit(&kv_empty[k_slot]);
+        else if (more && at.count() == 1) commit(&kv_empty[slot]);
       }
-      if (!ok) break;
-      commit(&kv_empty[v_slot]);
-      if (next) commit(&kv_empty[slot]);
+      if (ok) commit(&kv_empty[v_slot]);
     }
     if (!ok) {
       commit(&q_full);
       bar_wait(&q_full, 1, abort);
     }
+    }
   }
   __syncthreads();
   if (warp == kMmaWarp) {
     fence_after();
-    tmem_free<512>(tmem);
+    tmem_free<Shape::kColumns>(tmem);
   }
 }
 
@@ -1050,7 +1061,7 @@ cudaError_t launch_fwd(const AttnParams& p, const CUtensorMap (&m)[4], cudaStrea
   cudaError_t e = abi::allow_smem(attn_tc_fwd_kernel<T, DP, MODS>, Shape::kSmem, set);
   if (e != cudaSuccess) return e;
   const dim3 grid((p.Sq + 2 * kTileTokens - 1) / (2 * kTileTokens), p.H, p.B);
-  attn_tc_fwd_kernel<T, DP, MODS><<<grid, kFwdThreads, Shape::kSmem, st>>>(p, m[0], m[1], m[2]);
+  attn_tc_fwd_kernel<T, DP, MODS><<<grid, Shape::kThreads, Shape::kSmem, st>>>(p, m[0], m[1], m[2]);
   return cudaGetLastError();
 }
 
