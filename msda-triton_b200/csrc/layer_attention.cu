@@ -81,8 +81,8 @@ int check(const char* fn, const msda_attention_args* a, bool backward) {
     return fail(MSDA_ERR_INVALID_ARGUMENT, "%s: num_heads=%d must be a multiple of num_key_heads=%d", fn, a->num_heads, a->num_key_heads);
   if (a->head_dim < 1 || a->head_dim > MSDA_ATTENTION_MAX_HEAD_DIM)
     return fail(MSDA_ERR_UNSUPPORTED, "%s: head_dim=%d outside [1, %d]", fn, a->head_dim, MSDA_ATTENTION_MAX_HEAD_DIM);
-  if (a->batch > 65535 || a->num_heads > 4096 || a->num_queries > (1 << 24) || a->num_keys > (1 << 30))
-    return fail(MSDA_ERR_UNSUPPORTED, "%s: sizes exceed batch 65535, 4096 heads, 2^24 queries or 2^30 keys", fn);
+  if (a->batch > 65535 || a->num_heads > 4096 || a->num_queries > (1 << 22) || a->num_keys > (backward ? 1 << 22 : 1 << 30))
+    return fail(MSDA_ERR_UNSUPPORTED, "%s: sizes exceed batch 65535, 4096 heads, 2^22 queries or 2^30 keys (2^22 in the backward)", fn);
   if (!std::isfinite(a->scale) || !std::isfinite(a->softcap) || a->softcap < 0)
     return fail(MSDA_ERR_INVALID_ARGUMENT, "%s: scale must be finite, softcap finite and >= 0", fn);
   if (!a->query_documents != !a->key_documents)

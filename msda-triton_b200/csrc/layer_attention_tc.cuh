@@ -57,51 +57,69 @@ __device__ __forceinline__ uint64_t pair_add(uint64_t a, uint64_t b) {
   return r;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+  float r;
+  asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // A row's largest value: four chains.
 template <int N>
 __device__ __forceinline__ float row_max(const float (&s)[N]) {
-  float m0 = s[0], m1 = s[1], m2 = s[2], m3 = s[3];
+  float m[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-  for (int c = 4; c < N; c += 8) {
-    m0 = fmaxf(fmaxf(m0, s[c]), s[c + 4 < N ? c + 4 : c]);
-    m1 = fmaxf(fmaxf(m1, s[c + 1]), s[c + 4 < N ? c + 5 : c]);
-    m2 = fmaxf(fmaxf(m2, s[c + 2]), s[c + 4 < N ? c + 6 : c]);
-    m3 = fmaxf(fmaxf(m3, s[c + 3]), s[c + 4 < N ? c + 7 : c]);
-  }
-  return fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
+  for (int c = 0; c < N; c += 8)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m[i] = max3(m[i], s[c + i], s[c + 4 + i]);
+  return fmaxf(max3(m[0], m[1], m[2]), m[3]);
 }
 
-// Scores of a thread's row to base 2, capped: cap2 tanh(inv_cap s). Well below
-// the cap, the common case, by tanh_small's polynomial with the factors worked
-// into its coefficients, two columns an instruction; else one by one.
+// s <- cap2 tanh(inv_cap s) by an odd polynomial in inv_cap s, whose factors are
+// worked into the coefficients: two columns an instruction.
+template <int K, int N>
+__device__ __forceinline__ void cap_polynomial(const ScoreForm& f, const float (&poly)[K], float (&s)[N]) {
+  const float i2 = f.inv_cap * f.inv_cap, unit = f.cap2 * f.inv_cap;
+  const uint64_t k = pair_of(unit, unit);
+  uint64_t a[K];
+  float factor = i2;
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    a[i] = pair_of(poly[i] * factor, poly[i] * factor);
+    factor *= i2;
+  }
+#pragma unroll
+  for (int c = 0; c < N; c += 2) {
+    const uint64_t x = pair_of(s[c], s[c + 1]), y = pair_mul(x, x), u = pair_mul(x, k);
+    uint64_t r = a[K - 1];
+#pragma unroll
+    for (int i = K - 2; i >= 0; --i) r = f2_fma(r, y, a[i]);
+    f2_unpack(f2_fma(pair_mul(u, y), r, u), s[c], s[c + 1]);
+  }
+}
+
+// Scores of a thread's row to base 2, capped. Scores well below the cap, the
+// common case, go by a polynomial: below a quarter of it (2 terms, 4.9e-7
+// relative at most), below three quarters (tanh_small's 5 terms), else one by one.
 template <int N>
 __device__ __forceinline__ void cap_scores(const ScoreForm& f, float (&s)[N]) {
-  const float i2 = f.inv_cap * f.inv_cap;
-  float top0 = 0.0f, top1 = 0.0f;
+  float top[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-  for (int c = 0; c < N; c += 2) top0 = fmaxf(top0, fabsf(s[c])), top1 = fmaxf(top1, fabsf(s[c + 1]));
-  if (__all_sync(kFullMask, fmaxf(top0, top1) * fabsf(f.inv_cap) < kTanhSmall)) {
-    const float unit = f.cap2 * f.inv_cap;
-    const uint64_t k = pair_of(unit, unit);
-    uint64_t a[5];
-    float factor = i2;
+  for (int c = 0; c < N; c += 8)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top[i] = max3_abs(top[i], s[c + i], s[c + 4 + i]);
+  const float big = fmaxf(max3(top[0], top[1], top[2]), top[3]) * fabsf(f.inv_cap);
+  if (__all_sync(kFullMask, big < 0.25f)) {
+    const float poly[2] = {-0.33324572443962097f, 0.12876421213150024f};
+    cap_polynomial(f, poly, s);
+  } else if (__all_sync(kFullMask, big < kTanhSmall)) {
     const float poly[5] = {-0.3333306908607483f, 0.13326521217823029f, -0.0533902570605278f, 0.019664911553263664f,
                            -0.004769488703459501f};
-#pragma unroll
-    for (int i = 0; i < 5; ++i) {
-      a[i] = pair_of(poly[i] * factor, poly[i] * factor);
-      factor *= i2;
-    }
-#pragma unroll
-    for (int c = 0; c < N; c += 2) {
-      const uint64_t x = pair_of(s[c], s[c + 1]), y = pair_mul(x, x), u = pair_mul(x, k);
-      uint64_t r = f2_fma(a[4], y, a[3]);
-      r = f2_fma(r, y, a[2]);
-      r = f2_fma(r, y, a[1]);
-      r = f2_fma(r, y, a[0]);
-      r = f2_fma(pair_mul(u, y), r, u);
-      f2_unpack(r, s[c], s[c + 1]);
-    }
+    cap_polynomial(f, poly, s);
   } else {
 #pragma unroll
     for (int c = 0; c < N; ++c) s[c] = tanh_of(s[c] * f.inv_cap) * f.cap2;
@@ -226,8 +244,8 @@ __global__ void __launch_bounds__(FwdShape<DP>::kThreads, FwdShape<DP>::kCtas)
   __shared__ int abort_flag;
   volatile int* abort = &abort_flag;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int h = blockIdx.y, b = blockIdx.z, hk = h / (p.H / p.Hkv);
-  const int i0 = (gridDim.x - 1 - blockIdx.x) * 2 * kTileTokens;  // long causal rows first
+  const int h = blockIdx.x % p.H, b = blockIdx.x / p.H, hk = h / (p.H / p.Hkv);
+  const int i0 = (gridDim.y - 1 - blockIdx.y) * 2 * kTileTokens;  // long causal rows first
   const int length = attn_length(p, b);
   const int limit = rows_limit(p, b, i0 + 2 * kTileTokens, length);
   if (threadIdx.x == 0) {
@@ -482,26 +500,30 @@ __global__ void __launch_bounds__(FwdShape<DP>::kThreads, FwdShape<DP>::kCtas)
 }
 
 // ---------------------------------------------------------------------------
-// Backward, in two kernels without atomics: dq by tiles of queries (which also
-// leaves delta_i = g_i . o_i), then dk and dv by tiles of keys. Scores are formed
-// in both: 7 products of a tile pair instead of 5, and a fixed order of sums.
-// Each half of the eight warps takes 64 of the 128 columns, so that a thread
-// holds 64 scores and 64 derivatives. The derivative goes to TMEM in 16 bits
-// without the scale, which its sums get at the end: in fp16 it would cost small
-// gradients digits.
+// Backward, in two kernels without atomics: dq by tiles of 128 queries (which
+// also leaves delta_i = g_i . o_i), then dk and dv by tiles of 128 keys. Scores are
+// formed in both: 7 products of a tile pair instead of 5, and a fixed order of
+// sums. A step is 128 columns (keys; queries) above 64 channels, 64 up to it,
+// where two CTAs share an SM's TMEM; each half of the eight warps takes half of
+// the columns. The derivative goes to TMEM in 16 bits without the scale, which
+// its sums get at the end: in fp16 it would cost small gradients digits.
 // ---------------------------------------------------------------------------
 template <int DP>
 struct BwdShape {
   static constexpr int kTile = tile_bytes<DP>();
   static constexpr int kSmem = 1024 + 6 * kTile;  // two tiles that stay, two stages of two
+  static constexpr int kStep = DP > 64 ? 128 : 64;
+  static constexpr int kCtas = DP > 64 ? 1 : 2;
+  static constexpr bool kSplit = DP > 64;  // registers, as in the forward
+  static constexpr int kThreads = kSplit ? tc::kThreads : kSoftmaxThreads + 64;
+  static constexpr int kColumns = DP > 64 ? 512 : 256;
 };
 
-// A thread's 64 probabilities from its scores, in place; with a cap its
-// derivative 1 - tanh^2 in t2. far(c): places between query and key; lse(c, i):
-// minus the log-sum-exp, to base 2, of columns c and c + 1 (i = 0) or c + 2 and
-// c + 3.
-template <bool MODS, typename Far, typename Lse>
-__device__ __forceinline__ void probabilities(const AttnParams& p, const ScoreForm& f, float (&s)[64], float (&t2)[MODS ? 64 : 2],
+// A thread's N probabilities from its scores, in place; with a cap its
+// derivative 1 - tanh^2 in t2. far(c): places between query and key; lse(c, ..):
+// minus the log-sum-exp, to base 2, of columns c and c + 1, and of c + 2 and c + 3.
+template <bool MODS, int N, typename Far, typename Lse>
+__device__ __forceinline__ void probabilities(const AttnParams& p, const ScoreForm& f, float (&s)[N], float (&t2)[MODS ? N : 2],
                                               Far far, Lse lse) {
   float factor = f.scale2;
   if constexpr (MODS) {
@@ -510,7 +532,7 @@ __device__ __forceinline__ void probabilities(const AttnParams& p, const ScoreFo
       const float inv = -1.0f / (f.cap2 * f.cap2);
       const uint64_t inv2 = pair_of(inv, inv), one = pair_of(1.0f, 1.0f);
 #pragma unroll
-      for (int c = 0; c < 64; c += 2) {
+      for (int c = 0; c < N; c += 2) {
         const uint64_t x = pair_of(s[c], s[c + 1]);
         f2_unpack(f2_fma(pair_mul(x, x), inv2, one), t2[c], t2[c + 1]);
       }
@@ -518,13 +540,13 @@ __device__ __forceinline__ void probabilities(const AttnParams& p, const ScoreFo
     }
     if (p.slopes) {
 #pragma unroll
-      for (int c = 0; c < 64; ++c) s[c] = fmaf(-f.slope2, fabsf(far(c)), s[c] * factor);
+      for (int c = 0; c < N; ++c) s[c] = fmaf(-f.slope2, fabsf(far(c)), s[c] * factor);
       factor = 1.0f;
     }
   }
   const uint64_t factor2 = pair_of(factor, factor);
 #pragma unroll
-  for (int c = 0; c < 64; c += 4) {
+  for (int c = 0; c < N; c += 4) {
     uint64_t l0, l1;
     lse(c, l0, l1);
     f2_unpack(f2_fma(pair_of(s[c], s[c + 1]), factor2, l0), s[c], s[c + 1]);
@@ -534,17 +556,18 @@ __device__ __forceinline__ void probabilities(const AttnParams& p, const ScoreFo
   }
 }
 
-__device__ __forceinline__ void multiply(float (&s)[64], const float (&t)[64]) {
+template <int N>
+__device__ __forceinline__ void multiply(float (&s)[N], const float (&t)[N]) {
 #pragma unroll
-  for (int c = 0; c < 64; c += 2) f2_unpack(pair_mul(pair_of(s[c], s[c + 1]), pair_of(t[c], t[c + 1])), s[c], s[c + 1]);
+  for (int c = 0; c < N; c += 2) f2_unpack(pair_mul(pair_of(s[c], s[c + 1]), pair_of(t[c], t[c + 1])), s[c], s[c + 1]);
 }
 
 // dp <- s (dp - delta); delta(c, ..): minus the columns' row sums, as lse above.
 // `clean`: masked columns (s = 0) stay 0 whatever dp holds there.
-template <typename Delta>
-__device__ __forceinline__ void derivatives(const float (&s)[64], float (&dp)[64], bool clean, Delta delta) {
+template <int N, typename Delta>
+__device__ __forceinline__ void derivatives(const float (&s)[N], float (&dp)[N], bool clean, Delta delta) {
 #pragma unroll
-  for (int c = 0; c < 64; c += 4) {
+  for (int c = 0; c < N; c += 4) {
     uint64_t d0, d1;
     delta(c, d0, d1);
     f2_unpack(pair_mul(pair_add(pair_of(dp[c], dp[c + 1]), d0), pair_of(s[c], s[c + 1])), dp[c], dp[c + 1]);
@@ -552,17 +575,31 @@ __device__ __forceinline__ void derivatives(const float (&s)[64], float (&dp)[64
   }
   if (clean) {
 #pragma unroll
-    for (int c = 0; c < 64; ++c) dp[c] = s[c] == 0.0f ? 0.0f : dp[c];
+    for (int c = 0; c < N; ++c) dp[c] = s[c] == 0.0f ? 0.0f : dp[c];
   }
 }
 
-// 64 values of a thread's row to TMEM in 16 bits.
-template <typename T>
-__device__ __forceinline__ void store_row(uint32_t at, const float (&v)[64]) {
-  uint32_t packed[32];
+template <int N>
+__device__ __forceinline__ void load_row(uint32_t at, float (&v)[N]) {
 #pragma unroll
-  for (int c = 0; c < 32; ++c) packed[c] = pack_pair<T>(v[2 * c], v[2 * c + 1]);
-  tmem_store32(at, packed);
+  for (int c = 0; c < N; c += 32) tmem_load32(at + c, v + c);
+  tmem_wait_load();
+}
+
+// N values of a thread's row to TMEM in 16 bits, and word of it to `bar`.
+template <typename T, int N>
+__device__ __forceinline__ void store_row(uint32_t at, const float (&v)[N], uint64_t* bar) {
+#pragma unroll
+  for (int from = 0; from < N; from += 32) {
+    uint32_t packed[16];
+#pragma unroll
+    for (int c = 0; c < 16; ++c) packed[c] = pack_pair<T>(v[from + 2 * c], v[from + 2 * c + 1]);
+    tmem_store16(at + from / 2, packed);
+  }
+  tmem_wait_store();
+  fence_before();
+  __syncwarp();
+  if (threadIdx.x % 32 == 0) bar_arrive(bar);
 }
 
 // COLS columns of a thread's row of a sum in TMEM, times mul, to global memory.
@@ -589,51 +626,43 @@ __device__ __forceinline__ void write_row(T* out, bool in, uint32_t at, int firs
   }
 }
 
-// Columns of a sum that each half of the warps writes: half of them, or all by
-// the first half where half would be less than a load's 32.
-template <int DP>
-struct HalfColumns {
-  static constexpr int kCols = DP >= 64 ? DP / 2 : DP;
-};
-
 template <typename T, int DP, bool MODS>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
     attn_tc_dq_kernel(const AttnParams p, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                       const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap gmap) {
   using Shape = BwdShape<DP>;
+  constexpr int STEP = Shape::kStep, N = STEP / 2;
   extern __shared__ char raw[];
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   char *sq = smem, *sg = smem + Shape::kTile, *ring = smem + 2 * Shape::kTile;  // stage: key tile, value tile
-  __shared__ uint64_t q_full, kv_full[2], kv_empty[2], s_full[2], dp_full, dp_empty, ds_full, done;
+  __shared__ uint64_t q_full, kv_full[2], kv_empty[2], s_full[2], dp_full, dp_empty, ds_full, done, cleared;
   __shared__ float delta_part[2][kTileTokens];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   volatile int* abort = &abort_flag;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int h = blockIdx.y, b = blockIdx.z, hk = h / (p.H / p.Hkv);
-  const int i0 = (gridDim.x - 1 - blockIdx.x) * kTileTokens;
+  const int h = blockIdx.x % p.H, b = blockIdx.x / p.H, hk = h / (p.H / p.Hkv);
+  const int i0 = (gridDim.y - 1 - blockIdx.y) * kTileTokens;
   const int length = attn_length(p, b);
   const int limit = rows_limit(p, b, i0 + kTileTokens, length);
-  const int tiles = (limit + kTileTokens - 1) / kTileTokens;
   if (threadIdx.x == 0) {
     abort_flag = 0;
-    bar_init(&q_full, 1);
-    bar_init(&done, 1);
+    bar_init(&q_full, 1), bar_init(&done, 1), bar_init(&cleared, 1), bar_init(&dp_full, 1);
     for (int i = 0; i < 2; ++i) bar_init(&kv_full[i], 1), bar_init(&kv_empty[i], 1), bar_init(&s_full[i], 1);
-    bar_init(&dp_full, 1);
     bar_init(&dp_empty, kSoftmaxThreads / 32), bar_init(&ds_full, kSoftmaxThreads / 32);
     fence_async_smem();
   }
-  if (warp == kMmaWarp) tmem_alloc<512>(&tmem_slot);
+  if (warp == kMmaWarp) tmem_alloc<Shape::kColumns>(&tmem_slot);
   fence_before();
   __syncthreads();
   fence_after();
-  const uint32_t tmem = tmem_slot;  // scores 0..127 and 128..255, derivatives 256..383, dq 384...
+  // Two buffers of scores, whose place the derivative takes; dp; dq.
+  const uint32_t tmem = tmem_slot, dp_at = tmem + 2 * STEP, dq_at = tmem + 3 * STEP;
 
   if (warp < kLoadWarp) {
-    take_registers();
+    if constexpr (Shape::kSplit) take_registers();
     const int half = warp / 4, r = threadIdx.x % kTileTokens, i = i0 + r;
-    const uint32_t at = tmem + ((uint32_t)(warp % 4) << 21);
+    const uint32_t lanes = (uint32_t)(warp % 4) << 21;
     const RowView row = row_view(p, b, i, length);
     const ScoreForm f = score_form(p, h);
     const int* kdoc = p.kdoc ? p.kdoc + (int64_t)b * p.Sk : nullptr;
@@ -667,19 +696,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float lse = in && row.limit > 0 ? p.lse[stat] * -kLog2e : 0.0f;
     const uint64_t lse2 = pair_of(lse, lse), delta2 = pair_of(-delta, -delta);
     bool ok = true;
-    int n = 0;
-    for (int j = 0; j < tiles && ok; ++j) {
-      const TileState st = tile_state(p, b, i0, 1, j, length);
-      if (st.skip) continue;
-      const int c0 = j * kTileTokens + half * 64;  // the thread's first key
-      const uint32_t s_at = at + (n % 2) * 128 + half * 64;
-      ok = warp_wait(&s_full[n % 2], (n / 2) & 1, abort);
+    int u = 0;
+    for (KeySteps<STEP> at(p, b, i0, 1, limit, length); !at.done && ok; at.advance(p, b, i0, 1, length), ++u) {
+      const int c0 = at.j * kTileTokens + at.half * 64 + half * N;  // the thread's first key
+      const uint32_t s_at = tmem + lanes + (u & 1) * STEP + half * N;
+      ok = warp_wait(&s_full[u & 1], (u >> 1) & 1, abort);
       if (!ok) break;
       fence_after();
-      float s[64], t2[MODS ? 64 : 2];
-      tmem_load32(s_at, s);
-      tmem_load32(s_at + 32, s + 32);
-      tmem_wait_load();
+      float s[N], t2[MODS ? N : 2];
+      load_row(s_at, s);
       const int seen = row.limit - c0;
       const float away = (float)(row.place - c0);
       probabilities<MODS>(p, f, s, t2, [&](int c) { return away - (float)c; }, [&](int, uint64_t& a, uint64_t& d) { a = d = lse2; });
@@ -687,213 +712,255 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (p.cap != 0.0f) multiply(s, t2);
       }
       bool masked = false;
-      if (!__all_sync(kFullMask, seen >= 64)) {
+      if (!__all_sync(kFullMask, seen >= N)) {
         masked = true;
 #pragma unroll
-        for (int c = 0; c < 64; ++c) s[c] = c < seen ? s[c] : 0.0f;
+        for (int c = 0; c < N; ++c) s[c] = c < seen ? s[c] : 0.0f;
       }
-      if (!st.agree) {
+      if (!at.state.agree) {
         masked = true;
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
+        for (int q = 0; q < N / 32; ++q) {
           const int k = c0 + q * 32 + lane, mine = k < p.Sk ? __ldg(kdoc + k) : -1;
 #pragma unroll
           for (int c = 0; c < 32; ++c)
             if (!same_document(row.doc, __shfl_sync(kFullMask, mine, c), p.shared)) s[q * 32 + c] = 0.0f;
         }
       }
-      ok = warp_wait(&dp_full, n & 1, abort);
+      ok = warp_wait(&dp_full, u & 1, abort);
       if (!ok) break;
       fence_after();
-      float dp[64];
-      tmem_load32(at + 256 + half * 64, dp);
-      tmem_load32(at + 256 + half * 64 + 32, dp + 32);
-      tmem_wait_load();
+      float dp[N];
+      load_row(dp_at + lanes + half * N, dp);
       fence_before();
       __syncwarp();
       if (lane == 0) bar_arrive(&dp_empty);
       derivatives(s, dp, masked, [&](int, uint64_t& a, uint64_t& d) { a = d = delta2; });
-      store_row<T>(s_at, dp);
-      tmem_wait_store();
-      fence_before();
-      __syncwarp();
-      if (lane == 0) bar_arrive(&ds_full);
-      ++n;
+      store_row<T>(s_at, dp, &ds_full);
     }
-    if (ok && n > 0) ok = warp_wait(&done, 0, abort);
+    if (ok && u > 0) ok = warp_wait(&done, 0, abort);
     fence_after();
-    constexpr int cols = HalfColumns<DP>::kCols;
+    // Each half of the warps writes half of the channels, or the first all of them
+    // where half would be less than a load's 32.
+    constexpr int cols = DP >= 64 ? DP / 2 : DP;
     if (half * cols < DP)
-      write_row<T, cols>(static_cast<T*>(p.dq) + (((int64_t)b * p.Sq + i) * p.H + h) * p.D + half * cols, in, at + 384 + half * cols,
-                         half * cols, p.D, ok ? p.scale : NAN, n > 0);
+      write_row<T, cols>(static_cast<T*>(p.dq) + (((int64_t)b * p.Sq + i) * p.H + h) * p.D + half * cols, in,
+                         dq_at + lanes + half * cols, half * cols, p.D, ok ? p.scale : NAN, u > 0);
     fence_before();
   } else {
-    leave_registers();
+    if constexpr (Shape::kSplit) leave_registers();
     if (warp == kLoadWarp) {
-      if (lane == 0 && tiles > 0) {
-        bar_expect(&q_full, 2 * Shape::kTile);
-        tma_tile<DP>(sq, &qmap, &q_full, h, i0, b);
-        tma_tile<DP>(sg, &gmap, &q_full, h, i0, b);
+      if (limit > 0) {
+        if (lane == 0) {
+          bar_expect(&q_full, 2 * Shape::kTile);
+          tma_tile<DP>(sq, &qmap, &q_full, h, i0, b);
+          tma_tile<DP>(sg, &gmap, &q_full, h, i0, b);
+        }
+        const int* kdoc = p.kdoc ? p.kdoc + (int64_t)b * p.Sk : nullptr;
         int n = 0;
         bool ok = true;
-        for (int j = 0; j < tiles && ok; ++j) {
-          if (tile_state(p, b, i0, 1, j, length).skip) continue;
+        for (KeySteps<STEP> at(p, b, i0, 1, limit, length); !at.done && ok; at.next_tile(p, b, i0, 1, length)) {
           const int slot = n % 2;
-          if (n >= 2) ok = bar_wait(&kv_empty[slot], (n / 2 - 1) & 1, abort);
+          if (n >= 2) ok = warp_wait(&kv_empty[slot], (n / 2 - 1) & 1, abort);
           if (!ok) break;
-          bar_expect(&kv_full[slot], 2 * Shape::kTile);
-          tma_tile<DP>(ring + slot * 2 * Shape::kTile, &kmap, &kv_full[slot], hk, j * kTileTokens, b);
-          tma_tile<DP>(ring + slot * 2 * Shape::kTile + Shape::kTile, &vmap, &kv_full[slot], hk, j * kTileTokens, b);
+          char* stage = ring + slot * 2 * Shape::kTile;
+          if (lane == 0) {
+            bar_expect(&kv_full[slot], 2 * Shape::kTile);
+            tma_tile<DP>(stage, &kmap, &kv_full[slot], hk, at.j * kTileTokens, b);
+            tma_tile<DP>(stage + Shape::kTile, &vmap, &kv_full[slot], hk, at.j * kTileTokens, b);
+          }
+          __syncwarp();
+          if (at.state.padded) {  // padded keys are cleared: dq's product goes over all of the tile's
+            ok = warp_wait(&kv_full[slot], (n / 2) & 1, abort);
+            clear_rows<DP>(stage, kdoc, at.j * kTileTokens, length);
+            if (lane == 0) bar_arrive(&cleared);
+          }
           ++n;
         }
-        bar_wait(&q_full, 0, abort);
-        for (int i = max(0, n - 2); i < n; ++i) bar_wait(&kv_full[i % 2], (i / 2) & 1, abort);
+        warp_wait(&q_full, 0, abort);
+        for (int i = max(0, n - 2); i < n; ++i) warp_wait(&kv_full[i % 2], (i / 2) & 1, abort);
       }
-    } else if (warp == kMmaWarp) {
-      constexpr uint32_t ds = instr_desc<IsBf16<T>::value>(128, false), dd = instr_desc<IsBf16<T>::value>(DP, true);
-      const uint32_t q_addr = smem_u32(sq), g_addr = smem_u32(sg), ring_addr = smem_u32(ring);
-      bool ok = tiles == 0 || warp_wait(&q_full, 0, abort);
-      int n = 0;  // tiles begun; tile n - 1 is the one whose dq is due
-      bool prev_padded = false;
-      int prev_j = 0;
-      for (int j = 0; j <= tiles && ok; ++j) {
-        TileState st{};
-        if (j < tiles) {
-          st = tile_state(p, b, i0, 1, j, length);
-          if (st.skip) continue;
-          // Scores into the buffer that the tile before last has left, ahead of
-          // the softmax of the tile before.
-          const uint32_t slot = ring_addr + (n % 2) * 2 * Shape::kTile;
-          ok = warp_wait(&kv_full[n % 2], (n / 2) & 1, abort);
-          if (!ok) break;
+    } else if (warp == kMmaWarp && elect_one()) {
+      constexpr uint32_t ds = instr_desc<IsBf16<T>::value>(STEP, false), dd = instr_desc<IsBf16<T>::value>(DP, true);
+      constexpr uint64_t kHalfTile = 64 * 128 >> 4, kTileDesc = Shape::kTile >> 4;
+      const uint64_t q_desc = by_channels(smem_u32(sq)), g_desc = q_desc + kTileDesc, kv_desc = by_channels(smem_u32(ring));
+      const uint64_t k_tokens = by_tokens(smem_u32(ring));
+      bool ok = limit == 0 || bar_wait(&q_full, 0, abort);
+      int u = 0, clears = 0, prev_slot = 0;
+      uint64_t prev_k = 0;      // keys of the step before, whose dq is due
+      bool prev_last = false;   // it was its tile's last
+      const auto finish = [&]() {
+        ok = bar_wait(&ds_full, (u - 1) & 1, abort);
+        fence_after();
+        if (!ok) return;
+        product_parts<STEP>(dq_at, tmem + ((u - 1) & 1) * STEP, prev_k, dd, u > 1);
+        if (prev_last) commit(&kv_empty[prev_slot]);
+      };
+      for (KeySteps<STEP> at(p, b, i0, 1, limit, length); !at.done && ok; at.next_tile(p, b, i0, 1, length)) {
+        const int slot = at.n & 1, count = at.count();
+        ok = bar_wait(&kv_full[slot], (at.n >> 1) & 1, abort);
+        if (ok && at.state.padded) ok = bar_wait(&cleared, clears++ & 1, abort);
+        for (int half = 0; half < count && ok; ++half, ++u) {
+          // Scores into the buffer that the step before last has left, ahead of
+          // the softmax of the step before.
+          const uint64_t k = kv_desc + slot * 2 * kTileDesc + half * kHalfTile;
           fence_after();
-          if (elect_one()) {
-            product_channels<DP>(tmem + (n % 2) * 128, by_channels(q_addr), by_channels(slot), ds);
-            commit(&s_full[n % 2]);
-          }
-          __syncwarp();
-          if (n > 0) ok = warp_wait(&dp_empty, (n - 1) & 1, abort);
-          if (!ok) break;
+          product_channels<DP>(tmem + (u & 1) * STEP, q_desc, k, ds);
+          commit(&s_full[u & 1]);
+          if (u > 0) ok = bar_wait(&dp_empty, (u - 1) & 1, abort);
           fence_after();
-          if (elect_one()) {
-            product_channels<DP>(tmem + 256, by_channels(g_addr), by_channels(slot + Shape::kTile), ds);
-            commit(&dp_full);
-          }
-          __syncwarp();
+          if (!ok) break;
+          product_channels<DP>(dp_at, g_desc, k + kTileDesc, ds);
+          commit(&dp_full);
+          if (u > 0) finish();
+          prev_slot = slot, prev_k = k_tokens + slot * 2 * kTileDesc + half * 4 * kTokenStep, prev_last = half + 1 == count;
         }
-        if (n > 0) {
-          const int slot = (n - 1) % 2;
-          ok = warp_wait(&ds_full, (n - 1) & 1, abort);
-          if (!ok) break;
-          if (prev_padded)
-            clear_rows<DP>(ring + slot * 2 * Shape::kTile, p.kdoc ? p.kdoc + (int64_t)b * p.Sk : nullptr, prev_j * kTileTokens, length);
-          fence_after();
-          if (elect_one()) {
-            product_tokens(tmem + 384, tmem + slot * 128, 64, by_tokens(ring_addr + slot * 2 * Shape::kTile), dd, n > 1);
-            commit(&kv_empty[slot]);
-            if (j == tiles) commit(&done);
-          }
-          __syncwarp();
-        }
-        prev_padded = st.padded, prev_j = j;
-        ++n;
       }
-      if (!ok) {
-        if (elect_one()) commit(&done);
-        __syncwarp();
-        warp_wait(&done, 0, abort);
-      }
+      if (ok && u > 0) finish();
+      commit(&done);
+      if (!ok) bar_wait(&done, 0, abort);
     }
   }
   __syncthreads();
   if (warp == kMmaWarp) {
     fence_after();
-    tmem_free<512>(tmem);
+    tmem_free<Shape::kColumns>(tmem);
   }
 }
 
-// What a key-tile thread needs of each query of a tile.
+// The steps that a block of keys goes through: every head of its group, the
+// tiles of queries from the first that may see it, or with STEP 64 their halves.
+template <int STEP>
+struct QuerySteps {
+  int g, i, half, n;  // head of the group, query tile, its half, the tile's number among those visited
+  int first, tiles, halves;
+  bool done;
+  TileState state;
+
+  __device__ __forceinline__ void seek(const AttnParams& p, int b, int group, int kt, int length) {
+    for (;;) {
+      if (i >= tiles) i = first, ++g;
+      done = g >= group || first >= tiles;
+      if (done) return;
+      if (!p.kdoc) {
+        state = TileState{false, true, false};
+        return;
+      }
+      state = tile_state(p, b, i * kTileTokens, 1, kt, length);
+      if (!state.skip) {
+        state.padded = p.qtile[(int64_t)b * tiles + i].padded;  // of the queries, here
+        return;
+      }
+      ++i;
+    }
+  }
+  __device__ __forceinline__ QuerySteps(const AttnParams& p, int b, int group, int kt, int length)
+      : g(0), half(0), n(0), tiles((p.Sq + kTileTokens - 1) / kTileTokens),
+        halves(STEP == 128 || (p.Sq - 1) % kTileTokens < 64 ? 1 : 2) {
+    const int j0 = kt * kTileTokens;
+    first = i = j0 < length ? first_query(p, b, j0, length) / kTileTokens : tiles;
+    seek(p, b, group, kt, length);
+  }
+  __device__ __forceinline__ int count() const { return STEP == 128 || i + 1 == tiles ? halves : 2; }
+  __device__ __forceinline__ void next_tile(const AttnParams& p, int b, int group, int kt, int length) {
+    half = 0, ++i, ++n;
+    seek(p, b, group, kt, length);
+  }
+  __device__ __forceinline__ void advance(const AttnParams& p, int b, int group, int kt, int length) {
+    if (half + 1 == count()) next_tile(p, b, group, kt, length);
+    else half = 1;
+  }
+  __device__ __forceinline__ int row() const { return i * kTileTokens + half * 64; }
+};
+
+// What a key-tile thread needs of each query of a step.
+template <int STEP>
 struct __align__(16) QueryStats {
-  float lse[kTileTokens], delta[kTileTokens];  // negative; lse to base 2
-  int limit[kTileTokens], place[kTileTokens], doc[kTileTokens];
+  float lse[STEP], delta[STEP];  // negative; lse to base 2
+  int limit[STEP], place[STEP], doc[STEP];
 };
 
 template <typename T, int DP, bool MODS>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
     attn_tc_dkv_kernel(const AttnParams p, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                        const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap gmap) {
   using Shape = BwdShape<DP>;
+  constexpr int STEP = Shape::kStep, N = STEP / 2;
   extern __shared__ char raw[];
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   char *sk = smem, *sv = smem + Shape::kTile, *ring = smem + 2 * Shape::kTile;  // stage: query tile, gradient tile
-  __shared__ uint64_t k_full, q_full[2], q_empty[2], s_full, p_full, dp_full, ds_full, done;
-  __shared__ QueryStats stats[2];
+  __shared__ uint64_t k_full, q_full[2], q_empty[2], s_full, p_full, dp_full, ds_full, done, cleared;
+  __shared__ QueryStats<STEP> stats[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   volatile int* abort = &abort_flag;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int hk = blockIdx.y, b = blockIdx.z, group = p.H / p.Hkv;
-  const int kt = blockIdx.x, j0 = kt * kTileTokens;  // early keys are seen by the most causal queries
+  const int hk = blockIdx.x % p.Hkv, b = blockIdx.x / p.Hkv, group = p.H / p.Hkv;
+  const int kt = blockIdx.y, j0 = kt * kTileTokens;  // early keys, which the most causal queries see, first
   const int length = attn_length(p, b);
-  const int q_tiles = (p.Sq + kTileTokens - 1) / kTileTokens;
-  const int first = j0 < length ? first_query(p, b, j0, length) / kTileTokens : q_tiles;
-  // Steps: each head of the group, its tiles of queries from `first` on.
-  const int per_head = q_tiles - first, steps = group * per_head;
   if (threadIdx.x == 0) {
     abort_flag = 0;
-    bar_init(&k_full, 1);
-    bar_init(&done, 1);
+    bar_init(&k_full, 1), bar_init(&done, 1), bar_init(&cleared, 1), bar_init(&s_full, 1), bar_init(&dp_full, 1);
     for (int i = 0; i < 2; ++i) bar_init(&q_full[i], 1), bar_init(&q_empty[i], 1);
-    bar_init(&s_full, 1), bar_init(&dp_full, 1);
     bar_init(&p_full, kSoftmaxThreads / 32), bar_init(&ds_full, kSoftmaxThreads / 32);
     fence_async_smem();
   }
-  if (warp == kMmaWarp) tmem_alloc<512>(&tmem_slot);
+  if (warp == kMmaWarp) tmem_alloc<Shape::kColumns>(&tmem_slot);
   fence_before();
   __syncthreads();
   fence_after();
-  const uint32_t tmem = tmem_slot;  // scores 0..127, derivatives 128..255, dv 256..., dk 384...
+  // Scores, then probabilities; dp, then its derivative; dv; dk.
+  const uint32_t tmem = tmem_slot, dp_at = tmem + STEP, dv_at = tmem + 2 * STEP, dk_at = dv_at + DP;
 
   if (warp < kLoadWarp) {
-    take_registers();
+    if constexpr (Shape::kSplit) take_registers();
     const int half = warp / 4, r = threadIdx.x % kTileTokens, j = j0 + r;  // key of this thread
-    const uint32_t at = tmem + ((uint32_t)(warp % 4) << 21) + half * 64;
+    const int c0 = half * N;
+    const uint32_t lanes = (uint32_t)(warp % 4) << 21, s_at = tmem + lanes + c0;
     const int kd = p.kdoc && j < length ? __ldg(p.kdoc + (int64_t)b * p.Sk + j) : 0;
     const bool live = j < length;
-    bool ok = true;
-    int n = 0;
-    // A warp whose wait gave up still comes to the others' barriers.
-    for (int u = 0; u < steps; ++u) {
-      const int h = hk * group + u / per_head, i0 = (first + u % per_head) * kTileTokens;
-      const TileState st = tile_state(p, b, i0, 1, kt, length);
-      if (st.skip) continue;
-      QueryStats& q = stats[n % 2];
-      const ScoreForm f = score_form(p, h);
-      bool whole;  // every query of the tile sees every key of the tile
-      {
-        // Filled two steps ahead of their buffer's next use: every thread has
-        // passed the barrier of the step between.
-        const RowView row = row_view(p, b, i0 + r, length);
-        const int64_t stat = ((int64_t)b * p.H + h) * p.Sq + i0 + r;
-        if (half == 0) {
-          q.lse[r] = row.limit > 0 ? p.lse[stat] * -kLog2e : 0.0f;
-          q.delta[r] = row.limit > 0 ? -p.delta[stat] : 0.0f;
-        } else {
-          q.limit[r] = row.limit, q.place[r] = row.place, q.doc[r] = row.doc;
-        }
-        int full;
-        asm volatile("{\n .reg .pred p, q;\n setp.ne.s32 p, %1, 0;\n barrier.cta.red.and.pred q, 1, %2, p;\n selp.s32 %0, 1, 0, q;\n}"
-                     : "=r"(full) : "r"((int)(row.limit >= j0 + kTileTokens)), "r"(kSoftmaxThreads) : "memory");
-        whole = full && st.agree;
+    // The queries' statistics of a step are fetched during the step before: the
+    // first half of the warps has a query's log-sum-exp and row sum, the second
+    // its view of the keys.
+    float lse = 0.0f, delta = 0.0f;
+    RowView view{};
+    const auto fetch = [&](const QuerySteps<STEP>& at) {
+      if (at.done || r >= STEP) return;
+      const int i = at.row() + r;
+      view = row_view(p, b, i, length);
+      if (half == 0) {
+        const int64_t stat = ((int64_t)b * p.H + hk * group + at.g) * p.Sq + i;
+        lse = view.limit > 0 ? __ldg(p.lse + stat) * -kLog2e : 0.0f;
+        delta = view.limit > 0 ? -__ldg(p.delta + stat) : 0.0f;
       }
-      ok = ok && warp_wait(&s_full, n & 1, abort);
+    };
+    bool ok = true;
+    int u = 0;
+    QuerySteps<STEP> at(p, b, group, kt, length);
+    fetch(at);
+    // A warp whose wait gave up still comes to the others' barriers.
+    while (!at.done) {
+      QueryStats<STEP>& q = stats[u & 1];
+      const ScoreForm f = score_form(p, hk * group + at.g);
+      const bool agree = at.state.agree;
+      // This buffer was read two steps ago: every thread has passed the barrier
+      // of the step between.
+      if (r < STEP) {
+        if (half == 0) q.lse[r] = lse, q.delta[r] = delta;
+        else q.limit[r] = view.limit, q.place[r] = view.place, q.doc[r] = view.doc;
+      }
+      int full;
+      asm volatile("{\n .reg .pred p, q;\n setp.ne.s32 p, %1, 0;\n barrier.cta.red.and.pred q, 1, %2, p;\n selp.s32 %0, 1, 0, q;\n}"
+                   : "=r"(full) : "r"((int)(r >= STEP || view.limit >= j0 + kTileTokens)), "r"(kSoftmaxThreads) : "memory");
+      const bool whole = full && agree;  // every query of the step sees every key of the tile
+      at.advance(p, b, group, kt, length);
+      fetch(at);
+      const int turn = u++ & 1;
+      ok = ok && warp_wait(&s_full, turn, abort);
       if (!ok) continue;
       fence_after();
-      float s[64], t2[MODS ? 64 : 2];
-      tmem_load32(at, s);
-      tmem_load32(at + 32, s + 32);
-      tmem_wait_load();
-      const int c0 = half * 64;
+      float s[N], t2[MODS ? N : 2];
+      load_row(s_at, s);
       const auto pairs = [&](const float* from, int c, uint64_t& a, uint64_t& d) {
         const float4 v = *reinterpret_cast<const float4*>(from + c0 + c);
         a = pair_of(v.x, v.y), d = pair_of(v.z, v.w);
@@ -902,18 +969,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                           [&](int c, uint64_t& a, uint64_t& d) { pairs(q.lse, c, a, d); });
       if (!whole) {
 #pragma unroll
-        for (int c = 0; c < 64; c += 4) {
+        for (int c = 0; c < N; c += 4) {
           const int4 limit = *reinterpret_cast<const int4*>(q.limit + c0 + c);
           s[c] = live & (j < limit.x) ? s[c] : 0.0f;
           s[c + 1] = live & (j < limit.y) ? s[c + 1] : 0.0f;
           s[c + 2] = live & (j < limit.z) ? s[c + 2] : 0.0f;
           s[c + 3] = live & (j < limit.w) ? s[c + 3] : 0.0f;
         }
-        if (!st.agree) {
-          // A key of the shared document is of every query's; a padded key of none.
+        if (!agree) {
+          // A key of the shared document is of every query's; padded queries' limit is 0.
           const bool any = kd >= 0 && kd == p.shared;
 #pragma unroll
-          for (int c = 0; c < 64; c += 4) {
+          for (int c = 0; c < N; c += 4) {
             const int4 doc = *reinterpret_cast<const int4*>(q.doc + c0 + c);
             s[c] = (any | (doc.x == kd)) ? s[c] : 0.0f;
             s[c + 1] = (any | (doc.y == kd)) ? s[c + 1] : 0.0f;
@@ -922,130 +989,115 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      store_row<T>(at, s);
-      tmem_wait_store();
-      fence_before();
-      __syncwarp();
-      if (lane == 0) bar_arrive(&p_full);
+      store_row<T>(s_at, s, &p_full);
       if constexpr (MODS) {
         if (p.cap != 0.0f) multiply(s, t2);
       }
-      ok = warp_wait(&dp_full, n & 1, abort);
+      ok = warp_wait(&dp_full, turn, abort);
       if (!ok) continue;
       fence_after();
-      float dp[64];
-      tmem_load32(at + 128, dp);
-      tmem_load32(at + 160, dp + 32);
-      tmem_wait_load();
+      float dp[N];
+      load_row(dp_at + lanes + c0, dp);
       derivatives(s, dp, !whole, [&](int c, uint64_t& a, uint64_t& d) { pairs(q.delta, c, a, d); });
-      store_row<T>(at + 128, dp);
-      tmem_wait_store();
-      fence_before();
-      __syncwarp();
-      if (lane == 0) bar_arrive(&ds_full);
-      ++n;
+      store_row<T>(dp_at + lanes + c0, dp, &ds_full);
     }
-    if (ok && n > 0) ok = warp_wait(&done, 0, abort);
+    if (ok && u > 0) ok = warp_wait(&done, 0, abort);
     fence_after();
     const bool in = j < p.Sk;
     const int64_t out = (((int64_t)b * p.Sk + j) * p.Hkv + hk) * p.D;
-    const uint32_t lanes = tmem + ((uint32_t)(warp % 4) << 21);
     // The first half of the warps writes dv, the second dk.
-    if (half == 0) write_row<T, DP>(static_cast<T*>(p.dv) + out, in, lanes + 256, 0, p.D, ok ? 1.0f : NAN, n > 0);
-    else write_row<T, DP>(static_cast<T*>(p.dk) + out, in, lanes + 384, 0, p.D, ok ? p.scale : NAN, n > 0);
+    if (half == 0) write_row<T, DP>(static_cast<T*>(p.dv) + out, in, dv_at + lanes, 0, p.D, ok ? 1.0f : NAN, u > 0);
+    else write_row<T, DP>(static_cast<T*>(p.dk) + out, in, dk_at + lanes, 0, p.D, ok ? p.scale : NAN, u > 0);
     fence_before();
   } else {
-    leave_registers();
+    if constexpr (Shape::kSplit) leave_registers();
     if (warp == kLoadWarp) {
-      if (lane == 0 && steps > 0) {
-        bar_expect(&k_full, 2 * Shape::kTile);
-        tma_tile<DP>(sk, &kmap, &k_full, hk, j0, b);
-        tma_tile<DP>(sv, &vmap, &k_full, hk, j0, b);
+      QuerySteps<STEP> at(p, b, group, kt, length);
+      if (!at.done) {
+        if (lane == 0) {
+          bar_expect(&k_full, 2 * Shape::kTile);
+          tma_tile<DP>(sk, &kmap, &k_full, hk, j0, b);
+          tma_tile<DP>(sv, &vmap, &k_full, hk, j0, b);
+        }
         int n = 0;
         bool ok = true;
-        for (int u = 0; u < steps && ok; ++u) {
-          const int h = hk * group + u / per_head, i0 = (first + u % per_head) * kTileTokens;
-          if (tile_state(p, b, i0, 1, kt, length).skip) continue;
-          const int slot = n % 2;
-          if (n >= 2) ok = bar_wait(&q_empty[slot], (n / 2 - 1) & 1, abort);
+        for (; !at.done && ok; at.next_tile(p, b, group, kt, length)) {
+          const int slot = n % 2, h = hk * group + at.g, i0 = at.i * kTileTokens;
+          if (n >= 2) ok = warp_wait(&q_empty[slot], (n / 2 - 1) & 1, abort);
           if (!ok) break;
-          bar_expect(&q_full[slot], 2 * Shape::kTile);
-          tma_tile<DP>(ring + slot * 2 * Shape::kTile, &qmap, &q_full[slot], h, i0, b);
-          tma_tile<DP>(ring + slot * 2 * Shape::kTile + Shape::kTile, &gmap, &q_full[slot], h, i0, b);
+          char* stage = ring + slot * 2 * Shape::kTile;
+          if (lane == 0) {
+            bar_expect(&q_full[slot], 2 * Shape::kTile);
+            tma_tile<DP>(stage, &qmap, &q_full[slot], h, i0, b);
+            tma_tile<DP>(stage + Shape::kTile, &gmap, &q_full[slot], h, i0, b);
+          }
+          __syncwarp();
+          if (at.state.padded) {  // padded queries and their gradients, whatever they hold, count for nothing
+            ok = warp_wait(&q_full[slot], (n / 2) & 1, abort);
+            clear_rows<DP>(stage, p.qdoc + (int64_t)b * p.Sq, i0, p.Sq);
+            clear_rows<DP>(stage + Shape::kTile, p.qdoc + (int64_t)b * p.Sq, i0, p.Sq);
+            if (lane == 0) bar_arrive(&cleared);
+          }
           ++n;
         }
-        bar_wait(&k_full, 0, abort);
-        for (int i = max(0, n - 2); i < n; ++i) bar_wait(&q_full[i % 2], (i / 2) & 1, abort);
+        warp_wait(&k_full, 0, abort);
+        for (int i = max(0, n - 2); i < n; ++i) warp_wait(&q_full[i % 2], (i / 2) & 1, abort);
       }
-    } else if (warp == kMmaWarp) {
-      constexpr uint32_t ds = instr_desc<IsBf16<T>::value>(128, false), dd = instr_desc<IsBf16<T>::value>(DP, true);
-      const uint32_t k_addr = smem_u32(sk), v_addr = smem_u32(sv), ring_addr = smem_u32(ring);
-      bool ok = steps == 0 || warp_wait(&k_full, 0, abort);
-      int n = 0;
-      for (int u = 0; u <= steps && ok; ++u) {
-        const int i0 = u < steps ? (first + u % per_head) * kTileTokens : 0;
-        if (u < steps && tile_state(p, b, i0, 1, kt, length).skip) continue;
-        const uint32_t next = ring_addr + (n % 2) * 2 * Shape::kTile, prev = ring_addr + ((n - 1) & 1) * 2 * Shape::kTile;
-        // dv of the step before, then this step's scores over its probabilities;
-        // dk of the step before, then this step's derivatives: each product runs
-        // while the softmax works on the other half.
-        if (n > 0) {
-          ok = warp_wait(&p_full, (n - 1) & 1, abort);
+    } else if (warp == kMmaWarp && elect_one()) {
+      constexpr uint32_t ds = instr_desc<IsBf16<T>::value>(STEP, false), dd = instr_desc<IsBf16<T>::value>(DP, true);
+      constexpr uint64_t kHalfTile = 64 * 128 >> 4, kTileDesc = Shape::kTile >> 4;
+      const uint64_t k_desc = by_channels(smem_u32(sk)), v_desc = k_desc + kTileDesc, qg_desc = by_channels(smem_u32(ring));
+      const uint64_t qg_tokens = by_tokens(smem_u32(ring));
+      QuerySteps<STEP> at(p, b, group, kt, length);
+      bool ok = at.done || bar_wait(&k_full, 0, abort);
+      int u = 0, clears = 0, prev_slot = 0;
+      uint64_t prev_q = 0;     // queries of the step before, whose sums are due
+      bool prev_last = false;  // it was its tile's last
+      // dv of the step before, then this step's scores over its probabilities;
+      // dk of the step before, then this step's dp over its derivative: each
+      // product runs while the softmax works on the other half.
+      const auto add_dv = [&]() {
+        ok = bar_wait(&p_full, (u - 1) & 1, abort);
+        fence_after();
+        if (ok) product_parts<STEP>(dv_at, tmem, prev_q + kTileDesc, dd, u > 1);
+      };
+      const auto add_dk = [&]() {
+        ok = ok && bar_wait(&ds_full, (u - 1) & 1, abort);
+        fence_after();
+        if (!ok) return;
+        product_parts<STEP>(dk_at, dp_at, prev_q, dd, u > 1);
+        if (prev_last) commit(&q_empty[prev_slot]);
+      };
+      for (; !at.done && ok; at.next_tile(p, b, group, kt, length)) {
+        const int slot = at.n & 1, count = at.count();
+        ok = bar_wait(&q_full[slot], (at.n >> 1) & 1, abort);
+        if (ok && at.state.padded) ok = bar_wait(&cleared, clears++ & 1, abort);
+        for (int half = 0; half < count && ok; ++half, ++u) {
+          const uint64_t q = qg_desc + slot * 2 * kTileDesc + half * kHalfTile;
+          if (u > 0) add_dv();
           if (!ok) break;
           fence_after();
-          if (elect_one()) product_tokens(tmem + 256, tmem, 64, by_tokens(prev + Shape::kTile), dd, n > 1);
-          __syncwarp();
-        }
-        if (u < steps) {
-          ok = warp_wait(&q_full[n % 2], (n / 2) & 1, abort);
+          product_channels<DP>(tmem, k_desc, q, ds);
+          commit(&s_full);
+          if (u > 0) add_dk();
           if (!ok) break;
-          fence_after();
-          if (p.qdoc) {
-            // Padded queries' rows and gradients, whatever they hold, count for nothing.
-            const int nq = (p.Sq + kDocTile - 1) / kDocTile;
-            if (p.qtile[(int64_t)b * nq + i0 / kDocTile].padded) {
-              char* stage = ring + (n % 2) * 2 * Shape::kTile;
-              clear_rows<DP>(stage, p.qdoc + (int64_t)b * p.Sq, i0, p.Sq);
-              clear_rows<DP>(stage + Shape::kTile, p.qdoc + (int64_t)b * p.Sq, i0, p.Sq);
-            }
-          }
-          if (elect_one()) {
-            product_channels<DP>(tmem, by_channels(k_addr), by_channels(next), ds);
-            commit(&s_full);
-          }
-          __syncwarp();
+          product_channels<DP>(dp_at, v_desc, q + kTileDesc, ds);
+          commit(&dp_full);
+          prev_slot = slot, prev_q = qg_tokens + slot * 2 * kTileDesc + half * 4 * kTokenStep, prev_last = half + 1 == count;
         }
-        if (n > 0) {
-          ok = warp_wait(&ds_full, (n - 1) & 1, abort);
-          if (!ok) break;
-          fence_after();
-          if (elect_one()) {
-            product_tokens(tmem + 384, tmem + 128, 64, by_tokens(prev), dd, n > 1);
-            commit(&q_empty[(n - 1) & 1]);
-            if (u == steps) commit(&done);
-          }
-          __syncwarp();
-        }
-        if (u < steps) {
-          if (elect_one()) {
-            product_channels<DP>(tmem + 128, by_channels(v_addr), by_channels(next + Shape::kTile), ds);
-            commit(&dp_full);
-          }
-          __syncwarp();
-        }
-        ++n;
       }
-      if (!ok) {
-        if (elect_one()) commit(&done);
-        __syncwarp();
-        warp_wait(&done, 0, abort);
+      if (ok && u > 0) {
+        add_dv();
+        add_dk();
       }
+      commit(&done);
+      if (!ok) bar_wait(&done, 0, abort);
     }
   }
   __syncthreads();
   if (warp == kMmaWarp) {
     fence_after();
-    tmem_free<512>(tmem);
+    tmem_free<Shape::kColumns>(tmem);
   }
 }
 
@@ -1060,7 +1112,7 @@ cudaError_t launch_fwd(const AttnParams& p, const CUtensorMap (&m)[4], cudaStrea
   static std::atomic<uint64_t> set{0};
   cudaError_t e = abi::allow_smem(attn_tc_fwd_kernel<T, DP, MODS>, Shape::kSmem, set);
   if (e != cudaSuccess) return e;
-  const dim3 grid((p.Sq + 2 * kTileTokens - 1) / (2 * kTileTokens), p.H, p.B);
+  const dim3 grid(p.H * p.B, (p.Sq + 2 * kTileTokens - 1) / (2 * kTileTokens));
   attn_tc_fwd_kernel<T, DP, MODS><<<grid, Shape::kThreads, Shape::kSmem, st>>>(p, m[0], m[1], m[2]);
   return cudaGetLastError();
 }
@@ -1072,9 +1124,10 @@ cudaError_t launch_bwd(const AttnParams& p, const CUtensorMap (&m)[4], cudaStrea
   cudaError_t e = abi::allow_smem(attn_tc_dq_kernel<T, DP, MODS>, Shape::kSmem, set_q);
   if (e == cudaSuccess) e = abi::allow_smem(attn_tc_dkv_kernel<T, DP, MODS>, Shape::kSmem, set_k);
   if (e != cudaSuccess) return e;
-  attn_tc_dq_kernel<T, DP, MODS><<<dim3((p.Sq + kTileTokens - 1) / kTileTokens, p.H, p.B), kThreads, Shape::kSmem, st>>>(p, m[0], m[1], m[2], m[3]);
+  const auto tiles = [](int n) { return (unsigned)((n + kTileTokens - 1) / kTileTokens); };
+  attn_tc_dq_kernel<T, DP, MODS><<<dim3(p.H * p.B, tiles(p.Sq)), Shape::kThreads, Shape::kSmem, st>>>(p, m[0], m[1], m[2], m[3]);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  attn_tc_dkv_kernel<T, DP, MODS><<<dim3((p.Sk + kTileTokens - 1) / kTileTokens, p.Hkv, p.B), kThreads, Shape::kSmem, st>>>(p, m[0], m[1], m[2], m[3]);
+  attn_tc_dkv_kernel<T, DP, MODS><<<dim3(p.Hkv * p.B, tiles(p.Sk)), Shape::kThreads, Shape::kSmem, st>>>(p, m[0], m[1], m[2], m[3]);
   return cudaGetLastError();
 }
 

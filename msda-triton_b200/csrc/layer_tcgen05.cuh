@@ -146,10 +146,13 @@ __device__ __forceinline__ void product_half(uint32_t d, uint32_t p, uint64_t t,
   for (int k = 0; k < 4; ++k) mma_ts(d, p + k * 8, t + k * kTokenStep, idesc, add || k > 0);
 }
 
-// The same over 128 tokens: tokens 64... of p from column p + high.
-__device__ __forceinline__ void product_tokens(uint32_t d, uint32_t p, int high, uint64_t t, uint32_t idesc, bool add) {
-  product_half(d, p, t, idesc, add);
-  product_half(d, p + high, t + 4 * kTokenStep, idesc, true);
+// The same over N tokens, p in two parts: the first half of the tokens from
+// column p, the others from column p + N / 2.
+template <int N>
+__device__ __forceinline__ void product_parts(uint32_t d, uint32_t p, uint64_t t, uint32_t idesc, bool add) {
+#pragma unroll
+  for (int k = 0; k < N / 16; ++k)
+    mma_ts(d, p + (k < N / 32 ? k * 8 : N / 2 + (k - N / 32) * 8), t + k * kTokenStep, idesc, add || k > 0);
 }
 
 __device__ __forceinline__ void commit(uint64_t* bar) {
