@@ -18,14 +18,17 @@
 namespace msda {
 namespace tc {
 
+// What the scores of a kernel's instance go through.
+constexpr int kCapped = 1, kSloped = 2;
+
 constexpr int kSoftmaxThreads = 256;
 constexpr int kThreads = kSoftmaxThreads + 128;  // two warpgroups of softmax, one of the other roles
 constexpr int kLoadWarp = 8, kMmaWarp = 9;
 
 // The launch has 168 registers a thread; the softmax takes what the other
-// warpgroup leaves: 256 x 224 + 128 x 56 = 384 x 168.
-__device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 224;"); }
-__device__ __forceinline__ void leave_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 56;"); }
+// warpgroup leaves: 256 x 216 + 128 x 72 = 384 x 168.
+__device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 216;"); }
+__device__ __forceinline__ void leave_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 72;"); }
 
 template <typename T> struct IsBf16 { static constexpr bool value = false; };
 template <> struct IsBf16<__nv_bfloat16> { static constexpr bool value = true; };
@@ -229,7 +232,7 @@ struct FwdShape {
   static constexpr int kColumns = DP > 64 ? 512 : 256;
 };
 
-template <typename T, int DP, bool MODS>
+template <typename T, int DP, int MODE>
 __global__ void __launch_bounds__(FwdShape<DP>::kThreads, FwdShape<DP>::kCtas)
     attn_tc_fwd_kernel(const AttnParams p, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                        const __grid_constant__ CUtensorMap vmap) {
@@ -284,12 +287,12 @@ __global__ void __launch_bounds__(FwdShape<DP>::kThreads, FwdShape<DP>::kCtas)
       tmem_wait_load();
       const int j0 = at.j * kTileTokens + at.half * 64;
       float factor = f.scale2;
-      if constexpr (MODS) {
-        if (p.cap != 0.0f) {
+      {
+        if constexpr ((MODE & kCapped) != 0) {
           cap_scores(f, s);
           factor = 1.0f;
         }
-        if (p.slopes) {
+        if constexpr ((MODE & kSloped) != 0) {
           const float far = (float)(row.place - j0);
 #pragma unroll
           for (int c = 0; c < STEP; ++c) s[c] = fmaf(-f.slope2, fabsf(far - (float)c), s[c] * factor);
@@ -522,12 +525,12 @@ struct BwdShape {
 // A thread's N probabilities from its scores, in place; with a cap its
 // derivative 1 - tanh^2 in t2. far(c): places between query and key; lse(c, ..):
 // minus the log-sum-exp, to base 2, of columns c and c + 1, and of c + 2 and c + 3.
-template <bool MODS, int N, typename Far, typename Lse>
-__device__ __forceinline__ void probabilities(const AttnParams& p, const ScoreForm& f, float (&s)[N], float (&t2)[MODS ? N : 2],
+template <int MODE, int N, typename Far, typename Lse>
+__device__ __forceinline__ void probabilities(const AttnParams& p, const ScoreForm& f, float (&s)[N], float (&t2)[MODE & kCapped ? N : 2],
                                               Far far, Lse lse) {
   float factor = f.scale2;
-  if constexpr (MODS) {
-    if (p.cap != 0.0f) {
+  {
+    if constexpr ((MODE & kCapped) != 0) {
       cap_scores(f, s);
       const float inv = -1.0f / (f.cap2 * f.cap2);
       const uint64_t inv2 = pair_of(inv, inv), one = pair_of(1.0f, 1.0f);
@@ -538,7 +541,7 @@ __device__ __forceinline__ void probabilities(const AttnParams& p, const ScoreFo
       }
       factor = 1.0f;
     }
-    if (p.slopes) {
+    if constexpr ((MODE & kSloped) != 0) {
 #pragma unroll
       for (int c = 0; c < N; ++c) s[c] = fmaf(-f.slope2, fabsf(far(c)), s[c] * factor);
       factor = 1.0f;
@@ -626,7 +629,7 @@ __device__ __forceinline__ void write_row(T* out, bool in, uint32_t at, int firs
   }
 }
 
-template <typename T, int DP, bool MODS>
+template <typename T, int DP, int MODE>
 __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
     attn_tc_dq_kernel(const AttnParams p, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                       const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap gmap) {
@@ -703,14 +706,12 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
       ok = warp_wait(&s_full[u & 1], (u >> 1) & 1, abort);
       if (!ok) break;
       fence_after();
-      float s[N], t2[MODS ? N : 2];
+      float s[N], t2[MODE & kCapped ? N : 2];
       load_row(s_at, s);
       const int seen = row.limit - c0;
       const float away = (float)(row.place - c0);
-      probabilities<MODS>(p, f, s, t2, [&](int c) { return away - (float)c; }, [&](int, uint64_t& a, uint64_t& d) { a = d = lse2; });
-      if constexpr (MODS) {
-        if (p.cap != 0.0f) multiply(s, t2);
-      }
+      probabilities<MODE>(p, f, s, t2, [&](int c) { return away - (float)c; }, [&](int, uint64_t& a, uint64_t& d) { a = d = lse2; });
+      if constexpr ((MODE & kCapped) != 0) multiply(s, t2);
       bool masked = false;
       if (!__all_sync(kFullMask, seen >= N)) {
         masked = true;
@@ -880,7 +881,7 @@ struct __align__(16) QueryStats {
   int limit[STEP], place[STEP], doc[STEP];
 };
 
-template <typename T, int DP, bool MODS>
+template <typename T, int DP, int MODE>
 __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
     attn_tc_dkv_kernel(const AttnParams p, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                        const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap gmap) {
@@ -959,13 +960,13 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
       ok = ok && warp_wait(&s_full, turn, abort);
       if (!ok) continue;
       fence_after();
-      float s[N], t2[MODS ? N : 2];
+      float s[N], t2[MODE & kCapped ? N : 2];
       load_row(s_at, s);
       const auto pairs = [&](const float* from, int c, uint64_t& a, uint64_t& d) {
         const float4 v = *reinterpret_cast<const float4*>(from + c0 + c);
         a = pair_of(v.x, v.y), d = pair_of(v.z, v.w);
       };
-      probabilities<MODS>(p, f, s, t2, [&](int c) { return (float)(q.place[c0 + c] - j); },
+      probabilities<MODE>(p, f, s, t2, [&](int c) { return (float)(q.place[c0 + c] - j); },
                           [&](int c, uint64_t& a, uint64_t& d) { pairs(q.lse, c, a, d); });
       if (!whole) {
 #pragma unroll
@@ -990,9 +991,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
         }
       }
       store_row<T>(s_at, s, &p_full);
-      if constexpr (MODS) {
-        if (p.cap != 0.0f) multiply(s, t2);
-      }
+      if constexpr ((MODE & kCapped) != 0) multiply(s, t2);
       ok = warp_wait(&dp_full, turn, abort);
       if (!ok) continue;
       fence_after();
@@ -1106,36 +1105,36 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
 // ---------------------------------------------------------------------------
 bool make_map(CUtensorMap* map, const void* base, bool bf16, int64_t D, int64_t H, int64_t S, int64_t B, const int64_t (&strides)[3]);
 
-template <typename T, int DP, bool MODS>
+template <typename T, int DP, int MODE>
 cudaError_t launch_fwd(const AttnParams& p, const CUtensorMap (&m)[4], cudaStream_t st) {
   using Shape = FwdShape<DP>;
   static std::atomic<uint64_t> set{0};
-  cudaError_t e = abi::allow_smem(attn_tc_fwd_kernel<T, DP, MODS>, Shape::kSmem, set);
+  cudaError_t e = abi::allow_smem(attn_tc_fwd_kernel<T, DP, MODE>, Shape::kSmem, set);
   if (e != cudaSuccess) return e;
   const dim3 grid(p.H * p.B, (p.Sq + 2 * kTileTokens - 1) / (2 * kTileTokens));
-  attn_tc_fwd_kernel<T, DP, MODS><<<grid, Shape::kThreads, Shape::kSmem, st>>>(p, m[0], m[1], m[2]);
+  attn_tc_fwd_kernel<T, DP, MODE><<<grid, Shape::kThreads, Shape::kSmem, st>>>(p, m[0], m[1], m[2]);
   return cudaGetLastError();
 }
 
-template <typename T, int DP, bool MODS>
+template <typename T, int DP, int MODE>
 cudaError_t launch_bwd(const AttnParams& p, const CUtensorMap (&m)[4], cudaStream_t st) {
   using Shape = BwdShape<DP>;
   static std::atomic<uint64_t> set_q{0}, set_k{0};
-  cudaError_t e = abi::allow_smem(attn_tc_dq_kernel<T, DP, MODS>, Shape::kSmem, set_q);
-  if (e == cudaSuccess) e = abi::allow_smem(attn_tc_dkv_kernel<T, DP, MODS>, Shape::kSmem, set_k);
+  cudaError_t e = abi::allow_smem(attn_tc_dq_kernel<T, DP, MODE>, Shape::kSmem, set_q);
+  if (e == cudaSuccess) e = abi::allow_smem(attn_tc_dkv_kernel<T, DP, MODE>, Shape::kSmem, set_k);
   if (e != cudaSuccess) return e;
   const auto tiles = [](int n) { return (unsigned)((n + kTileTokens - 1) / kTileTokens); };
-  attn_tc_dq_kernel<T, DP, MODS><<<dim3(p.H * p.B, tiles(p.Sq)), Shape::kThreads, Shape::kSmem, st>>>(p, m[0], m[1], m[2], m[3]);
+  attn_tc_dq_kernel<T, DP, MODE><<<dim3(p.H * p.B, tiles(p.Sq)), Shape::kThreads, Shape::kSmem, st>>>(p, m[0], m[1], m[2], m[3]);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  attn_tc_dkv_kernel<T, DP, MODS><<<dim3(p.Hkv * p.B, tiles(p.Sk)), Shape::kThreads, Shape::kSmem, st>>>(p, m[0], m[1], m[2], m[3]);
+  attn_tc_dkv_kernel<T, DP, MODE><<<dim3(p.Hkv * p.B, tiles(p.Sk)), Shape::kThreads, Shape::kSmem, st>>>(p, m[0], m[1], m[2], m[3]);
   return cudaGetLastError();
 }
 
-template <typename T, bool MODS>
+template <typename T, int MODE>
 cudaError_t launch_by_size(const AttnParams& p, const CUtensorMap (&m)[4], bool backward, cudaStream_t st) {
-  if (p.D <= 32) return backward ? launch_bwd<T, 32, MODS>(p, m, st) : launch_fwd<T, 32, MODS>(p, m, st);
-  if (p.D <= 64) return backward ? launch_bwd<T, 64, MODS>(p, m, st) : launch_fwd<T, 64, MODS>(p, m, st);
-  return backward ? launch_bwd<T, 128, MODS>(p, m, st) : launch_fwd<T, 128, MODS>(p, m, st);
+  if (p.D <= 32) return backward ? launch_bwd<T, 32, MODE>(p, m, st) : launch_fwd<T, 32, MODE>(p, m, st);
+  if (p.D <= 64) return backward ? launch_bwd<T, 64, MODE>(p, m, st) : launch_fwd<T, 64, MODE>(p, m, st);
+  return backward ? launch_bwd<T, 128, MODE>(p, m, st) : launch_fwd<T, 128, MODE>(p, m, st);
 }
 
 template <typename T>
@@ -1146,8 +1145,12 @@ int run(const AttnParams& p, bool backward, cudaStream_t st) {
       !make_map(&m[2], p.v, bf16, p.D, p.Hkv, p.Sk, p.B, p.vs) ||
       (backward && !make_map(&m[3], p.go, bf16, p.D, p.H, p.Sq, p.B, p.gs)))
     return -1;
-  const bool mods = p.cap != 0.0f || p.slopes;
-  return (int)(mods ? launch_by_size<T, true>(p, m, backward, st) : launch_by_size<T, false>(p, m, backward, st));
+  switch ((p.cap != 0.0f ? kCapped : 0) | (p.slopes ? kSloped : 0)) {
+    case 0: return (int)launch_by_size<T, 0>(p, m, backward, st);
+    case kCapped: return (int)launch_by_size<T, kCapped>(p, m, backward, st);
+    case kSloped: return (int)launch_by_size<T, kSloped>(p, m, backward, st);
+    default: return (int)launch_by_size<T, kCapped | kSloped>(p, m, backward, st);
+  }
 }
 
 }  // namespace tc
