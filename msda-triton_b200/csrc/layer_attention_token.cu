@@ -3,14 +3,16 @@
 //
 // Bound by HBM: the visible keys and values are read once. The heads that share
 // a key head and the queries are packed into the 16 rows of an m16n8k16 product,
-// so that shared heads cost no further reads. Keys and values go from global
-// memory straight to the registers of that product, 16 bytes a thread: the
-// order of channels within a product is free as long as both sides agree, so a
-// thread takes 8 neighbouring channels of a key for four k-slots of two products;
-// for the values a thread takes a few neighbouring channels of four keys and
-// pairs the keys by byte permutes. No shared memory, no barrier in the loop: the
-// latency is covered by the loads of the SM's other warps. The keys are split
-// over CTAs, whose parts the combining kernel joins.
+// so that shared heads cost no further reads. Each warp has a ring of its own in
+// shared memory, which asynchronous copies of 16 bytes fill two steps of 16 keys
+// ahead (padded keys as zeros): no barrier in the loop, and enough bytes in
+// flight. (Loading straight to registers, a step at a time, read a cache of 1.3 GB
+// at 3.6 TB/s.) The order of channels within a product is free as long as both
+// sides agree, so a thread takes 8 neighbouring channels of a key for four k-slots
+// of two products; for the values it takes a few neighbouring channels of four keys
+// and pairs the keys by byte permutes. The rows' pitches keep both kinds of read
+// free of bank conflicts. The keys are split over CTAs, whose parts the combining
+// kernel joins.
 #include "layer_attention.cuh"
 
 namespace msda {
@@ -39,22 +41,36 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return u.raw;
 }
 
-// 16 bytes of the cache, which is read once: past L1.
-__device__ __forceinline__ uint4 load_cache(const void* p) {
-  uint4 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
-  return r;
+// 16 bytes to shared memory, or zeros.
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool in) {
+  const int bytes = in ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
 
+constexpr int kAhead = 3;  // slots of a warp's ring
+
+// Pitches in bytes: of a key, an odd multiple of 64 bytes (two keys' quarters of 64
+// bytes fill the banks); of a value, 16 bytes past a multiple of 64 (four pairs of
+// values' first 16 bytes lie 32 bytes apart).
+template <int DP>
+struct Ring {
+  static constexpr int kKey = DP == 32 ? 64 : DP * 2 + 64;
+  static constexpr int kValue = DP * 2 + 16;
+  static constexpr int kSlot = kStep * (kKey + kValue);
+  static constexpr int kBytes = kWarps * kAhead * kSlot;
+};
+
 template <typename T, int DP>
-__global__ void __launch_bounds__(kWarps * 32, DP == 128 ? 2 : 4) attn_token_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(kWarps * 32, DP == 128 ? 2 : DP == 64 ? 3 : 4) attn_token_kernel(const AttnParams p) {
   constexpr int KC = DP / 32;               // 32-channel chunks of a key
   constexpr int VE = DP == 32 ? 4 : 8;      // neighbouring channels of a value that a thread takes
   constexpr int VC = DP / (8 * VE);         // groups of them
   constexpr int NT = DP / 8;                // output tiles of 8 channels
-  __shared__ float part_o[kWarps - 1][16][DP + 4];
+  using R = Ring<DP>;
+  extern __shared__ __align__(128) char ring[];
   __shared__ float2 part_ml[kWarps][16];
+  static_assert((kWarps - 1) * 16 * (DP + 4) * 4 <= R::kBytes, "the parts take the ring's place");
+  float (*part_o)[16][DP + 4] = reinterpret_cast<float (*)[16][DP + 4]>(ring);
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, t = lane % 4;
   const int group = p.H / p.Hkv, rows = p.Sq * group;
   const int tiles = (rows + 15) / 16;
@@ -90,35 +106,53 @@ __global__ void __launch_bounds__(kWarps * 32, DP == 128 ? 2 : 4) attn_token_ker
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[n][i] = 0.0f;
 
-  for (int j0 = first + warp * kStep; j0 < last; j0 += kWarps * kStep) {
+  char* mine_ring = ring + warp * kAhead * R::kSlot;
+  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(mine_ring);
+  // A step's keys and values, 16 bytes a lane at a time; a group of copies each.
+  const auto fill = [&](int j0, int slot) {
+    if (j0 < last) {
+      constexpr int kPieces = DP / 8;
+      const uint32_t key_at = ring_at + slot * R::kSlot, value_at = key_at + kStep * R::kKey;
+#pragma unroll
+      for (int i = 0; i < kStep * kPieces / 32; ++i) {
+        const int at = i * 32 + lane, r = at / kPieces, d = at % kPieces * 8, j = j0 + r;
+        const bool in = j < last && d < p.D && (!kdoc || __ldg(kdoc + j) >= 0);
+        const int64_t jj = in ? j : first;  // an address in the cache, whether read or not
+        copy16(key_at + r * R::kKey + d * 2, kb + jj * p.ks[1] + (in ? d : 0), in);
+        copy16(value_at + r * R::kValue + d * 2, vb + jj * p.vs[1] + (in ? d : 0), in);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  const int start = first + warp * kStep;
+#pragma unroll
+  for (int i = 0; i < kAhead - 1; ++i) fill(start + i * kWarps * kStep, i);
+  int slot = 0;
+  for (int j0 = start; j0 < last; j0 += kWarps * kStep) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 2) : "memory");
+    __syncwarp();
+    // The slot that the step before has left.
+    fill(j0 + (kAhead - 1) * kWarps * kStep, slot == 0 ? kAhead - 1 : slot - 1);
+    const char* key_row = mine_ring + slot * R::kSlot;
+    const char* value_row = key_row + kStep * R::kKey;
+    slot = slot + 1 == kAhead ? 0 : slot + 1;
     uint4 kr[2][KC];
     uint32_t vr[4][VC][VE / 2];
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      const int j = j0 + g + 8 * n;
-      const bool in = j < last && (!kdoc || __ldg(kdoc + j) >= 0);
+    for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int c = 0; c < KC; ++c) {
-        const int d = c * 32 + t * 8;
-        kr[n][c] = make_uint4(0, 0, 0, 0);
-        if (in && d < p.D) kr[n][c] = load_cache(kb + j * p.ks[1] + d);
-      }
-    }
+      for (int c = 0; c < KC; ++c)
+        kr[n][c] = *reinterpret_cast<const uint4*>(key_row + (g + 8 * n) * R::kKey + c * 64 + t * 16);
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
-      const int j = j0 + t * 2 + (n & 1) + (n >> 1) * 8;
-      const bool in = j < last && (!kdoc || __ldg(kdoc + j) >= 0);
+      const char* v = value_row + (t * 2 + (n & 1) + (n >> 1) * 8) * R::kValue;
 #pragma unroll
       for (int c = 0; c < VC; ++c) {
-        const int d = c * 64 + g * VE;
-        const T* v = vb + j * p.vs[1] + d;
         if constexpr (VE == 8) {
-          uint4 u = make_uint4(0, 0, 0, 0);
-          if (in && d < p.D) u = load_cache(v);
+          const uint4 u = *reinterpret_cast<const uint4*>(v + c * 128 + g * 16);
           vr[n][c][0] = u.x, vr[n][c][1] = u.y, vr[n][c][2] = u.z, vr[n][c][3] = u.w;
         } else {
-          uint2 u = make_uint2(0, 0);
-          if (in && d < p.D) u = __ldg(reinterpret_cast<const uint2*>(v));
+          const uint2 u = *reinterpret_cast<const uint2*>(v + g * 8);
           vr[n][c][0] = u.x, vr[n][c][1] = u.y;
         }
       }
@@ -183,7 +217,9 @@ __global__ void __launch_bounds__(kWarps * 32, DP == 128 ? 2 : 4) attn_token_ker
         mma16816<T>(o[c * VE + e], pa, b0, b1);
       }
   }
-  // Join the CTA's warps.
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();
+  // Join the CTA's warps, in the ring's place.
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     l[i] += __shfl_xor_sync(kFullMask, l[i], 1);
@@ -285,10 +321,16 @@ template <typename T>
 cudaError_t token_t(const AttnParams& p, cudaStream_t st) {
   const int rows = p.Sq * (p.H / p.Hkv);
   const dim3 grid(p.splits, p.Hkv * ((rows + 15) / 16), p.B);
-  if (p.D <= 32) attn_token_kernel<T, 32><<<grid, kWarps * 32, 0, st>>>(p);
-  else if (p.D <= 64) attn_token_kernel<T, 64><<<grid, kWarps * 32, 0, st>>>(p);
-  else attn_token_kernel<T, 128><<<grid, kWarps * 32, 0, st>>>(p);
-  return cudaGetLastError();
+  const auto launch = [&](auto kernel, int smem, std::atomic<uint64_t>& set) {
+    cudaError_t e = abi::allow_smem(kernel, smem, set);
+    if (e != cudaSuccess) return e;
+    kernel<<<grid, kWarps * 32, smem, st>>>(p);
+    return cudaGetLastError();
+  };
+  static std::atomic<uint64_t> set[3];
+  if (p.D <= 32) return launch(attn_token_kernel<T, 32>, Ring<32>::kBytes, set[0]);
+  if (p.D <= 64) return launch(attn_token_kernel<T, 64>, Ring<64>::kBytes, set[1]);
+  return launch(attn_token_kernel<T, 128>, Ring<128>::kBytes, set[2]);
 }
 
 }  // namespace

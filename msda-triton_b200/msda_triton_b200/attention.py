@@ -14,10 +14,9 @@ import math
 import struct
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import _DTYPE_CODE, _FLOAT_DTYPES, _device_guard, _raw_stream
+from .ops import _DTYPE_CODE, _FLOAT_DTYPES, _apply, _device_guard, _once, _raw_stream
 
 # msda_attention_args of include/msda_layer_b200.h, packed in one call.
 _ARGS = struct.Struct("@10P3q4i12q2f5P2iPN")
@@ -88,7 +87,7 @@ class _AttentionFunction(torch.autograd.Function):
         return out, lse
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad_out, _):
         if grad_out is None:
             return (None,) * 5
@@ -196,7 +195,7 @@ def attention(
         raise ValueError("attention: all tensors must be on the same CUDA device")
     options = (scale, softcap, 1 if causal else 0, -1 if shared_document is None else int(shared_document))
     if (query.requires_grad or key.requires_grad or value.requires_grad) and torch.is_grad_enabled():
-        out, lse = _AttentionFunction.apply(query, key, value, options, tensors)
+        out, lse = _apply(_AttentionFunction, query, key, value, options, tensors)
     else:
         out, lse, *_ = _forward(query, key, value, options, tensors, return_lse, False)
     return (out, lse) if return_lse else out

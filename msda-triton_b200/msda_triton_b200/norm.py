@@ -10,10 +10,9 @@ bitwise reproducible. There is no CPU path.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import _DTYPE_CODE, _FLOAT_DTYPES, _device_guard, _raw_stream
+from .ops import _DTYPE_CODE, _FLOAT_DTYPES, _apply, _device_guard, _once, _raw_stream
 
 
 def _as_rows(x: torch.Tensor) -> torch.Tensor:
@@ -67,7 +66,7 @@ class _LayerNormFunction(torch.autograd.Function):
         return (y, total) if want_sum else y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad_y, grad_sum=None):
         weight, bias, rows, res, stats = ctx.saved_tensors
         N, C = rows.shape
@@ -154,6 +153,6 @@ def layer_norm(
     if bias is not None:
         bias = bias.contiguous()
     if grad and torch.is_grad_enabled():
-        return _LayerNormFunction.apply(x, residual, weight, bias, float(eps), bool(return_sum))
+        return _apply(_LayerNormFunction, x, residual, weight, bias, float(eps), bool(return_sum))
     y, total, *_ = _forward(x, residual, weight, bias, float(eps), return_sum, False)
     return (y, total) if return_sum else y

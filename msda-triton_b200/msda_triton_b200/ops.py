@@ -83,6 +83,25 @@ def _raw_stream(device: torch.device) -> int:
     return _stream_of_index(torch.cuda.current_device() if index is None else index)
 
 
+def _once(backward):
+    """once_differentiable for the layer operators: its checks run only where a
+    graph of the gradient is asked for (create_graph=True), and raise there."""
+    checked = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return checked(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return run
+
+
+def _apply(function, *args):
+    """function.apply, past its search for functorch wrappers (5 us a call)
+    where no functorch transform is active."""
+    if torch._C._are_functorch_transforms_active():
+        return function.apply(*args)
+    return super(torch.autograd.Function, function).apply(*args)
+
+
 def _forward(value, spatial_shapes, level_start_index, sampling_locations, attention_weights):
     B, S, M, D = value.shape
     _, Q, _, L, K, _ = sampling_locations.shape

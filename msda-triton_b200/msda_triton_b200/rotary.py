@@ -12,10 +12,9 @@ import ctypes
 from collections.abc import Sequence
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import _DTYPE_CODE, _FLOAT_DTYPES, _device_guard, _raw_stream
+from .ops import _DTYPE_CODE, _FLOAT_DTYPES, _apply, _device_guard, _once, _raw_stream
 
 _LADDER = {"axis": 0, "shared": 1}
 _PAIRING = {"half": 0, "interleaved": 1}
@@ -60,7 +59,7 @@ class _RotaryFunction(torch.autograd.Function):
         return out if key is None else (out, key_out)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad_query, grad_key=None):
         positions, = ctx.saved_tensors
         if grad_query is None and grad_key is None:
@@ -145,6 +144,6 @@ def rotary(
     args = (query, key, positions.contiguous(), (ctypes.c_int32 * A)(*axis_dims), float(base), _LADDER[ladder],
             _PAIRING[pairing])
     if (query.requires_grad or (key is not None and key.requires_grad)) and torch.is_grad_enabled():
-        return _RotaryFunction.apply(*args)
+        return _apply(_RotaryFunction, *args)
     out, key_out = _turn(*args, 0)
     return out if key is None else (out, key_out)
