@@ -74,7 +74,10 @@ __global__ void __launch_bounds__(kWarps * 32, DP == 128 ? 2 : DP == 64 ? 3 : 4)
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, t = lane % 4;
   const int group = p.H / p.Hkv, rows = p.Sq * group;
   const int tiles = (rows + 15) / 16;
-  const int hk = blockIdx.y / tiles, r0 = blockIdx.y % tiles * 16, b = blockIdx.z, split = blockIdx.x;
+  // The heads are the fast dimension: they read neighbouring bytes of the cache's
+  // rows at about the same time.
+  const int hk = blockIdx.x / tiles, r0 = blockIdx.x % tiles * 16, b = blockIdx.z, split = blockIdx.y;
+  pdl_trigger();
   const int length = attn_length(p, b);
   int first, last;
   split_range(rows_limit(p, b, (min(r0 + 16, rows) + group - 1) / group, length), p.splits, split, first, last);
@@ -168,6 +171,15 @@ __global__ void __launch_bounds__(kWarps * 32, DP == 128 ? 2 : DP == 64 ? 3 : 4)
       }
     }
     // s[n][2 i + e]: row g + 8 i, key j0 + 8 n + 2 t + e.
+    bool small = true;  // scores well below the cap, the common case
+    if (p.cap != 0.0f) {
+      float big = 0.0f;
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) big = fmaxf(big, fabsf(s[n][i]));
+      small = __all_sync(kFullMask, big * fabsf(f.inv_cap) < kTanhSmall);
+    }
     float top[2] = {m[0], m[1]};
 #pragma unroll
     for (int n = 0; n < 2; ++n)
@@ -178,7 +190,10 @@ __global__ void __launch_bounds__(kWarps * 32, DP == 128 ? 2 : DP == 64 ? 3 : 4)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           float x = s[n][2 * i + e] * f.scale2;
-          if (p.cap != 0.0f) x = tanh_of(s[n][2 * i + e] * f.inv_cap) * f.cap2;
+          if (p.cap != 0.0f) {
+            x = s[n][2 * i + e] * f.inv_cap;
+            x = (small ? tanh_small(x) : tanh_of(x)) * f.cap2;
+          }
           if (p.slopes) x = fmaf(-slope[i], (float)abs(row[i].place - j), x);
           const bool seen = j < last && j < row[i].limit && (!kdoc || same_document(row[i].doc, kd, p.shared));
           s[n][2 * i + e] = seen ? x : -INFINITY;
@@ -280,7 +295,7 @@ __global__ void __launch_bounds__(kWarps * 32, DP == 128 ? 2 : DP == 64 ? 3 : 4)
   }
 }
 
-// Joins the parts of each row in the parts' order: a warp a row.
+// Joins the parts of each row (at most 64) in the parts' order: a warp a row.
 template <typename T>
 __global__ void __launch_bounds__(128) attn_combine_kernel(const AttnParams p) {
   pdl_wait();
@@ -288,24 +303,34 @@ __global__ void __launch_bounds__(128) attn_combine_kernel(const AttnParams p) {
   const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / 32;
   if (row >= rows) return;
   const int lane = threadIdx.x % 32;
-  float top = -INFINITY;
-  for (int s = lane; s < p.splits; s += 32) top = fmaxf(top, __ldcg(&p.part_ml[s * rows + row]).x);
+  // A lane has two parts' maximum and sum.
+  float2 ml[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    ml[i] = make_float2(-INFINITY, 0.0f);
+    if (lane + 32 * i < p.splits) ml[i] = __ldcg(&p.part_ml[(lane + 32 * i) * rows + row]);
+  }
+  float top = fmaxf(ml[0].x, ml[1].x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, o));
   const float base = top == -INFINITY ? 0.0f : top;
+  // A part without keys has no weight, and its sums were not written.
+  const float weight[2] = {ml[0].y == 0.0f ? 0.0f : exp2f(ml[0].x - base), ml[1].y == 0.0f ? 0.0f : exp2f(ml[1].x - base)};
   float total = 0.0f, acc[8];
 #pragma unroll
   for (int c = 0; c < 8; ++c) acc[c] = 0.0f;
-#pragma unroll 4
+#pragma unroll 8
   for (int s = 0; s < p.splits; ++s) {
-    const float2 ml = __ldcg(&p.part_ml[s * rows + row]);
-    const float w = exp2f(ml.x - base);
-    total = fmaf(ml.y, w, total);
-    if (ml.y == 0.0f) continue;  // a part without keys
+    const float w = __shfl_sync(kFullMask, s < 32 ? weight[0] : weight[1], s & 31);
+    const float sum = __shfl_sync(kFullMask, s < 32 ? ml[0].y : ml[1].y, s & 31);
+    total = fmaf(sum, w, total);
     const float* o = p.part_o + (s * rows + row) * p.D;
 #pragma unroll
-    for (int c = 0; c < 8; ++c)
-      if (lane + 32 * c < p.D) acc[c] = fmaf(__ldcg(o + lane + 32 * c), w, acc[c]);
+    for (int c = 0; c < 8; ++c) {
+      float v = 0.0f;
+      if (sum != 0.0f && lane + 32 * c < p.D) v = __ldcg(o + lane + 32 * c);
+      acc[c] = fmaf(v, w, acc[c]);
+    }
   }
   const float mul = total > 0.0f ? 1.0f / total : (total == 0.0f ? 0.0f : total);
   const int i = (int)(row % p.Sq), h = (int)(row / p.Sq % p.H);
@@ -320,7 +345,7 @@ __global__ void __launch_bounds__(128) attn_combine_kernel(const AttnParams p) {
 template <typename T>
 cudaError_t token_t(const AttnParams& p, cudaStream_t st) {
   const int rows = p.Sq * (p.H / p.Hkv);
-  const dim3 grid(p.splits, p.Hkv * ((rows + 15) / 16), p.B);
+  const dim3 grid(p.Hkv * ((rows + 15) / 16), p.splits, p.B);
   const auto launch = [&](auto kernel, int smem, std::atomic<uint64_t>& set) {
     cudaError_t e = abi::allow_smem(kernel, smem, set);
     if (e != cudaSuccess) return e;
