@@ -72,7 +72,7 @@ using namespace msda::abi;
 constexpr int64_t kTokenRows = 64;
 constexpr int kMaxSplits = 64;
 
-enum class Path { kSimt, kToken, kTensor };
+enum class Path { kAny, kToken, kTensor };
 
 int check(const char* fn, const msda_attention_args* a, bool backward) {
   if (!a) return fail(MSDA_ERR_INVALID_ARGUMENT, "%s: null arguments", fn);
@@ -124,7 +124,8 @@ bool tensor_layout(const msda_attention_args* a, bool backward) {
 }
 
 struct Plan {
-  Path path = Path::kSimt;
+  Path path = Path::kAny;
+  bool few = false;  // few query rows
   int splits = 1;
   int64_t q_tiles = 0, k_tiles = 0;  // document summary entries
   size_t delta = 0, part_ml = 0, part_o = 0, bytes = 0;  // byte offsets, after the summary; total
@@ -135,22 +136,22 @@ Plan plan_of(const msda_attention_args* a, bool backward) {
   const int64_t group = a->num_heads / a->num_key_heads, rows = a->num_queries * group;
   const bool tensor = tensor_layout(a, backward);
   if (tensor && a->num_keys > 0) p.path = Path::kTensor;
-  if (!backward && rows <= kTokenRows) {
+  p.few = !backward && rows <= kTokenRows;
+  if (p.few) {
     if (tensor) p.path = Path::kToken;
     // Parts of at least 512 keys, up to 16 CTAs an SM, so that streams of
     // different lengths even out; of at least 128 keys where that leaves fewer
     // than 2 CTAs an SM. (Parts of 128 keys throughout: 8 streams of 4096 keys on 8
     // heads of 128 channels took 60 us.)
-    const int64_t tiles = tensor ? (rows + 15) / 16 : (rows + 31) / 32;
+    const int64_t tiles = (rows + 15) / 16;
     const int64_t ctas = std::max<int64_t>(1, a->batch * a->num_key_heads * tiles);
     const int64_t even = std::min<int64_t>(16 * sm_count() / ctas, a->num_keys / 512);
     const int64_t fill = std::min<int64_t>(2 * sm_count() / ctas, (a->num_keys + 127) / 128);
     const int64_t s = std::min<int64_t>(std::max(even, fill), kMaxSplits);
     p.splits = s < 1 ? 1 : (int)s;
-    if (!tensor && p.splits < 2 && a->num_keys > 64) p.splits = 2;  // the packed rows' form
   }
   size_t at = 0;
-  const bool documents = a->query_documents && p.path != Path::kToken && p.splits == 1;
+  const bool documents = a->query_documents && !p.few;
   if (documents) {
     p.q_tiles = a->batch * ((a->num_queries + kDocTile - 1) / kDocTile);
     p.k_tiles = a->batch * ((a->num_keys + kDocTile - 1) / kDocTile);
@@ -241,7 +242,7 @@ int msda_attention_forward(const msda_attention_args* a, void* stream) {
     if (rc < 0) return fail(MSDA_ERR_CUDA, "%s: no tensor map for these sizes and strides", fn);
     e = (cudaError_t)rc;
   } else if (e == cudaSuccess) {
-    e = plan.path == Path::kToken ? attn_token_forward(p, a->dtype, st) : attn_simt_forward(p, a->dtype, st);
+    e = plan.path == Path::kToken ? attn_token_forward(p, a->dtype, st) : attn_tf32_forward(p, a->dtype, plan.few, st);
   }
   if (e == cudaSuccess && plan.splits > 1) e = attn_combine_launch(p, a->dtype, st);
   if (e != cudaSuccess) return cuda_fail(e, "attention launch");
@@ -280,7 +281,7 @@ int msda_attention_backward(const msda_attention_args* a, void* stream) {
     if (rc < 0) return fail(MSDA_ERR_CUDA, "%s: no tensor map for these sizes and strides", fn);
     e = (cudaError_t)rc;
   } else if (e == cudaSuccess) {
-    e = attn_simt_backward(p, a->dtype, st);
+    e = attn_tf32_backward(p, a->dtype, st);
   }
   if (e != cudaSuccess) return cuda_fail(e, "attention backward launch");
   return succeed();

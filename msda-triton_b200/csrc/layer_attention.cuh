@@ -160,10 +160,11 @@ __device__ __forceinline__ void split_range(int limit, int splits, int split, in
 
 // Launches (each returns the launch's error).
 cudaError_t attn_documents_launch(const AttnParams& p, DocTile* qtile, DocTile* ktile, cudaStream_t st);
-// p.splits > 1: the heads that share a key head are packed into row tiles and
-// the keys are split; attn_combine_launch joins the parts.
-cudaError_t attn_simt_forward(const AttnParams& p, int dtype, cudaStream_t st);
-cudaError_t attn_simt_backward(const AttnParams& p, int dtype, cudaStream_t st);
+// Any type, head size and stride. token: few queries, the keys in p.splits parts,
+// which attn_combine_launch joins where there are more than one.
+cudaError_t attn_tf32_forward(const AttnParams& p, int dtype, bool token, cudaStream_t st);
+cudaError_t attn_tf32_backward(const AttnParams& p, int dtype, cudaStream_t st);
+// The form for single tokens: 16-bit types in the tensor-core kernels' layout.
 cudaError_t attn_token_forward(const AttnParams& p, int dtype, cudaStream_t st);
 // Tensor-core kernels: 16-bit types, D a multiple of 8 up to 128, rows that
 // start on 16 bytes at strides of whole 16 bytes. 0 or a cudaError_t; -1 where a
