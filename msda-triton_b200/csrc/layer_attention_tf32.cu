@@ -2,8 +2,8 @@
 // the tensor-core kernels of layer_attention_tc.cuh do not take.
 //
 // The products run on the tensor cores by register fragments (m16n8k8, tf32 in,
-// fp32 sums): an fp32 number is the sum of two tf32 numbers to 2^-22 of its size,
-//   x y = xh yh + xh yl + xl yh  (+ xl yl, below 2^-22),
+// fp32 sums): an fp32 number is the sum of two tf32 numbers to 2^-21 of its size,
+//   x y = xh yh + xh yl + xl yh  (+ xl yl, below 2^-20 x y),
 // three products for one, at 92 TFLOP/s a bound above the 72 of the FMA pipes.
 // 16-bit inputs are tf32 numbers as they stand: their scores need one product,
 // probabilities with values two. (On the FMA pipes, with 8 x 4 sums a thread, a
@@ -31,10 +31,17 @@ struct Pitch {
   static constexpr int kRowTile = kRows * kFloats, kColTile = kCols * kFloats;
 };
 
-// x as a tf32 number and what is left of it (which the product cuts to one).
+// x cut to a tf32 number, and what is left of it, which the product cuts in turn:
+// 2^-21 of x at most is lost, in sums whose own rounding is a few times that.
 __device__ __forceinline__ void split(float x, uint32_t& high, uint32_t& low) {
-  high = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
-  low = __float_as_uint(x - __uint_as_float(high)) + 0x1000u;
+  high = __float_as_uint(x) & 0xffffe000u;
+  low = __float_as_uint(x - __uint_as_float(high));
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
 
 // d = a b (+ c)
@@ -60,17 +67,14 @@ __device__ __forceinline__ void parts(const uint32_t (&x)[N], uint32_t (&high)[N
   }
 }
 
-// c[n] += a b[n] over 8 k-slots for N tiles at a time, whose products take turns
-// in the pipe. The small products come first, from zero, and their sum joins c by
-// a rounded addition: the tensor cores cut their running sum, which over the steps
-// of a long sum would cost several digits. `rest`: what is left of b past its two
-// parts, or nothing (WHOLE).
+// d[n] += a b[n] over 8 k-slots for N tiles at a time, whose products take turns in
+// the pipe, the small ones first. The tensor cores cut their running sum, which
+// over the steps of a long sum would cost several digits: d begins at zero every
+// second step, and `join` adds it to the long sum, rounded. `rest`: what is left of
+// b past its two parts, or nothing (WHOLE).
 template <bool EXACT_A, bool EXACT_B, bool WHOLE, int N>
-__device__ __forceinline__ void products(float (*c)[4], const uint32_t (&ah)[4], const uint32_t (&al)[4], const uint32_t (&bh)[N][2],
+__device__ __forceinline__ void products(float (&d)[N][4], const uint32_t (&ah)[4], const uint32_t (&al)[4], const uint32_t (&bh)[N][2],
                                          const uint32_t (&bl)[N][2], const uint32_t (&rest)[WHOLE ? N : 1][2]) {
-  float d[N][4];
-#pragma unroll
-  for (int n = 0; n < N; ++n) d[n][0] = d[n][1] = d[n][2] = d[n][3] = 0.0f;
   if constexpr (WHOLE) {
 #pragma unroll
     for (int n = 0; n < N; ++n) mma(d[n], ah, rest[n][0], rest[n][1], d[n][0], d[n][1], d[n][2], d[n][3]);
@@ -85,6 +89,16 @@ __device__ __forceinline__ void products(float (*c)[4], const uint32_t (&ah)[4],
   }
 #pragma unroll
   for (int n = 0; n < N; ++n) mma(d[n], ah, bh[n][0], bh[n][1], d[n][0], d[n][1], d[n][2], d[n][3]);
+}
+
+template <int N>
+__device__ __forceinline__ void clear(float (&d)[N][4]) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) d[n][0] = d[n][1] = d[n][2] = d[n][3] = 0.0f;
+}
+
+template <int N>
+__device__ __forceinline__ void join(float (*c)[4], const float (&d)[N][4]) {
 #pragma unroll
   for (int n = 0; n < N; ++n)
 #pragma unroll
@@ -100,23 +114,29 @@ __device__ __forceinline__ void scores(const float* a, const float* b, int D, fl
   // b's columns 0.. with both groups of channels, then columns 8...
   const uint32_t a_at = (uint32_t)__cvta_generic_to_shared(a + (lane % 16) * P + lane / 16 * 4);
   const uint32_t b_at = (uint32_t)__cvta_generic_to_shared(b + (lane % 8 + lane / 16 * 8) * P + lane / 8 % 2 * 4);
-#pragma unroll
-  for (int n = 0; n < NT; ++n) c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.0f;
-  const int steps = (D + 7) / 8;
+  clear(c);
   const uint32_t none[1][2] = {{0, 0}};
-#pragma unroll 2
-  for (int k = 0; k < steps; ++k) {
-    uint32_t x[4], ah[4], al[4], y[(NT + 1) / 2][4], bh[NT][2], bl[NT][2];
-    ldmatrix4(x, a_at + k * 32);
+  // Two steps of 8 channels at a time (tiles are padded with zeros).
+  const int pairs = (D + 15) / 16;
+#pragma unroll 1
+  for (int k = 0; k < pairs; ++k) {
+    float d[NT][4];
+    clear(d);
 #pragma unroll
-    for (int n = 0; n < NT; n += 2) ldmatrix4(y[n / 2], b_at + n * 8 * P * 4 + k * 32);
-    parts<EXACT>(x, ah, al);
+    for (int half = 0; half < 2; ++half) {
+      uint32_t x[4], ah[4], al[4], y[(NT + 1) / 2][4], bh[NT][2], bl[NT][2];
+      ldmatrix4(x, a_at + k * 64 + half * 32);
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const uint32_t z[2] = {y[n / 2][n % 2 * 2], y[n / 2][n % 2 * 2 + 1]};
-      parts<EXACT>(z, bh[n], bl[n]);
+      for (int n = 0; n < NT; n += 2) ldmatrix4(y[n / 2], b_at + n * 8 * P * 4 + k * 64 + half * 32);
+      parts<EXACT>(x, ah, al);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const uint32_t z[2] = {y[n / 2][n % 2 * 2], y[n / 2][n % 2 * 2 + 1]};
+        parts<EXACT>(z, bh[n], bl[n]);
+      }
+      products<EXACT, EXACT, false, NT>(d, ah, al, bh, bl, none);
     }
-    products<EXACT, EXACT, false, NT>(c, ah, al, bh, bl, none);
+    join(c, d);
   }
 }
 
@@ -130,26 +150,38 @@ __device__ __forceinline__ void gather(const float (&p)[NT][4], const float* t, 
   constexpr bool REST = WHOLE && !EXACT;
   const int lane = threadIdx.x % 32;
   const float* at = t + lane % 4 * 2 * P + lane / 4;
+  constexpr int PAIR = NT < 2 ? 1 : 2;  // tiles of 8 tokens that are summed before they join
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    // Row g: tokens 2 t and 2 t + 1 are slots t and t + 4.
-    const uint32_t x[4] = {__float_as_uint(p[n][0]), __float_as_uint(p[n][2]), __float_as_uint(p[n][1]), __float_as_uint(p[n][3])};
-    uint32_t ah[4], al[4];
-    parts<false>(x, ah, al);
+  for (int n0 = 0; n0 < NT; n0 += PAIR) {
+    uint32_t ah[PAIR][4], al[PAIR][4];
+#pragma unroll
+    for (int m = 0; m < PAIR; ++m) {
+      // Row g: tokens 2 t and 2 t + 1 are slots t and t + 4.
+      const float* q = p[n0 + m];
+      const uint32_t x[4] = {__float_as_uint(q[0]), __float_as_uint(q[2]), __float_as_uint(q[1]), __float_as_uint(q[3])};
+      parts<false>(x, ah[m], al[m]);
+    }
 #pragma unroll
     for (int d = 0; d < DP / 8; d += N) {
-      uint32_t bh[N][2], bl[N][2], rest[REST ? N : 1][2];
+      float c[N][4];
+      clear(c);
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const uint32_t y[2] = {__float_as_uint(at[n * 8 * P + (d + i) * 8]), __float_as_uint(at[n * 8 * P + P + (d + i) * 8])};
-        parts<EXACT>(y, bh[i], bl[i]);
-        if constexpr (REST) {
+      for (int m = 0; m < PAIR; ++m) {
+        uint32_t bh[N][2], bl[N][2], rest[REST ? N : 1][2];
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-            rest[i][e] = __float_as_uint(__uint_as_float(y[e]) - __uint_as_float(bh[i][e]) - __uint_as_float(bl[i][e] & 0xffffe000u));
+        for (int i = 0; i < N; ++i) {
+          const float* z = at + (n0 + m) * 8 * P + (d + i) * 8;
+          const uint32_t y[2] = {__float_as_uint(z[0]), __float_as_uint(z[P])};
+          parts<EXACT>(y, bh[i], bl[i]);
+          if constexpr (REST) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              rest[i][e] = __float_as_uint(__uint_as_float(bl[i][e]) - __uint_as_float(bl[i][e] & 0xffffe000u));
+          }
         }
+        products<false, EXACT, REST, N>(c, ah[m], al[m], bh, bl, rest);
       }
-      products<false, EXACT, REST, N>(out + d, ah, al, bh, bl, rest);
+      join(out + d, c);
     }
   }
 }
@@ -232,10 +264,11 @@ __device__ __forceinline__ float inverse(float s) { return s > 0.0f ? 1.0f / s :
 
 // Scores of a warp's 16 rows and 8 NT columns to probabilities, with the rows'
 // running maximum and sum; what the rows' sums have to be multiplied by in `old`.
-// column(n, e): the key of tile n's column 2 t + e.
+// column(n, e): the key of tile n's column 2 t + e. `whole`: every row sees every
+// column.
 template <int NT, typename Far>
 __device__ __forceinline__ void softmax_step(const AttnParams& p, const ScoreForm (&f)[2], const RowView (&row)[2], float (&s)[NT][4],
-                                             const int (&kd)[NT][2], int j0, int end, Far column, float (&m)[2], float (&l)[2],
+                                             const int (&kd)[NT][2], int j0, int end, bool whole, Far column, float (&m)[2], float (&l)[2],
                                              float (&old)[2]) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -245,29 +278,37 @@ __device__ __forceinline__ void softmax_step(const AttnParams& p, const ScoreFor
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int j = j0 + column(n, e);
-        const bool seen = j < end && j < row[i].limit && (!p.kdoc || same_document(row[i].doc, kd[n][e], p.shared));
+        const bool seen = whole || (j < end && j < row[i].limit && (!p.kdoc || same_document(row[i].doc, kd[n][e], p.shared)));
         s[n][2 * i + e] = seen ? score2(p, f[i], s[n][2 * i + e], row[i].place - j, t) : -INFINITY;
         top = fmaxf(top, s[n][2 * i + e]);
       }
     top = fmaxf(m[i], max4(top));
     const float base = top == -INFINITY ? 0.0f : top;
-    old[i] = exp2f(m[i] - base);
+    old[i] = ex2(m[i] - base);
     m[i] = top;
     l[i] *= old[i];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        s[n][2 * i + e] = exp2f(s[n][2 * i + e] - base);
+        s[n][2 * i + e] = ex2(s[n][2 * i + e] - base);
         l[i] += s[n][2 * i + e];
       }
   }
 }
 
+// Slots of the forward's ring: with one, three CTAs of 128 channels share an SM,
+// and cover one another's copies (2 x 1500 tokens, 8 heads: 872 us with two).
+template <int DP>
+__host__ __device__ constexpr int forward_slots() {
+  return DP == 128 ? 1 : 2;
+}
+
 template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) attn_tf32_fwd_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(kThreads, DP == 128 ? 3 : 1) attn_tf32_fwd_kernel(const AttnParams p) {
   constexpr int NT = kCols / 8;
   constexpr bool EXACT = sizeof(T) == 2;
+  constexpr int SLOTS = forward_slots<DP>();
   using S = Pitch<DP>;
   extern __shared__ __align__(16) float smem[];
   float *qs = smem, *ring = smem + S::kRowTile;  // slots: keys, then values
@@ -303,10 +344,14 @@ __global__ void __launch_bounds__(kThreads) attn_tf32_fwd_kernel(const AttnParam
 #pragma unroll
   for (int d = 0; d < DP / 8; ++d) out[d][0] = out[d][1] = out[d][2] = out[d][3] = 0.0f;
   const auto column = [&](int n, int e) { return n * 8 + 2 * t + e; };
-  for (int slot = 0; j0 < limit; slot ^= 1) {
+  for (int slot = 0; j0 < limit; slot ^= SLOTS - 1) {
     const int j1 = next(j0 + kCols);
-    fill(j1, slot ^ 1);
-    copies_wait<1>();
+    if constexpr (SLOTS == 2) {
+      fill(j1, slot ^ 1);
+      copies_wait<1>();
+    } else {
+      copies_wait<0>();
+    }
     __syncthreads();
     const float* ks = ring + slot * 2 * S::kColTile;
     float s[NT][4], old[2];
@@ -319,7 +364,8 @@ __global__ void __launch_bounds__(kThreads) attn_tf32_fwd_kernel(const AttnParam
         const int j = j0 + column(n, e);
         kd[n][e] = p.kdoc && j < length ? __ldg(p.kdoc + (int64_t)b * p.Sk + j) : 0;
       }
-    softmax_step<NT>(p, f, row, s, kd, j0, limit, column, m, l, old);
+    const bool whole = !p.kdoc && __all_sync(kFullMask, j0 + kCols <= min(row[0].limit, row[1].limit));
+    softmax_step<NT>(p, f, row, s, kd, j0, limit, whole, column, m, l, old);
 #pragma unroll
     for (int d = 0; d < DP / 8; ++d) {
       out[d][0] *= old[0], out[d][1] *= old[0];
@@ -327,6 +373,7 @@ __global__ void __launch_bounds__(kThreads) attn_tf32_fwd_kernel(const AttnParam
     }
     gather<DP, NT, EXACT, true>(s, ks + S::kColTile, out);
     __syncthreads();
+    if constexpr (SLOTS == 1) fill(j1, 0);
     j0 = j1;
   }
 #pragma unroll
@@ -405,7 +452,7 @@ __global__ void __launch_bounds__(kThreads) attn_tf32_token_kernel(const AttnPar
       const int j = j0 + column(0, e);
       kd[0][e] = p.kdoc && j < length ? __ldg(p.kdoc + (int64_t)b * p.Sk + j) : 0;
     }
-    softmax_step<1>(p, f, row, s, kd, j0, last, column, m, l, old);
+    softmax_step<1>(p, f, row, s, kd, j0, last, false, column, m, l, old);
 #pragma unroll
     for (int d = 0; d < DP / 8; ++d) {
       out[d][0] *= old[0], out[d][1] *= old[0];
@@ -531,6 +578,7 @@ __global__ void __launch_bounds__(kThreads) attn_tf32_dq_kernel(const AttnParams
 #pragma unroll
   for (int d = 0; d < DP / 8; ++d) dq[d][0] = dq[d][1] = dq[d][2] = dq[d][3] = 0.0f;
   while (j0 < limit) {
+    const bool whole = !p.kdoc && __all_sync(kFullMask, j0 + kCols <= min(row[0].limit, row[1].limit));
     float s[NT][4], dp[NT][4];
     scores<DP, NT, EXACT>(qs + warp * 16 * S::kFloats, ring, p.D, s);
     scores<DP, NT, EXACT>(gs + warp * 16 * S::kFloats, ring + S::kColTile, p.D, dp);
@@ -542,9 +590,9 @@ __global__ void __launch_bounds__(kThreads) attn_tf32_dq_kernel(const AttnParams
         const int kd = p.kdoc && j < length ? __ldg(p.kdoc + (int64_t)b * p.Sk + j) : 0;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const bool seen = j < row[i].limit && (!p.kdoc || same_document(row[i].doc, kd, p.shared));
+          const bool seen = whole || (j < row[i].limit && (!p.kdoc || same_document(row[i].doc, kd, p.shared)));
           float th;
-          const float x = exp2f(score2(p, f, s[n][2 * i + e], row[i].place - j, th) - lse2[i]);
+          const float x = ex2(score2(p, f, s[n][2 * i + e], row[i].place - j, th) - lse2[i]);
           s[n][2 * i + e] = seen ? x * (dp[n][2 * i + e] - delta[i]) * fmaf(-th, th, 1.0f) : 0.0f;
         }
       }
@@ -639,7 +687,7 @@ __global__ void __launch_bounds__(kThreads) attn_tf32_dkv_kernel(const AttnParam
             const int j = j0 + warp * 16 + g + 8 * i;
             const bool seen = j < row.limit && (!p.kdoc || same_document(row.doc, kd[i], p.shared));
             float th;
-            const float y = exp2f(score2(p, f, s[n][2 * i + e], row.place - j, th) - lse2);
+            const float y = ex2(score2(p, f, s[n][2 * i + e], row.place - j, th) - lse2);
             s[n][2 * i + e] = seen ? y : 0.0f;
             if constexpr (DK) dp[n][2 * i + e] = seen ? y * (dp[n][2 * i + e] - delta) * fmaf(-th, th, 1.0f) : 0.0f;
           }
@@ -714,7 +762,8 @@ cudaError_t forward(const AttnParams& p, bool token, cudaStream_t st) {
     return launch(attn_tf32_token_kernel<T, DP>, dim3(p.Hkv * ((rows + 15) / 16), p.splits, p.B), 16 * S::kFloats + 4 * S::kColTile,
                   set[0], p, st);
   }
-  return launch(attn_tf32_fwd_kernel<T, DP>, dim3(p.H * p.B, row_tiles(p.Sq)), S::kRowTile + 4 * S::kColTile, set[1], p, st);
+  return launch(attn_tf32_fwd_kernel<T, DP>, dim3(p.H * p.B, row_tiles(p.Sq)), S::kRowTile + 2 * forward_slots<DP>() * S::kColTile, set[1],
+                p, st);
 }
 
 template <typename T, int DP>
