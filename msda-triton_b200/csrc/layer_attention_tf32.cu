@@ -21,7 +21,8 @@
 namespace msda {
 namespace {
 
-constexpr int kThreads = 128;
+constexpr int kThreads = 128;      // forward: a warp has 16 rows
+constexpr int kBwdThreads = 256;  // backward: two groups of four warps
 constexpr int kRows = 64;  // rows of a CTA, 16 a warp
 constexpr int kCols = 32;  // columns of a step
 
@@ -189,11 +190,11 @@ __device__ __forceinline__ void gather(const float (&p)[NT][4], const float* t, 
 // Rows r0 + [0, n) of a (S, D) slice to shared memory; rows that `keep` rejects
 // and channels from D on are zeros. fp32 by asynchronous copies. `vec`: 16 bytes
 // at a time.
-template <typename T, int DP, typename Keep>
+template <typename T, int DP, int THREADS = kThreads, typename Keep>
 __device__ __forceinline__ void load_rows(float* to, int n, const T* base, int64_t stride, int r0, int D, bool vec, Keep keep) {
   constexpr int P = Pitch<DP>::kFloats;
   if (sizeof(T) == 4 && vec) {
-    for (int i = threadIdx.x; i < n * (DP / 4); i += kThreads) {
+    for (int i = threadIdx.x; i < n * (DP / 4); i += THREADS) {
       const int r = i / (DP / 4), d = i % (DP / 4) * 4;
       const bool in = d < D && keep(r);
       const T* from = in ? base + (int64_t)(r0 + r) * stride + d : base;
@@ -201,14 +202,14 @@ __device__ __forceinline__ void load_rows(float* to, int n, const T* base, int64
                    "l"(from), "r"(in ? 16 : 0) : "memory");
     }
   } else if (sizeof(T) == 2 && vec) {
-    for (int i = threadIdx.x; i < n * (DP / 4); i += kThreads) {
+    for (int i = threadIdx.x; i < n * (DP / 4); i += THREADS) {
       const int r = i / (DP / 4), d = i % (DP / 4) * 4;
       float f[4] = {0.0f, 0.0f, 0.0f, 0.0f};
       if (d < D && keep(r)) load_vec<T, 4>(base + (int64_t)(r0 + r) * stride + d, f);
       *reinterpret_cast<float4*>(to + r * P + d) = make_float4(f[0], f[1], f[2], f[3]);
     }
   } else {
-    for (int i = threadIdx.x; i < n * DP; i += kThreads) {
+    for (int i = threadIdx.x; i < n * DP; i += THREADS) {
       const int r = i / DP, d = i % DP;
       float f = 0.0f;
       if (d < D && keep(r)) f = to_f32(__ldg(base + (int64_t)(r0 + r) * stride + d));
@@ -305,7 +306,7 @@ __host__ __device__ constexpr int forward_slots() {
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads, DP == 128 ? 3 : 1) attn_tf32_fwd_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(kThreads, DP <= 64 ? 4 : DP == 128 ? 3 : 1) attn_tf32_fwd_kernel(const AttnParams p) {
   constexpr int NT = kCols / 8;
   constexpr bool EXACT = sizeof(T) == 2;
   constexpr int SLOTS = forward_slots<DP>();
@@ -501,16 +502,17 @@ __global__ void __launch_bounds__(kThreads) attn_tf32_token_kernel(const AttnPar
   }
 }
 
-// dq, and delta_i = g_i . o_i for the key gradient that follows.
+// dq, and delta_i = g_i . o_i for the key gradient that follows. Each group of four
+// warps has half of a step's keys; their sums are added at the end.
 template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) attn_tf32_dq_kernel(const AttnParams p) {
-  constexpr int NT = kCols / 8;
+__global__ void __launch_bounds__(kBwdThreads, DP <= 128 ? 2 : 1) attn_tf32_dq_kernel(const AttnParams p) {
+  constexpr int NT = kCols / 16;
   constexpr bool EXACT = sizeof(T) == 2;
   using S = Pitch<DP>;
   extern __shared__ __align__(16) float smem[];
   float *qs = smem, *gs = smem + S::kRowTile, *ring = smem + 2 * S::kRowTile;
   __shared__ float delta_s[kRows];
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
+  const int side = threadIdx.x / 128, warp = threadIdx.x / 32 % 4, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
   const int h = blockIdx.x % p.H, b = blockIdx.x / p.H, hk = h / (p.H / p.Hkv);
   const int i0 = (gridDim.y - 1 - blockIdx.y) * kRows;
   const int length = attn_length(p, b);
@@ -525,19 +527,19 @@ __global__ void __launch_bounds__(kThreads) attn_tf32_dq_kernel(const AttnParams
   const auto fill = [&](int j) {
     if (j < limit) {
       const auto keep = [&](int r) { return !key_padded(p, b, j + r, length); };
-      load_rows<T, DP>(ring, kCols, k, p.ks[1], j, p.D, kvec, keep);
-      load_rows<T, DP>(ring + S::kColTile, kCols, v, p.vs[1], j, p.D, vvec, keep);
+      load_rows<T, DP, kBwdThreads>(ring, kCols, k, p.ks[1], j, p.D, kvec, keep);
+      load_rows<T, DP, kBwdThreads>(ring + S::kColTile, kCols, v, p.vs[1], j, p.D, vvec, keep);
     }
     copies_done();
   };
   const auto in = [&](int r) { return row_view(p, b, i0 + r, length).limit > 0; };
-  load_rows<T, DP>(qs, kRows, static_cast<const T*>(p.q) + b * p.qs[0] + h * p.qs[2], p.qs[1], i0, p.D,
+  load_rows<T, DP, kBwdThreads>(qs, kRows, static_cast<const T*>(p.q) + b * p.qs[0] + h * p.qs[2], p.qs[1], i0, p.D,
                    can_vec<T>(p.q, p.qs, p.D), in);
-  load_rows<T, DP>(gs, kRows, static_cast<const T*>(p.go) + b * p.gs[0] + h * p.gs[2], p.gs[1], i0, p.D,
+  load_rows<T, DP, kBwdThreads>(gs, kRows, static_cast<const T*>(p.go) + b * p.gs[0] + h * p.gs[2], p.gs[1], i0, p.D,
                    can_vec<T>(p.go, p.gs, p.D), in);
   // delta from the outputs, which take the ring's 64 rows, by the arithmetic that
   // forms g . v: where a row sees one key the two cancel.
-  for (int i = threadIdx.x; i < kRows * DP; i += kThreads) {
+  for (int i = threadIdx.x; i < kRows * DP; i += kBwdThreads) {
     const int r = i / DP, d = i % DP;
     float o = 0.0f;
     if (d < p.D && in(r)) {
@@ -550,7 +552,7 @@ __global__ void __launch_bounds__(kThreads) attn_tf32_dq_kernel(const AttnParams
   copies_done();
   copies_wait<0>();
   __syncthreads();
-  {
+  if (side == 0) {
     float c[2][4];
     scores<DP, 2, false>(gs + warp * 16 * S::kFloats, ring + warp * 16 * S::kFloats, p.D, c);
     if (t == g / 2) {
@@ -579,14 +581,15 @@ __global__ void __launch_bounds__(kThreads) attn_tf32_dq_kernel(const AttnParams
   for (int d = 0; d < DP / 8; ++d) dq[d][0] = dq[d][1] = dq[d][2] = dq[d][3] = 0.0f;
   while (j0 < limit) {
     const bool whole = !p.kdoc && __all_sync(kFullMask, j0 + kCols <= min(row[0].limit, row[1].limit));
+    const float* ks = ring + side * (kCols / 2) * S::kFloats;
     float s[NT][4], dp[NT][4];
-    scores<DP, NT, EXACT>(qs + warp * 16 * S::kFloats, ring, p.D, s);
-    scores<DP, NT, EXACT>(gs + warp * 16 * S::kFloats, ring + S::kColTile, p.D, dp);
+    scores<DP, NT, EXACT>(qs + warp * 16 * S::kFloats, ks, p.D, s);
+    scores<DP, NT, EXACT>(gs + warp * 16 * S::kFloats, ks + S::kColTile, p.D, dp);
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int j = j0 + n * 8 + 2 * t + e;
+        const int j = j0 + side * (kCols / 2) + n * 8 + 2 * t + e;
         const int kd = p.kdoc && j < length ? __ldg(p.kdoc + (int64_t)b * p.Sk + j) : 0;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -596,55 +599,62 @@ __global__ void __launch_bounds__(kThreads) attn_tf32_dq_kernel(const AttnParams
           s[n][2 * i + e] = seen ? x * (dp[n][2 * i + e] - delta[i]) * fmaf(-th, th, 1.0f) : 0.0f;
         }
       }
-    gather<DP, NT, EXACT, false>(s, ring, dq);
+    gather<DP, NT, EXACT, false>(s, ks, dq);
     __syncthreads();
     j0 = next(j0 + kCols);
     fill(j0);
     copies_wait<0>();
     __syncthreads();
   }
+  // The second group's sums go through the queries' place.
+  if (side == 1) {
+#pragma unroll
+    for (int d = 0; d < DP / 8; ++d)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        *reinterpret_cast<float2*>(qs + (warp * 16 + g + 8 * i) * S::kFloats + d * 8 + 2 * t) = make_float2(dq[d][2 * i], dq[d][2 * i + 1]);
+  }
+  __syncthreads();
+  if (side == 1) return;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int r = i0 + warp * 16 + g + 8 * i;
     if (r >= p.Sq) continue;
     T* to = static_cast<T*>(p.dq) + (((int64_t)b * p.Sq + r) * p.H + h) * p.D;
 #pragma unroll
-    for (int d = 0; d < DP / 8; ++d)
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-        if (d * 8 + 2 * t + e < p.D) to[d * 8 + 2 * t + e] = from_f32<T>(dq[d][2 * i + e] * p.scale);
+    for (int d = 0; d < DP / 8; ++d) {
+      const float2 other = *reinterpret_cast<const float2*>(qs + (warp * 16 + g + 8 * i) * S::kFloats + d * 8 + 2 * t);
+      const int c = d * 8 + 2 * t;
+      if (c < p.D) to[c] = from_f32<T>((dq[d][2 * i] + other.x) * p.scale);
+      if (c + 1 < p.D) to[c + 1] = from_f32<T>((dq[d][2 * i + 1] + other.y) * p.scale);
+    }
   }
 }
 
 // dk and dv of 64 keys: every query of every head that shares them, in a fixed
-// order. WHAT: 3 both, 1 dv, 2 dk (above 128 channels one does not leave registers
-// for the other).
-template <typename T, int DP, int WHAT>
-__global__ void __launch_bounds__(kThreads) attn_tf32_dkv_kernel(const AttnParams p) {
+// order. One group of four warps has dv, the other dk, with the scores formed by
+// both: five products where one group needs four, but twice the warps.
+template <typename T, int DP>
+__global__ void __launch_bounds__(kBwdThreads, DP <= 128 ? 2 : 1) attn_tf32_dkv_kernel(const AttnParams p) {
   constexpr int NT = kCols / 8;
-  constexpr bool EXACT = sizeof(T) == 2, DV = (WHAT & 1) != 0, DK = (WHAT & 2) != 0;
+  constexpr bool EXACT = sizeof(T) == 2;
   using S = Pitch<DP>;
   extern __shared__ __align__(16) float smem[];
   float *ks = smem, *vs = smem + S::kRowTile, *qs = smem + 2 * S::kRowTile, *gs = qs + S::kColTile;
   __shared__ float lse_s[kCols], delta_s[kCols];
   __shared__ RowView view_s[kCols];
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
+  const bool keys = threadIdx.x >= 128;  // this group has dk
+  const int warp = threadIdx.x / 32 % 4, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
   const int hk = blockIdx.x % p.Hkv, b = blockIdx.x / p.Hkv, group = p.H / p.Hkv;
   const int j0 = blockIdx.y * kRows;
   const int length = attn_length(p, b);
   const auto keep = [&](int r) { return !key_padded(p, b, j0 + r, length); };
-  load_rows<T, DP>(ks, kRows, static_cast<const T*>(p.k) + b * p.ks[0] + hk * p.ks[2], p.ks[1], j0, p.D,
+  load_rows<T, DP, kBwdThreads>(ks, kRows, static_cast<const T*>(p.k) + b * p.ks[0] + hk * p.ks[2], p.ks[1], j0, p.D,
                    can_vec<T>(p.k, p.ks, p.D), keep);
-  load_rows<T, DP>(vs, kRows, static_cast<const T*>(p.v) + b * p.vs[0] + hk * p.vs[2], p.vs[1], j0, p.D,
+  load_rows<T, DP, kBwdThreads>(vs, kRows, static_cast<const T*>(p.v) + b * p.vs[0] + hk * p.vs[2], p.vs[1], j0, p.D,
                    can_vec<T>(p.v, p.vs, p.D), keep);
-  float dk[DK ? DP / 8 : 1][4], dv[DV ? DP / 8 : 1][4];
-#pragma unroll
-  for (int d = 0; d < DP / 8; ++d)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (DK) dk[d][i] = 0.0f;
-      if constexpr (DV) dv[d][i] = 0.0f;
-    }
+  float out[DP / 8][4];
+  clear(out);
   int kd[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -667,14 +677,14 @@ __global__ void __launch_bounds__(kThreads) attn_tf32_dkv_kernel(const AttnParam
         delta_s[threadIdx.x] = i < p.Sq ? p.delta[at] : 0.0f;
       }
       const auto in = [&](int r) { return row_view(p, b, i0 + r, length).limit > 0; };
-      load_rows<T, DP>(qs, kCols, static_cast<const T*>(p.q) + b * p.qs[0] + h * p.qs[2], p.qs[1], i0, p.D, qvec, in);
-      load_rows<T, DP>(gs, kCols, static_cast<const T*>(p.go) + b * p.gs[0] + h * p.gs[2], p.gs[1], i0, p.D, gvec, in);
+      load_rows<T, DP, kBwdThreads>(qs, kCols, static_cast<const T*>(p.q) + b * p.qs[0] + h * p.qs[2], p.qs[1], i0, p.D, qvec, in);
+      load_rows<T, DP, kBwdThreads>(gs, kCols, static_cast<const T*>(p.go) + b * p.gs[0] + h * p.gs[2], p.gs[1], i0, p.D, gvec, in);
       copies_done();
       copies_wait<0>();
       __syncthreads();
-      float s[NT][4], dp[DK ? NT : 1][4];
+      float s[NT][4], dp[NT][4];
       scores<DP, NT, EXACT>(ks + warp * 16 * S::kFloats, qs, p.D, s);
-      if constexpr (DK) scores<DP, NT, EXACT>(vs + warp * 16 * S::kFloats, gs, p.D, dp);
+      if (keys) scores<DP, NT, EXACT>(vs + warp * 16 * S::kFloats, gs, p.D, dp);
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -688,14 +698,15 @@ __global__ void __launch_bounds__(kThreads) attn_tf32_dkv_kernel(const AttnParam
             const bool seen = j < row.limit && (!p.kdoc || same_document(row.doc, kd[i], p.shared));
             float th;
             const float y = ex2(score2(p, f, s[n][2 * i + e], row.place - j, th) - lse2);
-            s[n][2 * i + e] = seen ? y : 0.0f;
-            if constexpr (DK) dp[n][2 * i + e] = seen ? y * (dp[n][2 * i + e] - delta) * fmaf(-th, th, 1.0f) : 0.0f;
+            const float z = keys ? y * (dp[n][2 * i + e] - delta) * fmaf(-th, th, 1.0f) : y;
+            s[n][2 * i + e] = seen ? z : 0.0f;
           }
         }
-      if constexpr (DV) gather<DP, NT, EXACT, false>(s, gs, dv);
-      if constexpr (DK) gather<DP, NT, EXACT, false>(dp, qs, dk);
+      gather<DP, NT, EXACT, false>(s, keys ? qs : gs, out);
     }
   }
+  T* to = static_cast<T*>(keys ? p.dk : p.dv);
+  const float mul = keys ? p.scale : 1.0f;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int j = j0 + warp * 16 + g + 8 * i;
@@ -707,8 +718,7 @@ __global__ void __launch_bounds__(kThreads) attn_tf32_dkv_kernel(const AttnParam
       for (int e = 0; e < 2; ++e) {
         const int c = d * 8 + 2 * t + e;
         if (c >= p.D) continue;
-        if constexpr (DK) static_cast<T*>(p.dk)[at + c] = from_f32<T>(dk[d][2 * i + e] * p.scale);
-        if constexpr (DV) static_cast<T*>(p.dv)[at + c] = from_f32<T>(dv[d][2 * i + e]);
+        to[at + c] = from_f32<T>(out[d][2 * i + e] * mul);
       }
   }
 }
@@ -744,10 +754,10 @@ __global__ void __launch_bounds__(128) attn_documents_kernel(const AttnParams p,
 }
 
 template <typename K>
-cudaError_t launch(K kernel, dim3 grid, int floats, std::atomic<uint64_t>& set, const AttnParams& p, cudaStream_t st) {
+cudaError_t launch(K kernel, dim3 grid, int threads, int floats, std::atomic<uint64_t>& set, const AttnParams& p, cudaStream_t st) {
   cudaError_t e = abi::allow_smem(kernel, floats * 4, set);
   if (e != cudaSuccess) return e;
-  kernel<<<grid, kThreads, floats * 4, st>>>(p);
+  kernel<<<grid, threads, floats * 4, st>>>(p);
   return cudaGetLastError();
 }
 
@@ -759,26 +769,21 @@ cudaError_t forward(const AttnParams& p, bool token, cudaStream_t st) {
   static std::atomic<uint64_t> set[2];
   if (token) {
     const int rows = p.Sq * (p.H / p.Hkv);
-    return launch(attn_tf32_token_kernel<T, DP>, dim3(p.Hkv * ((rows + 15) / 16), p.splits, p.B), 16 * S::kFloats + 4 * S::kColTile,
-                  set[0], p, st);
+    return launch(attn_tf32_token_kernel<T, DP>, dim3(p.Hkv * ((rows + 15) / 16), p.splits, p.B), kThreads,
+                  16 * S::kFloats + 4 * S::kColTile, set[0], p, st);
   }
-  return launch(attn_tf32_fwd_kernel<T, DP>, dim3(p.H * p.B, row_tiles(p.Sq)), S::kRowTile + 2 * forward_slots<DP>() * S::kColTile, set[1],
-                p, st);
+  return launch(attn_tf32_fwd_kernel<T, DP>, dim3(p.H * p.B, row_tiles(p.Sq)), kThreads,
+                S::kRowTile + 2 * forward_slots<DP>() * S::kColTile, set[1], p, st);
 }
 
 template <typename T, int DP>
 cudaError_t backward(const AttnParams& p, cudaStream_t st) {
   using S = Pitch<DP>;
-  static std::atomic<uint64_t> set[3];
+  static std::atomic<uint64_t> set[2];
   constexpr int floats = 2 * S::kRowTile + 2 * S::kColTile;
-  cudaError_t e = launch(attn_tf32_dq_kernel<T, DP>, dim3(p.H * p.B, row_tiles(p.Sq)), floats, set[0], p, st);
-  const dim3 grid(p.Hkv * p.B, row_tiles(p.Sk));
-  if constexpr (DP <= 128) {
-    if (e == cudaSuccess) e = launch(attn_tf32_dkv_kernel<T, DP, 3>, grid, floats, set[1], p, st);
-  } else {
-    if (e == cudaSuccess) e = launch(attn_tf32_dkv_kernel<T, DP, 1>, grid, floats, set[1], p, st);
-    if (e == cudaSuccess) e = launch(attn_tf32_dkv_kernel<T, DP, 2>, grid, floats, set[2], p, st);
-  }
+  cudaError_t e = launch(attn_tf32_dq_kernel<T, DP>, dim3(p.H * p.B, row_tiles(p.Sq)), kBwdThreads, floats, set[0], p, st);
+  if (e == cudaSuccess)
+    e = launch(attn_tf32_dkv_kernel<T, DP>, dim3(p.Hkv * p.B, row_tiles(p.Sk)), kBwdThreads, floats, set[1], p, st);
   return e;
 }
 
