@@ -11,20 +11,21 @@ attention logits) the kernels can take fused
 skeleton. Beside them stand the operators that complete a transformer layer:
 ``attention`` (capped scores, distance bias, document, prefix and length masks,
 training and single tokens), ``rotary`` (positions over several axes) and
-``layer_norm`` (with a residual). The kernels live in ``libmsda_b200.so`` behind
+``layer_norm`` (with a residual); ``DeformableDecoderLayer`` runs them together.
+The kernels live in ``libmsda_b200.so`` behind
 the C ABI of include/msda_b200.h and include/msda_layer_b200.h.
 """
 
 from .attention import attention
 from .gather import grid_sample, roi_align
-from .layers import MSDACrossAttention
+from .layers import DeformableDecoderLayer, MSDACrossAttention
 from .norm import layer_norm
 from .ops import (MultiScaleDeformableAttnFunction, multi_scale_deformable_attention,
                   multi_scale_deformable_attention_fused)
 from .rotary import rotary
 
-# The sampling operators' names; the layer operators (attention, rotary,
-# layer_norm) are imported by name.
+# The sampling operators' names; attention, rotary, layer_norm and
+# DeformableDecoderLayer are imported by name.
 __all__ = ["multi_scale_deformable_attention", "MultiScaleDeformableAttnFunction",
            "MSDACrossAttention", "multi_scale_deformable_attention_fused", "grid_sample", "roi_align"]
 __version__ = "0.1.0"

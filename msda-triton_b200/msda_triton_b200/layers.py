@@ -23,6 +23,12 @@ the bandwidth-bound tensor operations cost, 2.52 vs 2.30 ms).
 Shapes: ``query`` (B, Q, C); ``reference_points`` (B, Q, 2), normalised
 (x, y) in [0, 1]; ``value`` (B, S, C), the pyramid flattened level by level;
 ``spatial_shapes`` (L, 2) as (H_l, W_l). Returns (B, Q, C).
+
+``DeformableDecoderLayer`` is the whole layer of a detection decoder around it:
+self-attention among the queries, rotated by their reference points and masked by
+denoising groups, the cross-attention above and a feed-forward step, each followed
+by a layer norm with its residual. ``step`` runs it for one new query of each item
+over a cache of the earlier ones, as a decoder of sequences does.
 """
 
 from __future__ import annotations
@@ -30,7 +36,10 @@ from __future__ import annotations
 import torch
 from torch import nn
 
+from .attention import attention
+from .norm import layer_norm
 from .ops import multi_scale_deformable_attention, multi_scale_deformable_attention_fused
+from .rotary import rotary
 
 
 class MSDACrossAttention(nn.Module):
@@ -85,3 +94,77 @@ class MSDACrossAttention(nn.Module):
             out = multi_scale_deformable_attention(v, spatial_shapes, level_start_index,
                                                    locations.contiguous(), weights.contiguous())
         return self.out_proj(out)
+
+
+class DeformableDecoderLayer(nn.Module):
+    """A detection decoder's layer on the B200 kernels (post-norm).
+
+    Args:
+        embed_dim, num_heads, num_levels, num_points: as in
+            :class:`MSDACrossAttention`; the channels of a head must be a
+            multiple of 4 (half of them turn with x, half with y).
+        ffn_dim: hidden channels of the feed-forward step.
+        position_scale: what a reference point's unit is in rotary positions.
+        eps: of the norms.
+    """
+
+    def __init__(self, embed_dim: int, num_heads: int, num_levels: int, num_points: int, ffn_dim: int = 1024,
+                 position_scale: float = 100.0, eps: float = 1e-5):
+        super().__init__()
+        self.cross_attn = MSDACrossAttention(embed_dim, num_heads, num_levels, num_points)
+        self.num_heads = num_heads
+        self.head_dim = embed_dim // num_heads
+        if self.head_dim % 4:
+            raise ValueError(f"head_dim={self.head_dim} is not a multiple of 4")
+        self.position_scale = position_scale
+        self.in_proj = nn.Linear(embed_dim, 3 * embed_dim)
+        self.self_out_proj = nn.Linear(embed_dim, embed_dim)
+        self.linear1 = nn.Linear(embed_dim, ffn_dim)
+        self.linear2 = nn.Linear(ffn_dim, embed_dim)
+        # Hold the weights; the sums and norms run as one kernel each.
+        self.norm1, self.norm2, self.norm3 = (nn.LayerNorm(embed_dim, eps=eps) for _ in range(3))
+
+    def _heads(self, query, reference_points):
+        """The rotated query and key heads and the value heads, (B, Q, M, D) each."""
+        B, Q, _ = query.shape
+        q, k, v = self.in_proj(query).view(B, Q, 3, self.num_heads, self.head_dim).unbind(2)
+        positions = reference_points.detach().float() * self.position_scale
+        q, k = rotary(q, positions, key=k, axis_dims=(self.head_dim // 2, self.head_dim // 2))
+        return q, k, v
+
+    @staticmethod
+    def _norm(norm, x, residual):
+        return layer_norm(x, norm.weight, norm.bias, residual=residual, eps=norm.eps)
+
+    def _after(self, x, query, reference_points, value, spatial_shapes, level_start_index):
+        x = self._norm(self.norm1, self.self_out_proj(x.flatten(2)), query)
+        x = self._norm(self.norm2, self.cross_attn(x, reference_points, value, spatial_shapes, level_start_index), x)
+        return self._norm(self.norm3, self.linear2(self.linear1(x).relu()), x)
+
+    def forward(self, query: torch.Tensor, reference_points: torch.Tensor, value: torch.Tensor,
+                spatial_shapes: torch.Tensor, level_start_index: torch.Tensor | None = None, *,
+                groups: torch.Tensor | None = None, shared_group: int | None = None,
+                causal: bool = False) -> torch.Tensor:
+        """(B, Q, C) from ``query`` (B, Q, C) and ``value`` (B, S, C).
+
+        ``groups`` (B, Q) int32: queries see those of their own group and of
+        ``shared_group`` (the matching queries beside denoising groups);
+        negative ids are padding. ``causal``: a query sees the earlier ones
+        and itself."""
+        q, k, v = self._heads(query, reference_points)
+        x = attention(q, k, v, query_documents=groups, key_documents=groups, shared_document=shared_group, causal=causal)
+        return self._after(x, query, reference_points, value, spatial_shapes, level_start_index)
+
+    def step(self, query: torch.Tensor, reference_points: torch.Tensor, value: torch.Tensor,
+             spatial_shapes: torch.Tensor, level_start_index: torch.Tensor | None, keys: torch.Tensor,
+             values: torch.Tensor, lengths: torch.Tensor) -> torch.Tensor:
+        """One new query (B, 1, C) of each item, as ``forward`` with
+        ``causal=True`` gives it. ``keys`` and ``values`` (B, longest, M, D)
+        cache the earlier queries' heads and get this one's at
+        ``lengths - 1``; ``lengths`` (B,) int32 counts the queries with it."""
+        q, k, v = self._heads(query, reference_points)
+        item = torch.arange(query.shape[0], device=query.device)
+        at = lengths.long() - 1
+        keys[item, at], values[item, at] = k[:, 0], v[:, 0]
+        x = attention(q, keys, values, causal=True, key_lengths=lengths)
+        return self._after(x, query, reference_points, value, spatial_shapes, level_start_index)
