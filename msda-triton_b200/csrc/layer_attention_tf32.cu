@@ -2,7 +2,7 @@
 // the tensor-core kernels of layer_attention_tc.cuh do not take.
 //
 // The products run on the tensor cores by register fragments (m16n8k8, tf32 in,
-// fp32 sums): an fp32 number is the sum of two tf32 numbers to 2^-21 of its size,
+// fp32 sums): an fp32 number is the sum of two tf32 numbers to 2^-22 of its size,
 //   x y = xh yh + xh yl + xl yh  (+ xl yl, below 2^-20 x y),
 // three products for one, at 92 TFLOP/s a bound above the 72 of the FMA pipes.
 // 16-bit inputs are tf32 numbers as they stand: their scores need one product,
@@ -32,11 +32,12 @@ struct Pitch {
   static constexpr int kRowTile = kRows * kFloats, kColTile = kCols * kFloats;
 };
 
-// x cut to a tf32 number, and what is left of it, which the product cuts in turn:
-// 2^-21 of x at most is lost, in sums whose own rounding is a few times that.
+// x cut to a tf32 number, and what is left of it, rounded to one (the product cuts
+// the bits below): 2^-22 of x at most is lost, to either side. (Cut as well, the
+// second part would lose 2^-21, always towards zero: twice the error of a gradient.)
 __device__ __forceinline__ void split(float x, uint32_t& high, uint32_t& low) {
   high = __float_as_uint(x) & 0xffffe000u;
-  low = __float_as_uint(x - __uint_as_float(high));
+  low = __float_as_uint(x - __uint_as_float(high)) + 0x1000u;
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -177,7 +178,7 @@ __device__ __forceinline__ void gather(const float (&p)[NT][4], const float* t, 
           if constexpr (REST) {
 #pragma unroll
             for (int e = 0; e < 2; ++e)
-              rest[i][e] = __float_as_uint(__uint_as_float(bl[i][e]) - __uint_as_float(bl[i][e] & 0xffffe000u));
+              rest[i][e] = __float_as_uint(__uint_as_float(y[e]) - __uint_as_float(bh[i][e]) - __uint_as_float(bl[i][e] & 0xffffe000u));
           }
         }
         products<false, EXACT, REST, N>(c, ah[m], al[m], bh, bl, rest);
