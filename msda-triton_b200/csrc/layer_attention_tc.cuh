@@ -19,7 +19,7 @@ namespace msda {
 namespace tc {
 
 // What the scores of a kernel's instance go through.
-constexpr int kCapped = 1, kSloped = 2;
+constexpr int kCapped = 1, kSloped = 2, kGrouped = 4;  // cap; distance bias; documents
 
 constexpr int kSoftmaxThreads = 256;
 constexpr int kThreads = kSoftmaxThreads + 128;  // two warpgroups of softmax, one of the other roles
@@ -129,26 +129,48 @@ __device__ __forceinline__ void cap_scores(const ScoreForm& f, float (&s)[N]) {
   }
 }
 
+// What documents say of a block of query tiles (bit t: tile t) and a key tile.
 struct TileState {
-  bool skip;    // no query of the rows sees a key of the tile by documents
-  bool agree;   // documents hide nothing
-  bool padded;  // some keys are padding: their values must be cleared
+  uint8_t apart;  // no query of the tile sees a key
+  uint8_t agree;  // documents hide nothing
+  bool skip;      // apart from every tile of the block
+  bool padded;    // some keys are padding: their rows must be cleared
 };
 
-// rows: [i0, i0 + n * 128); keys: tile j.
+// rows: [i0, i0 + n * 128), n <= 2; keys: tile j.
 __device__ __forceinline__ TileState tile_state(const AttnParams& p, int b, int i0, int n, int j, int length) {
-  TileState s{false, true, (j + 1) * kTileTokens > length && length < p.Sk};
+  TileState s{0, 3, false, (j + 1) * kTileTokens > length && length < p.Sk};
   if (!p.kdoc) return s;
   const int nq = (p.Sq + kDocTile - 1) / kDocTile, nk = (p.Sk + kDocTile - 1) / kDocTile;
   const DocTile k = p.ktile[(int64_t)b * nk + j];
-  s.skip = true;
+  s.apart = 3, s.agree = 0;
   for (int t = 0; t < n && i0 / kDocTile + t < nq; ++t) {
     const DocTile q = p.qtile[(int64_t)b * nq + i0 / kDocTile + t];
-    s.skip = s.skip && tiles_apart(q, k);
-    s.agree = s.agree && tiles_agree(q, k, p.shared);
+    if (!tiles_apart(q, k)) s.apart &= ~(1 << t);
+    if (tiles_agree(q, k, p.shared)) s.agree |= 1 << t;
   }
+  s.skip = s.apart == 3;
   s.padded = s.padded || k.padded;
   return s;
+}
+
+// Which of the keys k0 ... (32 a word) a thread's query sees by its document: a
+// ballot for each document among the warp's queries, of which there are few.
+template <int W>
+__device__ __forceinline__ void document_masks(const AttnParams& p, const int* kdoc, int k0, int doc, uint32_t (&mask)[W]) {
+  const int lane = threadIdx.x % 32;
+  int mine[W];
+#pragma unroll
+  for (int w = 0; w < W; ++w) mine[w] = k0 + w * 32 + lane < p.Sk ? __ldg(kdoc + k0 + w * 32 + lane) : -1;
+  for (uint32_t todo = kFullMask; todo;) {
+    const int d = __shfl_sync(kFullMask, doc, __ffs(todo) - 1);
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const uint32_t seen = __ballot_sync(kFullMask, same_document(d, mine[w], p.shared));
+      if (doc == d) mask[w] = seen;
+    }
+    todo &= ~__ballot_sync(kFullMask, doc == d);
+  }
 }
 
 // Clears the rows of a tile whose token is padding (a warp): 0 x NaN is NaN, and
@@ -171,7 +193,7 @@ __device__ __forceinline__ void clear_rows(char* tile, const int* doc, int first
 // The steps that a block of queries goes through: its key tiles, or with STEP 64
 // their halves, less what the limit or the documents leave out. Every role walks
 // them by itself.
-template <int STEP>
+template <int STEP, bool DOCS>
 struct KeySteps {
   int j, half, n;  // key tile, its half, the tile's number among those visited
   int tiles, halves;  // key tiles below the limit; halves of the last of them
@@ -179,16 +201,16 @@ struct KeySteps {
   TileState state;
 
   __device__ __forceinline__ void seek(const AttnParams& p, int b, int i0, int rows, int length) {
-    if (!p.kdoc) {
+    if constexpr (!DOCS) {
       done = j >= tiles;
-      state = TileState{false, true, j * kTileTokens + kTileTokens > length && length < p.Sk};
-      return;
-    }
-    for (;; ++j) {
-      done = j >= tiles;
-      if (done) return;
-      state = tile_state(p, b, i0, rows, j, length);
-      if (!state.skip) return;
+      state = TileState{0, 3, false, j * kTileTokens + kTileTokens > length && length < p.Sk};
+    } else {
+      for (;; ++j) {
+        done = j >= tiles;
+        if (done) return;
+        state = tile_state(p, b, i0, rows, j, length);
+        if (!state.skip) return;
+      }
     }
   }
   __device__ __forceinline__ KeySteps(const AttnParams& p, int b, int i0, int rows, int limit, int length)
@@ -237,6 +259,7 @@ __global__ void __launch_bounds__(FwdShape<DP>::kThreads, FwdShape<DP>::kCtas)
     attn_tc_fwd_kernel(const AttnParams p, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                        const __grid_constant__ CUtensorMap vmap) {
   using Shape = FwdShape<DP>;
+  constexpr bool DOCS = (MODE & kGrouped) != 0;
   constexpr int NS = Shape::kStages, STEP = Shape::kStep, OUT = 2 * STEP;  // OUT: first TMEM column of the sums
   extern __shared__ char raw[];
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
@@ -277,10 +300,20 @@ __global__ void __launch_bounds__(FwdShape<DP>::kThreads, FwdShape<DP>::kCtas)
     constexpr float kSlack = 8.0f;
     bool ok = true;
     int u = 0;
-    for (KeySteps<STEP> at(p, b, i0, 2, limit, length); !at.done && ok; at.advance(p, b, i0, 2, length), ++u) {
+    for (KeySteps<STEP, DOCS> at(p, b, i0, 2, limit, length); !at.done && ok; at.advance(p, b, i0, 2, length), ++u) {
       ok = warp_wait(&s_full[t], u & 1, abort);
       if (!ok) break;
       fence_after();
+      if (DOCS && (at.state.apart >> t & 1)) {  // the step is the other tile's: no probabilities
+        const uint32_t none[16] = {};
+#pragma unroll
+        for (int c = 0; c < STEP / 2; c += 16) tmem_store16(s_at + c, none);
+        tmem_wait_store();
+        fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(&p_full[t]);
+        continue;
+      }
       float s[STEP];
 #pragma unroll
       for (int c = 0; c < STEP; c += 32) tmem_load32(s_at + c, s + c);
@@ -304,14 +337,11 @@ __global__ void __launch_bounds__(FwdShape<DP>::kThreads, FwdShape<DP>::kCtas)
 #pragma unroll
         for (int c = 0; c < STEP; ++c) s[c] = c < seen ? s[c] : -INFINITY;
       }
-      if (!at.state.agree) {
+      if (DOCS && !(at.state.agree >> t & 1)) {
+        uint32_t mask[STEP / 32];
+        document_masks(p, kdoc, j0, row.doc, mask);
 #pragma unroll
-        for (int q = 0; q < STEP / 32; ++q) {
-          const int k = j0 + q * 32 + lane, mine = k < p.Sk ? __ldg(kdoc + k) : -1;
-#pragma unroll
-          for (int c = 0; c < 32; ++c)
-            if (!same_document(row.doc, __shfl_sync(kFullMask, mine, c), p.shared)) s[q * 32 + c] = -INFINITY;
-        }
+        for (int c = 0; c < STEP; ++c) s[c] = mask[c / 32] >> (c % 32) & 1 ? s[c] : -INFINITY;
       }
       if (factor <= 0.0f) {  // a negative scale: its own factor now, so that the largest score is the largest value
 #pragma unroll
@@ -413,7 +443,7 @@ __global__ void __launch_bounds__(FwdShape<DP>::kThreads, FwdShape<DP>::kCtas)
         tma_tile<DP>(sq, &qmap, &q_full, h, i0, b);
         tma_tile<DP>(sq + Shape::kTile, &qmap, &q_full, h, i0 + kTileTokens, b);
       }
-      for (KeySteps<STEP> at(p, b, i0, 2, limit, length); !at.done && ok; at.next_tile(p, b, i0, 2, length)) {
+      for (KeySteps<STEP, DOCS> at(p, b, i0, 2, limit, length); !at.done && ok; at.next_tile(p, b, i0, 2, length)) {
         for (int kv = 0; kv < 2 && ok; ++kv, ++n) {
           const int slot = n % NS;
           if (n >= NS) ok = warp_wait(&kv_empty[slot], (n / NS - 1) & 1, abort);
@@ -441,7 +471,7 @@ __global__ void __launch_bounds__(FwdShape<DP>::kThreads, FwdShape<DP>::kCtas)
     constexpr uint64_t kHalfTile = 64 * 128 >> 4, kSlot = Shape::kTile >> 4;
     const uint64_t q_desc = by_channels(smem_u32(sq)), k_desc = by_channels(smem_u32(ring)), v_desc = by_tokens(smem_u32(ring));
     bool ok = limit == 0 || bar_wait(&q_full, 0, abort);
-    KeySteps<STEP> at(p, b, i0, 2, limit, length);
+    KeySteps<STEP, DOCS> at(p, b, i0, 2, limit, length);
     int slot = 0, clears = 0;  // slot of the tile's keys; its values': the next
     uint32_t phase = 0, turn = 0;
     const auto scores = [&](int t, uint64_t k) {
@@ -634,6 +664,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
     attn_tc_dq_kernel(const AttnParams p, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                       const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap gmap) {
   using Shape = BwdShape<DP>;
+  constexpr bool DOCS = (MODE & kGrouped) != 0;
   constexpr int STEP = Shape::kStep, N = STEP / 2;
   extern __shared__ char raw[];
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
@@ -700,7 +731,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
     const uint64_t lse2 = pair_of(lse, lse), delta2 = pair_of(-delta, -delta);
     bool ok = true;
     int u = 0;
-    for (KeySteps<STEP> at(p, b, i0, 1, limit, length); !at.done && ok; at.advance(p, b, i0, 1, length), ++u) {
+    for (KeySteps<STEP, DOCS> at(p, b, i0, 1, limit, length); !at.done && ok; at.advance(p, b, i0, 1, length), ++u) {
       const int c0 = at.j * kTileTokens + at.half * 64 + half * N;  // the thread's first key
       const uint32_t s_at = tmem + lanes + (u & 1) * STEP + half * N;
       ok = warp_wait(&s_full[u & 1], (u >> 1) & 1, abort);
@@ -718,15 +749,12 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
 #pragma unroll
         for (int c = 0; c < N; ++c) s[c] = c < seen ? s[c] : 0.0f;
       }
-      if (!at.state.agree) {
+      if (DOCS && !(at.state.agree & 1)) {
         masked = true;
+        uint32_t mask[N / 32];
+        document_masks(p, kdoc, c0, row.doc, mask);
 #pragma unroll
-        for (int q = 0; q < N / 32; ++q) {
-          const int k = c0 + q * 32 + lane, mine = k < p.Sk ? __ldg(kdoc + k) : -1;
-#pragma unroll
-          for (int c = 0; c < 32; ++c)
-            if (!same_document(row.doc, __shfl_sync(kFullMask, mine, c), p.shared)) s[q * 32 + c] = 0.0f;
-        }
+        for (int c = 0; c < N; ++c) s[c] = mask[c / 32] >> (c % 32) & 1 ? s[c] : 0.0f;
       }
       ok = warp_wait(&dp_full, u & 1, abort);
       if (!ok) break;
@@ -760,7 +788,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
         const int* kdoc = p.kdoc ? p.kdoc + (int64_t)b * p.Sk : nullptr;
         int n = 0;
         bool ok = true;
-        for (KeySteps<STEP> at(p, b, i0, 1, limit, length); !at.done && ok; at.next_tile(p, b, i0, 1, length)) {
+        for (KeySteps<STEP, DOCS> at(p, b, i0, 1, limit, length); !at.done && ok; at.next_tile(p, b, i0, 1, length)) {
           const int slot = n % 2;
           if (n >= 2) ok = warp_wait(&kv_empty[slot], (n / 2 - 1) & 1, abort);
           if (!ok) break;
@@ -797,7 +825,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
         product_parts<STEP>(dq_at, tmem + ((u - 1) & 1) * STEP, prev_k, dd, u > 1);
         if (prev_last) commit(&kv_empty[prev_slot]);
       };
-      for (KeySteps<STEP> at(p, b, i0, 1, limit, length); !at.done && ok; at.next_tile(p, b, i0, 1, length)) {
+      for (KeySteps<STEP, DOCS> at(p, b, i0, 1, limit, length); !at.done && ok; at.next_tile(p, b, i0, 1, length)) {
         const int slot = at.n & 1, count = at.count();
         ok = bar_wait(&kv_full[slot], (at.n >> 1) & 1, abort);
         if (ok && at.state.padded) ok = bar_wait(&cleared, clears++ & 1, abort);
@@ -831,7 +859,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
 
 // The steps that a block of keys goes through: every head of its group, the
 // tiles of queries from the first that may see it, or with STEP 64 their halves.
-template <int STEP>
+template <int STEP, bool DOCS>
 struct QuerySteps {
   int g, i, half, n;  // head of the group, query tile, its half, the tile's number among those visited
   int first, tiles, halves;
@@ -843,16 +871,17 @@ struct QuerySteps {
       if (i >= tiles) i = first, ++g;
       done = g >= group || first >= tiles;
       if (done) return;
-      if (!p.kdoc) {
-        state = TileState{false, true, false};
+      if constexpr (!DOCS) {
+        state = TileState{0, 3, false, false};
         return;
+      } else {
+        state = tile_state(p, b, i * kTileTokens, 1, kt, length);
+        if (!state.skip) {
+          state.padded = p.qtile[(int64_t)b * tiles + i].padded;  // of the queries, here
+          return;
+        }
+        ++i;
       }
-      state = tile_state(p, b, i * kTileTokens, 1, kt, length);
-      if (!state.skip) {
-        state.padded = p.qtile[(int64_t)b * tiles + i].padded;  // of the queries, here
-        return;
-      }
-      ++i;
     }
   }
   __device__ __forceinline__ QuerySteps(const AttnParams& p, int b, int group, int kt, int length)
@@ -886,6 +915,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
     attn_tc_dkv_kernel(const AttnParams p, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                        const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap gmap) {
   using Shape = BwdShape<DP>;
+  constexpr bool DOCS = (MODE & kGrouped) != 0;
   constexpr int STEP = Shape::kStep, N = STEP / 2;
   extern __shared__ char raw[];
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
@@ -925,7 +955,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
     // its view of the keys.
     float lse = 0.0f, delta = 0.0f;
     RowView view{};
-    const auto fetch = [&](const QuerySteps<STEP>& at) {
+    const auto fetch = [&](const QuerySteps<STEP, DOCS>& at) {
       if (at.done || r >= STEP) return;
       const int i = at.row() + r;
       view = row_view(p, b, i, length);
@@ -937,13 +967,13 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
     };
     bool ok = true;
     int u = 0;
-    QuerySteps<STEP> at(p, b, group, kt, length);
+    QuerySteps<STEP, DOCS> at(p, b, group, kt, length);
     fetch(at);
     // A warp whose wait gave up still comes to the others' barriers.
     while (!at.done) {
       QueryStats<STEP>& q = stats[u & 1];
       const ScoreForm f = score_form(p, hk * group + at.g);
-      const bool agree = at.state.agree;
+      const bool agree = at.state.agree & 1;
       // This buffer was read two steps ago: every thread has passed the barrier
       // of the step between.
       if (r < STEP) {
@@ -977,7 +1007,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
           s[c + 2] = live & (j < limit.z) ? s[c + 2] : 0.0f;
           s[c + 3] = live & (j < limit.w) ? s[c + 3] : 0.0f;
         }
-        if (!agree) {
+        if (DOCS && !agree) {
           // A key of the shared document is of every query's; padded queries' limit is 0.
           const bool any = kd >= 0 && kd == p.shared;
 #pragma unroll
@@ -1011,7 +1041,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
   } else {
     if constexpr (Shape::kSplit) leave_registers();
     if (warp == kLoadWarp) {
-      QuerySteps<STEP> at(p, b, group, kt, length);
+      QuerySteps<STEP, DOCS> at(p, b, group, kt, length);
       if (!at.done) {
         if (lane == 0) {
           bar_expect(&k_full, 2 * Shape::kTile);
@@ -1047,7 +1077,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
       constexpr uint64_t kHalfTile = 64 * 128 >> 4, kTileDesc = Shape::kTile >> 4;
       const uint64_t k_desc = by_channels(smem_u32(sk)), v_desc = k_desc + kTileDesc, qg_desc = by_channels(smem_u32(ring));
       const uint64_t qg_tokens = by_tokens(smem_u32(ring));
-      QuerySteps<STEP> at(p, b, group, kt, length);
+      QuerySteps<STEP, DOCS> at(p, b, group, kt, length);
       bool ok = at.done || bar_wait(&k_full, 0, abort);
       int u = 0, clears = 0, prev_slot = 0;
       uint64_t prev_q = 0;     // queries of the step before, whose sums are due
@@ -1145,11 +1175,15 @@ int run(const AttnParams& p, bool backward, cudaStream_t st) {
       !make_map(&m[2], p.v, bf16, p.D, p.Hkv, p.Sk, p.B, p.vs) ||
       (backward && !make_map(&m[3], p.go, bf16, p.D, p.H, p.Sq, p.B, p.gs)))
     return -1;
-  switch ((p.cap != 0.0f ? kCapped : 0) | (p.slopes ? kSloped : 0)) {
+  switch ((p.cap != 0.0f ? kCapped : 0) | (p.slopes ? kSloped : 0) | (p.kdoc ? kGrouped : 0)) {
     case 0: return (int)launch_by_size<T, 0>(p, m, backward, st);
-    case kCapped: return (int)launch_by_size<T, kCapped>(p, m, backward, st);
-    case kSloped: return (int)launch_by_size<T, kSloped>(p, m, backward, st);
-    default: return (int)launch_by_size<T, kCapped | kSloped>(p, m, backward, st);
+    case 1: return (int)launch_by_size<T, 1>(p, m, backward, st);
+    case 2: return (int)launch_by_size<T, 2>(p, m, backward, st);
+    case 3: return (int)launch_by_size<T, 3>(p, m, backward, st);
+    case 4: return (int)launch_by_size<T, 4>(p, m, backward, st);
+    case 5: return (int)launch_by_size<T, 5>(p, m, backward, st);
+    case 6: return (int)launch_by_size<T, 6>(p, m, backward, st);
+    default: return (int)launch_by_size<T, 7>(p, m, backward, st);
   }
 }
 
