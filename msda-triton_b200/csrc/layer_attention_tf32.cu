@@ -306,15 +306,24 @@ __host__ __device__ constexpr int forward_slots() {
   return DP == 128 ? 1 : 2;
 }
 
+// Groups of four warps that have 32 keys of a step each: two up to 64 channels,
+// whose sums are joined at the end. (With one, 2 x 1201 tokens on 8 heads of 32
+// channels took 112 us: 304 CTAs of four warps leave the schedulers idle.)
+template <int DP>
+__host__ __device__ constexpr int forward_groups() {
+  return DP <= 64 ? 2 : 1;
+}
+
 template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads, DP <= 64 ? 4 : DP == 128 ? 3 : 1) attn_tf32_fwd_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(kThreads * forward_groups<DP>(), DP <= 64 ? 2 : DP == 128 ? 3 : 1) attn_tf32_fwd_kernel(const AttnParams p) {
   constexpr int NT = kCols / 8;
   constexpr bool EXACT = sizeof(T) == 2;
-  constexpr int SLOTS = forward_slots<DP>();
+  constexpr int SLOTS = forward_slots<DP>(), GROUPS = forward_groups<DP>(), COLS = kCols * GROUPS, THREADS = kThreads * GROUPS;
+  constexpr int kTile = COLS * Pitch<DP>::kFloats;
   using S = Pitch<DP>;
   extern __shared__ __align__(16) float smem[];
   float *qs = smem, *ring = smem + S::kRowTile;  // slots: keys, then values
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
+  const int side = threadIdx.x / kThreads, warp = threadIdx.x / 32 % 4, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
   const int h = blockIdx.x % p.H, b = blockIdx.x / p.H, hk = h / (p.H / p.Hkv);
   const int i0 = (gridDim.y - 1 - blockIdx.y) * kRows;  // long causal rows first
   const int length = attn_length(p, b);
@@ -323,18 +332,18 @@ __global__ void __launch_bounds__(kThreads, DP <= 64 ? 4 : DP == 128 ? 3 : 1) at
   const T* v = static_cast<const T*>(p.v) + b * p.vs[0] + hk * p.vs[2];
   const bool kvec = can_vec<T>(p.k, p.ks, p.D), vvec = can_vec<T>(p.v, p.vs, p.D);
   const auto next = [&](int j) {
-    while (j < limit && skip_tiles(p, b, i0, j)) j += kCols;
+    while (j < limit && skip_tiles(p, b, i0, j)) j += COLS;
     return j;
   };
   const auto fill = [&](int j, int slot) {
     if (j < limit) {
       const auto keep = [&](int r) { return !key_padded(p, b, j + r, length); };
-      load_rows<T, DP>(ring + slot * 2 * S::kColTile, kCols, k, p.ks[1], j, p.D, kvec, keep);
-      load_rows<T, DP>(ring + (slot * 2 + 1) * S::kColTile, kCols, v, p.vs[1], j, p.D, vvec, keep);
+      load_rows<T, DP, THREADS>(ring + slot * 2 * kTile, COLS, k, p.ks[1], j, p.D, kvec, keep);
+      load_rows<T, DP, THREADS>(ring + (slot * 2 + 1) * kTile, COLS, v, p.vs[1], j, p.D, vvec, keep);
     }
     copies_done();
   };
-  load_rows<T, DP>(qs, kRows, static_cast<const T*>(p.q) + b * p.qs[0] + h * p.qs[2], p.qs[1], i0, p.D,
+  load_rows<T, DP, THREADS>(qs, kRows, static_cast<const T*>(p.q) + b * p.qs[0] + h * p.qs[2], p.qs[1], i0, p.D,
                    can_vec<T>(p.q, p.qs, p.D), [&](int r) { return i0 + r < p.Sq; });
   int j0 = next(0);
   fill(j0, 0);
@@ -345,9 +354,9 @@ __global__ void __launch_bounds__(kThreads, DP <= 64 ? 4 : DP == 128 ? 3 : 1) at
   for (int i = 0; i < 2; ++i) row[i] = row_view(p, b, i0 + warp * 16 + g + 8 * i, length);
 #pragma unroll
   for (int d = 0; d < DP / 8; ++d) out[d][0] = out[d][1] = out[d][2] = out[d][3] = 0.0f;
-  const auto column = [&](int n, int e) { return n * 8 + 2 * t + e; };
+  const auto column = [&](int n, int e) { return side * kCols + n * 8 + 2 * t + e; };
   for (int slot = 0; j0 < limit; slot ^= SLOTS - 1) {
-    const int j1 = next(j0 + kCols);
+    const int j1 = next(j0 + COLS);
     if constexpr (SLOTS == 2) {
       fill(j1, slot ^ 1);
       copies_wait<1>();
@@ -355,7 +364,7 @@ __global__ void __launch_bounds__(kThreads, DP <= 64 ? 4 : DP == 128 ? 3 : 1) at
       copies_wait<0>();
     }
     __syncthreads();
-    const float* ks = ring + slot * 2 * S::kColTile;
+    const float* ks = ring + slot * 2 * kTile + side * S::kColTile;
     float s[NT][4], old[2];
     scores<DP, NT, EXACT>(qs + warp * 16 * S::kFloats, ks, p.D, s);
     int kd[NT][2];
@@ -366,21 +375,54 @@ __global__ void __launch_bounds__(kThreads, DP <= 64 ? 4 : DP == 128 ? 3 : 1) at
         const int j = j0 + column(n, e);
         kd[n][e] = p.kdoc && j < length ? __ldg(p.kdoc + (int64_t)b * p.Sk + j) : 0;
       }
-    const bool whole = !p.kdoc && __all_sync(kFullMask, j0 + kCols <= min(row[0].limit, row[1].limit));
+    const bool whole = !p.kdoc && __all_sync(kFullMask, j0 + COLS <= min(row[0].limit, row[1].limit));
     softmax_step<NT>(p, f, row, s, kd, j0, limit, whole, column, m, l, old);
 #pragma unroll
     for (int d = 0; d < DP / 8; ++d) {
       out[d][0] *= old[0], out[d][1] *= old[0];
       out[d][2] *= old[1], out[d][3] *= old[1];
     }
-    gather<DP, NT, EXACT, true>(s, ks + S::kColTile, out);
+    gather<DP, NT, EXACT, true>(s, ks + kTile, out);
     __syncthreads();
     if constexpr (SLOTS == 1) fill(j1, 0);
     j0 = j1;
   }
+  l[0] = sum4(l[0]), l[1] = sum4(l[1]);
+  if constexpr (GROUPS == 2) {
+    // The second group's parts take the queries' and the ring's place.
+    copies_wait<0>();
+    __syncthreads();
+    float* ml = ring;
+    if (side == 1) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = warp * 16 + g + 8 * i;
+        if (t == 0) ml[2 * r] = m[i], ml[2 * r + 1] = l[i];
+#pragma unroll
+        for (int d = 0; d < DP / 8; ++d)
+          *reinterpret_cast<float2*>(qs + r * S::kFloats + d * 8 + 2 * t) = make_float2(out[d][2 * i], out[d][2 * i + 1]);
+      }
+    }
+    __syncthreads();
+    if (side == 1) return;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = warp * 16 + g + 8 * i;
+      const float other = ml[2 * r], top = fmaxf(m[i], other), base = top == -INFINITY ? 0.0f : top;
+      const float w0 = ex2(m[i] - base), w1 = ex2(other - base);
+      m[i] = top;
+      l[i] = fmaf(l[i], w0, ml[2 * r + 1] * w1);
+#pragma unroll
+      for (int d = 0; d < DP / 8; ++d) {
+        const float2 o = *reinterpret_cast<const float2*>(qs + r * S::kFloats + d * 8 + 2 * t);
+        out[d][2 * i] = fmaf(out[d][2 * i], w0, o.x * w1);
+        out[d][2 * i + 1] = fmaf(out[d][2 * i + 1], w0, o.y * w1);
+      }
+    }
+  }
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const float sum = sum4(l[i]), mul = inverse(sum);
+    const float sum = l[i], mul = inverse(sum);
     const int r = i0 + warp * 16 + g + 8 * i;
     if (r >= p.Sq) continue;
     if (p.lse && t == 0)
@@ -507,7 +549,7 @@ __global__ void __launch_bounds__(kThreads) attn_tf32_token_kernel(const AttnPar
 // warps has half of a step's keys; their sums are added at the end.
 template <typename T, int DP>
 __global__ void __launch_bounds__(kBwdThreads, DP <= 128 ? 2 : 1) attn_tf32_dq_kernel(const AttnParams p) {
-  constexpr int NT = kCols / 16;
+  constexpr int COLS = DP <= 64 ? 2 * kCols : kCols, NT = COLS / 16, kTile = COLS * Pitch<DP>::kFloats;
   constexpr bool EXACT = sizeof(T) == 2;
   using S = Pitch<DP>;
   extern __shared__ __align__(16) float smem[];
@@ -522,14 +564,14 @@ __global__ void __launch_bounds__(kBwdThreads, DP <= 128 ? 2 : 1) attn_tf32_dq_k
   const T* v = static_cast<const T*>(p.v) + b * p.vs[0] + hk * p.vs[2];
   const bool kvec = can_vec<T>(p.k, p.ks, p.D), vvec = can_vec<T>(p.v, p.vs, p.D);
   const auto next = [&](int j) {
-    while (j < limit && skip_tiles(p, b, i0, j)) j += kCols;
+    while (j < limit && skip_tiles(p, b, i0, j)) j += COLS;
     return j;
   };
   const auto fill = [&](int j) {
     if (j < limit) {
       const auto keep = [&](int r) { return !key_padded(p, b, j + r, length); };
-      load_rows<T, DP, kBwdThreads>(ring, kCols, k, p.ks[1], j, p.D, kvec, keep);
-      load_rows<T, DP, kBwdThreads>(ring + S::kColTile, kCols, v, p.vs[1], j, p.D, vvec, keep);
+      load_rows<T, DP, kBwdThreads>(ring, COLS, k, p.ks[1], j, p.D, kvec, keep);
+      load_rows<T, DP, kBwdThreads>(ring + kTile, COLS, v, p.vs[1], j, p.D, vvec, keep);
     }
     copies_done();
   };
@@ -581,16 +623,16 @@ __global__ void __launch_bounds__(kBwdThreads, DP <= 128 ? 2 : 1) attn_tf32_dq_k
 #pragma unroll
   for (int d = 0; d < DP / 8; ++d) dq[d][0] = dq[d][1] = dq[d][2] = dq[d][3] = 0.0f;
   while (j0 < limit) {
-    const bool whole = !p.kdoc && __all_sync(kFullMask, j0 + kCols <= min(row[0].limit, row[1].limit));
-    const float* ks = ring + side * (kCols / 2) * S::kFloats;
+    const bool whole = !p.kdoc && __all_sync(kFullMask, j0 + COLS <= min(row[0].limit, row[1].limit));
+    const float* ks = ring + side * (COLS / 2) * S::kFloats;
     float s[NT][4], dp[NT][4];
     scores<DP, NT, EXACT>(qs + warp * 16 * S::kFloats, ks, p.D, s);
-    scores<DP, NT, EXACT>(gs + warp * 16 * S::kFloats, ks + S::kColTile, p.D, dp);
+    scores<DP, NT, EXACT>(gs + warp * 16 * S::kFloats, ks + kTile, p.D, dp);
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int j = j0 + side * (kCols / 2) + n * 8 + 2 * t + e;
+        const int j = j0 + side * (COLS / 2) + n * 8 + 2 * t + e;
         const int kd = p.kdoc && j < length ? __ldg(p.kdoc + (int64_t)b * p.Sk + j) : 0;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -602,7 +644,7 @@ __global__ void __launch_bounds__(kBwdThreads, DP <= 128 ? 2 : 1) attn_tf32_dq_k
       }
     gather<DP, NT, EXACT, false>(s, ks, dq);
     __syncthreads();
-    j0 = next(j0 + kCols);
+    j0 = next(j0 + COLS);
     fill(j0);
     copies_wait<0>();
     __syncthreads();
@@ -773,16 +815,16 @@ cudaError_t forward(const AttnParams& p, bool token, cudaStream_t st) {
     return launch(attn_tf32_token_kernel<T, DP>, dim3(p.Hkv * ((rows + 15) / 16), p.splits, p.B), kThreads,
                   16 * S::kFloats + 4 * S::kColTile, set[0], p, st);
   }
-  return launch(attn_tf32_fwd_kernel<T, DP>, dim3(p.H * p.B, row_tiles(p.Sq)), kThreads,
-                S::kRowTile + 2 * forward_slots<DP>() * S::kColTile, set[1], p, st);
+  return launch(attn_tf32_fwd_kernel<T, DP>, dim3(p.H * p.B, row_tiles(p.Sq)), kThreads * forward_groups<DP>(),
+                S::kRowTile + 2 * forward_slots<DP>() * forward_groups<DP>() * S::kColTile, set[1], p, st);
 }
 
 template <typename T, int DP>
 cudaError_t backward(const AttnParams& p, cudaStream_t st) {
   using S = Pitch<DP>;
   static std::atomic<uint64_t> set[2];
-  constexpr int floats = 2 * S::kRowTile + 2 * S::kColTile;
-  cudaError_t e = launch(attn_tf32_dq_kernel<T, DP>, dim3(p.H * p.B, row_tiles(p.Sq)), kBwdThreads, floats, set[0], p, st);
+  constexpr int floats = 2 * S::kRowTile + 2 * S::kColTile, wide = DP <= 64 ? floats + 2 * S::kColTile : floats;
+  cudaError_t e = launch(attn_tf32_dq_kernel<T, DP>, dim3(p.H * p.B, row_tiles(p.Sq)), kBwdThreads, wide, set[0], p, st);
   if (e == cudaSuccess)
     e = launch(attn_tf32_dkv_kernel<T, DP>, dim3(p.Hkv * p.B, row_tiles(p.Sk)), kBwdThreads, floats, set[1], p, st);
   return e;
