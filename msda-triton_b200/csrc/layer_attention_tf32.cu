@@ -145,10 +145,10 @@ __device__ __forceinline__ void scores(const float* a, const float* b, int D, fl
 // out += p (16 x 8 NT, in the layout of `scores`) . t over tokens; EXACT: t is of
 // tf32 numbers. WHOLE: t's last bits too, by a fourth product, so that a
 // probability of 1 gives the value itself (and the row's gradient, g . v - g . o,
-// nothing).
-template <int DP, int NT, bool EXACT, bool WHOLE>
-__device__ __forceinline__ void gather(const float (&p)[NT][4], const float* t, float (&out)[DP / 8][4]) {
-  constexpr int P = Pitch<DP>::kFloats, N = 4;
+// nothing). W channels of rows of DP.
+template <int DP, int W, int NT, bool EXACT, bool WHOLE>
+__device__ __forceinline__ void gather(const float (&p)[NT][4], const float* t, float (&out)[W / 8][4]) {
+  constexpr int P = Pitch<DP>::kFloats, N = W < 32 ? W / 8 : 4;
   constexpr bool REST = WHOLE && !EXACT;
   const int lane = threadIdx.x % 32;
   const float* at = t + lane % 4 * 2 * P + lane / 4;
@@ -164,7 +164,7 @@ __device__ __forceinline__ void gather(const float (&p)[NT][4], const float* t, 
       parts<false>(x, ah[m], al[m]);
     }
 #pragma unroll
-    for (int d = 0; d < DP / 8; d += N) {
+    for (int d = 0; d < W / 8; d += N) {
       float c[N][4];
       clear(c);
 #pragma unroll
@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(kThreads * forward_groups<DP>(), DP <= 64 ? 2 
       out[d][0] *= old[0], out[d][1] *= old[0];
       out[d][2] *= old[1], out[d][3] *= old[1];
     }
-    gather<DP, NT, EXACT, true>(s, ks + kTile, out);
+    gather<DP, DP, NT, EXACT, true>(s, ks + kTile, out);
     __syncthreads();
     if constexpr (SLOTS == 1) fill(j1, 0);
     j0 = j1;
@@ -502,7 +502,7 @@ __global__ void __launch_bounds__(kThreads) attn_tf32_token_kernel(const AttnPar
       out[d][0] *= old[0], out[d][1] *= old[0];
       out[d][2] *= old[1], out[d][3] *= old[1];
     }
-    gather<DP, 1, EXACT, true>(s, ks + S::kColTile, out);
+    gather<DP, DP, 1, EXACT, true>(s, ks + S::kColTile, out);
     __syncthreads();
   }
   copies_wait<0>();
@@ -544,6 +544,13 @@ __global__ void __launch_bounds__(kThreads) attn_tf32_token_kernel(const AttnPar
     }
   }
 }
+
+// Warp w of either group, which have the same 16 rows.
+__device__ __forceinline__ void pair_sync(int w) { asm volatile("bar.sync %0, 64;" ::"r"(w + 1) : "memory"); }
+__device__ __forceinline__ void pair_arrive(int w) { asm volatile("bar.arrive %0, 64;" ::"r"(w + 1) : "memory"); }
+
+// z x, z being p (1 - tanh^2) >= 0 or, of a key that a row does not see, -0.
+__device__ __forceinline__ float times_seen(float z, float x) { return __float_as_uint(z) == 0x80000000u ? 0.0f : z * x; }
 
 // dq, and delta_i = g_i . o_i for the key gradient that follows. Each group of four
 // warps has half of a step's keys; their sums are added at the end.
@@ -642,7 +649,7 @@ __global__ void __launch_bounds__(kBwdThreads, DP <= 128 ? 2 : 1) attn_tf32_dq_k
           s[n][2 * i + e] = seen ? x * (dp[n][2 * i + e] - delta[i]) * fmaf(-th, th, 1.0f) : 0.0f;
         }
       }
-    gather<DP, NT, EXACT, false>(s, ks, dq);
+    gather<DP, DP, NT, EXACT, false>(s, ks, dq);
     __syncthreads();
     j0 = next(j0 + COLS);
     fill(j0);
@@ -675,8 +682,9 @@ __global__ void __launch_bounds__(kBwdThreads, DP <= 128 ? 2 : 1) attn_tf32_dq_k
 }
 
 // dk and dv of 64 keys: every query of every head that shares them, in a fixed
-// order. One group of four warps has dv, the other dk, with the scores formed by
-// both: five products where one group needs four, but twice the warps.
+// order. One group of four warps forms the probabilities and has dv, the other
+// forms g . v and has dk: two products each, and 16 sums a thread and step handed
+// over within a pair of warps.
 template <typename T, int DP>
 __global__ void __launch_bounds__(kBwdThreads, DP <= 128 ? 2 : 1) attn_tf32_dkv_kernel(const AttnParams p) {
   constexpr int NT = kCols / 8;
@@ -684,6 +692,7 @@ __global__ void __launch_bounds__(kBwdThreads, DP <= 128 ? 2 : 1) attn_tf32_dkv_
   using S = Pitch<DP>;
   extern __shared__ __align__(16) float smem[];
   float *ks = smem, *vs = smem + S::kRowTile, *qs = smem + 2 * S::kRowTile, *gs = qs + S::kColTile;
+  float4* mid = reinterpret_cast<float4*>(gs + S::kColTile) + threadIdx.x % 128;  // a pair of warps' p (1 - tanh^2)
   __shared__ float lse_s[kCols], delta_s[kCols];
   __shared__ RowView view_s[kCols];
   const bool keys = threadIdx.x >= 128;  // this group has dk
@@ -725,27 +734,44 @@ __global__ void __launch_bounds__(kBwdThreads, DP <= 128 ? 2 : 1) attn_tf32_dkv_
       copies_done();
       copies_wait<0>();
       __syncthreads();
-      float s[NT][4], dp[NT][4];
-      scores<DP, NT, EXACT>(ks + warp * 16 * S::kFloats, qs, p.D, s);
-      if (keys) scores<DP, NT, EXACT>(vs + warp * 16 * S::kFloats, gs, p.D, dp);
+      float s[NT][4];
+      scores<DP, NT, EXACT>((keys ? vs : ks) + warp * 16 * S::kFloats, keys ? gs : qs, p.D, s);
+      if (keys) {
+        pair_sync(warp);
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n) {
+          const float4 z = mid[n * 128];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int c = n * 8 + 2 * t + e;
-          const RowView row = view_s[c];
-          const float lse2 = lse_s[c], delta = delta_s[c];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int j = j0 + warp * 16 + g + 8 * i;
-            const bool seen = j < row.limit && (!p.kdoc || same_document(row.doc, kd[i], p.shared));
-            float th;
-            const float y = ex2(score2(p, f, s[n][2 * i + e], row.place - j, th) - lse2);
-            const float z = keys ? y * (dp[n][2 * i + e] - delta) * fmaf(-th, th, 1.0f) : y;
-            s[n][2 * i + e] = seen ? z : 0.0f;
+          for (int e = 0; e < 2; ++e) {
+            const float delta = delta_s[n * 8 + 2 * t + e];
+            s[n][e] = times_seen(e ? z.y : z.x, s[n][e] - delta);
+            s[n][2 + e] = times_seen(e ? z.w : z.z, s[n][2 + e] - delta);
           }
         }
-      gather<DP, NT, EXACT, false>(s, keys ? qs : gs, out);
+      } else {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float z[4];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int c = n * 8 + 2 * t + e;
+            const RowView row = view_s[c];
+            const float lse2 = lse_s[c];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int j = j0 + warp * 16 + g + 8 * i;
+              const bool seen = j < row.limit && (!p.kdoc || same_document(row.doc, kd[i], p.shared));
+              float th;
+              const float y = ex2(score2(p, f, s[n][2 * i + e], row.place - j, th) - lse2);
+              s[n][2 * i + e] = seen ? y : 0.0f;
+              z[2 * i + e] = seen ? y * fmaf(-th, th, 1.0f) : -0.0f;
+            }
+          }
+          mid[n * 128] = make_float4(z[0], z[1], z[2], z[3]);
+        }
+        pair_arrive(warp);
+      }
+      gather<DP, DP, NT, EXACT, false>(s, keys ? qs : gs, out);
     }
   }
   T* to = static_cast<T*>(keys ? p.dk : p.dv);
@@ -826,7 +852,7 @@ cudaError_t backward(const AttnParams& p, cudaStream_t st) {
   constexpr int floats = 2 * S::kRowTile + 2 * S::kColTile, wide = DP <= 64 ? floats + 2 * S::kColTile : floats;
   cudaError_t e = launch(attn_tf32_dq_kernel<T, DP>, dim3(p.H * p.B, row_tiles(p.Sq)), kBwdThreads, wide, set[0], p, st);
   if (e == cudaSuccess)
-    e = launch(attn_tf32_dkv_kernel<T, DP>, dim3(p.Hkv * p.B, row_tiles(p.Sk)), kBwdThreads, floats, set[1], p, st);
+    e = launch(attn_tf32_dkv_kernel<T, DP>, dim3(p.Hkv * p.B, row_tiles(p.Sk)), kBwdThreads, floats + 128 * kCols / 2, set[1], p, st);
   return e;
 }
 
