@@ -67,9 +67,6 @@ namespace {
 using namespace msda;
 using namespace msda::abi;
 
-// Query rows (queries x heads that share a key head) up to which the few-rows
-// kernels run, whose CTAs split the keys.
-constexpr int64_t kTokenRows = 64;
 constexpr int kMaxSplits = 64;
 
 enum class Path { kAny, kToken, kTensor };
@@ -131,12 +128,34 @@ struct Plan {
   size_t delta = 0, part_ml = 0, part_o = 0, bytes = 0;  // byte offsets, after the summary; total
 };
 
+// Whether the few-rows kernels, whose CTAs split the keys of 16 query rows (queries
+// x heads that share a key head), are the faster ones. Both walk over the same keys,
+// so their times compare by tiles of 16 rows against waves of the other kernel's
+// CTAs. Measured over 8192 keys, few-rows / other kernel: 1 x 8 heads of 64 16-bit
+// channels 128 rows 59 / 139 us, 512 rows 139 / 133 us; 8 x 32 heads on 8 of 128
+// channels 64 rows 262 / 283 us, 128 rows 432 / 285 us; fp32, 1 x 8 heads of 64
+// channels 512 rows 454 / 718 us; 8 x 32 on 8 of 128 channels 128 rows 1719 / 2637
+// us, 256 rows 3368 / 2638 us. Over few keys in one wave the start counts: 10 / 7 us
+// over 100 keys of 128 channels, 3.7 / 4.8 us over 10 of 32. (Over 300 random
+// calls the rule's choice takes 1.5% more time than the better one.) Documents, of
+// which the other kernels skip tiles, leave the single tokens' 64 rows.
+bool few_rows_faster(const msda_attention_args* a, bool tensor) {
+  const int64_t rows = a->num_queries * (a->num_heads / a->num_key_heads), heads = a->batch * a->num_heads;
+  const int64_t tiles = a->batch * a->num_key_heads * ((rows + 15) / 16);
+  if (a->query_documents && rows > 64) return false;
+  if (!tensor) return tiles <= std::max<int64_t>(300, 2 * heads * ((a->num_queries + 63) / 64));
+  const bool narrow = a->head_dim <= 64;
+  const int64_t room = sm_count() * (narrow ? 2 : 1), waves = (heads * ((a->num_queries + 255) / 256) + room - 1) / room;
+  if (waves == 1 && a->num_keys < (narrow ? 256 : 512)) return narrow && rows <= 16;
+  return narrow ? tiles + 90 <= 350 * waves : tiles + 100 <= 215 * waves;
+}
+
 Plan plan_of(const msda_attention_args* a, bool backward) {
   Plan p;
   const int64_t group = a->num_heads / a->num_key_heads, rows = a->num_queries * group;
   const bool tensor = tensor_layout(a, backward);
   if (tensor && a->num_keys > 0) p.path = Path::kTensor;
-  p.few = !backward && rows <= kTokenRows;
+  p.few = !backward && few_rows_faster(a, tensor);
   if (p.few) {
     if (tensor) p.path = Path::kToken;
     // Parts of at least 512 keys, up to 16 CTAs an SM, so that streams of

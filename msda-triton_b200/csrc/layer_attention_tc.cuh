@@ -239,6 +239,11 @@ struct KeySteps {
 // buffers of 64 keys a tile with one CTA took 606 us and 544 us for 8192 x 16
 // heads of 128 and of 32 channels: products of 64 columns run at half rate, and
 // two warps left the exponential units idle for half of the time.)
+// bf16, 8192 tokens on 16 heads, without a mask / causal: 128 channels 518 us (1062
+// TFLOP/s) / 260 us, bound by products and exponentials that do not cover one
+// another wholly; 64 channels 415 / 212 us, 32 channels 382 / 194 us, bound by the
+// exponential units (of which the cap's tanh, a polynomial, takes none: causal and
+// capped at 128 channels 343 us).
 // ---------------------------------------------------------------------------
 template <int DP>
 struct FwdShape {
@@ -540,6 +545,14 @@ __global__ void __launch_bounds__(FwdShape<DP>::kThreads, FwdShape<DP>::kCtas)
 // where two CTAs share an SM's TMEM; each half of the eight warps takes half of
 // the columns. The derivative goes to TMEM in 16 bits without the scale, which
 // its sums get at the end: in fp16 it would cost small gradients digits.
+// Rounding it costs dq and dk as much again as rounding their results does (2.4e-3
+// of bf16 gradients against 1.7e-3): a second 16-bit part would take a fourth
+// product and TMEM that is not there.
+// bf16, 8192 tokens on 16 heads, dq / dkv without a mask: 128 channels (4 key heads)
+// 748 / 1039 us (1100 and 1058 TFLOP/s counting what is formed), 64 channels 439 /
+// 711 us, 32 channels 402 / 667 us; causal at 128 channels 419 / 459 us, capped
+// too 439 / 540 us. Bound as the forward is: by products at 128 channels, below by
+// the exponentials and the traffic of scores between TMEM and registers.
 // ---------------------------------------------------------------------------
 template <int DP>
 struct BwdShape {
