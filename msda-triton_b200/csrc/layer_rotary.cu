@@ -7,10 +7,11 @@
 // a few tokens, forms the cosines and sines of their pairs once in shared
 // memory, and turns every query and key head of those tokens with them, 16
 // bytes a thread at a time, four loads in flight. Query and key of 4 x 22223
-// tokens, 16 heads of 32 bf16 channels in all (182 MB) take 46 us, 4.0 TB/s: the
-// issue slots are half taken, by the items' index arithmetic (three 32-bit
-// products an item, no division) and the cosines, of which a token's 16 serve
-// only 16 heads there.
+// tokens, 16 heads of 32 bf16 channels in all (182 MB) take 38 us, 4.8 TB/s; of 2 x
+// 16384 tokens, 40 heads of 128 (671 MB), 115 us interleaved, 5.8 TB/s, 138 us by
+// halves, 4.9 TB/s. What is above the bytes' time is the items' index arithmetic,
+// the cosines, of which a token's 16 serve only 16 heads in the first case, and the
+// last wave of CTAs.
 #include <cmath>
 
 #include "msda_abi.cuh"
@@ -42,7 +43,7 @@ struct RotaryParams {
   int64_t tokens;  // B * S
   uint32_t seq;
   int32_t heads[2], D, pairs, num_axes, position_type, tokens_per_cta, items, all_heads;
-  uint32_t items_magic, heads_magic;  // ceil(2^32 / d): n / d = umulhi(n, magic) for n * d < 2^32
+  uint32_t items_magic, heads_magic, pairs_magic;  // ceil(2^32 / d): n / d = umulhi(n, magic) for n * d < 2^32
   float sign;
 };
 
@@ -68,22 +69,37 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryPara
   constexpr bool TWO = HALF || VP == 0;                 // an item is two loads
   constexpr int U = 4;                                  // items in flight a thread
   using Raw = typename Pack<T, W>::Raw;
-  __shared__ float2 turn[kMaxCached];
-  __shared__ int64_t from[2][kMaxTokens];  // the tokens' rows of query and key
+  __shared__ __align__(16) float2 turn[kMaxCached];
+  __shared__ int64_t from[3][kMaxTokens];  // the tokens' rows of query and key, and their positions
+  // The table, which lanes read at places of their own: constant memory would
+  // serve these one after the other (4 x 8000 tokens, 12 heads of 74 fp32 channels
+  // on three axes: 226 us).
+  __shared__ float2 frequency[kMaxPairs];
+  __shared__ ushort2 channels[kMaxPairs];
+  __shared__ uint8_t axis[kMaxPairs];
+  for (int k = threadIdx.x; k < p.pairs; k += kRotaryThreads) {
+    frequency[k] = make_float2(table.hi[k], table.lo[k]);
+    channels[k] = make_ushort2(table.first[k], table.second[k]);
+    axis[k] = table.axis[k];
+  }
   const int64_t token0 = (int64_t)blockIdx.x * p.tokens_per_cta;
   const int count = (int)min((int64_t)p.tokens_per_cta, p.tokens - token0);
-  if ((int)threadIdx.x < 2 * count) {
-    const int which = threadIdx.x & 1, t = threadIdx.x >> 1;
+  if ((int)threadIdx.x < count) {
+    const int t = threadIdx.x;
     const int64_t b = (token0 + t) / p.seq, s = token0 + t - b * p.seq;
-    from[which][t] = b * p.stride[which][0] + s * p.stride[which][1];
+    from[0][t] = b * p.stride[0][0] + s * p.stride[0][1];
+    from[1][t] = b * p.stride[1][0] + s * p.stride[1][1];
+    from[2][t] = b * p.position_batch_stride + s * p.num_axes;
   }
-  for (int i = threadIdx.x; i < count * p.pairs; i += kRotaryThreads) {
-    const int t = i / p.pairs, k = i - t * p.pairs;
-    const int64_t b = (token0 + t) / p.seq, s = token0 + t - b * p.seq;
-    const float pos = position_at(p, b * p.position_batch_stride + s * p.num_axes + table.axis[k]);
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < (uint32_t)(count * p.pairs); i += kRotaryThreads) {
+    const uint32_t t = quotient(i, p.pairs, p.pairs_magic);
+    const int k = i - t * p.pairs;
+    const float pos = position_at(p, from[2][t] + axis[k]);
     // pos * frequency exactly, as h + l; whole turns leave h without a rounding.
-    const float f = table.hi[k], h = pos * f, l = fmaf(pos, f, -h);
-    const float turns = (h - rintf(h)) + fmaf(pos, table.lo[k], l);
+    const float2 freq = frequency[k];
+    const float f = freq.x, h = pos * f, l = fmaf(pos, f, -h);
+    const float turns = (h - rintf(h)) + fmaf(pos, freq.y, l);
     float sn, cs;
     sincospif(2.0f * turns, &sn, &cs);
     turn[i] = make_float2(cs, sn * p.sign);
@@ -111,7 +127,7 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryPara
       if (item < pair_items) {
         const int k = item * N;
         at[u] = t * p.pairs + k;
-        if constexpr (TWO) c = table.first[k], apart[u] = table.second[k] - c;
+        if constexpr (TWO) c = channels[k].x, apart[u] = channels[k].y - c;
         else c = 2 * k;
       }
       const T* x = static_cast<const T*>(p.x[which]) + from[which][t] + h * p.stride[which][2] + c;
@@ -126,7 +142,16 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryPara
         *reinterpret_cast<Raw*>(y[u]) = first[u];
         continue;
       }
-      const float2* cs = turn + at[u];
+      float2 cs[N];
+      if constexpr (N > 1) {  // `at` is a multiple of N
+#pragma unroll
+        for (int j = 0; j < N; j += 2) {
+          const float4 r = *reinterpret_cast<const float4*>(turn + at[u] + j);
+          cs[j] = make_float2(r.x, r.y), cs[j + 1] = make_float2(r.z, r.w);
+        }
+      } else {
+        cs[0] = turn[at[u]];
+      }
       float a[W];
       unpack_raw<T, W>(first[u], a);
       if constexpr (TWO) {
@@ -287,6 +312,7 @@ extern "C" int msda_rotary(const void* query, const void* key, const void* posit
   p.all_heads = num_heads + num_key_heads;
   p.items_magic = magic_of(p.items);
   p.heads_magic = magic_of(p.all_heads);
+  p.pairs_magic = magic_of(p.pairs);
   // Tokens a CTA: 4096 items (16 a thread) spread the cosines' cost over the
   // heads and keep the loop busy, as long as the grid still fills the GPU twice.
   const int64_t per_token = (int64_t)p.items * p.all_heads;
