@@ -9,13 +9,22 @@
 // probabilities with values two. (On the FMA pipes, with 8 x 4 sums a thread, a
 // training step of 2 x 1500 tokens, 8 heads of 128 channels took 5.8 ms.)
 //
-// A CTA has 64 rows (queries; keys in their gradient), 16 a warp, and walks over
-// steps of 32 columns in two slots of shared memory, the next of which is filled
-// by asynchronous copies meanwhile. All tiles lie as rows of DP + 4 floats: four
+// A CTA has 64 rows (queries; keys in their gradient), 16 a warp, in one group of
+// four warps or two that share the work of a step of 32 or 64 columns (keys between
+// them in the forward and in dq, products in the key gradient). Steps come by
+// asynchronous copies, in the forward into the other of two slots; elsewhere the
+// SM's other CTAs cover them. All tiles lie as rows of DP + 4 floats: four
 // words past a multiple of 32, so that the fragments of both kinds of product (over
 // channels, by ldmatrix; over tokens, word by word) are free of bank conflicts. The
 // second product takes the probabilities from the first one's registers: its eight
 // k-slots are the tokens in the order 0 2 4 6 1 3 5 7, in which a thread has them.
+//
+// fp32, 2 x 1201 tokens, 8 heads of 32 channels, causal with prefixes: forward 79
+// us, dq 106 us, dk and dv 145 us, 20 to 33 TFLOP/s of products formed; 2 x 1500
+// tokens, 8 heads of 128: forward 585 us, 31 TFLOP/s, a training step 2.2 ms, 38
+// TFLOP/s. Bound by what stands around the products, the splitting of fragments and
+// their waits (the tensor pipe is a quarter to a third active), and at these sizes by
+// CTAs that fill the GPU one and a third times.
 #include "layer_attention.cuh"
 
 namespace msda {

@@ -16,6 +16,12 @@
 // 1000 bf16 forward 91 us for 29.) Rows wider than 8192 are read again from L2
 // for each step. Each CTA leaves one partial row of the two column sums; a second
 // kernel adds the partial rows in a fixed order.
+//
+// 88892 x 256 bf16 with a residual: forward 29 us (137 MB, 4.7 TB/s; three quarters
+// of the issue slots are taken, by the sums' shuffles), backward 42 us (182 MB, 4.3
+// TB/s) and 5 us for the columns. 2500 x 8192 fp32 with a residual: 45 and 61 us
+// (5.5 and 5.4 TB/s); 4095 x 5001 fp32, one element a load: 51 and 89 us (3.2 and
+// 2.8 TB/s).
 #include <algorithm>
 
 #include "msda_abi.cuh"
@@ -408,7 +414,11 @@ struct NormShape {
 };
 
 // Threads a row and channels a thread by the width alone: 8 channels, or 16
-// where a warp (up to 512) or 512 threads (up to 8192) hold the row with them.
+// where a warp (up to 512) or 512 threads (up to 8192) hold the row with them. A
+// barrier for each sum costs more than the threads bring, forward and backward: 40000
+// x 512 bf16 28 and 42 us by warps, 37 and 69 us by 128 threads; 20000 x 768 bf16 23
+// and 41 us by 128 threads, 38 and 57 us by 256; 10000 x 2048 bf16 25 and 42 us by
+// 256, 45 and 59 us by 512.
 int norm_threads_of(int64_t width) { return width <= 512 ? 32 : width <= 1024 ? 128 : width <= 2048 ? 256 : 512; }
 int norm_channels_of(int64_t width) { return width <= 8 * norm_threads_of(width) ? 8 : 16; }
 

@@ -6,12 +6,13 @@
 // is bound by HBM: each head vector is read once and written once. A CTA takes
 // a few tokens, forms the cosines and sines of their pairs once in shared
 // memory, and turns every query and key head of those tokens with them, 16
-// bytes a thread at a time, four loads in flight. Query and key of 4 x 22223
+// bytes a thread at a time, two items in flight. Query and key of 4 x 22223
 // tokens, 16 heads of 32 bf16 channels in all (182 MB) take 38 us, 4.8 TB/s; of 2 x
-// 16384 tokens, 40 heads of 128 (671 MB), 115 us interleaved, 5.8 TB/s, 138 us by
-// halves, 4.9 TB/s. What is above the bytes' time is the items' index arithmetic,
+// 16384 tokens, 40 heads of 128 (671 MB), 110 us interleaved, 6.1 TB/s, 131 us by
+// halves, 5.1 TB/s. What is above the bytes' time is the items' index arithmetic,
 // the cosines, of which a token's 16 serve only 16 heads in the first case, and the
-// last wave of CTAs.
+// last wave of CTAs. (Four items in flight: 138 us by halves, at fewer CTAs an SM;
+// one: 44 us in the first case.)
 #include <cmath>
 
 #include "msda_abi.cuh"
@@ -67,13 +68,13 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryPara
   constexpr int N = VP == 0 ? 1 : VP;                   // pairs an item
   constexpr int W = HALF ? N : (VP == 0 ? 1 : 2 * VP);  // elements a load
   constexpr bool TWO = HALF || VP == 0;                 // an item is two loads
-  constexpr int U = 4;                                  // items in flight a thread
+  constexpr int U = 2;                                  // items in flight a thread
   using Raw = typename Pack<T, W>::Raw;
   __shared__ __align__(16) float2 turn[kMaxCached];
   __shared__ int64_t from[3][kMaxTokens];  // the tokens' rows of query and key, and their positions
   // The table, which lanes read at places of their own: constant memory would
   // serve these one after the other (4 x 8000 tokens, 12 heads of 74 fp32 channels
-  // on three axes: 226 us).
+  // on three axes: 226 us for 79).
   __shared__ float2 frequency[kMaxPairs];
   __shared__ ushort2 channels[kMaxPairs];
   __shared__ uint8_t axis[kMaxPairs];
