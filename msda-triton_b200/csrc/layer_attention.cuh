@@ -45,7 +45,14 @@ struct AttnParams {
   int splits;          // parts of the keys; above 1 the parts' results go to part_o, part_ml
   float* part_o;       // (splits, B, H, Sq, D)
   float2* part_ml;     // (splits, B, H, Sq): maximum (base 2) and sum
+  int kv_parts;        // parts of a key head's query heads in its gradient; above 1 the sums go to part_kv
+  float* part_kv;      // (kv_parts, 2, B, Sk, Hkv, D): dv's parts and dk's
 };
+
+// A part's sums of dv, or of dk.
+__device__ __forceinline__ float* kv_part(const AttnParams& p, int part, bool keys) {
+  return p.part_kv + (part * 2 + (keys ? 1 : 0)) * ((int64_t)p.B * p.Sk * p.Hkv * p.D);
+}
 
 __device__ __forceinline__ int attn_length(const AttnParams& p, int b) {
   if (!p.klen) return p.Sk;
@@ -173,6 +180,7 @@ int attn_tc_forward(const AttnParams& p, int dtype, cudaStream_t st);
 int attn_tc_backward(const AttnParams& p, int dtype, cudaStream_t st);
 // Waits of the tensor-core kernels that gave up so far (reads device memory).
 cudaError_t attn_tc_gave_up(int* count);
+cudaError_t attn_kv_sum_launch(const AttnParams& p, int dtype, cudaStream_t st);
 cudaError_t attn_combine_launch(const AttnParams& p, int dtype, cudaStream_t st);
 
 }  // namespace msda

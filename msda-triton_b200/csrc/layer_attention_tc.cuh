@@ -662,6 +662,15 @@ __device__ __forceinline__ void write_row(T* out, bool in, uint32_t at, int firs
 #pragma unroll
     for (int e = 0; e < 32; e += 8) {
       if (first + c + e >= D) continue;
+      if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int x = 0; x < 8; x += 4) {
+          float4 v = make_float4(mul - mul, mul - mul, mul - mul, mul - mul);
+          if (any) v = make_float4(o[e + x] * mul, o[e + x + 1] * mul, o[e + x + 2] * mul, o[e + x + 3] * mul);
+          *reinterpret_cast<float4*>(out + c + e + x) = v;
+        }
+        continue;
+      }
       uint4 v;
       uint32_t* w = reinterpret_cast<uint32_t*>(&v);
 #pragma unroll
@@ -939,7 +948,8 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
   __shared__ int abort_flag;
   volatile int* abort = &abort_flag;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int hk = blockIdx.x % p.Hkv, b = blockIdx.x / p.Hkv, group = p.H / p.Hkv;
+  const int hk = blockIdx.x % p.Hkv, part = blockIdx.x / p.Hkv % p.kv_parts, b = blockIdx.x / (p.Hkv * p.kv_parts);
+  const int group = p.H / p.Hkv / p.kv_parts, head0 = (hk * p.kv_parts + part) * group;  // this CTA's query heads
   const int kt = blockIdx.y, j0 = kt * kTileTokens;  // early keys, which the most causal queries see, first
   const int length = attn_length(p, b);
   if (threadIdx.x == 0) {
@@ -973,7 +983,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
       const int i = at.row() + r;
       view = row_view(p, b, i, length);
       if (half == 0) {
-        const int64_t stat = ((int64_t)b * p.H + hk * group + at.g) * p.Sq + i;
+        const int64_t stat = ((int64_t)b * p.H + head0 + at.g) * p.Sq + i;
         lse = view.limit > 0 ? __ldg(p.lse + stat) * -kLog2e : 0.0f;
         delta = view.limit > 0 ? -__ldg(p.delta + stat) : 0.0f;
       }
@@ -985,7 +995,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
     // A warp whose wait gave up still comes to the others' barriers.
     while (!at.done) {
       QueryStats<STEP>& q = stats[u & 1];
-      const ScoreForm f = score_form(p, hk * group + at.g);
+      const ScoreForm f = score_form(p, head0 + at.g);
       const bool agree = at.state.agree & 1;
       // This buffer was read two steps ago: every thread has passed the barrier
       // of the step between.
@@ -1048,8 +1058,10 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
     const bool in = j < p.Sk;
     const int64_t out = (((int64_t)b * p.Sk + j) * p.Hkv + hk) * p.D;
     // The first half of the warps writes dv, the second dk.
-    if (half == 0) write_row<T, DP>(static_cast<T*>(p.dv) + out, in, dv_at + lanes, 0, p.D, ok ? 1.0f : NAN, u > 0);
-    else write_row<T, DP>(static_cast<T*>(p.dk) + out, in, dk_at + lanes, 0, p.D, ok ? p.scale : NAN, u > 0);
+    const uint32_t sums = (half == 0 ? dv_at : dk_at) + lanes;
+    const float mul = !ok ? NAN : half == 0 ? 1.0f : p.scale;
+    if (p.kv_parts > 1) write_row<float, DP>(kv_part(p, part, half != 0) + out, in, sums, 0, p.D, mul, u > 0);
+    else write_row<T, DP>(static_cast<T*>(half == 0 ? p.dv : p.dk) + out, in, sums, 0, p.D, mul, u > 0);
     fence_before();
   } else {
     if constexpr (Shape::kSplit) leave_registers();
@@ -1064,7 +1076,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
         int n = 0;
         bool ok = true;
         for (; !at.done && ok; at.next_tile(p, b, group, kt, length)) {
-          const int slot = n % 2, h = hk * group + at.g, i0 = at.i * kTileTokens;
+          const int slot = n % 2, h = head0 + at.g, i0 = at.i * kTileTokens;
           if (n >= 2) ok = warp_wait(&q_empty[slot], (n / 2 - 1) & 1, abort);
           if (!ok) break;
           char* stage = ring + slot * 2 * Shape::kTile;
@@ -1169,7 +1181,7 @@ cudaError_t launch_bwd(const AttnParams& p, const CUtensorMap (&m)[4], cudaStrea
   const auto tiles = [](int n) { return (unsigned)((n + kTileTokens - 1) / kTileTokens); };
   attn_tc_dq_kernel<T, DP, MODE><<<dim3(p.H * p.B, tiles(p.Sq)), Shape::kThreads, Shape::kSmem, st>>>(p, m[0], m[1], m[2], m[3]);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  attn_tc_dkv_kernel<T, DP, MODE><<<dim3(p.Hkv * p.B, tiles(p.Sk)), Shape::kThreads, Shape::kSmem, st>>>(p, m[0], m[1], m[2], m[3]);
+  attn_tc_dkv_kernel<T, DP, MODE><<<dim3(p.Hkv * p.kv_parts * p.B, tiles(p.Sk)), Shape::kThreads, Shape::kSmem, st>>>(p, m[0], m[1], m[2], m[3]);
   return cudaGetLastError();
 }
 

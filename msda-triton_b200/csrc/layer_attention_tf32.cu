@@ -20,7 +20,7 @@
 // k-slots are the tokens in the order 0 2 4 6 1 3 5 7, in which a thread has them.
 //
 // fp32, 2 x 1201 tokens, 8 heads of 32 channels, causal with prefixes: forward 79
-// us, dq 106 us, dk and dv 145 us, 20 to 33 TFLOP/s of products formed; 2 x 1500
+// us, dq 106 us, dk and dv 145 us, 26 to 29 TFLOP/s of products formed; 2 x 1500
 // tokens, 8 heads of 128: forward 585 us, 31 TFLOP/s, a training step 2.2 ms, 38
 // TFLOP/s. Bound by what stands around the products, the splitting of fragments and
 // their waits (the tensor pipe is a quarter to a third active), and at these sizes by
@@ -706,7 +706,8 @@ __global__ void __launch_bounds__(kBwdThreads, DP <= 128 ? 2 : 1) attn_tf32_dkv_
   __shared__ RowView view_s[kCols];
   const bool keys = threadIdx.x >= 128;  // this group has dk
   const int warp = threadIdx.x / 32 % 4, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
-  const int hk = blockIdx.x % p.Hkv, b = blockIdx.x / p.Hkv, group = p.H / p.Hkv;
+  const int hk = blockIdx.x % p.Hkv, part = blockIdx.x / p.Hkv % p.kv_parts, b = blockIdx.x / (p.Hkv * p.kv_parts);
+  const int group = p.H / p.Hkv / p.kv_parts, head0 = (hk * p.kv_parts + part) * group;  // this CTA's query heads
   const int j0 = blockIdx.y * kRows;
   const int length = attn_length(p, b);
   const auto keep = [&](int r) { return !key_padded(p, b, j0 + r, length); };
@@ -725,7 +726,7 @@ __global__ void __launch_bounds__(kBwdThreads, DP <= 128 ? 2 : 1) attn_tf32_dkv_
   const bool qvec = can_vec<T>(p.q, p.qs, p.D), gvec = can_vec<T>(p.go, p.gs, p.D);
   const int first = j0 < length ? first_query(p, b, j0, length) / kCols * kCols : p.Sq;
   for (int x = 0; x < group; ++x) {
-    const int h = hk * group + x;
+    const int h = head0 + x;
     const ScoreForm f = score_form(p, h);
     for (int i0 = first; i0 < p.Sq; i0 += kCols) {
       if (skip_tiles(p, b, i0, j0)) continue;
@@ -784,6 +785,7 @@ __global__ void __launch_bounds__(kBwdThreads, DP <= 128 ? 2 : 1) attn_tf32_dkv_
     }
   }
   T* to = static_cast<T*>(keys ? p.dk : p.dv);
+  float* sums = p.kv_parts > 1 ? kv_part(p, part, keys) : nullptr;
   const float mul = keys ? p.scale : 1.0f;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -796,7 +798,8 @@ __global__ void __launch_bounds__(kBwdThreads, DP <= 128 ? 2 : 1) attn_tf32_dkv_
       for (int e = 0; e < 2; ++e) {
         const int c = d * 8 + 2 * t + e;
         if (c >= p.D) continue;
-        to[at + c] = from_f32<T>(out[d][2 * i + e] * mul);
+        if (p.kv_parts > 1) sums[at + c] = out[d][2 * i + e] * mul;
+        else to[at + c] = from_f32<T>(out[d][2 * i + e] * mul);
       }
   }
 }
@@ -861,7 +864,7 @@ cudaError_t backward(const AttnParams& p, cudaStream_t st) {
   constexpr int floats = 2 * S::kRowTile + 2 * S::kColTile, wide = DP <= 64 ? floats + 2 * S::kColTile : floats;
   cudaError_t e = launch(attn_tf32_dq_kernel<T, DP>, dim3(p.H * p.B, row_tiles(p.Sq)), kBwdThreads, wide, set[0], p, st);
   if (e == cudaSuccess)
-    e = launch(attn_tf32_dkv_kernel<T, DP>, dim3(p.Hkv * p.B, row_tiles(p.Sk)), kBwdThreads, floats + 128 * kCols / 2, set[1], p, st);
+    e = launch(attn_tf32_dkv_kernel<T, DP>, dim3(p.Hkv * p.kv_parts * p.B, row_tiles(p.Sk)), kBwdThreads, floats + 128 * kCols / 2, set[1], p, st);
   return e;
 }
 

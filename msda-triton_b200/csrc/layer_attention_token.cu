@@ -345,6 +345,24 @@ __global__ void __launch_bounds__(128) attn_combine_kernel(const AttnParams p) {
   if (p.lse && lane == 0) p.lse[row] = total == 0.0f ? -INFINITY : (top + log2f(total)) * kLn2;
 }
 
+// dv (blockIdx.y 0) and dk from the parts' sums, in the parts' order.
+template <typename T>
+__global__ void __launch_bounds__(256) attn_kv_sum_kernel(const AttnParams p) {
+  const int64_t all = (int64_t)p.B * p.Sk * p.Hkv * p.D, step = (int64_t)gridDim.x * 1024;
+  const float* from = kv_part(p, 0, blockIdx.y != 0);
+  T* to = static_cast<T*>(blockIdx.y ? p.dk : p.dv);
+  for (int64_t i0 = (int64_t)blockIdx.x * 1024 + threadIdx.x; i0 < all; i0 += step) {
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int part = 0; part < p.kv_parts; ++part)
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (i0 + u * 256 < all) sum[u] += __ldg(from + part * 2 * all + i0 + u * 256);
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (i0 + u * 256 < all) to[i0 + u * 256] = from_f32<T>(sum[u]);
+  }
+}
+
 template <typename T>
 cudaError_t token_t(const AttnParams& p, cudaStream_t st) {
   const int rows = p.Sq * (p.H / p.Hkv);
@@ -365,6 +383,15 @@ cudaError_t token_t(const AttnParams& p, cudaStream_t st) {
 
 cudaError_t attn_token_forward(const AttnParams& p, int dtype, cudaStream_t st) {
   return dtype == MSDA_DTYPE_F16 ? token_t<__half>(p, st) : token_t<__nv_bfloat16>(p, st);
+}
+
+cudaError_t attn_kv_sum_launch(const AttnParams& p, int dtype, cudaStream_t st) {
+  const int64_t blocks = ((int64_t)p.B * p.Sk * p.Hkv * p.D + 1023) / 1024;
+  const dim3 grid((unsigned)(blocks < 4096 ? blocks : 4096), 2);
+  if (dtype == MSDA_DTYPE_F32) attn_kv_sum_kernel<float><<<grid, 256, 0, st>>>(p);
+  else if (dtype == MSDA_DTYPE_F16) attn_kv_sum_kernel<__half><<<grid, 256, 0, st>>>(p);
+  else attn_kv_sum_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(p);
+  return cudaGetLastError();
 }
 
 cudaError_t attn_combine_launch(const AttnParams& p, int dtype, cudaStream_t st) {

@@ -11,6 +11,11 @@ the result's root mean square.
   the inputs' type before the second product: two errors of at most u each,
   and 3 u leaves room for the sums; a single element meets them at full size
   and may be smaller than its terms: 12 u.
+* Where early keys meet many terms far above the result's root mean square (long
+  causal calls), an element is held to its own terms instead: each is rounded
+  once, by at most u, and their sum once more; the sum over g . out that enters
+  each ds has its own terms rounded; a quarter above that is for the sums in 32
+  bits. What lies below fp16's normal numbers, 2^-14, is rounded as they are.
 * In 32 bits the sums dominate: n terms in order are off by at most n u, near
   sqrt(n) u for signs at random; n is at most a few thousand here, and scores
   of size s turn an error of s u into one of the exponential's: 64 u in the
@@ -111,8 +116,10 @@ def visible(B, Sq, Sk, device, causal=False, prefix_lengths=None, query_document
     return torch.stack(seen), torch.stack(places)
 
 
-def attention(q, k, v, g=None, scale=None, softcap=0.0, distance_slopes=None, **masks):
-    """out, lse and, for an output gradient g, (dq, dk, dv)."""
+def attention(q, k, v, g=None, scale=None, softcap=0.0, distance_slopes=None, terms=None, **masks):
+    """out, lse and, for an output gradient g, (dq, dk, dv); with `terms` also the
+    sums of the sizes of out's, dq's, dk's and dv's terms, of which the rounded
+    factor counts for `terms` at least."""
     B, Sq, H, D = q.shape
     Sk, Hkv = k.shape[1:3]
     scale = D ** -0.5 if scale is None else scale
@@ -140,5 +147,13 @@ def attention(q, k, v, g=None, scale=None, softcap=0.0, distance_slopes=None, **
     dp = torch.einsum("bihd,bjhd->bhij", g, vv)
     ds = p * (dp - (p * dp).sum(-1, keepdim=True)) * (1 - t * t) * scale
     fold = lambda x: x.reshape(B, Sk, Hkv, G, D).sum(3)  # noqa: E731
-    return out, lse, (torch.einsum("bhij,bjhd->bihd", ds, kk), fold(torch.einsum("bhij,bihd->bjhd", ds, q)),
-                      fold(torch.einsum("bhij,bihd->bjhd", p, g)))
+    grads = (torch.einsum("bhij,bjhd->bihd", ds, kk), fold(torch.einsum("bhij,bihd->bjhd", ds, q)),
+             fold(torch.einsum("bhij,bihd->bjhd", p, g)))
+    if terms is None:
+        return out, lse, grads
+    # The output's rounded probabilities reach every ds of a row by sum(g . out).
+    ds = ds.abs() + p * (p * dp.abs()).sum(-1, keepdim=True) * (1 - t * t) * scale
+    ds = (ds / scale).clamp_min(terms).masked_fill(~seen[:, None], 0) * scale
+    p = p.clamp_min(terms).masked_fill(~seen[:, None], 0)
+    return out, lse, grads, (torch.einsum("bhij,bjhd->bihd", p, vv.abs()), torch.einsum("bhij,bjhd->bihd", ds, kk.abs()),
+                             fold(torch.einsum("bhij,bihd->bjhd", ds, q.abs())), fold(torch.einsum("bhij,bihd->bjhd", p, g.abs())))

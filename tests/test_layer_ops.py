@@ -343,6 +343,23 @@ def _check(q, k, v, dtype, train=True, size=64, **how):
     return out.detach(), None
 
 
+def _check_by_terms(q, k, v, dtype, **how):
+    """As _check with gradients, in 16 bits with each element held to its terms."""
+    if dtype == torch.float32:
+        return _check(q, k, v, dtype, **how)
+    q, k, v = (t.detach().requires_grad_() for t in (q, k, v))
+    g = randn(*q.shape, dtype=dtype, seed=11)
+    with torch.no_grad():
+        want, _, grads, terms = ref.attention(q, k, v, g, terms=2.0**-14 if dtype == torch.float16 else 0.0, **how)
+    out = attention(q, k, v, **how)
+    got = (out, *torch.autograd.grad(out, (q, k, v), g))
+    u = ref.U[dtype]
+    for n, a, b, size in zip(("out", "dq", "dk", "dv"), got, (want, *grads), terms):
+        off = (a.detach().double() - b).abs()
+        assert off.norm() <= 3 * u * b.norm(), n
+        assert (off <= 1.25 * u * (size + b.abs()) + 1e-5 * b.square().mean().sqrt()).all(), n
+
+
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("kind", MASKS)
@@ -372,6 +389,28 @@ def test_attention_sizes(Sq, Sk, D, dtype, cuda_lib):
     q, k, v = randn(2, Sq, 2, D, dtype=dtype), randn(2, Sk, 2, D, dtype=dtype, seed=1), randn(2, Sk, 2, D, dtype=dtype, seed=2)
     for kind in ("none", "causal", "lengths"):
         _check(q, k, v, dtype, **_masks(kind, 2, Sq, Sk))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B, S, H, Hkv, D", [(1, 70, 24, 2, 32), (1, 260, 8, 1, 128), (30, 130, 12, 4, 32), (20, 130, 24, 4, 40),
+                                             (70, 130, 8, 4, 24)])
+def test_attention_shared_heads(B, S, H, Hkv, D, dtype, cuda_lib):
+    """Key gradients whose query heads share CTAs wholly, in parts or not at all."""
+    q, k, v = randn(B, S, H, D, dtype=dtype), randn(B, S, Hkv, D, dtype=dtype, seed=1), randn(B, S, Hkv, D, dtype=dtype, seed=2)
+    for kind in ("causal", "shared"):
+        _check_by_terms(q, k, v, dtype, **_masks(kind, B, S, S))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B, Sq, Sk, H, Hkv, D", [(1, 100, 2000, 4, 4, 64), (1, 61, 3000, 8, 2, 128), (2, 250, 900, 2, 1, 32),
+                                                  (9, 130, 600, 8, 8, 40)])
+def test_attention_some_queries_over_more_keys(B, Sq, Sk, H, Hkv, D, dtype, cuda_lib):
+    q, k, v = randn(B, Sq, H, D, dtype=dtype), randn(B, Sk, Hkv, D, dtype=dtype, seed=1), randn(B, Sk, Hkv, D, dtype=dtype, seed=2)
+    s = 0.01 * torch.arange(H, device=DEV, dtype=torch.float32)
+    for kind in ("none", "prefix", "causal_lengths", "scattered"):
+        _check_by_terms(q, k, v, dtype, distance_slopes=s, **_masks(kind, B, Sq, Sk))
 
 
 @gpu
