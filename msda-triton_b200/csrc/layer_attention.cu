@@ -37,9 +37,20 @@ bool make_map(CUtensorMap* map, const void* base, bool bf16, int64_t D, int64_t 
   // A dimension of one element may have any stride; 16 bytes stand for it.
   for (int i = 0; i < 3; ++i) stride[i] = size[i + 1] > 1 ? (cuuint64_t)from[i] * 2 : 16;
   const cuuint32_t box[4] = {64, 1, 128, 1}, step[4] = {1, 1, 1, 1};
-  return encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), size,
-                stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  const auto run = [&] {
+    return encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), size,
+                  stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = run();
+  if (r == CUDA_ERROR_INVALID_CONTEXT || r == CUDA_ERROR_NOT_INITIALIZED) {
+    // A thread that has not used its device so far (autograd's, when the memory comes
+    // from a cache) has no context: the runtime would bind it at its first launch.
+    int device;
+    if (cudaGetDevice(&device) != cudaSuccess || cudaSetDevice(device) != cudaSuccess) return false;
+    r = run();
+  }
+  return r == CUDA_SUCCESS;
 }
 
 }  // namespace tc

@@ -6,7 +6,10 @@ differences, and their refusals."""
 from __future__ import annotations
 
 import ctypes
+import os
 import re
+import subprocess
+import sys
 import zlib
 from pathlib import Path
 
@@ -523,6 +526,27 @@ def test_attention_repeats_bitwise_and_on_other_streams(dtype, cuda_lib):
     side.synchronize()
     for a in again:
         assert all(torch.equal(x, y) for x, y in zip(first, a))
+
+
+@gpu
+def test_attention_backward_as_a_threads_first_cuda_call(cuda_lib):
+    """A fresh process whose backward takes its memory from the allocator's cache:
+    autograd's thread has made no CUDA call before it asks for tensor maps."""
+    code = """
+import torch
+from msda_triton_b200 import attention
+q = torch.randn(1, 300, 2, 64, device="cuda", dtype=torch.bfloat16).requires_grad_()
+cached = [torch.empty(n, device="cuda", dtype=torch.bfloat16) for n in (1 << 16, 1 << 20, 1 << 24) for _ in range(4)]
+g = torch.randn_like(q)
+del cached
+out = attention(q, q, q, causal=True)
+grad, = torch.autograd.grad(out, q, g)
+assert bool(torch.isfinite(grad).all()) and bool(grad.any())
+"""
+    path = os.pathsep.join([str(Path(_lib.__file__).resolve().parent.parent), os.environ.get("PYTHONPATH", "")])
+    done = subprocess.run([sys.executable, "-c", code], env={**os.environ, "PYTHONPATH": path}, capture_output=True, text=True,
+                          timeout=300)
+    assert done.returncode == 0, done.stderr
 
 
 @gpu
