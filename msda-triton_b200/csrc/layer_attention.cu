@@ -185,13 +185,15 @@ Plan plan_of(const msda_attention_args* a, bool backward) {
   p.few = !backward && few_rows_faster(a, tensor);
   if (p.few) {
     if (tensor) p.path = Path::kToken;
-    // Parts of at least 512 keys, up to 16 CTAs an SM, so that streams of
-    // different lengths even out; of at least 128 keys where that leaves fewer
-    // than 2 CTAs an SM. (Parts of 128 keys throughout: 8 streams of 4096 keys on 8
-    // heads of 128 channels took 60 us.)
+    // Parts of at least 2048 keys (512 for the slower kernel of 32 bits), up to 16
+    // CTAs an SM, so that streams of different lengths even out; of at least 128
+    // keys where that leaves fewer than 2 CTAs an SM. With at least 512 and 2048
+    // keys, 32 heads on 8 of 128 16-bit channels: 4 streams of 4096 to 16384 keys 69
+    // and 44 us, 8 of up to 8192 58 and 46 us, 32 of 16384 377 and 366 us; fp32, 16
+    // of up to 8192 on 8 heads of 64 channels 129 and 184 us.
     const int64_t tiles = (rows + 15) / 16;
     const int64_t ctas = std::max<int64_t>(1, a->batch * a->num_key_heads * tiles);
-    const int64_t even = std::min<int64_t>(16 * sm_count() / ctas, a->num_keys / 512);
+    const int64_t even = std::min<int64_t>(16 * sm_count() / ctas, a->num_keys / (tensor ? 2048 : 512));
     const int64_t fill = std::min<int64_t>(2 * sm_count() / ctas, (a->num_keys + 127) / 128);
     const int64_t s = std::min<int64_t>(std::max(even, fill), kMaxSplits);
     p.splits = s < 1 ? 1 : (int)s;
