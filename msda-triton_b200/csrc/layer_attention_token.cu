@@ -13,9 +13,9 @@
 // and pairs the keys by byte permutes. The rows' pitches keep both kinds of read
 // free of bank conflicts. The keys are split over CTAs, whose parts the combining
 // kernel joins. 32 streams of 16384 keys, 32 heads on 8 key heads of 128 channels
-// (2.15 GB) take 370 us, 5.8 TB/s; of 4096 to 16384 keys each, capped (1.34 GB), 294
-// us, 4.5 TB/s: there the lengths' spread and a cap's arithmetic in one warp at a
-// time hold it up.
+// (2.15 GB) take 357 us, 6.0 TB/s; of 4096 to 16384 keys each 276 us, 5.3 TB/s, the
+// lengths' spread holding it up, and with capped scores 303 us, 4.8 TB/s, the cap's
+// arithmetic too (with the softmax of rows 8.. that are empty there: 329 us).
 #include "layer_attention.cuh"
 
 namespace msda {
@@ -80,6 +80,7 @@ __global__ void __launch_bounds__(kWarps * 32, DP == 128 ? 2 : DP == 64 ? 3 : 4)
   // The heads are the fast dimension: they read neighbouring bytes of the cache's
   // rows at about the same time.
   const int hk = blockIdx.x / tiles, r0 = blockIdx.x % tiles * 16, b = blockIdx.z, split = blockIdx.y;
+  const bool both = rows - r0 > 8;  // rows 8.. too
   pdl_trigger();
   const int length = attn_length(p, b);
   int first, last;
@@ -173,7 +174,7 @@ __global__ void __launch_bounds__(kWarps * 32, DP == 128 ? 2 : DP == 64 ? 3 : 4)
         mma16816<T>(s[n], qa[c][1], kr[n][c].z, kr[n][c].w);
       }
     }
-    // s[n][2 i + e]: row g + 8 i, key j0 + 8 n + 2 t + e.
+    // s[n][2 i + e]: row g + 8 i, key j0 + 8 n + 2 t + e. Rows 8.. may all be empty.
     bool small = true;  // scores well below the cap, the common case
     if (p.cap != 0.0f) {
       float big = 0.0f;
@@ -192,6 +193,7 @@ __global__ void __launch_bounds__(kWarps * 32, DP == 128 ? 2 : DP == 64 ? 3 : 4)
         const int kd = kdoc && j < last ? __ldg(kdoc + j) : 0;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
+          if (i == 1 && !both) continue;
           float x = s[n][2 * i + e] * f.scale2;
           if (p.cap != 0.0f) {
             x = s[n][2 * i + e] * f.inv_cap;
@@ -203,9 +205,10 @@ __global__ void __launch_bounds__(kWarps * 32, DP == 128 ? 2 : DP == 64 ? 3 : 4)
           top[i] = fmaxf(top[i], s[n][2 * i + e]);
         }
       }
-    uint32_t pa[4];
+    uint32_t pa[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
+      if (i == 1 && !both) continue;
       top[i] = fmaxf(top[i], __shfl_xor_sync(kFullMask, top[i], 1));
       top[i] = fmaxf(top[i], __shfl_xor_sync(kFullMask, top[i], 2));
       const float base = top[i] == -INFINITY ? 0.0f : top[i];
