@@ -173,6 +173,20 @@ __device__ __forceinline__ void document_masks(const AttnParams& p, const int* k
   }
 }
 
+// Parities of the barriers that say a ring's stage has been cleared, one for each
+// stage: a stage is not filled again before its products are done, so that none of
+// these can end two phases ahead of the wait for the first. (One barrier for all
+// stages could: the ring's tiles may be loaded and cleared before the issuing
+// thread looks at it, and its parity stands as if nothing had come.)
+struct StagePhases {
+  uint32_t bits = 0;
+  __device__ __forceinline__ uint32_t next(int stage) {
+    const uint32_t parity = bits >> stage & 1;
+    bits ^= 1u << stage;
+    return parity;
+  }
+};
+
 // Clears the rows of a tile whose token is padding (a warp): 0 x NaN is NaN, and
 // a product over tokens would spread what padding holds.
 template <int DP>
@@ -270,7 +284,7 @@ __global__ void __launch_bounds__(FwdShape<DP>::kThreads, FwdShape<DP>::kCtas)
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   char* sq = smem;
   char* ring = smem + 2 * Shape::kTile;  // slots: a visited tile's keys, then its values
-  __shared__ uint64_t q_full, kv_full[NS], kv_empty[NS], s_full[2], p_full[2], o_full[2], cleared;
+  __shared__ uint64_t q_full, kv_full[NS], kv_empty[NS], s_full[2], p_full[2], o_full[2], cleared[NS / 2];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   volatile int* abort = &abort_flag;
@@ -282,7 +296,7 @@ __global__ void __launch_bounds__(FwdShape<DP>::kThreads, FwdShape<DP>::kCtas)
   if (threadIdx.x == 0) {
     abort_flag = 0;
     bar_init(&q_full, 1);
-    bar_init(&cleared, 1);
+    for (int i = 0; i < NS / 2; ++i) bar_init(&cleared[i], 1);
     for (int i = 0; i < NS; ++i) bar_init(&kv_full[i], 1), bar_init(&kv_empty[i], 1);
     for (int t = 0; t < 2; ++t) bar_init(&s_full[t], 1), bar_init(&p_full[t], 4), bar_init(&o_full[t], 1);
     fence_async_smem();
@@ -461,7 +475,7 @@ __global__ void __launch_bounds__(FwdShape<DP>::kThreads, FwdShape<DP>::kCtas)
           if (kv && at.state.padded) {  // padded keys' values are cleared before their product
             ok = warp_wait(&kv_full[slot], (n / NS) & 1, abort);
             clear_rows<DP>(ring + slot * Shape::kTile, kdoc, at.j * kTileTokens, length);
-            if (lane == 0) bar_arrive(&cleared);
+            if (lane == 0) bar_arrive(&cleared[slot / 2]);
           }
         }
       }
@@ -477,8 +491,9 @@ __global__ void __launch_bounds__(FwdShape<DP>::kThreads, FwdShape<DP>::kCtas)
     const uint64_t q_desc = by_channels(smem_u32(sq)), k_desc = by_channels(smem_u32(ring)), v_desc = by_tokens(smem_u32(ring));
     bool ok = limit == 0 || bar_wait(&q_full, 0, abort);
     KeySteps<STEP, DOCS> at(p, b, i0, 2, limit, length);
-    int slot = 0, clears = 0;  // slot of the tile's keys; its values': the next
+    int slot = 0;  // of the tile's keys; its values': the next
     uint32_t phase = 0, turn = 0;
+    StagePhases cleared_phase;
     const auto scores = [&](int t, uint64_t k) {
       product_channels<DP>(tmem + t * STEP, q_desc + t * kSlot, k, ds);
       commit(&s_full[t]);
@@ -497,7 +512,7 @@ __global__ void __launch_bounds__(FwdShape<DP>::kThreads, FwdShape<DP>::kCtas)
       const int count = at.count(), k_slot = slot, v_slot = slot + 1;
       const uint64_t v = v_desc + v_slot * kSlot;
       ok = bar_wait(&kv_full[v_slot], phase, abort);
-      if (ok && at.state.padded) ok = bar_wait(&cleared, clears++ & 1, abort);
+      if (ok && at.state.padded) ok = bar_wait(&cleared[v_slot / 2], cleared_phase.next(v_slot / 2), abort);
       at.next_tile(p, b, i0, 2, length);
       slot += 2;
       if (slot == NS) slot = 0, phase ^= 1;
@@ -691,7 +706,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
   extern __shared__ char raw[];
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   char *sq = smem, *sg = smem + Shape::kTile, *ring = smem + 2 * Shape::kTile;  // stage: key tile, value tile
-  __shared__ uint64_t q_full, kv_full[2], kv_empty[2], s_full[2], dp_full, dp_empty, ds_full, done, cleared;
+  __shared__ uint64_t q_full, kv_full[2], kv_empty[2], s_full[2], dp_full, dp_empty, ds_full, done, cleared[2];
   __shared__ float delta_part[2][kTileTokens];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
@@ -703,8 +718,8 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
   const int limit = rows_limit(p, b, i0 + kTileTokens, length);
   if (threadIdx.x == 0) {
     abort_flag = 0;
-    bar_init(&q_full, 1), bar_init(&done, 1), bar_init(&cleared, 1), bar_init(&dp_full, 1);
-    for (int i = 0; i < 2; ++i) bar_init(&kv_full[i], 1), bar_init(&kv_empty[i], 1), bar_init(&s_full[i], 1);
+    bar_init(&q_full, 1), bar_init(&done, 1), bar_init(&dp_full, 1);
+    for (int i = 0; i < 2; ++i) bar_init(&kv_full[i], 1), bar_init(&kv_empty[i], 1), bar_init(&s_full[i], 1), bar_init(&cleared[i], 1);
     bar_init(&dp_empty, kSoftmaxThreads / 32), bar_init(&ds_full, kSoftmaxThreads / 32);
     fence_async_smem();
   }
@@ -824,7 +839,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
           if (at.state.padded) {  // padded keys are cleared: dq's product goes over all of the tile's
             ok = warp_wait(&kv_full[slot], (n / 2) & 1, abort);
             clear_rows<DP>(stage, kdoc, at.j * kTileTokens, length);
-            if (lane == 0) bar_arrive(&cleared);
+            if (lane == 0) bar_arrive(&cleared[slot]);
           }
           ++n;
         }
@@ -837,7 +852,8 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
       const uint64_t q_desc = by_channels(smem_u32(sq)), g_desc = q_desc + kTileDesc, kv_desc = by_channels(smem_u32(ring));
       const uint64_t k_tokens = by_tokens(smem_u32(ring));
       bool ok = limit == 0 || bar_wait(&q_full, 0, abort);
-      int u = 0, clears = 0, prev_slot = 0;
+      int u = 0, prev_slot = 0;
+      StagePhases cleared_phase;
       uint64_t prev_k = 0;      // keys of the step before, whose dq is due
       bool prev_last = false;   // it was its tile's last
       const auto finish = [&]() {
@@ -850,7 +866,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
       for (KeySteps<STEP, DOCS> at(p, b, i0, 1, limit, length); !at.done && ok; at.next_tile(p, b, i0, 1, length)) {
         const int slot = at.n & 1, count = at.count();
         ok = bar_wait(&kv_full[slot], (at.n >> 1) & 1, abort);
-        if (ok && at.state.padded) ok = bar_wait(&cleared, clears++ & 1, abort);
+        if (ok && at.state.padded) ok = bar_wait(&cleared[slot], cleared_phase.next(slot), abort);
         for (int half = 0; half < count && ok; ++half, ++u) {
           // Scores into the buffer that the step before last has left, ahead of
           // the softmax of the step before.
@@ -942,7 +958,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
   extern __shared__ char raw[];
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   char *sk = smem, *sv = smem + Shape::kTile, *ring = smem + 2 * Shape::kTile;  // stage: query tile, gradient tile
-  __shared__ uint64_t k_full, q_full[2], q_empty[2], s_full, p_full, dp_full, ds_full, done, cleared;
+  __shared__ uint64_t k_full, q_full[2], q_empty[2], s_full, p_full, dp_full, ds_full, done, cleared[2];
   __shared__ QueryStats<STEP> stats[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
@@ -954,8 +970,8 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
   const int length = attn_length(p, b);
   if (threadIdx.x == 0) {
     abort_flag = 0;
-    bar_init(&k_full, 1), bar_init(&done, 1), bar_init(&cleared, 1), bar_init(&s_full, 1), bar_init(&dp_full, 1);
-    for (int i = 0; i < 2; ++i) bar_init(&q_full[i], 1), bar_init(&q_empty[i], 1);
+    bar_init(&k_full, 1), bar_init(&done, 1), bar_init(&s_full, 1), bar_init(&dp_full, 1);
+    for (int i = 0; i < 2; ++i) bar_init(&q_full[i], 1), bar_init(&q_empty[i], 1), bar_init(&cleared[i], 1);
     bar_init(&p_full, kSoftmaxThreads / 32), bar_init(&ds_full, kSoftmaxThreads / 32);
     fence_async_smem();
   }
@@ -1090,7 +1106,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
             ok = warp_wait(&q_full[slot], (n / 2) & 1, abort);
             clear_rows<DP>(stage, p.qdoc + (int64_t)b * p.Sq, i0, p.Sq);
             clear_rows<DP>(stage + Shape::kTile, p.qdoc + (int64_t)b * p.Sq, i0, p.Sq);
-            if (lane == 0) bar_arrive(&cleared);
+            if (lane == 0) bar_arrive(&cleared[slot]);
           }
           ++n;
         }
@@ -1104,7 +1120,8 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
       const uint64_t qg_tokens = by_tokens(smem_u32(ring));
       QuerySteps<STEP, DOCS> at(p, b, group, kt, length);
       bool ok = at.done || bar_wait(&k_full, 0, abort);
-      int u = 0, clears = 0, prev_slot = 0;
+      int u = 0, prev_slot = 0;
+      StagePhases cleared_phase;
       uint64_t prev_q = 0;     // queries of the step before, whose sums are due
       bool prev_last = false;  // it was its tile's last
       // dv of the step before, then this step's scores over its probabilities;
@@ -1125,7 +1142,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
       for (; !at.done && ok; at.next_tile(p, b, group, kt, length)) {
         const int slot = at.n & 1, count = at.count();
         ok = bar_wait(&q_full[slot], (at.n >> 1) & 1, abort);
-        if (ok && at.state.padded) ok = bar_wait(&cleared, clears++ & 1, abort);
+        if (ok && at.state.padded) ok = bar_wait(&cleared[slot], cleared_phase.next(slot), abort);
         for (int half = 0; half < count && ok; ++half, ++u) {
           const uint64_t q = qg_desc + slot * 2 * kTileDesc + half * kHalfTile;
           if (u > 0) add_dv();

@@ -1,0 +1,50 @@
+"""The layer operators at their edges: what padding and empty rows hold, hand-overs
+between the tensor-core kernels' roles, caps, offsets and sizes at their limits."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+import layer_reference as ref
+from layer_reference import close
+from msda_triton_b200 import _lib, attention
+from test_layer_ops import DEV, DTYPES, HALF, randn
+
+gpu = pytest.mark.gpu
+
+
+def tolerance(dtype):
+    return (3, 12) if dtype != torch.float32 else (64, 1024)
+
+
+def waits_given_up():
+    n = ctypes.c_int32(-1)
+    _lib.check("msda_attention_gave_up", _lib.load().msda_attention_gave_up(ctypes.byref(n)))
+    return n.value
+
+
+@gpu
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_padding_in_every_tile(D, dtype, cuda_lib):
+    """Scattered padding: each tile of keys, and of queries in the key gradient, is
+    cleared before its products, in calls of one tile to many."""
+    before = waits_given_up()
+    for B, S in ((1, 100), (3, 250), (2, 1300), (40, 700)):
+        q, k, v, g = (randn(B, S, 2, D, dtype=dtype, seed=i) for i in range(4))
+        ids = (torch.arange(S, device=DEV) // 400).int().expand(B, S).clone()
+        pad = torch.arange(S, device=DEV)[None] * 7 % (13 + torch.arange(B, device=DEV)[:, None]) == 0
+        ids[pad] = -1
+        how = dict(query_documents=ids, key_documents=ids)
+        want, _, grads = ref.attention(q, k, v, g.masked_fill(pad[:, :, None, None], 0), **how)
+        k[pad], v[pad], q[pad], g[pad] = float("nan"), float("inf"), float("nan"), float("inf")
+        q, k, v = (t.requires_grad_() for t in (q, k, v))
+        for _ in range(4):
+            out = attention(q, k, v, **how)
+            close(out.detach(), want, dtype, *tolerance(dtype), floor=0.02, what="out")
+            for n, a, b in zip(("dq", "dk", "dv"), torch.autograd.grad(out, (q, k, v), g), grads):
+                close(a, b, dtype, *tolerance(dtype), floor=0.02, what=n)
+    assert waits_given_up() == before
