@@ -706,7 +706,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
   extern __shared__ char raw[];
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   char *sq = smem, *sg = smem + Shape::kTile, *ring = smem + 2 * Shape::kTile;  // stage: key tile, value tile
-  __shared__ uint64_t q_full, kv_full[2], kv_empty[2], s_full[2], dp_full, dp_empty, ds_full, done, cleared[2];
+  __shared__ uint64_t q_full, kv_full[2], kv_empty[2], s_full[2], dp_full, dp_empty, ds_full[2], done, cleared[2];
   __shared__ float delta_part[2][kTileTokens];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
@@ -720,7 +720,8 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
     abort_flag = 0;
     bar_init(&q_full, 1), bar_init(&done, 1), bar_init(&dp_full, 1);
     for (int i = 0; i < 2; ++i) bar_init(&kv_full[i], 1), bar_init(&kv_empty[i], 1), bar_init(&s_full[i], 1), bar_init(&cleared[i], 1);
-    bar_init(&dp_empty, kSoftmaxThreads / 32), bar_init(&ds_full, kSoftmaxThreads / 32);
+    bar_init(&dp_empty, kSoftmaxThreads / 32);
+    for (int i = 0; i < 2; ++i) bar_init(&ds_full[i], kSoftmaxThreads / 32);
     fence_async_smem();
   }
   if (warp == kMmaWarp) tmem_alloc<Shape::kColumns>(&tmem_slot);
@@ -802,7 +803,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
       __syncwarp();
       if (lane == 0) bar_arrive(&dp_empty);
       derivatives(s, dp, masked, [&](int, uint64_t& a, uint64_t& d) { a = d = delta2; });
-      store_row<T>(s_at, dp, &ds_full);
+      store_row<T>(s_at, dp, &ds_full[u & 1]);
     }
     if (ok && u > 0) ok = warp_wait(&done, 0, abort);
     fence_after();
@@ -856,8 +857,10 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
       StagePhases cleared_phase;
       uint64_t prev_k = 0;      // keys of the step before, whose dq is due
       bool prev_last = false;   // it was its tile's last
+      // A barrier for each of the two buffers: a step's scores and dp are issued before
+      // the step before is waited for, so that its derivative too may be there by then.
       const auto finish = [&]() {
-        ok = bar_wait(&ds_full, (u - 1) & 1, abort);
+        ok = bar_wait(&ds_full[(u - 1) & 1], ((u - 1) >> 1) & 1, abort);
         fence_after();
         if (!ok) return;
         product_parts<STEP>(dq_at, tmem + ((u - 1) & 1) * STEP, prev_k, dd, u > 1);

@@ -48,3 +48,23 @@ def test_padding_in_every_tile(D, dtype, cuda_lib):
             for n, a, b in zip(("dq", "dk", "dv"), torch.autograd.grad(out, (q, k, v), g), grads):
                 close(a, b, dtype, *tolerance(dtype), floor=0.02, what=n)
     assert waits_given_up() == before
+
+
+@gpu
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_query_gradient_of_many_steps(D, dtype, cuda_lib):
+    """Odd and even numbers of steps, of whole tiles and halves; the same each time."""
+    before = waits_given_up()
+    for Sk in (60, 128, 190, 300, 449, 2050):
+        q, k, v, g = (randn(2, 130 if i in (0, 3) else Sk, 2, D, dtype=dtype, seed=i) for i in range(4))
+        _, _, grads = ref.attention(q, k, v, g)
+        q, k, v = (t.requires_grad_() for t in (q, k, v))
+        out = attention(q, k, v)
+        first = None
+        for _ in range(20):
+            dq, = torch.autograd.grad(out, q, g, retain_graph=True)
+            first = dq if first is None else first
+            assert torch.equal(dq, first)
+        close(first, grads[0], dtype, *tolerance(dtype), floor=0.02, what="dq")
+    assert waits_given_up() == before
