@@ -1063,7 +1063,14 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
         }
       }
       store_row<T>(s_at, s, &p_full);
-      if constexpr ((MODE & kCapped) != 0) multiply(s, t2);
+      if constexpr ((MODE & kCapped) != 0) {
+        // Padded keys lie in the tile as they came: a score of NaN has a derivative of NaN.
+        if (!whole) {
+#pragma unroll
+          for (int c = 0; c < N; ++c) t2[c] = s[c] == 0.0f ? 0.0f : t2[c];
+        }
+        multiply(s, t2);
+      }
       ok = warp_wait(&dp_full, turn, abort);
       if (!ok) continue;
       fence_after();

@@ -11,7 +11,7 @@ import torch
 import layer_reference as ref
 from layer_reference import close
 from msda_triton_b200 import _lib, attention
-from test_layer_ops import DEV, DTYPES, HALF, randn
+from test_layer_ops import DEV, DTYPES, HALF, _ids, randn
 
 gpu = pytest.mark.gpu
 
@@ -68,3 +68,30 @@ def test_query_gradient_of_many_steps(D, dtype, cuda_lib):
             assert torch.equal(dq, first)
         close(first, grads[0], dtype, *tolerance(dtype), floor=0.02, what="dq")
     assert waits_given_up() == before
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [40, 64, 128])
+@pytest.mark.parametrize("softcap, documents", [(20.0, False), (20.0, True), (1.0, True), (0.0, False)])
+def test_capped_scores_ignore_what_padding_holds(softcap, documents, D, dtype, cuda_lib):
+    """Not-a-numbers past the lengths, in padded keys and in padded queries' rows."""
+    B, S = 2, 300
+    q, k, v, g = (randn(B, S, 2, D, dtype=dtype, seed=i) for i in range(4))
+    lengths = torch.tensor([S - 1, 211], dtype=torch.int32, device=DEV)
+    how = dict(key_lengths=lengths, softcap=softcap)
+    pad = torch.arange(S, device=DEV)[None] >= lengths[:, None]
+    idle = torch.zeros_like(pad)
+    if documents:
+        ids = _ids(B, S, 3, 4, pad=45)
+        ids[:, 130:140] = -1
+        how.update(query_documents=ids, key_documents=ids)
+        idle = ids < 0
+        pad = pad | idle
+    want, _, grads = ref.attention(q, k, v, g.masked_fill(idle[:, :, None, None], 0), **how)
+    k[pad], v[pad], q[idle], g[idle] = float("nan"), float("inf"), float("nan"), float("inf")
+    q, k, v = (t.requires_grad_() for t in (q, k, v))
+    out = attention(q, k, v, **how)
+    close(out.detach(), want, dtype, *tolerance(dtype), floor=0.02, what="out")
+    for n, a, b in zip(("dq", "dk", "dv"), torch.autograd.grad(out, (q, k, v), g), grads):
+        close(a, b, dtype, *tolerance(dtype), floor=0.02, what=n)
