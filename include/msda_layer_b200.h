@@ -113,7 +113,8 @@ MSDA_API int msda_layer_norm_backward(const void* x, const void* residual, const
  * distance_slopes[h] |place - j|. A query that sees no key gets zeros, an lse
  * of -inf and no gradient. Keys past length_b and of negative documents are
  * never read into a result, whatever they hold; a key that other queries see
- * must be finite.
+ * must be finite. The rows of query and grad_out of a query that sees no key
+ * may hold anything too.
  */
 typedef struct msda_attention_args {
   const void *query, *key, *value;

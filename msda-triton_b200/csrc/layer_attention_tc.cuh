@@ -187,13 +187,12 @@ struct StagePhases {
   }
 };
 
-// Clears the rows of a tile whose token is padding (a warp): 0 x NaN is NaN, and
-// a product over tokens would spread what padding holds.
-template <int DP>
-__device__ __forceinline__ void clear_rows(char* tile, const int* doc, int first, int count) {
+// Clears the rows of a tile that `keep` rejects (a warp): 0 x NaN is NaN, and a
+// product over tokens would spread what padding holds.
+template <int DP, typename Keep>
+__device__ __forceinline__ void clear_rows(char* tile, Keep keep) {
   for (int r = threadIdx.x % 32; r < kTileTokens; r += 32) {
-    const int at = first + r;
-    if (at < count && (!doc || __ldg(doc + at) >= 0)) continue;
+    if (keep(r)) continue;
 #pragma unroll
     for (int c = 0; c < (DP + kChunk - 1) / kChunk; ++c)
 #pragma unroll
@@ -203,6 +202,15 @@ __device__ __forceinline__ void clear_rows(char* tile, const int* doc, int first
   fence_async_smem();
   __syncwarp();
 }
+
+// Key tile j's rows that are no padding.
+struct KeyRows {
+  const int* doc;  // nullable
+  int first, length;
+  __device__ __forceinline__ bool operator()(int r) const {
+    return first + r < length && (!doc || __ldg(doc + first + r) >= 0);
+  }
+};
 
 // The steps that a block of queries goes through: its key tiles, or with STEP 64
 // their halves, less what the limit or the documents leave out. Every role walks
@@ -474,7 +482,7 @@ __global__ void __launch_bounds__(FwdShape<DP>::kThreads, FwdShape<DP>::kCtas)
           __syncwarp();
           if (kv && at.state.padded) {  // padded keys' values are cleared before their product
             ok = warp_wait(&kv_full[slot], (n / NS) & 1, abort);
-            clear_rows<DP>(ring + slot * Shape::kTile, kdoc, at.j * kTileTokens, length);
+            clear_rows<DP>(ring + slot * Shape::kTile, KeyRows{kdoc, at.j * kTileTokens, length});
             if (lane == 0) bar_arrive(&cleared[slot / 2]);
           }
         }
@@ -839,7 +847,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
           __syncwarp();
           if (at.state.padded) {  // padded keys are cleared: dq's product goes over all of the tile's
             ok = warp_wait(&kv_full[slot], (n / 2) & 1, abort);
-            clear_rows<DP>(stage, kdoc, at.j * kTileTokens, length);
+            clear_rows<DP>(stage, KeyRows{kdoc, at.j * kTileTokens, length});
             if (lane == 0) bar_arrive(&cleared[slot]);
           }
           ++n;
@@ -900,6 +908,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
 
 // The steps that a block of keys goes through: every head of its group, the
 // tiles of queries from the first that may see it, or with STEP 64 their halves.
+// state.padded: some queries of the tile may see no key at all.
 template <int STEP, bool DOCS>
 struct QuerySteps {
   int g, i, half, n;  // head of the group, query tile, its half, the tile's number among those visited
@@ -913,12 +922,12 @@ struct QuerySteps {
       done = g >= group || first >= tiles;
       if (done) return;
       if constexpr (!DOCS) {
-        state = TileState{0, 3, false, false};
+        state = TileState{0, 3, false, p.causal && i * kTileTokens < p.Sq - length};
         return;
       } else {
         state = tile_state(p, b, i * kTileTokens, 1, kt, length);
         if (!state.skip) {
-          state.padded = p.qtile[(int64_t)b * tiles + i].padded;  // of the queries, here
+          state.padded = true;
           return;
         }
         ++i;
@@ -1112,10 +1121,22 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kCtas)
             tma_tile<DP>(stage + Shape::kTile, &gmap, &q_full[slot], h, i0, b);
           }
           __syncwarp();
-          if (at.state.padded) {  // padded queries and their gradients, whatever they hold, count for nothing
-            ok = warp_wait(&q_full[slot], (n / 2) & 1, abort);
-            clear_rows<DP>(stage, p.qdoc + (int64_t)b * p.Sq, i0, p.Sq);
-            clear_rows<DP>(stage + Shape::kTile, p.qdoc + (int64_t)b * p.Sq, i0, p.Sq);
+          if (at.state.padded) {
+            // Queries that see no key (padding, an id that no key has, a place before
+            // the first key) and their gradients count for nothing, whatever they hold.
+            const float* lse = p.lse + ((int64_t)b * p.H + h) * p.Sq;
+            uint32_t idle = 0;
+#pragma unroll
+            for (int x = 0; x < kTileTokens / 32; ++x) {
+              const int i = i0 + x * 32 + lane;
+              if (i < p.Sq && __ldg(lse + i) == -INFINITY) idle |= 1u << x;
+            }
+            if (__any_sync(kFullMask, idle != 0)) {
+              const auto keep = [&](int r) { return !(idle >> (r / 32) & 1); };
+              ok = warp_wait(&q_full[slot], (n / 2) & 1, abort);
+              clear_rows<DP>(stage, keep);
+              clear_rows<DP>(stage + Shape::kTile, keep);
+            }
             if (lane == 0) bar_arrive(&cleared[slot]);
           }
           ++n;

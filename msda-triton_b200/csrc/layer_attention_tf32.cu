@@ -738,7 +738,9 @@ __global__ void __launch_bounds__(kBwdThreads, DP <= 128 ? 2 : 1) attn_tf32_dkv_
         lse_s[threadIdx.x] = i < p.Sq ? p.lse[at] * kLog2e : 0.0f;
         delta_s[threadIdx.x] = i < p.Sq ? p.delta[at] : 0.0f;
       }
-      const auto in = [&](int r) { return row_view(p, b, i0 + r, length).limit > 0; };
+      // A query that sees no key counts for nothing, whatever its rows hold.
+      const float* lse = p.lse + ((int64_t)b * p.H + h) * p.Sq + i0;
+      const auto in = [&](int r) { return i0 + r < p.Sq && __ldg(lse + r) != -INFINITY; };
       load_rows<T, DP, kBwdThreads>(qs, kCols, static_cast<const T*>(p.q) + b * p.qs[0] + h * p.qs[2], p.qs[1], i0, p.D, qvec, in);
       load_rows<T, DP, kBwdThreads>(gs, kCols, static_cast<const T*>(p.go) + b * p.gs[0] + h * p.gs[2], p.gs[1], i0, p.D, gvec, in);
       copies_done();

@@ -95,3 +95,32 @@ def test_capped_scores_ignore_what_padding_holds(softcap, documents, D, dtype, c
     close(out.detach(), want, dtype, *tolerance(dtype), floor=0.02, what="out")
     for n, a, b in zip(("dq", "dk", "dv"), torch.autograd.grad(out, (q, k, v), g), grads):
         close(a, b, dtype, *tolerance(dtype), floor=0.02, what=n)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [20, 64, 128])
+@pytest.mark.parametrize("kind", ["before the first key", "document without keys", "both"])
+def test_queries_that_see_no_key_have_no_gradient(kind, D, dtype, cuda_lib):
+    """Whatever their rows of the query and of the output's gradient hold."""
+    B, S = 2, 300
+    q, k, v, g = (randn(B, S, 4 if i in (0, 3) else 2, D, dtype=dtype, seed=i) for i in range(4))
+    how, idle = {}, torch.zeros(B, S, dtype=torch.bool, device=DEV)
+    if kind != "document without keys":
+        lengths = torch.tensor([S, 120], dtype=torch.int32, device=DEV)
+        how.update(causal=True, key_lengths=lengths)
+        idle |= torch.arange(S, device=DEV)[None] < S - lengths[:, None]
+    if kind != "before the first key":
+        ids = _ids(B, S, 3, 4)
+        theirs = ids.clone()
+        theirs[:, 5::7] = 9
+        how.update(query_documents=theirs, key_documents=ids)
+        seen, _ = ref.visible(B, S, S, DEV, **how)
+        idle = ~seen.any(-1)
+    want, _, grads = ref.attention(q, k, v, g.masked_fill(idle[:, :, None, None], 0), **how)
+    q[idle], g[idle] = float("nan"), float("inf")
+    q, k, v = (t.requires_grad_() for t in (q, k, v))
+    out = attention(q, k, v, **how)
+    close(out.detach(), want, dtype, *tolerance(dtype), floor=0.02, what="out")
+    for n, a, b in zip(("dq", "dk", "dv"), torch.autograd.grad(out, (q, k, v), g), grads):
+        close(a, b, dtype, *tolerance(dtype), floor=0.02, what=n)
