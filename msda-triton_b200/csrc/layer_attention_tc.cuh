@@ -82,30 +82,26 @@ __device__ __forceinline__ float row_max(const float (&s)[N]) {
   return fmaxf(max3(m[0], m[1], m[2]), m[3]);
 }
 
-// s <- cap2 tanh(inv_cap s) by an odd polynomial in inv_cap s, whose factors are
-// worked into the coefficients: two columns an instruction.
+// s <- tanh(inv_cap s) by an odd polynomial, two columns an instruction. (The cap
+// comes in as the scores' factor, further on: powers of inv_cap worked into the
+// coefficients would leave fp32's range where the cap is wide.)
 template <int K, int N>
 __device__ __forceinline__ void cap_polynomial(const ScoreForm& f, const float (&poly)[K], float (&s)[N]) {
-  const float i2 = f.inv_cap * f.inv_cap, unit = f.cap2 * f.inv_cap;
-  const uint64_t k = pair_of(unit, unit);
+  const uint64_t inv = pair_of(f.inv_cap, f.inv_cap);
   uint64_t a[K];
-  float factor = i2;
 #pragma unroll
-  for (int i = 0; i < K; ++i) {
-    a[i] = pair_of(poly[i] * factor, poly[i] * factor);
-    factor *= i2;
-  }
+  for (int i = 0; i < K; ++i) a[i] = pair_of(poly[i], poly[i]);
 #pragma unroll
   for (int c = 0; c < N; c += 2) {
-    const uint64_t x = pair_of(s[c], s[c + 1]), y = pair_mul(x, x), u = pair_mul(x, k);
+    const uint64_t x = pair_mul(pair_of(s[c], s[c + 1]), inv), y = pair_mul(x, x);
     uint64_t r = a[K - 1];
 #pragma unroll
     for (int i = K - 2; i >= 0; --i) r = f2_fma(r, y, a[i]);
-    f2_unpack(f2_fma(pair_mul(u, y), r, u), s[c], s[c + 1]);
+    f2_unpack(f2_fma(pair_mul(x, y), r, x), s[c], s[c + 1]);
   }
 }
 
-// Scores of a thread's row to base 2, capped. Scores well below the cap, the
+// Scores of a thread's row as shares of the cap. Scores well below the cap, the
 // common case, go by a polynomial: below a quarter of it (2 terms, 4.9e-7
 // relative at most), below three quarters (tanh_small's 5 terms), else one by one.
 template <int N>
@@ -125,7 +121,7 @@ __device__ __forceinline__ void cap_scores(const ScoreForm& f, float (&s)[N]) {
     cap_polynomial(f, poly, s);
   } else {
 #pragma unroll
-    for (int c = 0; c < N; ++c) s[c] = tanh_of(s[c] * f.inv_cap) * f.cap2;
+    for (int c = 0; c < N; ++c) s[c] = tanh_of(s[c] * f.inv_cap);
   }
 }
 
@@ -350,7 +346,7 @@ __global__ void __launch_bounds__(FwdShape<DP>::kThreads, FwdShape<DP>::kCtas)
       {
         if constexpr ((MODE & kCapped) != 0) {
           cap_scores(f, s);
-          factor = 1.0f;
+          factor = f.cap2;
         }
         if constexpr ((MODE & kSloped) != 0) {
           const float far = (float)(row.place - j0);
@@ -598,14 +594,13 @@ __device__ __forceinline__ void probabilities(const AttnParams& p, const ScoreFo
   {
     if constexpr ((MODE & kCapped) != 0) {
       cap_scores(f, s);
-      const float inv = -1.0f / (f.cap2 * f.cap2);
-      const uint64_t inv2 = pair_of(inv, inv), one = pair_of(1.0f, 1.0f);
+      const uint64_t less = pair_of(-1.0f, -1.0f), one = pair_of(1.0f, 1.0f);
 #pragma unroll
       for (int c = 0; c < N; c += 2) {
         const uint64_t x = pair_of(s[c], s[c + 1]);
-        f2_unpack(f2_fma(pair_mul(x, x), inv2, one), t2[c], t2[c + 1]);
+        f2_unpack(f2_fma(pair_mul(x, x), less, one), t2[c], t2[c + 1]);
       }
-      factor = 1.0f;
+      factor = f.cap2;
     }
     if constexpr ((MODE & kSloped) != 0) {
 #pragma unroll

@@ -124,3 +124,29 @@ def test_queries_that_see_no_key_have_no_gradient(kind, D, dtype, cuda_lib):
     close(out.detach(), want, dtype, *tolerance(dtype), floor=0.02, what="out")
     for n, a, b in zip(("dq", "dk", "dv"), torch.autograd.grad(out, (q, k, v), g), grads):
         close(a, b, dtype, *tolerance(dtype), floor=0.02, what=n)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("scale, softcap", [(1 / 128, 500.0), (0.01, 1000.0), (0.125, 5000.0), (64.0, 30.0), (1e-4, 0.01)])
+@pytest.mark.parametrize("Sq, H", [(1, 2), (300, 2), (300, 16)])
+@pytest.mark.parametrize("share", [0.15, 0.6, 0.74, 1.5])
+def test_scores_at_a_share_of_the_cap(share, Sq, H, scale, softcap, dtype, cuda_lib):
+    """Scores of about `share` of the cap, before it, with wide and narrow caps. A score
+    may be off by 16 u (32 bits) of itself, which its probability is off by too."""
+    S, D, u = 300, 64, ref.U[torch.float32]
+    size = (share * softcap / scale / D) ** 0.5
+    g = torch.Generator(DEV).manual_seed(1)
+    q = torch.full((1, Sq, H, D), size, device=DEV).to(dtype)
+    k = (size * (1 - 0.02 * torch.rand(1, S, H, D, device=DEV, generator=g))).to(dtype)
+    v, grad = randn(1, S, H, D, dtype=dtype, seed=2), randn(1, Sq, H, D, dtype=dtype, seed=3)
+    how = dict(scale=scale, softcap=softcap)
+    want, want_lse, grads = ref.attention(q, k, v, grad, **how)
+    v.requires_grad_()
+    out, lse = attention(q, k, v, return_lse=True, **how)
+    top = float(want_lse.abs().max())
+    assert float((lse.double() - want_lse).abs().max()) <= 16 * u * softcap + 4 * u * top
+    more = 16 * u * softcap / ref.U[dtype]
+    norm, element = tolerance(dtype)
+    close(out.detach(), want, dtype, norm + more, element + 4 * more, floor=0.02, what="out")
+    close(torch.autograd.grad(out, v, grad)[0], grads[2], dtype, norm + more, element + 4 * more, floor=0.02, what="dv")
