@@ -5,6 +5,10 @@
 //   dh = s (gw - mean(gw) - z mean(gw z)) (+ dsum),  z = (h - mu) s,  gw = g w
 //   dw = sum_rows g z,  db = sum_rows g
 //
+// The mean that is kept for the backward is rounded, which shows where a row lies
+// many deviations from zero: both directions take out what is left of the centred
+// row's own mean.
+//
 // Bound by HBM: a row is read once, kept in registers by the threads that
 // share it (a warp up to 512 channels, 128 to 512 threads up to 8192), and
 // written once; the variance is taken about the mean, from the registers. Rows
@@ -41,6 +45,7 @@ struct NormParams {
   void *y, *sum_out, *grad_x;
   float *mean, *rstd;
   float *partial;  // [2][gridDim.x][width]: weight's and bias's column sums
+  float *rest;     // (rows,): what the wide rows' kept means leave, in deviations; with columns only
   int64_t rows, x_stride, residual_stride, grad_stride;
   int32_t width;
   int32_t param_f32;  // weight and bias are fp32, not T
@@ -63,27 +68,66 @@ __device__ __forceinline__ float param_at(const void* p, int f32, int c) {
   return to_f32(*reinterpret_cast<const T*>(&bits));
 }
 
-// Sums of two values over the TPR threads that share a row, the same in each of
-// them. `red`: a pair for each warp of the CTA in each of two buffers, which
+// Sums of N values over the TPR threads that share a row, the same in each of
+// them. `red`: N values for each warp of the CTA in each of two buffers, which
 // consecutive calls take in turn, so that one barrier a call is enough.
-template <int TPR>
-__device__ __forceinline__ float2 row_sums(float2 v, float2 (*red)[32], int buffer) {
+template <int TPR, int N, int M>
+__device__ __forceinline__ void row_sums(float (&v)[N], float (*red)[M][32], int buffer) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    v.x += __shfl_xor_sync(kFullMask, v.x, o);
-    v.y += __shfl_xor_sync(kFullMask, v.y, o);
-  }
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int n = 0; n < N; ++n) v[n] += __shfl_xor_sync(kFullMask, v[n], o);
   if constexpr (TPR > 32) {
-    if ((threadIdx.x & 31) == 0) red[buffer][threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = red[buffer][threadIdx.x & (TPR / 32 - 1)];
+    if ((threadIdx.x & 31) == 0) {
 #pragma unroll
-    for (int o = TPR / 64; o > 0; o >>= 1) {
-      v.x += __shfl_xor_sync(kFullMask, v.x, o);
-      v.y += __shfl_xor_sync(kFullMask, v.y, o);
+      for (int n = 0; n < N; ++n) red[buffer][n][threadIdx.x >> 5] = v[n];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < N; ++n) v[n] = red[buffer][n][threadIdx.x & (TPR / 32 - 1)];
+#pragma unroll
+    for (int o = TPR / 64; o > 0; o >>= 1)
+#pragma unroll
+      for (int n = 0; n < N; ++n) v[n] += __shfl_xor_sync(kFullMask, v[n], o);
+  }
+}
+
+// The same for three values, as the backward wants them: the first two exchanges
+// leave a quarter of a warp with each value, 6 shuffles for 15.
+template <int TPR>
+__device__ __forceinline__ void row_sums_of_three(float (&v)[3], float (*red)[3][32], int buffer) {
+  const int lane = threadIdx.x & 31;
+  const bool upper = lane & 16, odd = lane & 8;
+  float a = upper ? v[2] : v[0], b = upper ? 0.0f : v[1];
+  a += __shfl_xor_sync(kFullMask, upper ? v[0] : v[2], 16);
+  b += __shfl_xor_sync(kFullMask, upper ? v[1] : 0.0f, 16);
+  float c = odd ? b : a;
+  c += __shfl_xor_sync(kFullMask, odd ? a : b, 8);
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) c += __shfl_xor_sync(kFullMask, c, o);
+  if constexpr (TPR == 32) {
+#pragma unroll
+    for (int n = 0; n < 3; ++n) v[n] = __shfl_sync(kFullMask, c, n * 8);
+  } else {
+    constexpr int W = TPR / 32;
+    if ((lane & 7) == 0 && lane < 24) red[buffer][lane >> 3][threadIdx.x >> 5] = c;
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < 3; ++n) {
+      if constexpr (W <= 8) {
+        v[n] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < W; w += 4) {
+          const float4 q = *reinterpret_cast<const float4*>(&red[buffer][n][w]);
+          v[n] += (q.x + q.y) + (q.z + q.w);
+        }
+      } else {
+        v[n] = red[buffer][n][threadIdx.x & (W - 1)];
+#pragma unroll
+        for (int o = W / 2; o > 0; o >>= 1) v[n] += __shfl_xor_sync(kFullMask, v[n], o);
+      }
     }
   }
-  return v;
 }
 
 // TPR threads share a row, NV vectors of VEC channels each.
@@ -167,7 +211,7 @@ template <typename T, int VEC, int NV, int TPR>
 __global__ void __launch_bounds__(norm_threads<TPR>()) norm_fwd_kernel(const NormParams p) {
   using R = RowTile<T, VEC, NV, TPR>;
   constexpr int E = R::E;
-  __shared__ float2 red[2][32];
+  __shared__ float red[2][2][32];
   const int width = p.width;
   const float inv = 1.0f / (float)width;
   const int64_t step = (int64_t)gridDim.x * norm_rows<TPR>();
@@ -185,22 +229,20 @@ __global__ void __launch_bounds__(norm_threads<TPR>()) norm_fwd_kernel(const Nor
     R::fetch(p.x, (row + step) * p.x_stride, width, row + step < p.rows, next);
     if (p.residual) R::fetch(p.residual, (row + step) * p.residual_stride, width, row + step < p.rows, more);
     if (p.sum_out) R::store(p.sum_out, row * width, width, h);
-    float2 s = make_float2(0.0f, 0.0f);
+    float sum[1] = {0.0f}, s[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int e = 0; e < E; ++e) s.x += h[e];
-    const float mean = row_sums<TPR>(s, red, 0).x * inv;
-    // The mean's rounding is taken out again: it would show where the row
-    // lies many deviations from zero.
-    s = make_float2(0.0f, 0.0f);
+    for (int e = 0; e < E; ++e) sum[0] += h[e];
+    row_sums<TPR>(sum, red, 0);
+    const float mean = sum[0] * inv;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       h[e] = R::inside(e, width) ? h[e] - mean : 0.0f;
-      s.x += h[e];
-      s.y = fmaf(h[e], h[e], s.y);
+      s[0] += h[e];
+      s[1] = fmaf(h[e], h[e], s[1]);
     }
-    s = row_sums<TPR>(s, red, 1);
-    const float rest = s.x * inv;
-    const float rstd = rsqrtf(fmaf(-rest, rest, s.y * inv) + p.eps);
+    row_sums<TPR>(s, red, 1);
+    const float rest = s[0] * inv;
+    const float rstd = rsqrtf(fmaf(-rest, rest, s[1] * inv) + p.eps);
 #pragma unroll
     for (int e = 0; e < E; ++e) h[e] = fmaf((h[e] - rest) * rstd, w[e], b[e]);
     R::store(p.y, row * width, width, h);
@@ -211,12 +253,16 @@ __global__ void __launch_bounds__(norm_threads<TPR>()) norm_fwd_kernel(const Nor
   }
 }
 
+// CTAs of 256 threads of the backward that an SM has room for, which the compiler is
+// held to (10000 x 1537 bf16: 66 us without, 42 us) and the grid goes by.
+__host__ __device__ constexpr int norm_bwd_ctas(int vec) { return vec > 1 ? 3 : 2; }
+
 template <typename T, int VEC, int NV, int TPR>
-__global__ void __launch_bounds__(norm_threads<TPR>()) norm_bwd_kernel(const NormParams p) {
+__global__ void __launch_bounds__(norm_threads<TPR>(), TPR == 256 ? norm_bwd_ctas(VEC) : 1) norm_bwd_kernel(const NormParams p) {
   using R = RowTile<T, VEC, NV, TPR>;
   constexpr int E = R::E, kRows = norm_rows<TPR>();
   constexpr bool kAhead = norm_ahead<TPR, E, true>();
-  __shared__ float2 red[2][32];
+  __shared__ __align__(16) float red[2][3][32];
   const int width = p.width;
   const float inv = 1.0f / (float)width;
   const int64_t step = (int64_t)gridDim.x * kRows;
@@ -243,20 +289,25 @@ __global__ void __launch_bounds__(norm_threads<TPR>()) norm_bwd_kernel(const Nor
     if (p.residual) R::add(more, h);
     const float mu = mean, rs = rstd;
     if (kAhead) fetch(row + step, row + step < p.rows);
-    float2 s = make_float2(0.0f, 0.0f);
+    float s[3] = {0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       h[e] = R::inside(e, width) ? (h[e] - mu) * rs : 0.0f;
+      const float gw = g[e] * w[e];
       db[e] += g[e];
       dw[e] = fmaf(g[e], h[e], dw[e]);
-      g[e] *= w[e];
-      s.x += g[e];
-      s.y = fmaf(g[e], h[e], s.y);
+      s[0] += gw;
+      s[1] = fmaf(gw, h[e], s[1]);
+      s[2] += h[e];
     }
-    s = row_sums<TPR>(s, red, turn);
-    s.x *= inv, s.y *= inv;
+    row_sums_of_three<TPR>(s, red, turn);
+    // z = h - rest, in what has been summed with h too.
+    const float rest = s[2] * inv, c2 = fmaf(-rest, s[0], s[1]) * inv, c1 = fmaf(-rest, c2, s[0] * inv);
 #pragma unroll
-    for (int e = 0; e < E; ++e) g[e] = (g[e] - s.x - h[e] * s.y) * rs;
+    for (int e = 0; e < E; ++e) {
+      dw[e] = fmaf(-rest, g[e], dw[e]);
+      g[e] = (g[e] * w[e] - c1 - h[e] * c2) * rs;
+    }
     if (p.grad_sum) {
       typename R::Raw sum[NV];
       R::fetch(p.grad_sum, row * width, width, true, sum);
@@ -309,20 +360,20 @@ __device__ __forceinline__ float wide_at(const NormParams& p, int64_t row, int c
 
 template <typename T>
 __global__ void __launch_bounds__(kWideThreads) norm_wide_fwd_kernel(const NormParams p) {
-  __shared__ float2 red[2][32];
+  __shared__ float red[2][2][32];
   const float inv = 1.0f / (float)p.width;
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-    float2 s = make_float2(0.0f, 0.0f);
-    for (int c = threadIdx.x; c < p.width; c += kWideThreads) s.x += wide_at<T>(p, row, c);
-    const float mean = row_sums<kWideThreads>(s, red, 0).x * inv;
-    s = make_float2(0.0f, 0.0f);
+    float sum[1] = {0.0f}, s[2] = {0.0f, 0.0f};
+    for (int c = threadIdx.x; c < p.width; c += kWideThreads) sum[0] += wide_at<T>(p, row, c);
+    row_sums<kWideThreads>(sum, red, 0);
+    const float mean = sum[0] * inv;
     for (int c = threadIdx.x; c < p.width; c += kWideThreads) {
       const float d = wide_at<T>(p, row, c) - mean;
-      s.x += d;
-      s.y = fmaf(d, d, s.y);
+      s[0] += d;
+      s[1] = fmaf(d, d, s[1]);
     }
-    s = row_sums<kWideThreads>(s, red, 1);
-    const float rest = s.x * inv, rstd = rsqrtf(fmaf(-rest, rest, s.y * inv) + p.eps);
+    row_sums<kWideThreads>(s, red, 1);
+    const float rest = s[0] * inv, rstd = rsqrtf(fmaf(-rest, rest, s[1] * inv) + p.eps);
     for (int c = threadIdx.x; c < p.width; c += kWideThreads) {
       const float h = wide_at<T>(p, row, c);
       const float w = p.weight ? param_at<T>(p.weight, p.param_f32, c) : 1.0f;
@@ -339,21 +390,24 @@ __global__ void __launch_bounds__(kWideThreads) norm_wide_fwd_kernel(const NormP
 
 template <typename T>
 __global__ void __launch_bounds__(kWideThreads) norm_wide_bwd_kernel(const NormParams p) {
-  __shared__ float2 red[2][32];
+  __shared__ __align__(16) float red[2][3][32];
   const float inv = 1.0f / (float)p.width;
   int turn = 0;
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
     const float mean = __ldg(p.mean + row), rstd = __ldg(p.rstd + row);
     const T* g = static_cast<const T*>(p.grad_y) + row * p.grad_stride;
-    float2 s = make_float2(0.0f, 0.0f);
+    float s[3] = {0.0f, 0.0f, 0.0f};
     for (int c = threadIdx.x; c < p.width; c += kWideThreads) {
       const float gw = to_f32(__ldg(g + c)) * (p.weight ? param_at<T>(p.weight, p.param_f32, c) : 1.0f);
-      s.x += gw;
-      s.y = fmaf(gw, (wide_at<T>(p, row, c) - mean) * rstd, s.y);
+      const float z = (wide_at<T>(p, row, c) - mean) * rstd;
+      s[0] += gw;
+      s[1] = fmaf(gw, z, s[1]);
+      s[2] += z;
     }
-    s = row_sums<kWideThreads>(s, red, turn);
+    row_sums_of_three<kWideThreads>(s, red, turn);
     turn ^= 1;
-    const float c1 = s.x * inv, c2 = s.y * inv;
+    const float rest = s[2] * inv, c2 = fmaf(-rest, s[0], s[1]) * inv, c1 = fmaf(-rest, c2, s[0] * inv);
+    if (p.want_columns && threadIdx.x == 0) p.rest[row] = rest;
     for (int c = threadIdx.x; c < p.width; c += kWideThreads) {
       const float gw = to_f32(__ldg(g + c)) * (p.weight ? param_at<T>(p.weight, p.param_f32, c) : 1.0f);
       float d = (gw - c1 - (wide_at<T>(p, row, c) - mean) * rstd * c2) * rstd;
@@ -372,7 +426,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_wide_columns_kernel(const N
   for (int64_t row = blockIdx.y; row < p.rows; row += gridDim.y) {
     const float g = to_f32(__ldg(static_cast<const T*>(p.grad_y) + row * p.grad_stride + c));
     db += g;
-    dw = fmaf(g, (wide_at<T>(p, row, c) - __ldg(p.mean + row)) * __ldg(p.rstd + row), dw);
+    dw = fmaf(g, (wide_at<T>(p, row, c) - __ldg(p.mean + row)) * __ldg(p.rstd + row) - __ldg(p.rest + row), dw);
   }
   p.partial[(int64_t)blockIdx.y * p.width + c] = dw;
   p.partial[((int64_t)gridDim.y + blockIdx.y) * p.width + c] = db;
@@ -442,7 +496,7 @@ int64_t norm_backward_most(int64_t width) {
 int norm_grid(int64_t rows, const NormShape& s, bool backward, int64_t width) {
   const bool warps = s.tpr == 32;
   const int64_t ctas = warps ? (rows + kNormThreads / 32 - 1) / (kNormThreads / 32) : rows;
-  const int64_t most = backward ? norm_backward_most(width)
+  const int64_t most = backward ? (s.tpr == 256 ? kNormSms * norm_bwd_ctas(s.vec) : norm_backward_most(width))
                                 : kNormSms * (width > kRegisterWidth ? 2 : 2048 / (warps ? kNormThreads : s.tpr));
   return (int)(ctas < most ? ctas : most);
 }
@@ -551,7 +605,8 @@ int msda_layer_norm_forward(const void* x, const void* residual, const void* wei
 
 size_t msda_layer_norm_backward_workspace_size(int64_t rows, int64_t width) {
   if (rows < 1 || width < 1 || width > MSDA_LAYER_NORM_MAX_WIDTH) return 0;
-  return sizeof(float) * 2 * (size_t)std::min(rows, msda::norm_backward_most(width)) * (size_t)width;
+  const size_t columns = 2 * (size_t)std::min(rows, msda::norm_backward_most(width)) * (size_t)width;
+  return sizeof(float) * (columns + (width > msda::kRegisterWidth ? (size_t)rows : 0));
 }
 
 int msda_layer_norm_backward(const void* x, const void* residual, const void* weight, const float* mean,
@@ -594,6 +649,7 @@ int msda_layer_norm_backward(const void* x, const void* residual, const void* we
   p.x = x, p.residual = residual, p.weight = weight, p.grad_y = grad_y, p.grad_sum = grad_sum, p.grad_x = grad_x;
   p.mean = const_cast<float*>(mean), p.rstd = const_cast<float*>(rstd);
   p.partial = static_cast<float*>(workspace);
+  if (columns) p.rest = p.partial + 2 * std::min(rows, norm_backward_most(width)) * width;
   p.rows = rows, p.width = (int32_t)width, p.x_stride = x_stride, p.residual_stride = residual_stride;
   p.grad_stride = grad_stride;
   p.param_f32 = param_dtype == MSDA_DTYPE_F32, p.want_columns = columns;

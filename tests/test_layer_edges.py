@@ -10,7 +10,7 @@ import torch
 
 import layer_reference as ref
 from layer_reference import close
-from msda_triton_b200 import _lib, attention
+from msda_triton_b200 import _lib, attention, layer_norm
 from test_layer_ops import DEV, DTYPES, HALF, _ids, randn
 
 gpu = pytest.mark.gpu
@@ -150,3 +150,27 @@ def test_scores_at_a_share_of_the_cap(share, Sq, H, scale, softcap, dtype, cuda_
     norm, element = tolerance(dtype)
     close(out.detach(), want, dtype, norm + more, element + 4 * more, floor=0.02, what="out")
     close(torch.autograd.grad(out, v, grad)[0], grads[2], dtype, norm + more, element + 4 * more, floor=0.02, what="dv")
+
+
+def _offset_case(C, residual):
+    grid = lambda t: (t * 4096).round() / 4096  # noqa: E731  (sums without a rounding)
+    x = grid(randn(37, C) + 1000.0)
+    r = grid(randn(37, C, seed=1) - 300.0) if residual else None
+    w = 1 + 0.3 * randn(C, seed=2)
+    return x, r, w, randn(37, C, seed=4)
+
+
+@gpu
+@pytest.mark.parametrize("C", [7, 256, 511, 1000, 2047, 5001, 8192, 8200])
+@pytest.mark.parametrize("residual", [False, True])
+def test_layer_norm_gradient_far_from_zero(C, residual, cuda_lib):
+    """Rows a thousand deviations from zero: the gradients take the rows that made y."""
+    x, r, w, g = _offset_case(C, residual)
+    leaves = [t.requires_grad_() for t in (x, r, w) if t is not None]
+    y = layer_norm(x, w, None, residual=r)
+    want, z, rstd = ref.layer_norm(x.detach(), w.detach(), None, None if r is None else r.detach(), 1e-5)
+    dx, dw, _ = ref.layer_norm_grad(z, rstd, w.detach(), g)
+    got = torch.autograd.grad(y, leaves, g)
+    close(y.detach(), want, torch.float32, 64, 1024, what="y")
+    close(got[0], dx, torch.float32, 64, 1024, what="dx")
+    close(got[-1], dw, torch.float32, 64, 1024, what="dw")
