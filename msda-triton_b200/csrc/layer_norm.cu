@@ -130,6 +130,13 @@ __device__ __forceinline__ void row_sums_of_three(float (&v)[3], float (*red)[3]
   }
 }
 
+// A row's variance from its mean square and what its mean left. The rounding of the
+// two can leave less than nothing of a constant row far from zero.
+__device__ __forceinline__ float variance(float square, float rest) {
+  const float v = fmaf(-rest, rest, square);
+  return v < 0.0f ? 0.0f : v;
+}
+
 // TPR threads share a row, NV vectors of VEC channels each.
 template <typename T, int VEC, int NV, int TPR>
 struct RowTile {
@@ -242,7 +249,7 @@ __global__ void __launch_bounds__(norm_threads<TPR>()) norm_fwd_kernel(const Nor
     }
     row_sums<TPR>(s, red, 1);
     const float rest = s[0] * inv;
-    const float rstd = rsqrtf(fmaf(-rest, rest, s[1] * inv) + p.eps);
+    const float rstd = rsqrtf(variance(s[1] * inv, rest) + p.eps);
 #pragma unroll
     for (int e = 0; e < E; ++e) h[e] = fmaf((h[e] - rest) * rstd, w[e], b[e]);
     R::store(p.y, row * width, width, h);
@@ -373,7 +380,7 @@ __global__ void __launch_bounds__(kWideThreads) norm_wide_fwd_kernel(const NormP
       s[1] = fmaf(d, d, s[1]);
     }
     row_sums<kWideThreads>(s, red, 1);
-    const float rest = s[0] * inv, rstd = rsqrtf(fmaf(-rest, rest, s[1] * inv) + p.eps);
+    const float rest = s[0] * inv, rstd = rsqrtf(variance(s[1] * inv, rest) + p.eps);
     for (int c = threadIdx.x; c < p.width; c += kWideThreads) {
       const float h = wide_at<T>(p, row, c);
       const float w = p.weight ? param_at<T>(p.weight, p.param_f32, c) : 1.0f;

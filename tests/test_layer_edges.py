@@ -174,3 +174,17 @@ def test_layer_norm_gradient_far_from_zero(C, residual, cuda_lib):
     close(y.detach(), want, torch.float32, 64, 1024, what="y")
     close(got[0], dx, torch.float32, 64, 1024, what="dx")
     close(got[-1], dw, torch.float32, 64, 1024, what="dw")
+
+
+@gpu
+@pytest.mark.parametrize("C", [3, 7, 100, 1000, 5001, 8192, 8200])
+def test_layer_norm_of_constant_rows(C, cuda_lib):
+    """Far from zero their variance is what rounding left: sums of up to 26 terms in a row
+    leave 28 u of the row and, of that, 28 u again, by at most 1 / sqrt(eps)."""
+    at = torch.tensor([0.1, 1e4, 1e8, -3.3e9, 514228608.0, 2063394304.0, 33778102272.0, 15217946624.0], device=DEV)
+    x = at[:, None].expand(8, C).contiguous().requires_grad_()
+    y = layer_norm(x)
+    off = (28 * ref.U[torch.float32]) ** 2 * at.abs() / 1e-5 ** 0.5
+    assert (y.abs() <= off[:, None]).all()
+    gx, = torch.autograd.grad(y, x, randn(8, C))
+    assert torch.isfinite(gx).all()
