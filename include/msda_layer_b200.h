@@ -115,6 +115,10 @@ MSDA_API int msda_layer_norm_backward(const void* x, const void* residual, const
  * never read into a result, whatever they hold; a key that other queries see
  * must be finite. The rows of query and grad_out of a query that sees no key
  * may hold anything too.
+ *
+ * At most 65535 items, 4096 heads, 2^22 queries and 2^30 keys, 2^22 in the
+ * backward; where the type is fp32 or a row is not of up to 128 channels in whole
+ * 16-byte vectors, 65535 x 64 for 2^22.
  */
 typedef struct msda_attention_args {
   const void *query, *key, *value;

@@ -79,10 +79,28 @@ using namespace msda;
 using namespace msda::abi;
 
 constexpr int kMaxSplits = 64;
+constexpr int kMaxRows = 1 << 22;  // queries, and keys that have a gradient
 
 enum class Path { kAny, kToken, kTensor };
 
-int check(const char* fn, const msda_attention_args* a, bool backward) {
+// 16-byte loads of 8 channels: the tensor-core kernels' layout.
+bool rows_of_16(const void* p, const int64_t (&s)[3], const int64_t (&n)[3]) {
+  for (int i = 0; i < 3; ++i)
+    if (n[i] > 1 && (s[i] <= 0 || s[i] % 8)) return false;
+  return aligned(p, 16);
+}
+
+bool tensor_layout(const msda_attention_args* a, bool backward) {
+  if (a->dtype == MSDA_DTYPE_F32 || a->head_dim % 8 || a->head_dim > 128) return false;
+  const int64_t nq[3] = {a->batch, a->num_queries, a->num_heads}, nk[3] = {a->batch, a->num_keys, a->num_key_heads};
+  return rows_of_16(a->query, a->query_strides, nq) && rows_of_16(a->key, a->key_strides, nk) &&
+         rows_of_16(a->value, a->value_strides, nk) && aligned(a->out, 16) && aligned(a->out_residue, 16) &&
+         (!backward || (rows_of_16(a->grad_out, a->grad_out_strides, nq) && aligned(a->grad_query, 16) &&
+                        aligned(a->grad_key, 16) && aligned(a->grad_value, 16)));
+}
+
+// Refusals by type and sizes, which the workspace's size goes by too.
+int check_sizes(const char* fn, const msda_attention_args* a, bool backward) {
   if (!a) return fail(MSDA_ERR_INVALID_ARGUMENT, "%s: null arguments", fn);
   if (elem_size(a->dtype) == 0) return fail(MSDA_ERR_UNSUPPORTED, "%s: unsupported dtype code %d (0=f32, 1=f16, 2=bf16)", fn, a->dtype);
   if (a->batch < 0 || a->num_queries < 0 || a->num_keys < 0) return fail(MSDA_ERR_INVALID_ARGUMENT, "%s: negative size", fn);
@@ -90,8 +108,17 @@ int check(const char* fn, const msda_attention_args* a, bool backward) {
     return fail(MSDA_ERR_INVALID_ARGUMENT, "%s: num_heads=%d must be a multiple of num_key_heads=%d", fn, a->num_heads, a->num_key_heads);
   if (a->head_dim < 1 || a->head_dim > MSDA_ATTENTION_MAX_HEAD_DIM)
     return fail(MSDA_ERR_UNSUPPORTED, "%s: head_dim=%d outside [1, %d]", fn, a->head_dim, MSDA_ATTENTION_MAX_HEAD_DIM);
-  if (a->batch > 65535 || a->num_heads > 4096 || a->num_queries > (1 << 22) || a->num_keys > (backward ? 1 << 22 : 1 << 30))
+  if (a->batch > 65535 || a->num_heads > 4096 || a->num_queries > kMaxRows || a->num_keys > (backward ? kMaxRows : 1 << 30))
     return fail(MSDA_ERR_UNSUPPORTED, "%s: sizes exceed batch 65535, 4096 heads, 2^22 queries or 2^30 keys (2^22 in the backward)", fn);
+  // The other kernels' grids have a tile of 64 rows for each of y's 65535 steps.
+  if (!tensor_layout(a, backward) && (a->num_queries > 65535 * 64 || (backward && a->num_keys > 65535 * 64)))
+    return fail(MSDA_ERR_UNSUPPORTED, "%s: more than %d rows of fp32, or of a layout without 16-byte rows of up to 128 channels", fn,
+                65535 * 64);
+  return MSDA_OK;
+}
+
+int check(const char* fn, const msda_attention_args* a, bool backward) {
+  if (int rc = check_sizes(fn, a, backward)) return rc;
   if (!std::isfinite(a->scale) || !std::isfinite(a->softcap) || a->softcap < 0)
     return fail(MSDA_ERR_INVALID_ARGUMENT, "%s: scale must be finite, softcap finite and >= 0", fn);
   if (!a->query_documents != !a->key_documents)
@@ -113,22 +140,6 @@ int check(const char* fn, const msda_attention_args* a, bool backward) {
     if (a->num_keys > 0 && (!a->grad_key || !a->grad_value)) return fail(MSDA_ERR_INVALID_ARGUMENT, "%s: null pointer argument", fn);
   }
   return MSDA_OK;
-}
-
-// 16-byte loads of 8 channels: the tensor-core kernels' layout.
-bool rows_of_16(const void* p, const int64_t (&s)[3], const int64_t (&n)[3]) {
-  for (int i = 0; i < 3; ++i)
-    if (n[i] > 1 && (s[i] <= 0 || s[i] % 8)) return false;
-  return aligned(p, 16);
-}
-
-bool tensor_layout(const msda_attention_args* a, bool backward) {
-  if (a->dtype == MSDA_DTYPE_F32 || a->head_dim % 8 || a->head_dim > 128) return false;
-  const int64_t nq[3] = {a->batch, a->num_queries, a->num_heads}, nk[3] = {a->batch, a->num_keys, a->num_key_heads};
-  return rows_of_16(a->query, a->query_strides, nq) && rows_of_16(a->key, a->key_strides, nk) &&
-         rows_of_16(a->value, a->value_strides, nk) && aligned(a->out, 16) && aligned(a->out_residue, 16) &&
-         (!backward || (rows_of_16(a->grad_out, a->grad_out_strides, nq) && aligned(a->grad_query, 16) &&
-                        aligned(a->grad_key, 16) && aligned(a->grad_value, 16)));
 }
 
 struct Plan {
@@ -277,9 +288,7 @@ cudaError_t documents(const AttnParams& p, const Plan& plan, cudaStream_t st) {
 extern "C" {
 
 size_t msda_attention_workspace_size(const msda_attention_args* a, int32_t backward) {
-  if (!a || elem_size(a->dtype) == 0 || a->batch < 1 || a->num_queries < 1 || a->num_keys < 0 || a->num_heads < 1 ||
-      a->num_key_heads < 1 || a->num_heads % a->num_key_heads || a->head_dim < 1 || a->head_dim > MSDA_ATTENTION_MAX_HEAD_DIM)
-    return 0;
+  if (check_sizes("msda_attention_workspace_size", a, backward != 0) || a->batch == 0 || a->num_queries == 0) return 0;
   return plan_of(a, backward != 0).bytes;
 }
 

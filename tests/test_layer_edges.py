@@ -9,6 +9,7 @@ import pytest
 import torch
 
 import layer_reference as ref
+from hostonly import host_only
 from layer_reference import close
 from msda_triton_b200 import _lib, attention, layer_norm
 from test_layer_ops import DEV, DTYPES, HALF, _ids, randn
@@ -188,3 +189,41 @@ def test_layer_norm_of_constant_rows(C, cuda_lib):
     assert (y.abs() <= off[:, None]).all()
     gx, = torch.autograd.grad(y, x, randn(8, C))
     assert torch.isfinite(gx).all()
+
+
+def _attention_args(**over):
+    a = _lib.AttentionArgs()
+    names = ("query", "key", "value", "out", "lse", "grad_out", "grad_query", "grad_key", "grad_value")
+    fields = dict.fromkeys(names, 16) | dict(batch=1, num_queries=100, num_keys=100, num_heads=2, num_key_heads=1, head_dim=8,
+                                             scale=1.0, shared_document=-1)
+    for n, v in (fields | over).items():
+        setattr(a, n, v)
+    for n in ("query_strides", "key_strides", "value_strides", "grad_out_strides"):
+        getattr(a, n)[:] = (8, 8, 8)
+    return ctypes.byref(a)
+
+
+REFUSED = [dict(batch=65536), dict(num_heads=4097), dict(num_queries=2**22 + 1), dict(num_queries=65535 * 64 + 1),
+           dict(num_queries=65535 * 64 + 1, head_dim=136, dtype=1), dict(num_keys=2**30 + 1), dict(head_dim=257), dict(dtype=3),
+           dict(num_heads=3, num_key_heads=2), dict(num_queries=-1)]
+REFUSED_BACKWARD = [dict(num_keys=65535 * 64 + 1), dict(num_keys=2**22 + 1, dtype=2)]
+
+
+@host_only
+def test_attention_refuses_sizes_that_no_grid_holds():
+    """The launches and the workspace's size by the same limits; one less or another layout passes them
+    (the launches then ask for a workspace)."""
+    lib = _lib.load()
+    for over in REFUSED:
+        assert lib.msda_attention_forward(_attention_args(**over), None) in (_lib.MSDA_ERR_UNSUPPORTED, _lib.MSDA_ERR_INVALID_ARGUMENT)
+        assert b"workspace" not in lib.msda_last_error()
+    for over in REFUSED + REFUSED_BACKWARD:
+        assert lib.msda_attention_workspace_size(_attention_args(**over), 1) == 0
+        assert lib.msda_attention_backward(_attention_args(**over), None) in (_lib.MSDA_ERR_UNSUPPORTED, _lib.MSDA_ERR_INVALID_ARGUMENT)
+        assert b"workspace" not in lib.msda_last_error()
+    for over in (dict(batch=65535), dict(num_queries=65535 * 64), dict(num_queries=2**22, dtype=1), dict(num_keys=65535 * 64),
+                 dict(num_keys=2**22, dtype=2)):
+        assert lib.msda_attention_workspace_size(_attention_args(**over), 1) > 0
+        assert lib.msda_attention_backward(_attention_args(**over), None) == _lib.MSDA_ERR_INVALID_ARGUMENT
+        assert b"workspace" in lib.msda_last_error()
+    assert lib.msda_attention_workspace_size(None, 0) == 0
