@@ -16,7 +16,7 @@ import struct
 import torch
 
 from . import _lib
-from .ops import _DTYPE_CODE, _FLOAT_DTYPES, _apply, _device_guard, _once, _raw_stream
+from .ops import _DTYPE_CODE, _FLOAT_DTYPES, _apply, _device_guard, _once, _raw_stream, _wants_node
 
 # msda_attention_args of include/msda_layer_b200.h, packed in one call.
 _ARGS = struct.Struct("@10P3q4i12q2f5P2iPN")
@@ -194,7 +194,7 @@ def attention(
     if key.device != device or value.device != device:
         raise ValueError("attention: all tensors must be on the same CUDA device")
     options = (scale, softcap, 1 if causal else 0, -1 if shared_document is None else int(shared_document))
-    if (query.requires_grad or key.requires_grad or value.requires_grad) and torch.is_grad_enabled():
+    if _wants_node(query, key, value):
         out, lse = _apply(_AttentionFunction, query, key, value, options, tensors)
     else:
         out, lse, *_ = _forward(query, key, value, options, tensors, return_lse, False)

@@ -12,7 +12,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .ops import _DTYPE_CODE, _FLOAT_DTYPES, _apply, _device_guard, _once, _raw_stream
+from .ops import _DTYPE_CODE, _FLOAT_DTYPES, _apply, _device_guard, _once, _raw_stream, _wants_node
 
 
 def _as_rows(x: torch.Tensor) -> torch.Tensor:
@@ -142,17 +142,14 @@ def layer_norm(
         raise ValueError(f"layer_norm: eps must be >= 0, got {eps}")
     if device.type != "cuda":
         raise ValueError("layer_norm requires CUDA tensors on a B200 (sm_100a) GPU")
-    grad = x.requires_grad
     for t in (weight, bias, residual):
-        if t is not None:
-            if t.device != device:
-                raise ValueError("layer_norm: all tensors must be on the same CUDA device")
-            grad = grad or t.requires_grad
+        if t is not None and t.device != device:
+            raise ValueError("layer_norm: all tensors must be on the same CUDA device")
     if weight is not None:
         weight = weight.contiguous()
     if bias is not None:
         bias = bias.contiguous()
-    if grad and torch.is_grad_enabled():
+    if _wants_node(x, weight, bias, residual):
         return _apply(_LayerNormFunction, x, residual, weight, bias, float(eps), bool(return_sum))
     y, total, *_ = _forward(x, residual, weight, bias, float(eps), return_sum, False)
     return (y, total) if return_sum else y

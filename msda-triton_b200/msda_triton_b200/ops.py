@@ -14,6 +14,7 @@ import contextlib
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -92,6 +93,15 @@ def _once(backward):
         return checked(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
 
     return run
+
+
+def _wants_node(*tensors: torch.Tensor | None) -> bool:
+    """Whether a layer operator's call goes through its autograd node: where an
+    input requires a gradient, and where forward-mode derivatives are under way,
+    which the node refuses (a dual tensor does not require a gradient)."""
+    if forward_ad._current_level >= 0:
+        return True
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def _apply(function, *args):

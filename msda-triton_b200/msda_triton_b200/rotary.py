@@ -14,7 +14,7 @@ from collections.abc import Sequence
 import torch
 
 from . import _lib
-from .ops import _DTYPE_CODE, _FLOAT_DTYPES, _apply, _device_guard, _once, _raw_stream
+from .ops import _DTYPE_CODE, _FLOAT_DTYPES, _apply, _device_guard, _once, _raw_stream, _wants_node
 
 _LADDER = {"axis": 0, "shared": 1}
 _PAIRING = {"half": 0, "interleaved": 1}
@@ -143,7 +143,7 @@ def rotary(
         return query.clone() if key is None else (query.clone(), key.clone())
     args = (query, key, positions.contiguous(), (ctypes.c_int32 * A)(*axis_dims), float(base), _LADDER[ladder],
             _PAIRING[pairing])
-    if (query.requires_grad or (key is not None and key.requires_grad)) and torch.is_grad_enabled():
+    if _wants_node(query, key):
         return _apply(_RotaryFunction, *args)
     out, key_out = _turn(*args, 0)
     return out if key is None else (out, key_out)

@@ -7,11 +7,12 @@ import ctypes
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import layer_reference as ref
 from hostonly import host_only
 from layer_reference import close
-from msda_triton_b200 import _lib, attention, layer_norm
+from msda_triton_b200 import _lib, attention, layer_norm, rotary
 from test_layer_ops import DEV, DTYPES, HALF, _ids, randn
 
 gpu = pytest.mark.gpu
@@ -227,3 +228,24 @@ def test_attention_refuses_sizes_that_no_grid_holds():
         assert lib.msda_attention_backward(_attention_args(**over), None) == _lib.MSDA_ERR_INVALID_ARGUMENT
         assert b"workspace" in lib.msda_last_error()
     assert lib.msda_attention_workspace_size(None, 0) == 0
+
+
+@gpu
+@pytest.mark.parametrize("recorded", [True, False])
+def test_forward_mode_is_refused(recorded, cuda_lib):
+    """A tangent is not dropped: the operators have no forward-mode derivative."""
+    x, q = randn(3, 8), randn(1, 3, 2, 8)
+    w = randn(8)
+    pos = torch.arange(3, device=DEV).view(3, 1)
+    plain = layer_norm(x), rotary(q, pos, axis_dims=[8]), attention(q, q, q)
+    with forward_ad.dual_level(), torch.set_grad_enabled(recorded):
+        dx, dw, dq = (forward_ad.make_dual(t, t.clone()) for t in (x, w, q))
+        for call in (lambda: layer_norm(dx), lambda: layer_norm(x, dw), lambda: layer_norm(x, w, dw), lambda: layer_norm(x, residual=dx),
+                     lambda: rotary(dq, pos, axis_dims=[8]), lambda: rotary(q, pos, key=dq, axis_dims=[8]),
+                     lambda: attention(dq, q, q), lambda: attention(q, dq, q), lambda: attention(q, q, dq)):
+            with pytest.raises(RuntimeError, match="forward mode AD"):
+                call()
+        for a, b in zip(plain, (layer_norm(x), rotary(q, pos, axis_dims=[8]), attention(q, q, q))):
+            assert torch.equal(a, b)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(layer_norm, (x,), (x,))
