@@ -13,6 +13,7 @@ import layer_reference as ref
 from hostonly import host_only
 from layer_reference import close
 from msda_triton_b200 import _lib, attention, layer_norm, rotary
+from msda_triton_b200.attention import _pack
 from test_layer_ops import DEV, DTYPES, HALF, _ids, randn
 
 gpu = pytest.mark.gpu
@@ -249,3 +250,60 @@ def test_forward_mode_is_refused(recorded, cuda_lib):
             assert torch.equal(a, b)
     with pytest.raises(RuntimeError):
         torch.func.jvp(layer_norm, (x,), (x,))
+
+
+def test_attention_arguments_are_packed_as_the_header_lays_them_out():
+    """The one-call packing against the structure by its fields."""
+    tensors = [torch.empty(2, 3 + i % 2, 4, 8).transpose(1, 2).contiguous().transpose(1, 2) for i in range(8)]
+    lse, slopes = torch.empty(2, 4, 3), torch.empty(4)
+    ints = [torch.empty(n, dtype=torch.int32) for n in (6, 8, 2, 2)]
+    q, k, v, out, residue, dq, dk, dv = tensors
+    packed = _pack(q, k, v, out, residue, lse, (q, dq, dk, dv), (0.5, 20.0, 1, 7), (slopes, *ints), 4096, 12345)
+    a = _lib.AttentionArgs()
+    pointers = dict(query=q, key=k, value=v, out=out, out_residue=residue, lse=lse, grad_out=q, grad_query=dq, grad_key=dk, grad_value=dv,
+                    distance_slopes=slopes, query_documents=ints[0], key_documents=ints[1], prefix_lengths=ints[2], key_lengths=ints[3])
+    for n, t in pointers.items():
+        setattr(a, n, t.data_ptr())
+    for n, value in dict(batch=2, num_queries=3, num_keys=4, num_heads=4, num_key_heads=4, head_dim=8, dtype=0, scale=0.5, softcap=20.0,
+                         shared_document=7, causal=1, workspace=4096, workspace_bytes=12345).items():
+        setattr(a, n, value)
+    for n, t in dict(query_strides=q, key_strides=k, value_strides=v, grad_out_strides=q).items():
+        getattr(a, n)[:] = t.stride()[:3]
+    assert packed == bytes(a)
+
+
+@gpu
+def test_offsets_past_32_bits(cuda_lib):
+    """Tensors of more than 2^32 bytes and 2^31 elements, of which the last rows count."""
+    dtype, D, heads, near = torch.bfloat16, 128, 8, 200
+    n = 2**31 // (heads * D) + near  # rows of heads x D
+    x = torch.zeros(1, n, heads, D, dtype=dtype, device=DEV)
+    end = x[:, -near:]
+    end.copy_(randn(1, near, heads, D, dtype=dtype))
+    value = torch.zeros_like(x)
+    value[:, -near:] = randn(1, near, heads, D, dtype=dtype, seed=1)
+    ids = torch.full((1, n), -1, dtype=torch.int32, device=DEV)
+    ids[:, -near:] = 0
+    for Sq in (1, 130):
+        q, g = randn(1, Sq, heads, D, dtype=dtype, seed=2), randn(1, Sq, heads, D, dtype=dtype, seed=3)
+        want, _, grads = ref.attention(q, end, value[:, -near:], g)
+        leaves = [t.detach().requires_grad_() for t in (q, x, value)]
+        out = attention(*leaves, query_documents=ids[:, -Sq:].contiguous(), key_documents=ids)
+        close(out.detach(), want, dtype, *tolerance(dtype), floor=0.02, what="out")
+        dq, dk, dv = torch.autograd.grad(out, leaves, g)
+        for what, a, b in zip(("dq", "dk", "dv"), (dq, dk[:, -near:], dv[:, -near:]), grads):
+            close(a, b, dtype, *tolerance(dtype), floor=0.02, what=what)
+        assert not dk[:, :-near].any() and not dv[:, :-near].any()
+        del leaves, out, dq, dk, dv
+    del value, ids
+    rows, g = x.view(n * heads, D), torch.zeros_like(x).view(n * heads, D)
+    g[-near:] = randn(near, D, dtype=dtype, seed=5)
+    rows = rows.requires_grad_()
+    y = layer_norm(rows)
+    want, z, rstd = ref.layer_norm(rows.detach()[-near:], None, None, None, 1e-5)
+    close(y.detach()[-near:], want, dtype, 1.5, 8, floor=0.1, what="y")
+    close(torch.autograd.grad(y, rows, g)[0][-near:], ref.layer_norm_grad(z, rstd, None, g[-near:])[0], dtype, 1.5, 8, floor=0.1, what="dx")
+    del y, g, rows
+    at = torch.arange(n, device=DEV)[:, None]
+    y = rotary(x.detach(), at, axis_dims=[D])
+    close(y[:, -near:], ref.rotary(x.detach()[:, -near:], at[-near:], [D]), dtype, 1.5, 8, what="rotary")
