@@ -109,11 +109,11 @@ MSDA_API int msda_layer_norm_backward(const void* x, const void* residual, const
  *   - with causal: j <= place, or j < prefix_lengths[b] where given;
  *   - with documents: neither id is negative (padding), and the ids agree or
  *     the key's is shared_document (-1: none).
- * Scores: s = scale q.k; s = softcap tanh(s / softcap) (softcap 0: not); s -=
- * distance_slopes[h] |place - j|. A query that sees no key gets zeros, an lse
- * of -inf and no gradient. Keys past length_b and of negative documents are
- * never read into a result, whatever they hold; a key that other queries see
- * must be finite. The rows of query and grad_out of a query that sees no key
+ * Scores: s = scale q.k; s = softcap tanh(s / softcap) (softcap from 2^-100 to
+ * 2^100, or 0: not); s -= distance_slopes[h] |place - j|. A query that sees no
+ * key gets zeros, an lse of -inf and no gradient. Keys past length_b and of
+ * negative documents are never read into a result, whatever they hold; a key
+ * that other queries see must be finite. The rows of query and grad_out of a query that sees no key
  * may hold anything too.
  *
  * At most 65535 items, 4096 heads, 2^22 queries and 2^30 keys, 2^22 in the

@@ -121,6 +121,9 @@ int check(const char* fn, const msda_attention_args* a, bool backward) {
   if (int rc = check_sizes(fn, a, backward)) return rc;
   if (!std::isfinite(a->scale) || !std::isfinite(a->softcap) || a->softcap < 0)
     return fail(MSDA_ERR_INVALID_ARGUMENT, "%s: scale must be finite, softcap finite and >= 0", fn);
+  // Beyond, the cap to base 2 or its inverse leaves 32 bits.
+  if (a->softcap != 0 && (a->softcap < 0x1p-100f || a->softcap > 0x1p100f || !std::isfinite(a->scale / a->softcap)))
+    return fail(MSDA_ERR_INVALID_ARGUMENT, "%s: softcap=%g outside [2^-100, 2^100], or scale / softcap not finite", fn, (double)a->softcap);
   if (!a->query_documents != !a->key_documents)
     return fail(MSDA_ERR_INVALID_ARGUMENT, "%s: documents of queries and keys come together", fn);
   if (a->prefix_lengths && !a->causal) return fail(MSDA_ERR_INVALID_ARGUMENT, "%s: prefix_lengths needs causal", fn);

@@ -10,7 +10,6 @@ reproducible. There is no CPU path.
 
 from __future__ import annotations
 
-import math
 import struct
 
 import torch
@@ -20,6 +19,10 @@ from .ops import _DTYPE_CODE, _FLOAT_DTYPES, _apply, _device_guard, _once, _raw_
 
 # msda_attention_args of include/msda_layer_b200.h, packed in one call.
 _ARGS = struct.Struct("@10P3q4i12q2f5P2iPN")
+
+_FLOAT_MAX = torch.finfo(torch.float32).max
+# Wider and narrower caps leave 32 bits once they are taken to base 2 or divided by.
+_CAP_MIN, _CAP_MAX = 2.0**-100, 2.0**100
 
 
 def _laid_out(x: torch.Tensor) -> torch.Tensor:
@@ -129,6 +132,7 @@ def attention(
             ``h`` reads key head ``h // (H // Hkv)``.
         scale: of the scores; ``D ** -0.5`` by default.
         softcap: ``c > 0`` makes a score ``c * tanh(score / c)``; 0: not.
+            From ``2**-100`` to ``2**100``.
         distance_slopes: ``(H,)`` fp32; subtracts ``slope * |place - j|``.
             A constant: may not require a gradient.
         causal: key ``j`` must lie at ``j <= place``...
@@ -165,12 +169,13 @@ def attention(
         raise ValueError(f"attention: unsupported dtype {query.dtype}; use fp32, fp16 or bf16")
     scale = D ** -0.5 if scale is None else float(scale)
     softcap = float(softcap or 0.0)
-    if not math.isfinite(scale) or not 0.0 <= softcap < math.inf:
-        raise ValueError(f"attention: scale must be finite and softcap finite and >= 0, got {scale} and {softcap}")
+    if not abs(scale) <= _FLOAT_MAX or not (softcap == 0.0 or _CAP_MIN <= softcap <= _CAP_MAX and abs(scale) <= _FLOAT_MAX * softcap):
+        raise ValueError(f"attention: scale must be finite in 32 bits and softcap 0 or from 2**-100 to 2**100 (scale / softcap "
+                         f"finite too), got {scale} and {softcap}")
     if (query_documents is None) != (key_documents is None):
         raise ValueError("attention: query_documents and key_documents come together")
-    if shared_document is not None and (key_documents is None or shared_document < 0):
-        raise ValueError("attention: shared_document is an id >= 0 and needs documents")
+    if shared_document is not None and (key_documents is None or not 0 <= shared_document < 2**31):
+        raise ValueError("attention: shared_document is an int32 id >= 0 and needs documents")
     if prefix_lengths is not None and not causal:
         raise ValueError("attention: prefix_lengths needs causal=True")
     device = query.device

@@ -307,3 +307,36 @@ def test_offsets_past_32_bits(cuda_lib):
     at = torch.arange(n, device=DEV)[:, None]
     y = rotary(x.detach(), at, axis_dims=[D])
     close(y[:, -near:], ref.rotary(x.detach()[:, -near:], at[-near:], [D]), dtype, 1.5, 8, what="rotary")
+
+
+@pytest.mark.parametrize("how, words", [(dict(shared_document=2**31), "shared_document"), (dict(shared_document=-1), "shared_document"),
+                                        (dict(scale=1e39), "scale"), (dict(scale=float("-inf")), "scale"), (dict(softcap=1e39), "softcap"),
+                                        (dict(softcap=float("nan")), "softcap"), (dict(softcap=3e38), "softcap"),
+                                        (dict(softcap=1e-40), "softcap"), (dict(softcap=1e-29, scale=1e10), "scale")])
+def test_attention_refuses_numbers_that_32_bits_do_not_hold(how, words):
+    x, ids = torch.zeros(1, 2, 2, 8), torch.zeros(1, 2, dtype=torch.int32)
+    with pytest.raises(ValueError, match=words):
+        attention(x, x, x, query_documents=ids, key_documents=ids, **how)
+
+
+@host_only
+def test_c_abi_refuses_caps_that_leave_32_bits():
+    lib = _lib.load()
+    for over in (dict(softcap=3e38), dict(softcap=1e-40), dict(softcap=1e-29, scale=1e10)):
+        assert lib.msda_attention_forward(_attention_args(**over), None) == _lib.MSDA_ERR_INVALID_ARGUMENT
+        assert b"softcap" in lib.msda_last_error()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("softcap", [2.0**100, 2.0**-100])
+@pytest.mark.parametrize("Sq, H", [(1, 2), (300, 16)])
+def test_caps_at_their_limits(Sq, H, softcap, dtype, cuda_lib):
+    """The widest changes nothing, the narrowest leaves equal scores."""
+    q, k, v, g = (randn(1, Sq if i in (0, 3) else 300, H, 64, dtype=dtype, seed=i) for i in range(4))
+    want, _, grads = ref.attention(q, k, v, g, softcap=softcap)
+    q, k, v = (t.requires_grad_() for t in (q, k, v))
+    out = attention(q, k, v, softcap=softcap)
+    close(out.detach(), want, dtype, *tolerance(dtype), floor=0.02, what="out")
+    for n, a, b in zip(("dq", "dk", "dv"), torch.autograd.grad(out, (q, k, v), g), grads):
+        close(a, b, dtype, *tolerance(dtype), floor=0.02, what=n)
