@@ -204,7 +204,8 @@ Plan plan_of(const msda_attention_args* a, bool backward) {
     // keys where that leaves fewer than 2 CTAs an SM. With at least 512 and 2048
     // keys, 32 heads on 8 of 128 16-bit channels: 4 streams of 4096 to 16384 keys 69
     // and 44 us, 8 of up to 8192 58 and 46 us, 32 of 16384 377 and 366 us; fp32, 16
-    // of up to 8192 on 8 heads of 64 channels 129 and 184 us.
+    // of up to 8192 on 8 heads of 64 channels 129 and 184 us. (At 32 and 64 16-bit
+    // channels, where 2048 keys are a quarter and half of the bytes, not measured.)
     const int64_t tiles = (rows + 15) / 16;
     const int64_t ctas = std::max<int64_t>(1, a->batch * a->num_key_heads * tiles);
     const int64_t even = std::min<int64_t>(16 * sm_count() / ctas, a->num_keys / (tensor ? 2048 : 512));

@@ -568,9 +568,9 @@ __global__ void __launch_bounds__(FwdShape<DP>::kThreads, FwdShape<DP>::kCtas)
 // of bf16 gradients against 1.7e-3): a second 16-bit part would take a fourth
 // product and TMEM that is not there.
 // bf16, 8192 tokens on 16 heads, dq / dkv without a mask: 128 channels (4 key heads)
-// 748 / 1039 us (1100 and 1058 TFLOP/s counting what is formed), 64 channels 439 /
-// 711 us, 32 channels 402 / 667 us; causal at 128 channels 419 / 459 us, capped
-// too 439 / 540 us. Bound as the forward is: by products at 128 channels, below by
+// 748 / 1064 us (1100 and 1033 TFLOP/s counting what is formed), 64 channels 447 /
+// 712 us, 32 channels 413 / 664 us; causal at 128 channels 419 / 470 us, capped
+// too 442 / 542 us. Bound as the forward is: by products at 128 channels, below by
 // the exponentials and the traffic of scores between TMEM and registers.
 // ---------------------------------------------------------------------------
 template <int DP>

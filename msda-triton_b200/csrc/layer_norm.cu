@@ -21,11 +21,13 @@
 // for each step. Each CTA leaves one partial row of the two column sums; a second
 // kernel adds the partial rows in a fixed order.
 //
-// 88892 x 256 bf16 with a residual: forward 29 us (137 MB, 4.7 TB/s; three quarters
+// 88892 x 256 bf16 with a residual: forward 28 us (137 MB, 4.8 TB/s; three quarters
 // of the issue slots are taken, by the sums' shuffles), backward 42 us (182 MB, 4.3
-// TB/s) and 5 us for the columns. 2500 x 8192 fp32 with a residual: 45 and 61 us
-// (5.5 and 5.4 TB/s); 4095 x 5001 fp32, one element a load: 51 and 89 us (3.2 and
-// 2.8 TB/s).
+// TB/s: it waits for its loads, with two CTAs an SM at 115 registers) and 5 us for
+// the columns. 2500 x 8192 fp32 with a residual: 45 and 63 us (5.5 and 5.2 TB/s);
+// 4095 x 5001 fp32, one element a load since rows start at any element: 51 and 88 us
+// (3.2 and 2.8 TB/s); wider, 2000 x 20000 bf16 with a residual, a scalar a load and
+// rows read again for each step: 142 us, and 209 with 117 for the columns.
 #include <algorithm>
 
 #include "msda_abi.cuh"
@@ -477,9 +479,9 @@ struct NormShape {
 // Threads a row and channels a thread by the width alone: 8 channels, or 16
 // where a warp (up to 512) or 512 threads (up to 8192) hold the row with them. A
 // barrier for each sum costs more than the threads bring, forward and backward: 40000
-// x 512 bf16 28 and 42 us by warps, 37 and 69 us by 128 threads; 20000 x 768 bf16 23
-// and 41 us by 128 threads, 38 and 57 us by 256; 10000 x 2048 bf16 25 and 42 us by
-// 256, 45 and 59 us by 512.
+// x 512 bf16 27 and 42 us by warps, 37 and 69 us by 128 threads; 20000 x 768 bf16 23
+// and 31 us by 128 threads, 38 and 57 us by 256; 10000 x 2048 bf16 25 and 44 us by
+// 256, 45 and 59 us by 512. (The slower side's backward had two sums a row, not three.)
 int norm_threads_of(int64_t width) { return width <= 512 ? 32 : width <= 1024 ? 128 : width <= 2048 ? 256 : 512; }
 int norm_channels_of(int64_t width) { return width <= 8 * norm_threads_of(width) ? 8 : 16; }
 
@@ -494,7 +496,8 @@ NormShape norm_shape(int64_t width, int es, int64_t unit) {
   return s;
 }
 
-// Most CTAs of a backward, each of which leaves a partial row.
+// Most CTAs of a backward, each of which leaves a partial row. (Of the four an SM by
+// warps two are resident; grids of two were not measured.)
 int64_t norm_backward_most(int64_t width) {
   if (width > kRegisterWidth) return kNormSms * 2;
   return kNormSms * (norm_threads_of(width) <= 256 ? 4 : norm_channels_of(width) == 8 ? 2 : 1);

@@ -126,6 +126,11 @@ def attention(
     ``j < length`` and the causal and document masks below allow it. A query
     that sees no key gives zeros and no gradient.
 
+    With ``Sq == Sk`` and items padded at their end, ``key_lengths`` would thus
+    shift an item's places, its causal mask and its distances by its padding:
+    such prompts mark their padding by negative document ids instead (all else
+    id 0), and leave ``key_lengths`` out.
+
     Args:
         query: ``(B, Sq, H, D)``, fp32, fp16 or bf16, ``D <= 256``.
         key, value: ``(B, Sk, Hkv, D)``, ``H`` a multiple of ``Hkv``: head
@@ -143,8 +148,9 @@ def attention(
             which sees nothing and is not seen.
         shared_document: a document whose keys every query that is no padding
             sees (the matching queries beside denoising groups).
-        key_lengths: ``(B,)`` int32, visible keys of each item. What lies past
-            them is never read into a result.
+        key_lengths: ``(B,)`` int32, visible keys of each item, the last of
+            which is the last query's own (see above). What lies past them is
+            never read into a result.
         return_lse: also return the log-sum-exp of the scores, ``(B, H, Sq)``
             fp32 (-inf for a row that sees no key); not differentiable.
 
