@@ -16,9 +16,9 @@
 // weights, and in the backward their gradients' running sums, in registers from
 // row to row, and the next row's loads are in flight while a row is reduced.
 // Longer rows are bound by the latency of their sums over the CTA, so that these
-// go together, two in the forward and three in the backward. (Staging rows in shared memory by bulk copies was slower: 20000 x
-// 1000 bf16 forward 91 us for 29.) Rows wider than 8192 are read again from L2
-// for each step. Each CTA leaves one partial row of the two column sums; a second
+// go together, two in the forward and three in the backward. (Staging rows in shared
+// memory by bulk copies was slower: 20000 x 1000 bf16 forward 91 us for 29.) Rows
+// wider than 8192 are read again from L2 for each step. Each CTA leaves one partial row of the two column sums; a second
 // kernel adds the partial rows in a fixed order.
 //
 // 88892 x 256 bf16 with a residual: forward 28 us (137 MB, 4.8 TB/s; three quarters
